@@ -407,15 +407,16 @@ def _plain_sample(s):
         w = w * ((before < p * w.sum(-1, keepdim=True)) | (rank == 0) | (p >= 1))
     if s["min_p"] is not None:
         w = w * ((w >= s["min_p"][:, None].double()) | (rank == 0))
-    w = torch.zeros_like(w).scatter_(-1, order, w)
     cdf = w.cumsum(-1)
     target = s["uniforms"][:, None].double() * cdf[:, -1:]
-    token = torch.searchsorted(cdf, target, right=True)
+    at = torch.searchsorted(cdf, target, right=True)
     # A target that rounding put on the sum: the last token with weight.
-    last = torch.where(w > 0, rank, -1).amax(-1, keepdim=True)
-    token = torch.minimum(token, last)
-    logprob = (w.gather(-1, token.clamp(min=0)) / cdf[:, -1:]).log().float()
-    return token[:, 0], logprob[:, 0].masked_fill(token[:, 0] < 0, float("-inf"))
+    at = torch.minimum(at, torch.where(w > 0, rank, -1).amax(-1, keepdim=True))
+    none = at[:, 0] < 0
+    at = at.clamp(min=0)
+    logprob = (w.gather(-1, at) / cdf[:, -1:]).log().float()[:, 0]
+    token = order.gather(-1, at)[:, 0]
+    return token.masked_fill(none, -1), logprob.masked_fill(none, float("-inf"))
 
 
 # ---------------------------------------------------------------------------
@@ -565,7 +566,6 @@ def _exact_sample(s):
             n = int((mass < p * mass[-1]).sum()) + 1
             head = head[:n]
         head = head[(w[head] >= m * w[order[0]]) | (head == order[0])]
-        head = head.sort().values
         mass = w[head].cumsum(0)
         at = int((mass <= s["uniforms"][r].double() * mass[-1]).sum().clamp(max=len(head) - 1))
         tokens.append(int(head[at]))
