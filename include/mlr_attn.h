@@ -597,6 +597,52 @@ int mlr_paged_kv_read_floor(const void *k_cache, const void *v_cache, int64_t nu
                             int64_t batch, int64_t tokens_per_item, uint32_t *out,
                             int64_t out_len, void *stream);
 
+/*
+ * RMSNorm of each q and k head, rotary positions and the append of k and v to
+ * the paged cache, from rows [q heads | k heads | v heads] x head_dim. With R =
+ * rotary_dim and i < R / 2, per q or k head x:
+ *   n_j = x_j w_j / sqrt(mean(x^2) + eps) (n = x where q_weight, k_weight, which
+ *   come together, are null); the pair (n_i, n_{i + R/2}), or (n_2i, n_2i+1) if
+ *   interleaved, is turned by positions[t] * inv_freq[i], cosine and sine times
+ *   attention_factor; elements from R on are n_j.
+ * FP32 arithmetic (angles in 64 bits), one rounding. q_out has rows of
+ * num_q_heads * head_dim; weights are in `dtype`. Any even head_dim up to 1024
+ * whose rows start at multiples of 16 bytes and whose head_dim / 2 and R / 2 are
+ * multiples of 16 bytes; up to 512 where they are so for 4 elements, and up to
+ * 128 otherwise. A slot outside [0, num_slots) writes no k and v.
+ */
+int mlr_qk_norm_rope_write(const void *qkv, int64_t qkv_stride_t, const void *q_weight,
+                           const void *k_weight, double eps, const int64_t *positions,
+                           const float *inv_freq, int64_t rotary_dim, int interleaved,
+                           double attention_factor, const void *slot_mapping, int index_dtype,
+                           void *q_out, int64_t q_out_stride_t, void *k_cache, void *v_cache,
+                           int64_t num_slots, int64_t num_tokens, int64_t num_q_heads,
+                           int64_t num_kv_heads, int64_t head_dim, int dtype, void *stream);
+
+/*
+ * One token per row of logits [num_logit_rows, vocab] (FP32, fp16, bf16), drawn
+ * with uniforms[r] in [0, 1) (FP32, or 64 bits with uniforms_f64). Row r reads
+ * logits row row_ids[r], or r where row_ids is null. temperature, top_k (index
+ * dtype top_k_dtype), top_p and min_p are arrays of num_rows, or where null the
+ * value beside them holds for every row:
+ *   w_i = exp((x_i - max x) / temperature); in descending order of x, ties by
+ *   index, keep the first top_k (all if <= 0), of those the shortest head that
+ *   weighs at least top_p times their sum (all if >= 1, one if <= 0), of those
+ *   the ones with w_i >= min_p (all if <= 0; the first always). The token is the
+ *   first of the order whose running sum exceeds u times the sum S of the kept,
+ *   and logprobs[r] (may be null) is log(w / S).
+ * temperature <= 0 (or NaN), or an infinite maximum: the first of the order,
+ * logprob 0. A row without a value above -inf, or a row id out of range: -1 and
+ * -inf. NaN logits are never drawn. vocab <= 2^23.
+ */
+int mlr_sample_tokens(const void *logits, int64_t row_stride, int64_t num_logit_rows, int dtype,
+                      const int64_t *row_ids, const void *uniforms, int uniforms_f64,
+                      const float *temperature, double temperature_value, const void *top_k,
+                      int top_k_dtype, int64_t top_k_value, const float *top_p,
+                      double top_p_value, const float *min_p, double min_p_value,
+                      int64_t *tokens, float *logprobs, int64_t num_rows, int64_t vocab,
+                      void *stream);
+
 #ifdef __cplusplus
 }
 #endif

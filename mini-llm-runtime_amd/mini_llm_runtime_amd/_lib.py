@@ -115,6 +115,17 @@ _PROTOTYPES = {
          _c_i64, _c_ptr, _c_ptr, _c_ptr, _c_ptr, _c_i64, _c_i64, _c_i64, _c_i64, _c_i64, _c_int,
          _c_ptr],
     ),
+    "mlr_qk_norm_rope_write": (
+        _c_int,
+        [_c_ptr, _c_i64, _c_ptr, _c_ptr, _c_f64, _c_ptr, _c_ptr, _c_i64, _c_int, _c_f64, _c_ptr,
+         _c_int, _c_ptr, _c_i64, _c_ptr, _c_ptr, _c_i64, _c_i64, _c_i64, _c_i64, _c_i64, _c_int,
+         _c_ptr],
+    ),
+    "mlr_sample_tokens": (
+        _c_int,
+        [_c_ptr, _c_i64, _c_i64, _c_int, _c_ptr, _c_ptr, _c_int, _c_ptr, _c_f64, _c_ptr, _c_int,
+         _c_i64, _c_ptr, _c_f64, _c_ptr, _c_f64, _c_ptr, _c_ptr, _c_i64, _c_i64, _c_ptr],
+    ),
     "mlr_pa_accumulate": (_c_int, [_c_ptr, _c_ptr, _c_ptr, _c_i64, _c_ptr]),
     "mlr_build_step_metadata": (
         _c_int,

@@ -12,12 +12,19 @@ apply_rotary_pos_emb -> kv_cache.write_slots (model/qwen2.py:125-209,
 rotation and KV write and the batched paged decode in one launch
 (``mlr_paged_decode_qkv``).
 
+``qk_norm_rope_write`` (``mlr_qk_norm_rope_write``) is the step for models
+that normalise each query and key head, or rotate neighbouring elements, part
+of the head or at the stretched positions of ``rotary_frequencies``; it
+computes in FP32 and rounds once.
+
 Checks are on shapes, dtypes and devices only; slot values are the caller's
 to validate (``PagedKVCache.check_slots`` runs the reference's write_slots
 checks). A slot outside the pool is not written.
 """
 
 from __future__ import annotations
+
+import math
 
 import torch
 
@@ -239,4 +246,140 @@ def qkv_rope_decode(qkv: torch.Tensor, inv_freq: torch.Tensor, kv_cache: PagedKV
             workspace.numel(), out.data_ptr(), out.stride(0), out.stride(1),
             _lib.stream_handle(device))
     _lib.check(status, "mlr_paged_decode_qkv")
+    return out
+
+
+def rotary_frequencies(rotary_dim: int, base: float = 10000.0, *, scaling: str | None = None,
+                       factor: float = 1.0, original_max_position: int = 0,
+                       beta_fast: float = 32.0, beta_slow: float = 1.0,
+                       device: torch.device | str | None = None) -> tuple[torch.Tensor, float]:
+    """(inv_freq [rotary_dim / 2] in FP32, attention_factor) for
+    ``qk_norm_rope_write``: f_i = base ** (-2 i / rotary_dim), stretched for
+    contexts ``factor`` times as long by
+
+    - None: not at all;
+    - "linear": f_i / factor;
+    - "ntk": base * factor ** (rotary_dim / (rotary_dim - 2)) in place of base;
+    - "yarn": f_i where a pair turns more than beta_fast times over
+      original_max_position positions, f_i / factor where fewer than beta_slow
+      times, and between the two a mix linear in the pair's index; attention_factor
+      is 0.1 ln(factor) + 1 (1 otherwise).
+    """
+    if rotary_dim <= 0 or rotary_dim % 2:
+        raise ValueError("rotary_dim must be a positive even number")
+    if not base > 0:
+        raise ValueError("base must be positive")
+    if not factor >= 1:
+        raise ValueError("factor must be at least 1")
+    if scaling not in (None, "linear", "ntk", "yarn"):
+        raise ValueError(f"unknown rotary scaling {scaling!r}")
+    half = rotary_dim // 2
+    index = torch.arange(half, dtype=torch.float64)
+    attention_factor = 1.0
+    if scaling == "ntk":
+        if rotary_dim < 4:
+            raise ValueError("ntk scaling needs a rotary_dim of at least 4")
+        base = base * factor ** (rotary_dim / (rotary_dim - 2))
+    freq = base ** (-index / half)
+    if scaling == "linear":
+        freq = freq / factor
+    elif scaling == "yarn":
+        if original_max_position <= 0:
+            raise ValueError("yarn scaling needs original_max_position")
+        if not beta_fast > beta_slow > 0:
+            raise ValueError("beta_fast must exceed beta_slow, which must be positive")
+
+        def index_of(turns: float) -> float:
+            return half * math.log(original_max_position / (turns * 2 * math.pi)) / math.log(base)
+
+        first = max(math.floor(index_of(beta_fast)), 0)
+        last = min(math.ceil(index_of(beta_slow)), rotary_dim - 1)
+        mix = ((index - first) / max(last - first, 1e-3)).clamp(0, 1)
+        freq = freq * (1 - mix) + freq / factor * mix
+        attention_factor = 0.1 * math.log(factor) + 1.0
+    return freq.to(torch.float32).to(device), attention_factor
+
+
+def qk_norm_rope_write(qkv: torch.Tensor, positions: torch.Tensor, inv_freq: torch.Tensor,
+                       k_cache: torch.Tensor, v_cache: torch.Tensor, slot_mapping: torch.Tensor,
+                       num_q_heads: int, *, q_weight: torch.Tensor | None = None,
+                       k_weight: torch.Tensor | None = None, eps: float = 1e-6,
+                       interleaved: bool = False, attention_factor: float = 1.0,
+                       out: torch.Tensor | None = None) -> torch.Tensor:
+    """qkv [T, (Hq + 2 Hkv) * D] -> rotated q [T, Hq, D]; k and v to the cache,
+    in one launch (``mlr_qk_norm_rope_write``).
+
+    Each q and k head x is normalised with q_weight and k_weight [D] if they
+    are given, x_j w_j / sqrt(mean(x^2) + eps), and its first R = 2 *
+    inv_freq.numel() elements are rotated by position * inv_freq[i]: the pairs
+    (x_i, x_{i + R/2}), or (x_2i, x_2i+1) if ``interleaved``; cosine and sine
+    are multiplied by attention_factor. Elements from R on keep their
+    (normalised) values. The arithmetic is FP32 (angles in 64 bits: exact
+    positions up to 2^53) with one rounding at the end.
+
+    positions int64 [T]; inv_freq [R / 2], used as FP32; k_cache and v_cache one
+    contiguous layer [num_blocks, block_size, Hkv, D] in qkv's dtype;
+    slot_mapping int32/int64 [T]: a token whose slot lies outside the cache
+    (-1 in a padded batch) writes no k and v, and no two tokens may share a slot.
+    """
+    if k_cache.ndim != 4 or k_cache.shape != v_cache.shape:
+        raise ValueError("k_cache and v_cache must both have shape [num_blocks, block_size, Hkv, D]")
+    num_blocks, block_size, hkv, d = k_cache.shape
+    if num_q_heads <= 0 or hkv == 0 or num_q_heads % hkv != 0:
+        raise ValueError("num_q_heads must be a positive multiple of the cache's KV heads")
+    width = (num_q_heads + 2 * hkv) * d
+    dtype = qkv.dtype
+    if qkv.ndim != 2 or qkv.shape[1] != width:
+        raise ValueError(f"qkv must have shape [num_tokens, {width}], got {tuple(qkv.shape)}")
+    tokens = qkv.shape[0]
+    if dtype not in _SUPPORTED:
+        raise TypeError(f"qkv dtype {dtype} is not supported")
+    if k_cache.dtype != dtype or v_cache.dtype != dtype:
+        raise TypeError("qkv dtype must match the KV cache dtype")
+    if tokens > 0 and (qkv.stride(1) != 1 or (tokens > 1 and qkv.stride(0) < width)):
+        raise ValueError("qkv rows must be contiguous")
+    if positions.shape != (tokens,) or positions.dtype != torch.long:
+        raise ValueError("positions must be an int64 tensor of shape [num_tokens]")
+    if slot_mapping.shape != (tokens,):
+        raise ValueError("slot_mapping must have shape [num_tokens]")
+    if slot_mapping.dtype not in _lib.INDEX_CODES:
+        raise TypeError("slot_mapping must use an integer index dtype")
+    rotary_dim = 2 * inv_freq.numel()
+    if inv_freq.ndim != 1 or not 0 < rotary_dim <= d:
+        raise ValueError(f"inv_freq must have shape [R / 2] with 0 < R <= {d}")
+    if (q_weight is None) != (k_weight is None):
+        raise ValueError("q_weight and k_weight must be given together")
+    tensors = (qkv, positions, inv_freq, slot_mapping, k_cache, v_cache)
+    if q_weight is not None:
+        if (q_weight.shape != (d,) or k_weight.shape != (d,) or q_weight.dtype != dtype
+                or k_weight.dtype != dtype):
+            raise ValueError(f"q_weight and k_weight must have shape [{d}] and the qkv dtype")
+        q_weight, k_weight = q_weight.contiguous(), k_weight.contiguous()
+        tensors += (q_weight, k_weight)
+    if out is None:
+        out = torch.empty((tokens, num_q_heads, d), dtype=dtype, device=qkv.device)
+    elif (out.shape != (tokens, num_q_heads, d) or out.dtype != dtype
+          or (tokens > 0 and (out.stride(2) != 1 or out.stride(1) != d
+                              or (tokens > 1 and out.stride(0) < num_q_heads * d)))):
+        raise ValueError("out must be [num_tokens, num_q_heads, head_dim] with contiguous heads")
+    device = _lib.require_hip(*tensors, out, what="qk_norm_rope_write")
+    if not (k_cache.is_contiguous() and v_cache.is_contiguous()):
+        raise ValueError("KV cache layers must be contiguous")
+    if tokens == 0:
+        return out
+    freq = _freq_fp32(inv_freq)
+    positions, slot_mapping = positions.contiguous(), slot_mapping.contiguous()
+    many = tokens > 1
+    lib = _lib.load()
+    with _lib.on(device):
+        status = lib.mlr_qk_norm_rope_write(
+            qkv.data_ptr(), qkv.stride(0) if many else width,
+            None if q_weight is None else q_weight.data_ptr(),
+            None if k_weight is None else k_weight.data_ptr(), eps, positions.data_ptr(),
+            freq.data_ptr(), rotary_dim, interleaved, attention_factor, slot_mapping.data_ptr(),
+            _lib.INDEX_CODES[slot_mapping.dtype], out.data_ptr(),
+            out.stride(0) if many else num_q_heads * d, k_cache.data_ptr(), v_cache.data_ptr(),
+            num_blocks * block_size, tokens, num_q_heads, hkv, d, _lib.DTYPE_CODES[dtype],
+            _lib.stream_handle(device))
+    _lib.check(status, "mlr_qk_norm_rope_write")
     return out
