@@ -620,6 +620,79 @@ int mlr_qk_norm_rope_write(const void *qkv, int64_t qkv_stride_t, const void *q_
                            int64_t num_kv_heads, int64_t head_dim, int dtype, void *stream);
 
 /*
+ * Paged attention with capped or biased scores over one layer's cache. For the
+ * query at position i of head h and key j:
+ *   x = scale * q.k;  softcap > 0: x = softcap * tanh(x / softcap);
+ *   alibi_slopes (FP32 [num_q_heads], may be null): x -= alibi_slopes[h] * |i - j|
+ * and out is the softmax of x over the visible keys times V; a query that sees
+ * no key (or none with a score above -inf) gets zeros. FP32, fp16 and bf16,
+ * head_dim a multiple of 8 (FP32: 4) up to 128, any block_size, fewer than 2^31
+ * positions per table; q rows, the cache and the row strides are 16-byte
+ * aligned, out rows have unit stride. FP32 scores and sums; 16-bit types round the
+ * probabilities once as operands of the matrix cores and the result once.
+ * Block ids out of range mask their keys, whose K and V are not read; V rows of
+ * keys that no query of the call sees may hold anything. Workspaces (sizes by
+ * the functions beside each call, 0 where none is needed) need no preparation
+ * and belong to the call until it has finished on its stream.
+ *
+ * mlr_paged_decode_scored: one token per sequence, q [batch, Hq, D] at position
+ * seq_lens[b] - 1, keys [0, seq_lens[b]). A length of 0 (a padded row) gives
+ * zeros.
+ *
+ * mlr_paged_prefill_scored: packed chunks as for mlr_paged_prefill: sequence s
+ * has the rows [query_start_loc[s], query_start_loc[s+1]) of q [total_q, Hq, D],
+ * the last of context_lens[s] positions. Key j is visible to the query at i if
+ * j <= i, or j < prefix_lens[s] (may be null; at most the context). Rows outside
+ * all sequences are not written. max_query_len is at least the longest chunk.
+ *
+ * mlr_paged_decode_shared_prefix: mlr_paged_decode_scored for a batch whose
+ * requests share their first prefix_len positions, which are read once for all
+ * of them through prefix_table [prefix_blocks]; positions from prefix_len on
+ * are looked up in block_tables (indexed by position as ever, so entries before
+ * prefix_len / block_size are not read). seq_lens count the prefix too.
+ *
+ * No counterpart in the reference.
+ */
+size_t mlr_paged_decode_scored_workspace_size(int64_t batch, int64_t num_q_heads,
+                                              int64_t num_kv_heads, int64_t head_dim,
+                                              int64_t max_context);
+int mlr_paged_decode_scored(const void *q, int64_t q_stride_b, int64_t q_stride_h,
+                            const void *k_cache, const void *v_cache, int64_t num_blocks,
+                            int64_t block_size, int64_t num_kv_heads, int64_t head_dim,
+                            const int64_t *block_tables, int64_t bt_stride, int64_t max_blocks,
+                            const int64_t *seq_lens, int64_t batch, int64_t num_q_heads,
+                            double scale, double softcap, const float *alibi_slopes, int dtype,
+                            void *workspace, size_t workspace_bytes, void *out,
+                            int64_t out_stride_b, int64_t out_stride_h, void *stream);
+size_t mlr_paged_prefill_scored_workspace_size(int64_t num_seqs, int64_t max_query_len,
+                                               int64_t max_context, int64_t num_q_heads,
+                                               int64_t num_kv_heads, int64_t head_dim, int dtype);
+int mlr_paged_prefill_scored(const void *q, int64_t q_stride_t, int64_t q_stride_h,
+                             const void *k_cache, const void *v_cache, int64_t num_blocks,
+                             int64_t block_size, int64_t num_kv_heads, int64_t head_dim,
+                             const int64_t *block_tables, int64_t bt_stride, int64_t max_blocks,
+                             const int64_t *query_start_loc, const int64_t *context_lens,
+                             const int64_t *prefix_lens, int64_t num_seqs, int64_t total_q,
+                             int64_t max_query_len, int64_t num_q_heads, double scale,
+                             double softcap, const float *alibi_slopes, int dtype,
+                             void *workspace, size_t workspace_bytes, void *out,
+                             int64_t out_stride_t, int64_t out_stride_h, void *stream);
+size_t mlr_paged_decode_shared_prefix_workspace_size(int64_t batch, int64_t num_q_heads,
+                                                     int64_t num_kv_heads, int64_t head_dim,
+                                                     int64_t prefix_len, int64_t max_context,
+                                                     int dtype);
+int mlr_paged_decode_shared_prefix(const void *q, int64_t q_stride_b, int64_t q_stride_h,
+                                   const void *k_cache, const void *v_cache, int64_t num_blocks,
+                                   int64_t block_size, int64_t num_kv_heads, int64_t head_dim,
+                                   const int64_t *prefix_table, int64_t prefix_blocks,
+                                   int64_t prefix_len, const int64_t *block_tables,
+                                   int64_t bt_stride, int64_t max_blocks,
+                                   const int64_t *seq_lens, int64_t batch, int64_t num_q_heads,
+                                   double scale, double softcap, const float *alibi_slopes,
+                                   int dtype, void *workspace, size_t workspace_bytes, void *out,
+                                   int64_t out_stride_b, int64_t out_stride_h, void *stream);
+
+/*
  * One token per row of logits [num_logit_rows, vocab] (FP32, fp16, bf16), drawn
  * with uniforms[r] in [0, 1) (FP32, or 64 bits with uniforms_f64). Row r reads
  * logits row row_ids[r], or r where row_ids is null. temperature, top_k (index

@@ -1,0 +1,113 @@
+// What the scored attention kernels share: a call's operands, the cut of its
+// work into items, the scores, and the layout of partial results.
+//
+// A unit is a group of query rows that share their keys: kRows consecutive rows
+// of one sequence and KV head, a row being one (token, query head of the KV
+// head's group), tokens first. Its keys are cut into splits of equal length;
+// an item is one (unit, split, KV head). The split length is chosen on the
+// device from the lengths themselves: the whole call makes about `target`
+// items whatever the table's width says, and the same lengths always give the
+// same splits.
+#pragma once
+
+#include "mlr_common.h"
+
+namespace mlr {
+
+enum ScoredMode {
+  kModePrefill = 0,  // packed chunks, causal, prefixes seen ahead
+  kModeDecode = 1,   // one token a sequence
+  kModePrefix = 2,   // one token a sequence, the keys [0, prefix) of one table
+};
+
+constexpr int kMinSplit = 128;  // keys of the shortest split
+
+struct ScoredParams {
+  const void *q, *k, *v;
+  int64_t q_st, q_sh;
+  int64_t num_blocks, block_size;
+  int hkv, group, d, hq;
+  const int64_t *bt, *ctx, *qsl, *ahead;
+  int64_t bt_st, bt_width;
+  int seqs, tiles;         // sequences; units of a sequence (kModePrefix: of the call)
+  int64_t total_q;         // rows of q
+  int64_t start;           // first key (kModeDecode), number of keys (kModePrefix)
+  float scale, cap;
+  const float *slopes;
+  void *out;
+  int64_t o_st, o_sh;
+  int mode, units;
+  bool force_partial;      // results go to the workspace even of a single split
+  int64_t target;          // items the call is cut into, about
+  int *first;              // [units + 1]: items before each unit (of one KV head)
+  float *ml, *acc;         // [items][kRows][2], [items][kRows][D] of partial results
+};
+
+// One unit's rows and keys.
+struct Unit {
+  int64_t q0;      // row of q of the sequence's first token
+  int64_t pos0;    // position of that token (kModePrefill)
+  int64_t ctx;     // keys of the sequence
+  int64_t ahead;   // keys visible to every query
+  int64_t lo, hi;  // keys [lo, hi) that some row sees
+  int rows, r0;    // rows of the sequence; first of the unit
+  int seq;
+};
+
+__device__ __forceinline__ int64_t clamp64(int64_t x, int64_t lo, int64_t hi) {
+  return x < lo ? lo : x > hi ? hi : x;
+}
+
+__device__ __forceinline__ Unit unit_of(const ScoredParams &p, int u, int kRows) {
+  Unit t;
+  t.seq = p.mode == kModePrefix ? 0 : u / p.tiles;
+  t.r0 = (u - t.seq * p.tiles) * kRows;
+  const int64_t covered = p.bt_width * p.block_size;
+  t.pos0 = t.ahead = 0;
+  t.lo = 0;
+  if (p.mode == kModePrefill) {
+    t.q0 = clamp64(p.qsl[t.seq], 0, p.total_q);
+    const int64_t end = clamp64(p.qsl[t.seq + 1], t.q0, p.total_q);
+    t.ctx = clamp64(p.ctx[t.seq], 0, covered);
+    t.pos0 = t.ctx - (end - t.q0);
+    t.ahead = p.ahead ? clamp64(p.ahead[t.seq], 0, t.ctx) : 0;
+    const int64_t rows = (end - t.q0) * p.group;
+    t.rows = static_cast<int>(rows);
+    const int64_t last = (rows < t.r0 + kRows ? rows : t.r0 + kRows) - 1;
+    t.hi = t.r0 < rows ? t.pos0 + last / p.group + 1 : 0;
+    if (t.hi < t.ahead && t.r0 < rows) t.hi = t.ahead;
+    if (t.hi < 0) t.hi = 0;
+  } else if (p.mode == kModeDecode) {
+    t.q0 = t.seq;
+    t.ctx = clamp64(p.ctx[t.seq], 0, covered);
+    t.rows = p.group;
+    t.hi = t.ctx;
+    t.lo = p.start;
+  } else {
+    t.q0 = 0;
+    t.ctx = 0;
+    t.rows = p.seqs * p.group;
+    t.hi = p.start < covered ? p.start : covered;
+  }
+  return t;
+}
+
+// Splits of a unit start at multiples of 16 keys.
+__device__ __forceinline__ int64_t unit_base(const Unit &t) { return t.lo & ~int64_t(15); }
+__device__ __forceinline__ int64_t unit_len(const Unit &t) {
+  return t.hi > t.lo && t.r0 < t.rows ? t.hi - unit_base(t) : 0;
+}
+// A unit with rows but no key has one item, which writes what an empty sum gives.
+__device__ __forceinline__ int unit_items(const Unit &t, int64_t split) {
+  if (t.r0 >= t.rows) return 0;
+  const int64_t n = (unit_len(t) + split - 1) / split;
+  return n > 0 ? static_cast<int>(n) : 1;
+}
+__device__ __forceinline__ int64_t split_of(int64_t total_keys, const ScoredParams &p) {
+  const int64_t s = (total_keys * p.hkv + p.target - 1) / p.target;
+  return ((s > kMinSplit ? s : kMinSplit) + 63) & ~int64_t(63);
+}
+
+int launch_scored_rows(const ScoredParams &p, int dtype, unsigned grid, hipStream_t stream);
+
+}  // namespace mlr

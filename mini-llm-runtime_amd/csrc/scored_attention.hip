@@ -1,0 +1,364 @@
+// Entry points of paged attention with capped or biased scores, and the sum of
+// the partial results that splits leave in the workspace.
+#include "scored_attention.h"
+
+#include <algorithm>
+
+namespace mlr {
+namespace {
+
+constexpr float kLog2e = 1.4426950408889634f;
+constexpr int kRows = 16;
+
+// out = sum_i 2^{m_i - M} O_i / sum_i 2^{m_i - M} l_i over a row's items, those
+// of `p` and, for a shared prefix, of `x` too. One workgroup per (unit of p, KV
+// head), 16 threads per row; items are added in their order. A unit that has
+// written its result itself is left alone.
+template <typename T, int D>
+__global__ __launch_bounds__(256) void scored_merge(ScoredParams p, ScoredParams x, bool prefixed,
+                                                    int x_rows) {
+  constexpr int kVe = D / 16;
+  const int u = blockIdx.x / p.hkv, kvh = blockIdx.x - u * p.hkv;
+  const int first = p.first[u], count = p.first[u + 1] - first;
+  if (count == 0 || (count == 1 && !p.force_partial)) return;
+  const Unit t = unit_of(p, u, kRows);
+  const int rr = threadIdx.x >> 4, d0 = (threadIdx.x & 15) * kVe;
+  const int r = t.r0 + rr;
+  if (r >= t.rows) return;
+  const int tok = r / p.group, g = r - tok * p.group;
+  // Items of the row: `count` from p, then `more` from x.
+  int64_t at = (static_cast<int64_t>(first) * p.hkv + kvh) * kRows + rr, x_at = 0;
+  int more = 0;
+  if (prefixed) {
+    const int xr = t.seq * p.group + g;
+    const int xu = xr / x_rows;
+    const int x_first = x.first[xu];
+    more = x.first[xu + 1] - x_first;
+    x_at = (static_cast<int64_t>(x_first) * x.hkv + kvh) * x_rows + (xr - xu * x_rows);
+  }
+  const int64_t step = static_cast<int64_t>(p.hkv) * kRows;
+  const int64_t x_step = static_cast<int64_t>(p.hkv) * x_rows;
+  float m = -INFINITY;
+  for (int i = threadIdx.x & 15; i < count; i += 16) m = fmaxf(m, p.ml[2 * (at + i * step)]);
+  for (int i = threadIdx.x & 15; i < more; i += 16) m = fmaxf(m, x.ml[2 * (x_at + i * x_step)]);
+#pragma unroll
+  for (int o = 8; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor(m, o));
+  const float ref = m == -INFINITY ? 0.f : m;
+  float sum = 0.f, acc[kVe];
+#pragma unroll
+  for (int n = 0; n < kVe; ++n) acc[n] = 0.f;
+  auto add = [&](const ScoredParams &s, int64_t row) __attribute__((always_inline)) {
+    const float f = __builtin_amdgcn_exp2f((s.ml[2 * row] - ref) * kLog2e);
+    sum += s.ml[2 * row + 1] * f;
+#pragma unroll
+    for (int n = 0; n < kVe; n += 4) {
+      const float4 v = *reinterpret_cast<const float4 *>(s.acc + row * D + d0 + n);
+      acc[n] += v.x * f;
+      acc[n + 1] += v.y * f;
+      acc[n + 2] += v.z * f;
+      acc[n + 3] += v.w * f;
+    }
+  };
+#pragma unroll 4
+  for (int i = 0; i < count; ++i) add(p, at + i * step);
+#pragma unroll 4
+  for (int i = 0; i < more; ++i) add(x, x_at + i * x_step);
+  const float inv = sum > 0.f ? 1.f / sum : sum == 0.f ? 0.f : sum;
+  T *dst = static_cast<T *>(p.out) + (t.q0 + tok) * p.o_st + (kvh * p.group + g) * p.o_sh;
+#pragma unroll
+  for (int n = 0; n < kVe; ++n)
+    if (d0 + n < p.d) dst[d0 + n] = Elem<T>::from_f32(acc[n] * inv);
+}
+
+int launch_merge(const ScoredParams &p, const ScoredParams &x, bool prefixed, int x_rows, int dtype,
+                 hipStream_t stream) {
+  const unsigned grid = static_cast<unsigned>(p.units) * p.hkv;
+#define MLR_MERGE(T)                                                                       \
+  if (p.d > 64) scored_merge<T, 128><<<grid, 256, 0, stream>>>(p, x, prefixed, x_rows);    \
+  else scored_merge<T, 64><<<grid, 256, 0, stream>>>(p, x, prefixed, x_rows)
+  if (dtype == MLR_DTYPE_F32) {
+    MLR_MERGE(float);
+  } else if (dtype == MLR_DTYPE_F16) {
+    MLR_MERGE(f16_t);
+  } else {
+    MLR_MERGE(bf16_t);
+  }
+#undef MLR_MERGE
+  return check_launch("scored_merge");
+}
+
+int64_t target_items() {
+  const int cus = current_device_cus();
+  return 2 * static_cast<int64_t>(cus > 0 ? cus : 256);
+}
+
+// Items of a call at most, over its KV heads.
+int64_t max_items(int64_t units, int64_t hkv, int64_t max_keys) {
+  const int64_t by_len = units * std::max<int64_t>(1, ceil_div(max_keys + 15, kMinSplit));
+  return std::min(by_len, units + ceil_div(target_items(), hkv) + 1) * hkv;
+}
+
+size_t align256(size_t n) { return (n + 255) & ~size_t(255); }
+
+// Workspace of one kernel's partial results: [first | ml | acc].
+size_t part_bytes(int64_t units, int64_t items, int64_t rows, int64_t d) {
+  const int64_t wide = d > 64 ? 128 : 64;
+  return align256((units + 1) * sizeof(int)) + align256(items * rows * 2 * sizeof(float)) +
+         align256(items * rows * wide * sizeof(float));
+}
+
+char *place_parts(ScoredParams &p, char *ws, int64_t items, int64_t rows) {
+  const int64_t wide = p.d > 64 ? 128 : 64;
+  p.first = reinterpret_cast<int *>(ws);
+  ws += align256((p.units + 1) * sizeof(int));
+  p.ml = reinterpret_cast<float *>(ws);
+  ws += align256(items * rows * 2 * sizeof(float));
+  p.acc = reinterpret_cast<float *>(ws);
+  return ws + align256(items * rows * wide * sizeof(float));
+}
+
+int64_t decode_units(int64_t batch, int64_t group) { return batch * ceil_div(group, kRows); }
+int64_t prefill_units(int64_t seqs, int64_t max_q, int64_t group) {
+  return seqs * ceil_div(max_q * group, kRows);
+}
+int64_t prefix_units(int64_t batch, int64_t group) { return ceil_div(batch * group, kRows); }
+
+bool head_dim_ok(int64_t d, int dtype) {
+  return d > 0 && d <= 128 && d % (dtype == MLR_DTYPE_F32 ? 4 : 8) == 0;
+}
+
+struct Operands {
+  const char *what;
+  const void *q;
+  int64_t q_st, q_sh;
+  const void *k, *v;
+  int64_t num_blocks, block_size, hkv, d;
+  const int64_t *bt;
+  int64_t bt_st, bt_width;
+  const int64_t *ctx;
+  int64_t seqs, hq;
+  double scale, cap;
+  const float *slopes;
+  int dtype;
+  const void *out;
+  int64_t o_st, o_sh;
+};
+
+int check_operands(const Operands &o) {
+  const char *w = o.what;
+  MLR_REQUIRE(o.dtype == MLR_DTYPE_F32 || o.dtype == MLR_DTYPE_F16 || o.dtype == MLR_DTYPE_BF16,
+              "%s: unsupported dtype %d", w, o.dtype);
+  MLR_REQUIRE(o.seqs >= 0 && o.seqs < (1 << 24), "%s: number of sequences must be in [0, 2^24)", w);
+  MLR_REQUIRE(o.hkv > 0 && o.hq > 0 && o.hq % o.hkv == 0 && o.hq < (1 << 16),
+              "%s: query heads must be a positive multiple of the KV heads, below 2^16", w);
+  MLR_REQUIRE(head_dim_ok(o.d, o.dtype),
+              "%s: head_dim must be a multiple of %d up to 128, got %lld", w,
+              o.dtype == MLR_DTYPE_F32 ? 4 : 8, static_cast<long long>(o.d));
+  MLR_REQUIRE(o.num_blocks > 0 && o.block_size > 0 && o.bt_width >= 0,
+              "%s: the cache needs blocks of a positive size", w);
+  MLR_REQUIRE(o.bt_width < (int64_t(1) << 31) / o.block_size,
+              "%s: a block table must cover fewer than 2^31 positions", w);
+  // A cap so small that its inverse is infinite would make NaN of scores of 0.
+  MLR_REQUIRE(o.cap == 0 || (o.cap >= 1e-30 && o.cap <= 1e30),
+              "%s: softcap must be 0 (off) or in [1e-30, 1e30]", w);
+  MLR_REQUIRE(o.scale == o.scale && o.scale - o.scale == 0, "%s: scale must be finite", w);
+  const int64_t vec = 16 / dtype_size(o.dtype);
+  MLR_REQUIRE(o.q_st % vec == 0 && o.q_sh % vec == 0 && reinterpret_cast<uintptr_t>(o.q) % 16 == 0,
+              "%s: q rows must start at multiples of 16 bytes", w);
+  MLR_REQUIRE((reinterpret_cast<uintptr_t>(o.k) | reinterpret_cast<uintptr_t>(o.v)) % 16 == 0,
+              "%s: the cache must be 16-byte aligned", w);
+  return MLR_OK;
+}
+
+ScoredParams params_of(const Operands &o, int mode) {
+  ScoredParams p{};
+  p.q = o.q;
+  p.k = o.k;
+  p.v = o.v;
+  p.q_st = o.q_st;
+  p.q_sh = o.q_sh;
+  p.num_blocks = o.num_blocks;
+  p.block_size = o.block_size;
+  p.hkv = static_cast<int>(o.hkv);
+  p.hq = static_cast<int>(o.hq);
+  p.group = static_cast<int>(o.hq / o.hkv);
+  p.d = static_cast<int>(o.d);
+  p.bt = o.bt;
+  p.bt_st = o.bt_st;
+  p.bt_width = o.bt_width;
+  p.ctx = o.ctx;
+  p.seqs = static_cast<int>(o.seqs);
+  p.total_q = o.seqs;
+  p.scale = static_cast<float>(o.scale);
+  p.cap = static_cast<float>(o.cap);
+  p.slopes = o.slopes;
+  p.out = const_cast<void *>(o.out);
+  p.o_st = o.o_st;
+  p.o_sh = o.o_sh;
+  p.mode = mode;
+  p.target = target_items();
+  return p;
+}
+
+unsigned grid_of(int64_t items) { return static_cast<unsigned>(std::min<int64_t>(items, 1024)); }
+
+}  // namespace
+}  // namespace mlr
+
+using namespace mlr;
+
+extern "C" size_t mlr_paged_decode_scored_workspace_size(int64_t batch, int64_t num_q_heads,
+                                                         int64_t num_kv_heads, int64_t head_dim,
+                                                         int64_t max_context) {
+  if (batch <= 0 || num_kv_heads <= 0 || num_q_heads <= 0 || max_context <= kMinSplit) return 0;
+  const int64_t units = decode_units(batch, num_q_heads / num_kv_heads);
+  return part_bytes(units, max_items(units, num_kv_heads, max_context), kRows, head_dim);
+}
+
+extern "C" int mlr_paged_decode_scored(
+    const void *q, int64_t q_stride_b, int64_t q_stride_h, const void *k_cache,
+    const void *v_cache, int64_t num_blocks, int64_t block_size, int64_t num_kv_heads,
+    int64_t head_dim, const int64_t *block_tables, int64_t bt_stride, int64_t max_blocks,
+    const int64_t *seq_lens, int64_t batch, int64_t num_q_heads, double scale, double softcap,
+    const float *alibi_slopes, int dtype, void *workspace, size_t workspace_bytes, void *out,
+    int64_t out_stride_b, int64_t out_stride_h, void *stream) {
+  clear_error();
+  const Operands o{"mlr_paged_decode_scored", q, q_stride_b, q_stride_h, k_cache, v_cache,
+                   num_blocks, block_size, num_kv_heads, head_dim, block_tables, bt_stride,
+                   max_blocks, seq_lens, batch, num_q_heads, scale, softcap, alibi_slopes, dtype,
+                   out, out_stride_b, out_stride_h};
+  if (const int rc = check_operands(o)) return rc;
+  if (batch == 0) return MLR_OK;
+  MLR_REQUIRE(q && k_cache && v_cache && (block_tables || max_blocks == 0) && seq_lens && out,
+              "mlr_paged_decode_scored: null pointer");
+  const int64_t max_keys = max_blocks * block_size;
+  const size_t need = mlr_paged_decode_scored_workspace_size(batch, num_q_heads, num_kv_heads,
+                                                             head_dim, max_keys);
+  MLR_REQUIRE(need == 0 || (workspace && workspace_bytes >= need),
+              "mlr_paged_decode_scored: workspace of %zu bytes, %zu needed", workspace_bytes, need);
+  ScoredParams p = params_of(o, kModeDecode);
+  p.tiles = static_cast<int>(ceil_div(p.group, kRows));
+  p.units = static_cast<int>(decode_units(batch, p.group));
+  const int64_t items = max_items(p.units, p.hkv, max_keys);
+  if (need) place_parts(p, static_cast<char *>(workspace), items, kRows);
+  hipStream_t s = static_cast<hipStream_t>(stream);
+  if (const int rc = launch_scored_rows(p, dtype, grid_of(items), s)) return rc;
+  return need ? launch_merge(p, p, false, kRows, dtype, s) : MLR_OK;
+}
+
+extern "C" size_t mlr_paged_prefill_scored_workspace_size(int64_t num_seqs, int64_t max_query_len,
+                                                          int64_t max_context, int64_t num_q_heads,
+                                                          int64_t num_kv_heads, int64_t head_dim,
+                                                          int dtype) {
+  (void)dtype;
+  if (num_seqs <= 0 || max_query_len <= 0 || num_kv_heads <= 0 || num_q_heads <= 0 ||
+      max_context <= kMinSplit)
+    return 0;
+  const int64_t units = prefill_units(num_seqs, max_query_len, num_q_heads / num_kv_heads);
+  return part_bytes(units, max_items(units, num_kv_heads, max_context), kRows, head_dim);
+}
+
+extern "C" int mlr_paged_prefill_scored(
+    const void *q, int64_t q_stride_t, int64_t q_stride_h, const void *k_cache,
+    const void *v_cache, int64_t num_blocks, int64_t block_size, int64_t num_kv_heads,
+    int64_t head_dim, const int64_t *block_tables, int64_t bt_stride, int64_t max_blocks,
+    const int64_t *query_start_loc, const int64_t *context_lens, const int64_t *prefix_lens,
+    int64_t num_seqs, int64_t total_q, int64_t max_query_len, int64_t num_q_heads, double scale,
+    double softcap, const float *alibi_slopes, int dtype, void *workspace, size_t workspace_bytes,
+    void *out, int64_t out_stride_t, int64_t out_stride_h, void *stream) {
+  clear_error();
+  const Operands o{"mlr_paged_prefill_scored", q, q_stride_t, q_stride_h, k_cache, v_cache,
+                   num_blocks, block_size, num_kv_heads, head_dim, block_tables, bt_stride,
+                   max_blocks, context_lens, num_seqs, num_q_heads, scale, softcap, alibi_slopes,
+                   dtype, out, out_stride_t, out_stride_h};
+  if (const int rc = check_operands(o)) return rc;
+  MLR_REQUIRE(total_q >= 0 && max_query_len >= 0,
+              "mlr_paged_prefill_scored: token counts must be >= 0");
+  if (num_seqs == 0 || total_q == 0 || max_query_len == 0) return MLR_OK;
+  MLR_REQUIRE(q && k_cache && v_cache && (block_tables || max_blocks == 0) && query_start_loc &&
+                  context_lens && out,
+              "mlr_paged_prefill_scored: null pointer");
+  max_query_len = std::min(max_query_len, total_q);
+  const int64_t group = num_q_heads / num_kv_heads;
+  MLR_REQUIRE(max_query_len < (int64_t(1) << 31) / group &&
+                  prefill_units(num_seqs, max_query_len, group) * num_kv_heads < (int64_t(1) << 30),
+              "mlr_paged_prefill_scored: too many query rows");
+  const int64_t max_keys = max_blocks * block_size;
+  const size_t need = mlr_paged_prefill_scored_workspace_size(
+      num_seqs, max_query_len, max_keys, num_q_heads, num_kv_heads, head_dim, dtype);
+  MLR_REQUIRE(need == 0 || (workspace && workspace_bytes >= need),
+              "mlr_paged_prefill_scored: workspace of %zu bytes, %zu needed", workspace_bytes,
+              need);
+  ScoredParams p = params_of(o, kModePrefill);
+  p.qsl = query_start_loc;
+  p.ahead = prefix_lens;
+  p.total_q = total_q;
+  p.tiles = static_cast<int>(ceil_div(max_query_len * group, kRows));
+  p.units = static_cast<int>(prefill_units(num_seqs, max_query_len, group));
+  const int64_t items = max_items(p.units, p.hkv, max_keys);
+  if (need) place_parts(p, static_cast<char *>(workspace), items, kRows);
+  hipStream_t s = static_cast<hipStream_t>(stream);
+  if (const int rc = launch_scored_rows(p, dtype, grid_of(items), s)) return rc;
+  return need ? launch_merge(p, p, false, kRows, dtype, s) : MLR_OK;
+}
+
+extern "C" size_t mlr_paged_decode_shared_prefix_workspace_size(
+    int64_t batch, int64_t num_q_heads, int64_t num_kv_heads, int64_t head_dim, int64_t prefix_len,
+    int64_t max_context, int dtype) {
+  (void)dtype;
+  if (batch <= 0 || num_kv_heads <= 0 || num_q_heads <= 0) return 0;
+  const int64_t group = num_q_heads / num_kv_heads;
+  const int64_t own = decode_units(batch, group), over = prefix_units(batch, group);
+  return part_bytes(own, max_items(own, num_kv_heads, max_context), kRows, head_dim) +
+         part_bytes(over, max_items(over, num_kv_heads, prefix_len), kRows, head_dim);
+}
+
+extern "C" int mlr_paged_decode_shared_prefix(
+    const void *q, int64_t q_stride_b, int64_t q_stride_h, const void *k_cache,
+    const void *v_cache, int64_t num_blocks, int64_t block_size, int64_t num_kv_heads,
+    int64_t head_dim, const int64_t *prefix_table, int64_t prefix_blocks, int64_t prefix_len,
+    const int64_t *block_tables, int64_t bt_stride, int64_t max_blocks, const int64_t *seq_lens,
+    int64_t batch, int64_t num_q_heads, double scale, double softcap, const float *alibi_slopes,
+    int dtype, void *workspace, size_t workspace_bytes, void *out, int64_t out_stride_b,
+    int64_t out_stride_h, void *stream) {
+  clear_error();
+  const Operands o{"mlr_paged_decode_shared_prefix", q, q_stride_b, q_stride_h, k_cache, v_cache,
+                   num_blocks, block_size, num_kv_heads, head_dim, block_tables, bt_stride,
+                   max_blocks, seq_lens, batch, num_q_heads, scale, softcap, alibi_slopes, dtype,
+                   out, out_stride_b, out_stride_h};
+  if (const int rc = check_operands(o)) return rc;
+  MLR_REQUIRE(prefix_len >= 0 && prefix_blocks >= 0 &&
+                  prefix_blocks < (int64_t(1) << 31) / block_size &&
+                  prefix_len <= prefix_blocks * block_size,
+              "mlr_paged_decode_shared_prefix: the prefix table does not cover the prefix");
+  if (batch == 0) return MLR_OK;
+  MLR_REQUIRE(q && k_cache && v_cache && (prefix_table || prefix_len == 0) &&
+                  (block_tables || max_blocks == 0) && seq_lens && out,
+              "mlr_paged_decode_shared_prefix: null pointer");
+  const int64_t max_keys = max_blocks * block_size;
+  const size_t need = mlr_paged_decode_shared_prefix_workspace_size(
+      batch, num_q_heads, num_kv_heads, head_dim, prefix_len, max_keys, dtype);
+  MLR_REQUIRE(workspace && workspace_bytes >= need,
+              "mlr_paged_decode_shared_prefix: workspace of %zu bytes, %zu needed",
+              workspace_bytes, need);
+  ScoredParams own = params_of(o, kModeDecode);
+  own.tiles = static_cast<int>(ceil_div(own.group, kRows));
+  own.units = static_cast<int>(decode_units(batch, own.group));
+  own.start = prefix_len;
+  own.force_partial = true;
+  const int64_t own_items = max_items(own.units, own.hkv, max_keys);
+  char *ws = place_parts(own, static_cast<char *>(workspace), own_items, kRows);
+  ScoredParams over = params_of(o, kModePrefix);
+  over.bt = prefix_table;
+  over.bt_st = 0;
+  over.bt_width = prefix_blocks;
+  over.units = over.tiles = static_cast<int>(prefix_units(batch, over.group));
+  over.start = prefix_len;
+  over.force_partial = true;
+  const int64_t over_items = max_items(over.units, over.hkv, prefix_len);
+  place_parts(over, ws, over_items, kRows);
+  hipStream_t s = static_cast<hipStream_t>(stream);
+  if (const int rc = launch_scored_rows(over, dtype, grid_of(over_items), s)) return rc;
+  if (const int rc = launch_scored_rows(own, dtype, grid_of(own_items), s)) return rc;
+  return launch_merge(own, over, true, kRows, dtype, s);
+}
