@@ -665,8 +665,9 @@ int mlr_paged_decode_scored(const void *q, int64_t q_stride_b, int64_t q_stride_
                             void *workspace, size_t workspace_bytes, void *out,
                             int64_t out_stride_b, int64_t out_stride_h, void *stream);
 size_t mlr_paged_prefill_scored_workspace_size(int64_t num_seqs, int64_t max_query_len,
-                                               int64_t max_context, int64_t num_q_heads,
-                                               int64_t num_kv_heads, int64_t head_dim, int dtype);
+                                               int64_t max_blocks, int64_t block_size,
+                                               int64_t num_q_heads, int64_t num_kv_heads,
+                                               int64_t head_dim, int dtype);
 int mlr_paged_prefill_scored(const void *q, int64_t q_stride_t, int64_t q_stride_h,
                              const void *k_cache, const void *v_cache, int64_t num_blocks,
                              int64_t block_size, int64_t num_kv_heads, int64_t head_dim,
@@ -679,8 +680,8 @@ int mlr_paged_prefill_scored(const void *q, int64_t q_stride_t, int64_t q_stride
                              int64_t out_stride_t, int64_t out_stride_h, void *stream);
 size_t mlr_paged_decode_shared_prefix_workspace_size(int64_t batch, int64_t num_q_heads,
                                                      int64_t num_kv_heads, int64_t head_dim,
-                                                     int64_t prefix_len, int64_t max_context,
-                                                     int dtype);
+                                                     int64_t prefix_len, int64_t max_blocks,
+                                                     int64_t block_size, int dtype);
 int mlr_paged_decode_shared_prefix(const void *q, int64_t q_stride_b, int64_t q_stride_h,
                                    const void *k_cache, const void *v_cache, int64_t num_blocks,
                                    int64_t block_size, int64_t num_kv_heads, int64_t head_dim,

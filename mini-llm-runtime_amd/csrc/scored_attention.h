@@ -39,6 +39,8 @@ struct ScoredParams {
   int mode, units;
   bool force_partial;      // results go to the workspace even of a single split
   int64_t target;          // items the call is cut into, about
+  bool whole;              // no splits: an item is a unit
+  int bs_log2, ncu;        // kernels that need them: log2 of block_size, CUs of the GPU
   int *first;              // [units + 1]: items before each unit (of one KV head)
   float *ml, *acc;         // [items][kRows][2], [items][kRows][D] of partial results
 };
@@ -71,12 +73,16 @@ __device__ __forceinline__ Unit unit_of(const ScoredParams &p, int u, int kRows)
     t.ctx = clamp64(p.ctx[t.seq], 0, covered);
     t.pos0 = t.ctx - (end - t.q0);
     t.ahead = p.ahead ? clamp64(p.ahead[t.seq], 0, t.ctx) : 0;
-    const int64_t rows = (end - t.q0) * p.group;
-    t.rows = static_cast<int>(rows);
-    const int64_t last = (rows < t.r0 + kRows ? rows : t.r0 + kRows) - 1;
-    t.hi = t.r0 < rows ? t.pos0 + last / p.group + 1 : 0;
-    if (t.hi < t.ahead && t.r0 < rows) t.hi = t.ahead;
-    if (t.hi < 0) t.hi = 0;
+    // Rows past the declared longest chunk have no unit.
+    const int64_t rows = (end - t.q0) * p.group, most = static_cast<int64_t>(p.tiles) * kRows;
+    t.rows = static_cast<int>(rows < most ? rows : most);
+    t.hi = 0;
+    if (t.r0 < t.rows) {
+      const int last = (t.rows < t.r0 + kRows ? t.rows : t.r0 + kRows) - 1;
+      t.hi = t.pos0 + last / p.group + 1;
+      if (t.hi < t.ahead) t.hi = t.ahead;
+      if (t.hi < 0) t.hi = 0;
+    }
   } else if (p.mode == kModeDecode) {
     t.q0 = t.seq;
     t.ctx = clamp64(p.ctx[t.seq], 0, covered);
@@ -109,5 +115,9 @@ __device__ __forceinline__ int64_t split_of(int64_t total_keys, const ScoredPara
 }
 
 int launch_scored_rows(const ScoredParams &p, int dtype, unsigned grid, hipStream_t stream);
+
+// Units of 128 rows; bf16 and fp16, block_size a power of two from 16 on.
+constexpr int kTileRows = 128;
+int launch_scored_tiles(const ScoredParams &p, int dtype, unsigned grid, hipStream_t stream);
 
 }  // namespace mlr

@@ -11,23 +11,24 @@ constexpr float kLog2e = 1.4426950408889634f;
 constexpr int kRows = 16;
 
 // out = sum_i 2^{m_i - M} O_i / sum_i 2^{m_i - M} l_i over a row's items, those
-// of `p` and, for a shared prefix, of `x` too. One workgroup per (unit of p, KV
-// head), 16 threads per row; items are added in their order. A unit that has
-// written its result itself is left alone.
+// of `p` and, for a shared prefix, of `x` too. One workgroup per 16 rows of a
+// (unit of p, KV head), 16 threads per row; items are added in their order. A
+// unit that has written its result itself is left alone.
 template <typename T, int D>
-__global__ __launch_bounds__(256) void scored_merge(ScoredParams p, ScoredParams x, bool prefixed,
-                                                    int x_rows) {
+__global__ __launch_bounds__(256) void scored_merge(ScoredParams p, int p_rows, ScoredParams x,
+                                                    int x_rows, bool prefixed) {
   constexpr int kVe = D / 16;
-  const int u = blockIdx.x / p.hkv, kvh = blockIdx.x - u * p.hkv;
+  const int slices = p_rows / kRows, slice = blockIdx.x % slices, uk = blockIdx.x / slices;
+  const int u = uk / p.hkv, kvh = uk - u * p.hkv;
   const int first = p.first[u], count = p.first[u + 1] - first;
   if (count == 0 || (count == 1 && !p.force_partial)) return;
-  const Unit t = unit_of(p, u, kRows);
-  const int rr = threadIdx.x >> 4, d0 = (threadIdx.x & 15) * kVe;
+  const Unit t = unit_of(p, u, p_rows);
+  const int rr = slice * kRows + (threadIdx.x >> 4), d0 = (threadIdx.x & 15) * kVe;
   const int r = t.r0 + rr;
   if (r >= t.rows) return;
   const int tok = r / p.group, g = r - tok * p.group;
   // Items of the row: `count` from p, then `more` from x.
-  int64_t at = (static_cast<int64_t>(first) * p.hkv + kvh) * kRows + rr, x_at = 0;
+  int64_t at = (static_cast<int64_t>(first) * p.hkv + kvh) * p_rows + rr, x_at = 0;
   int more = 0;
   if (prefixed) {
     const int xr = t.seq * p.group + g;
@@ -36,7 +37,7 @@ __global__ __launch_bounds__(256) void scored_merge(ScoredParams p, ScoredParams
     more = x.first[xu + 1] - x_first;
     x_at = (static_cast<int64_t>(x_first) * x.hkv + kvh) * x_rows + (xr - xu * x_rows);
   }
-  const int64_t step = static_cast<int64_t>(p.hkv) * kRows;
+  const int64_t step = static_cast<int64_t>(p.hkv) * p_rows;
   const int64_t x_step = static_cast<int64_t>(p.hkv) * x_rows;
   float m = -INFINITY;
   for (int i = threadIdx.x & 15; i < count; i += 16) m = fmaxf(m, p.ml[2 * (at + i * step)]);
@@ -70,12 +71,12 @@ __global__ __launch_bounds__(256) void scored_merge(ScoredParams p, ScoredParams
     if (d0 + n < p.d) dst[d0 + n] = Elem<T>::from_f32(acc[n] * inv);
 }
 
-int launch_merge(const ScoredParams &p, const ScoredParams &x, bool prefixed, int x_rows, int dtype,
-                 hipStream_t stream) {
-  const unsigned grid = static_cast<unsigned>(p.units) * p.hkv;
-#define MLR_MERGE(T)                                                                       \
-  if (p.d > 64) scored_merge<T, 128><<<grid, 256, 0, stream>>>(p, x, prefixed, x_rows);    \
-  else scored_merge<T, 64><<<grid, 256, 0, stream>>>(p, x, prefixed, x_rows)
+int launch_merge(const ScoredParams &p, int p_rows, const ScoredParams &x, int x_rows,
+                 bool prefixed, int dtype, hipStream_t stream) {
+  const unsigned grid = static_cast<unsigned>(p.units) * p.hkv * (p_rows / kRows);
+#define MLR_MERGE(T)                                                                            \
+  if (p.d > 64) scored_merge<T, 128><<<grid, 256, 0, stream>>>(p, p_rows, x, x_rows, prefixed); \
+  else scored_merge<T, 64><<<grid, 256, 0, stream>>>(p, p_rows, x, x_rows, prefixed)
   if (dtype == MLR_DTYPE_F32) {
     MLR_MERGE(float);
   } else if (dtype == MLR_DTYPE_F16) {
@@ -87,15 +88,16 @@ int launch_merge(const ScoredParams &p, const ScoredParams &x, bool prefixed, in
   return check_launch("scored_merge");
 }
 
-int64_t target_items() {
-  const int cus = current_device_cus();
-  return 2 * static_cast<int64_t>(cus > 0 ? cus : 256);
+int cus() {
+  const int n = current_device_cus();
+  return n > 0 ? n : 256;
 }
+int64_t target_items() { return 2 * static_cast<int64_t>(cus()); }
 
-// Items of a call at most, over its KV heads.
-int64_t max_items(int64_t units, int64_t hkv, int64_t max_keys) {
+// Items of a call at most, over its KV heads, cut into about `target`.
+int64_t max_items(int64_t units, int64_t hkv, int64_t max_keys, int64_t target) {
   const int64_t by_len = units * std::max<int64_t>(1, ceil_div(max_keys + 15, kMinSplit));
-  return std::min(by_len, units + ceil_div(target_items(), hkv) + 1) * hkv;
+  return std::min(by_len, units + ceil_div(target, hkv) + 1) * hkv;
 }
 
 size_t align256(size_t n) { return (n + 255) & ~size_t(255); }
@@ -118,10 +120,39 @@ char *place_parts(ScoredParams &p, char *ws, int64_t items, int64_t rows) {
 }
 
 int64_t decode_units(int64_t batch, int64_t group) { return batch * ceil_div(group, kRows); }
-int64_t prefill_units(int64_t seqs, int64_t max_q, int64_t group) {
-  return seqs * ceil_div(max_q * group, kRows);
+int64_t prefill_units(int64_t seqs, int64_t max_q, int64_t group, int64_t rows) {
+  return seqs * ceil_div(max_q * group, rows);
 }
-int64_t prefix_units(int64_t batch, int64_t group) { return ceil_div(batch * group, kRows); }
+int64_t prefix_units(int64_t batch, int64_t group, int64_t rows) {
+  return ceil_div(batch * group, rows);
+}
+
+// Whether a call with `rows` query rows per sequence and KV head goes to the
+// kernel of 128 rows a unit: more than two of the other kernel's units.
+bool takes_tiles(int64_t rows, int64_t block_size, int dtype) {
+  return dtype != MLR_DTYPE_F32 && rows > 2 * kRows && block_size >= 16 &&
+         log2_if_pow2(block_size) >= 4;
+}
+
+// A prefill's rows per unit, units, items, and whether units stay whole: with a
+// unit for every CU there is nothing to gain from splits, which cost a pass over
+// FP32 partial results.
+struct PrefillPlan {
+  int64_t rows, units, items;
+  bool whole, parts;
+};
+PrefillPlan plan_prefill(int64_t seqs, int64_t max_q, int64_t max_keys, int64_t block_size,
+                         int64_t hq, int64_t hkv, int dtype) {
+  const int64_t group = hq / hkv;
+  PrefillPlan n;
+  const bool tiles = takes_tiles(max_q * group, block_size, dtype);
+  n.rows = tiles ? kTileRows : kRows;
+  n.units = prefill_units(seqs, max_q, group, n.rows);
+  n.whole = tiles && (n.units * hkv >= cus() || max_keys <= kMinSplit);
+  n.items = n.whole ? n.units * hkv : max_items(n.units, hkv, max_keys, target_items());
+  n.parts = !n.whole && max_keys > kMinSplit;
+  return n;
+}
 
 bool head_dim_ok(int64_t d, int dtype) {
   return d > 0 && d <= 128 && d % (dtype == MLR_DTYPE_F32 ? 4 : 8) == 0;
@@ -197,6 +228,8 @@ ScoredParams params_of(const Operands &o, int mode) {
   p.o_sh = o.o_sh;
   p.mode = mode;
   p.target = target_items();
+  p.ncu = cus();
+  p.bs_log2 = std::max(0, log2_if_pow2(o.block_size));
   return p;
 }
 
@@ -212,7 +245,8 @@ extern "C" size_t mlr_paged_decode_scored_workspace_size(int64_t batch, int64_t 
                                                          int64_t max_context) {
   if (batch <= 0 || num_kv_heads <= 0 || num_q_heads <= 0 || max_context <= kMinSplit) return 0;
   const int64_t units = decode_units(batch, num_q_heads / num_kv_heads);
-  return part_bytes(units, max_items(units, num_kv_heads, max_context), kRows, head_dim);
+  return part_bytes(units, max_items(units, num_kv_heads, max_context, target_items()), kRows,
+                    head_dim);
 }
 
 extern "C" int mlr_paged_decode_scored(
@@ -239,23 +273,22 @@ extern "C" int mlr_paged_decode_scored(
   ScoredParams p = params_of(o, kModeDecode);
   p.tiles = static_cast<int>(ceil_div(p.group, kRows));
   p.units = static_cast<int>(decode_units(batch, p.group));
-  const int64_t items = max_items(p.units, p.hkv, max_keys);
+  const int64_t items = max_items(p.units, p.hkv, max_keys, p.target);
   if (need) place_parts(p, static_cast<char *>(workspace), items, kRows);
   hipStream_t s = static_cast<hipStream_t>(stream);
   if (const int rc = launch_scored_rows(p, dtype, grid_of(items), s)) return rc;
-  return need ? launch_merge(p, p, false, kRows, dtype, s) : MLR_OK;
+  return need ? launch_merge(p, kRows, p, kRows, false, dtype, s) : MLR_OK;
 }
 
 extern "C" size_t mlr_paged_prefill_scored_workspace_size(int64_t num_seqs, int64_t max_query_len,
-                                                          int64_t max_context, int64_t num_q_heads,
+                                                          int64_t max_blocks, int64_t block_size,
+                                                          int64_t num_q_heads,
                                                           int64_t num_kv_heads, int64_t head_dim,
                                                           int dtype) {
-  (void)dtype;
-  if (num_seqs <= 0 || max_query_len <= 0 || num_kv_heads <= 0 || num_q_heads <= 0 ||
-      max_context <= kMinSplit)
-    return 0;
-  const int64_t units = prefill_units(num_seqs, max_query_len, num_q_heads / num_kv_heads);
-  return part_bytes(units, max_items(units, num_kv_heads, max_context), kRows, head_dim);
+  if (num_seqs <= 0 || max_query_len <= 0 || num_kv_heads <= 0 || num_q_heads <= 0) return 0;
+  const PrefillPlan n = plan_prefill(num_seqs, max_query_len, max_blocks * block_size, block_size,
+                                     num_q_heads, num_kv_heads, dtype);
+  return n.parts ? part_bytes(n.units, n.items, n.rows, head_dim) : 0;
 }
 
 extern "C" int mlr_paged_prefill_scored(
@@ -281,11 +314,14 @@ extern "C" int mlr_paged_prefill_scored(
   max_query_len = std::min(max_query_len, total_q);
   const int64_t group = num_q_heads / num_kv_heads;
   MLR_REQUIRE(max_query_len < (int64_t(1) << 31) / group &&
-                  prefill_units(num_seqs, max_query_len, group) * num_kv_heads < (int64_t(1) << 30),
+                  prefill_units(num_seqs, max_query_len, group, kRows) * num_kv_heads <
+                      (int64_t(1) << 28),
               "mlr_paged_prefill_scored: too many query rows");
   const int64_t max_keys = max_blocks * block_size;
+  const PrefillPlan n = plan_prefill(num_seqs, max_query_len, max_keys, block_size, num_q_heads,
+                                     num_kv_heads, dtype);
   const size_t need = mlr_paged_prefill_scored_workspace_size(
-      num_seqs, max_query_len, max_keys, num_q_heads, num_kv_heads, head_dim, dtype);
+      num_seqs, max_query_len, max_blocks, block_size, num_q_heads, num_kv_heads, head_dim, dtype);
   MLR_REQUIRE(need == 0 || (workspace && workspace_bytes >= need),
               "mlr_paged_prefill_scored: workspace of %zu bytes, %zu needed", workspace_bytes,
               need);
@@ -293,24 +329,29 @@ extern "C" int mlr_paged_prefill_scored(
   p.qsl = query_start_loc;
   p.ahead = prefix_lens;
   p.total_q = total_q;
-  p.tiles = static_cast<int>(ceil_div(max_query_len * group, kRows));
-  p.units = static_cast<int>(prefill_units(num_seqs, max_query_len, group));
-  const int64_t items = max_items(p.units, p.hkv, max_keys);
-  if (need) place_parts(p, static_cast<char *>(workspace), items, kRows);
+  p.units = static_cast<int>(n.units);
+  p.tiles = static_cast<int>(n.units / num_seqs);
+  p.whole = n.whole;
+  const int rows = static_cast<int>(n.rows);
+  if (n.parts) place_parts(p, static_cast<char *>(workspace), n.items, rows);
   hipStream_t s = static_cast<hipStream_t>(stream);
-  if (const int rc = launch_scored_rows(p, dtype, grid_of(items), s)) return rc;
-  return need ? launch_merge(p, p, false, kRows, dtype, s) : MLR_OK;
+  const int rc = rows == kTileRows
+                     ? launch_scored_tiles(p, dtype, static_cast<unsigned>(n.items), s)
+                     : launch_scored_rows(p, dtype, grid_of(n.items), s);
+  if (rc) return rc;
+  return n.parts ? launch_merge(p, rows, p, rows, false, dtype, s) : MLR_OK;
 }
 
 extern "C" size_t mlr_paged_decode_shared_prefix_workspace_size(
     int64_t batch, int64_t num_q_heads, int64_t num_kv_heads, int64_t head_dim, int64_t prefix_len,
-    int64_t max_context, int dtype) {
-  (void)dtype;
+    int64_t max_blocks, int64_t block_size, int dtype) {
   if (batch <= 0 || num_kv_heads <= 0 || num_q_heads <= 0) return 0;
-  const int64_t group = num_q_heads / num_kv_heads;
-  const int64_t own = decode_units(batch, group), over = prefix_units(batch, group);
-  return part_bytes(own, max_items(own, num_kv_heads, max_context), kRows, head_dim) +
-         part_bytes(over, max_items(over, num_kv_heads, prefix_len), kRows, head_dim);
+  const int64_t group = num_q_heads / num_kv_heads, target = target_items();
+  const int64_t rows = takes_tiles(batch * group, block_size, dtype) ? kTileRows : kRows;
+  const int64_t own = decode_units(batch, group), over = prefix_units(batch, group, rows);
+  return part_bytes(own, max_items(own, num_kv_heads, max_blocks * block_size, target), kRows,
+                    head_dim) +
+         part_bytes(over, max_items(over, num_kv_heads, prefix_len, target), rows, head_dim);
 }
 
 extern "C" int mlr_paged_decode_shared_prefix(
@@ -337,7 +378,7 @@ extern "C" int mlr_paged_decode_shared_prefix(
               "mlr_paged_decode_shared_prefix: null pointer");
   const int64_t max_keys = max_blocks * block_size;
   const size_t need = mlr_paged_decode_shared_prefix_workspace_size(
-      batch, num_q_heads, num_kv_heads, head_dim, prefix_len, max_keys, dtype);
+      batch, num_q_heads, num_kv_heads, head_dim, prefix_len, max_blocks, block_size, dtype);
   MLR_REQUIRE(workspace && workspace_bytes >= need,
               "mlr_paged_decode_shared_prefix: workspace of %zu bytes, %zu needed",
               workspace_bytes, need);
@@ -346,19 +387,23 @@ extern "C" int mlr_paged_decode_shared_prefix(
   own.units = static_cast<int>(decode_units(batch, own.group));
   own.start = prefix_len;
   own.force_partial = true;
-  const int64_t own_items = max_items(own.units, own.hkv, max_keys);
+  const int64_t own_items = max_items(own.units, own.hkv, max_keys, own.target);
   char *ws = place_parts(own, static_cast<char *>(workspace), own_items, kRows);
   ScoredParams over = params_of(o, kModePrefix);
+  const bool tiles = takes_tiles(batch * over.group, block_size, dtype);
+  const int rows = tiles ? kTileRows : kRows;
   over.bt = prefix_table;
   over.bt_st = 0;
   over.bt_width = prefix_blocks;
-  over.units = over.tiles = static_cast<int>(prefix_units(batch, over.group));
+  over.units = over.tiles = static_cast<int>(prefix_units(batch, over.group, rows));
   over.start = prefix_len;
   over.force_partial = true;
-  const int64_t over_items = max_items(over.units, over.hkv, prefix_len);
-  place_parts(over, ws, over_items, kRows);
+  const int64_t over_items = max_items(over.units, over.hkv, prefix_len, over.target);
+  place_parts(over, ws, over_items, rows);
   hipStream_t s = static_cast<hipStream_t>(stream);
-  if (const int rc = launch_scored_rows(over, dtype, grid_of(over_items), s)) return rc;
-  if (const int rc = launch_scored_rows(own, dtype, grid_of(own_items), s)) return rc;
-  return launch_merge(own, over, true, kRows, dtype, s);
+  const int rc = tiles ? launch_scored_tiles(over, dtype, static_cast<unsigned>(over_items), s)
+                       : launch_scored_rows(over, dtype, grid_of(over_items), s);
+  if (rc) return rc;
+  if (const int rc2 = launch_scored_rows(own, dtype, grid_of(own_items), s)) return rc2;
+  return launch_merge(own, kRows, over, rows, true, dtype, s);
 }

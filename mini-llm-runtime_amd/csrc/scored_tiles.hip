@@ -1,0 +1,652 @@
+// Paged attention with capped or biased scores, for many query rows per key
+// (bf16, fp16): packed prompt chunks, and a decode batch over the prefix that
+// its requests share. The scores are those of scored_rows.hip.
+//
+// A unit is 128 query rows of one KV head, a row being one (token, head of the
+// group): the heads of a group share every K/V tile that is loaded. Eight
+// waves: four groups of 32 rows, twice, for two halves of the unit's keys
+// (joined through LDS at the end). Keys stream through LDS in tiles of 64,
+// two stages per half, copied there from memory without registers on the way
+// (buffer_load ... lds), one tile ahead of its use, one barrier per tile.
+//
+// Per tile and wave, v_mfma_f32_32x32x16:
+//   S^T[64 keys x 32 rows] = K Q^T: operand A = K rows from LDS, B = Q^T in
+//     registers. Lane l holds row l % 32 and, of each 32 keys, keys
+//     8 (i / 4) + 4 (l / 32) + i % 4, i < 16.
+//   scores in base 2, relative to the row's reference point m, which follows
+//     the running maximum only when a tile exceeds it by 2^kLazy: probabilities
+//     stay below 2^kLazy, numerator and sum share m, and most tiles rescale nothing.
+//   O^T[D x 32 rows] += V^T P^T: B = P^T straight from the S^T registers, rounded
+//     to the 16-bit type (relative 2^-9, 2^-12), A = V^T by transposing LDS reads.
+//
+// What bounds it is the vector work per score beside the matrix work (D = 64:
+// 16 cycles of MFMA per wave and score): 28 cycles plain, of which the
+// exponential takes 16. The cap as exponential and reciprocal would add 40;
+// tanh(y) = y P(y^2) with three terms beyond the first (relative error 5.1e-7
+// for |y| <= 1/2) adds 16, so a tile whose scores all lie within half the cap
+// takes that, and others the exponential form.
+//
+// LDS rows are unpadded; the 16-byte chunk c of row r lies at c ^ swizzle(r),
+// which keeps the row reads of K and the transposing reads of V free of bank
+// conflicts.
+#include "scored_attention.h"
+
+namespace mlr {
+namespace {
+
+typedef __bf16 bf16x8_t __attribute__((ext_vector_type(8)));
+typedef _Float16 f16x8_t __attribute__((ext_vector_type(8)));
+typedef float f32x16_t __attribute__((ext_vector_type(16)));
+typedef short s16x4_t __attribute__((ext_vector_type(4)));
+typedef __attribute__((address_space(3))) void lds_void_t;
+typedef __attribute__((address_space(3))) s16x4_t lds_s16x4_t;
+
+constexpr float kLog2e = 1.4426950408889634f;
+constexpr float kLazy = 8.f;
+constexpr int kTile = 64;    // keys
+constexpr int kHalves = 2;   // of the keys
+constexpr int kThreads = 256 * kHalves;
+constexpr int kRankUnits = 4096;  // most units that are ranked by their keys
+
+template <typename T> struct Wide;
+template <> struct Wide<bf16_t> {
+  using v8 = bf16x8_t;
+  using h = __bf16;
+  __device__ static f32x16_t mfma(v8 a, v8 b, f32x16_t c) {
+    return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0);
+  }
+  // Whether a half of w is an infinity or NaN.
+  __device__ static bool odd(uint32_t w) {
+    return ((w & 0x7f807f80u) + 0x00800080u) & 0x80008000u;
+  }
+};
+template <> struct Wide<f16_t> {
+  using v8 = f16x8_t;
+  using h = _Float16;
+  __device__ static f32x16_t mfma(v8 a, v8 b, f32x16_t c) {
+    return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0);
+  }
+  __device__ static bool odd(uint32_t w) {
+    return ((w & 0x7c007c00u) + 0x04000400u) & 0x80008000u;
+  }
+};
+
+template <typename T>
+__device__ __forceinline__ uint32_t pack2(float a, float b) {
+  typedef float f32x2_v __attribute__((ext_vector_type(2)));
+  typedef typename Wide<T>::h h2 __attribute__((ext_vector_type(2)));
+  return __builtin_bit_cast(uint32_t, __builtin_convertvector(f32x2_v{a, b}, h2));
+}
+
+__device__ __forceinline__ float max3(float a, float b, float c) {
+  return __builtin_elementwise_maximum(__builtin_elementwise_maximum(a, b), c);
+}
+__device__ __forceinline__ float pair_max(float x) {  // lanes l and l ^ 32
+  const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false,
+                                                  false);
+  return __builtin_elementwise_maximum(__uint_as_float(r[0]), __uint_as_float(r[1]));
+}
+__device__ __forceinline__ float pair_sum(float x) {
+  const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false,
+                                                  false);
+  return __uint_as_float(r[0]) + __uint_as_float(r[1]);
+}
+
+template <int D>
+__device__ __forceinline__ int swizzle(int r) {
+  if (D == 64) return (((r >> 1) & 1) << 2) | (((r >> 2) & 1) << 1) | ((r >> 3) & 1);
+  return ((r & 1) << 1) | (((r >> 1) & 3) << 2) | ((r >> 3) & 1);
+}
+
+// Units of a sequence that see more than `keys` keys: those whose last row
+// belongs to token keys - pos0 or a later one.
+__device__ __forceinline__ int units_past(const ScoredParams &p, int seq, int64_t keys) {
+  const Unit t = unit_of(p, seq * p.tiles, kTileRows);
+  if (t.rows == 0) return 0;
+  const int all = (t.rows + kTileRows - 1) / kTileRows;
+  if (t.ahead > keys) return all;
+  const int64_t tok = keys - t.pos0;
+  if (tok <= 0) return all;
+  const int64_t row = tok * p.group;
+  return row >= t.rows ? 0 : all - static_cast<int>(row / kTileRows);
+}
+
+template <typename T, int D, bool kCap, bool kBias>
+__global__ __launch_bounds__(kThreads)
+    __attribute__((amdgpu_waves_per_eu(2)))
+void scored_tiles_kernel(ScoredParams p) {
+  using W = Wide<T>;
+  using v8 = typename W::v8;
+  constexpr int QS = D / 16, NB = D / 32, KB = kTile / 32;
+  constexpr int kRowB = 2 * D, kChunks = D / 8;
+  constexpr int kCopies = 16 * kRowB / 1024;  // 1 KB copies of a wave's 16 rows
+  constexpr int kTileB = kTile * kRowB;
+  // Each stage is an object of its own, so that the compiler does not make reads
+  // of one wait for copies into another.
+  __shared__ __align__(1024) unsigned char ks0[kHalves][kTileB], ks1[kHalves][kTileB];
+  __shared__ __align__(1024) unsigned char vs0[kHalves][kTileB], vs1[kHalves][kTileB];
+  __shared__ int64_t s_keys[kThreads / 64];
+  __shared__ int s_count[kThreads / 64], s_unit, s_part, s_of;
+  const int tid = threadIdx.x, lane = tid & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int w = wave & 3, half = wave >> 2;
+  const int m32 = lane & 31, hh = lane >> 5;
+
+  // Which item this workgroup takes.
+  int64_t split = int64_t(1) << 40;
+  int64_t item;
+  int kvh;
+  if (p.whole) {
+    // Heaviest units first, so that the last to start are short. Where two
+    // workgroups fit a CU (D = 64), b and b + ncu share one: the second ncu go in
+    // reverse, light beside heavy.
+    const int n = gridDim.x;
+    int b = blockIdx.x;
+    if (D == 64 && b >= p.ncu && b < 2 * p.ncu) b = min(n, 2 * p.ncu) - 1 - (b - p.ncu);
+    const int rank = b / p.hkv;
+    kvh = b - rank * p.hkv;
+    if (p.units > kRankUnits) {
+      const int seq = rank / p.tiles;
+      if (tid == 0) s_unit = seq * p.tiles + p.tiles - 1 - (rank - seq * p.tiles);
+    } else {
+      // By keys, then by sequence, then later rows first.
+      if (tid == 0) s_unit = -1;
+      __syncthreads();
+      for (int u = tid; u < p.units; u += kThreads) {
+        const Unit t = unit_of(p, u, kTileRows);
+        if (t.r0 >= t.rows) continue;
+        int r = (t.rows + kTileRows - 1) / kTileRows - 1 - t.r0 / kTileRows;
+        for (int q = 0; q < p.seqs; ++q)
+          if (q != t.seq) r += units_past(p, q, q < t.seq ? t.hi - 1 : t.hi);
+        if (r == rank) s_unit = u;
+      }
+    }
+    if (tid == 0) {
+      s_part = 0;
+      s_of = 1;
+    }
+    item = rank;
+  } else {
+    const int per = (p.units + kThreads - 1) / kThreads;
+    const int u_lo = min(tid * per, p.units), u_hi = min(u_lo + per, p.units);
+    int64_t keys = 0;
+    for (int u = u_lo; u < u_hi; ++u) keys += unit_len(unit_of(p, u, kTileRows));
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) keys += __shfl_xor(keys, o);
+    if (lane == 0) s_keys[wave] = keys;
+    __syncthreads();
+    keys = 0;
+    for (int i = 0; i < kThreads / 64; ++i) keys += s_keys[i];
+    split = split_of(keys, p);
+    int own = 0;
+    for (int u = u_lo; u < u_hi; ++u) own += unit_items(unit_of(p, u, kTileRows), split);
+    int before = own;
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) {
+      const int x = __shfl_up(before, o);
+      if (lane >= o) before += x;
+    }
+    if (lane == 63) s_count[wave] = before;
+    before -= own;
+    if (tid == 0) s_unit = -1;
+    __syncthreads();
+    int items = 0;
+    for (int i = 0; i < kThreads / 64; ++i) {
+      if (i < wave) before += s_count[i];
+      items += s_count[i];
+    }
+    item = blockIdx.x / p.hkv;
+    kvh = blockIdx.x - static_cast<int>(item) * p.hkv;
+    int at = before;
+    for (int u = u_lo; u < u_hi; ++u) {
+      const int n = unit_items(unit_of(p, u, kTileRows), split);
+      if (blockIdx.x == 0) p.first[u] = at;
+      if (item >= at && item < at + n) {
+        s_unit = u;
+        s_part = static_cast<int>(item) - at;
+        s_of = n;
+      }
+      at += n;
+    }
+    if (blockIdx.x == 0 && tid == kThreads - 1) p.first[p.units] = items;
+  }
+  __syncthreads();
+  const int unit = __builtin_amdgcn_readfirstlane(s_unit);
+  if (unit < 0) return;  // uniform: no item left for this workgroup
+  const int part = __builtin_amdgcn_readfirstlane(s_part);
+  const bool alone = s_of == 1 && !p.force_partial;
+  const Unit t = unit_of(p, unit, kTileRows);
+  if (t.r0 >= t.rows) return;
+  const int k_lo = __builtin_amdgcn_readfirstlane(static_cast<int>(p.whole ? 0 : part * split));
+  const int k_hi = __builtin_amdgcn_readfirstlane(
+      static_cast<int>(min(t.hi, static_cast<int64_t>(k_lo) + split)));
+
+  // This half's tiles [t_lo, t_hi) of the item's.
+  const int tiles = (k_hi - k_lo + kTile - 1) / kTile;
+  const int chunk = (tiles + kHalves - 1) / kHalves;
+  const int t_lo = half * chunk, t_hi = min(tiles, t_lo + chunk);
+
+  // The lane's row: token, head, position, first key that it does not see.
+  const int r = t.r0 + 32 * w + m32;
+  const bool live = r < t.rows;
+  const int rc = live ? r : t.rows - 1;
+  const int tok = rc / p.group, head = kvh * p.group + rc - tok * p.group;
+  const int64_t row = t.q0 + tok;
+  int pos, limit;
+  if (p.mode == kModePrefill) {
+    pos = static_cast<int>(t.pos0) + tok;
+    limit = max(pos + 1, static_cast<int>(t.ahead));
+  } else {
+    const int64_t ctx = clamp64(p.ctx[row], 0, 0x7fffffff);
+    pos = static_cast<int>(ctx) - 1;
+    limit = static_cast<int>(min(t.hi, ctx));
+  }
+  if (!live) limit = 0;
+  // Keys that all of the wave's rows see, and that any does.
+  int all = live ? limit : 0x7fffffff, any = limit;
+#pragma unroll
+  for (int o = 32; o > 0; o >>= 1) {
+    all = min(all, __shfl_xor(all, o));
+    any = max(any, __shfl_xor(any, o));
+  }
+  all = __builtin_amdgcn_readfirstlane(all);
+  any = __builtin_amdgcn_readfirstlane(any);
+
+  // Q^T fragments: Q[row][16 s + 8 hh ..]. A negative scale goes into Q's sign,
+  // so that the factor of the scores is positive.
+  const uint32_t flip = p.scale < 0 ? 0x80008000u : 0u;
+  v8 qf[QS];
+  const uint16_t *qr = static_cast<const uint16_t *>(p.q) + row * p.q_st + head * p.q_sh;
+#pragma unroll
+  for (int s = 0; s < QS; ++s) {
+    const int e = 16 * s + 8 * hh;
+    uint4 q = make_uint4(0, 0, 0, 0);
+    if (live && e < p.d) q = *reinterpret_cast<const uint4 *>(qr + e);
+    q.x ^= flip;
+    q.y ^= flip;
+    q.z ^= flip;
+    q.w ^= flip;
+    qf[s] = __builtin_bit_cast(v8, q);
+  }
+  // Score in base 2: c2 s, or with the cap s (b0 + s^2 (b1 + ...)).
+  const float scale = fabsf(p.scale);
+  const float c2 = scale * kLog2e;
+  const float c1 = kCap ? scale / p.cap : 0.f;     // y = c1 s
+  const float top = kCap ? p.cap * kLog2e : 0.f;   // the cap in base 2
+  const float b0 = 0.99999949f * c1 * top;
+  const float b1 = -0.33326618f * c1 * c1 * c1 * top;
+  const float b2 = 0.13193061f * c1 * c1 * c1 * c1 * c1 * top;
+  const float b3 = -0.044465f * c1 * c1 * c1 * c1 * c1 * c1 * c1 * top;
+  const float near = 0.5f / c1;                    // |s| up to which that holds
+  const float slope = kBias ? p.slopes[head] * kLog2e : 0.f;
+
+  // Copies: copy i of a wave's 16 rows moves chunk places [64 i, 64 i + 64);
+  // lane l fills place 64 i + l, row rr, physical chunk pc, with the logical
+  // chunk pc ^ swizzle(rr). Chunks past the head lie outside every resource.
+  const uint32_t row_bytes = static_cast<uint32_t>(p.hkv) * p.d * 2;
+  uint32_t src_off[kCopies];
+#pragma unroll
+  for (int i = 0; i < kCopies; ++i) {
+    const int place = 64 * i + lane, rr = place / kChunks;
+    const int c = (place % kChunks) ^ swizzle<D>(rr);
+    src_off[i] = 8 * c < p.d ? rr * row_bytes + 16 * c : 0x7fffffffu;
+  }
+  typedef __attribute__((address_space(4))) const int64_t const_i64;
+  const const_i64 *table =
+      (const const_i64 *)p.bt + (p.mode == kModePrefix ? 0 : static_cast<int64_t>(t.seq) * p.bt_st);
+  const int bs_log2 = p.bs_log2, bs_mask = (1 << bs_log2) - 1;
+  const uint32_t kv_bytes = static_cast<uint32_t>(kvh) * (2 * p.d);
+  const int64_t block_bytes = static_cast<int64_t>(row_bytes) << bs_log2;
+
+  // The block ids of tile i's four runs of 16 keys, and which are out of range.
+  struct Ids {
+    int64_t id[4];
+  };
+  auto ids_of = [&](int i) __attribute__((always_inline)) -> Ids {
+    Ids x;
+#pragma unroll
+    for (int b = 0; b < 4; ++b)
+      x.id[b] = table[min(k_lo + i * kTile + 16 * b, k_hi - 1) >> bs_log2];
+    return x;
+  };
+  auto bad_of = [&](const Ids &x) __attribute__((always_inline)) -> uint32_t {
+    uint32_t bad = 0;
+#pragma unroll
+    for (int b = 0; b < 4; ++b)
+      if (x.id[b] < 0 || x.id[b] >= p.num_blocks) bad |= 1u << b;
+    return bad;
+  };
+  // Copies the wave's 16 rows of tile i into a stage; rows past k_hi and of
+  // blocks out of range arrive as zeros.
+  auto copy = [&](int i, const Ids &x, unsigned char *kt, unsigned char *vt)
+      __attribute__((always_inline)) {
+    const int key = k_lo + i * kTile + 16 * w;
+    const int64_t id = w == 0 ? x.id[0] : w == 1 ? x.id[1] : w == 2 ? x.id[2] : x.id[3];
+    const bool ok = i < t_hi && key < k_hi && id >= 0 && id < p.num_blocks;
+    const uint32_t nrec =
+        ok ? static_cast<uint32_t>(min(k_hi - key, 16) - 1) * row_bytes + 2 * p.d : 0u;
+    const int64_t at = ok ? id * block_bytes +
+                                static_cast<int64_t>(key & bs_mask) * row_bytes + kv_bytes
+                          : 0;
+    const __amdgpu_buffer_rsrc_t rk = __builtin_amdgcn_make_buffer_rsrc(
+        const_cast<unsigned char *>(static_cast<const unsigned char *>(p.k) + at), 0, nrec,
+        0x00020000);
+    const __amdgpu_buffer_rsrc_t rv = __builtin_amdgcn_make_buffer_rsrc(
+        const_cast<unsigned char *>(static_cast<const unsigned char *>(p.v) + at), 0, nrec,
+        0x00020000);
+    kt += 16 * w * kRowB;
+    vt += 16 * w * kRowB;
+#pragma unroll
+    for (int c = 0; c < kCopies; ++c) {
+      const uint32_t off = src_off[c];
+      __builtin_amdgcn_raw_ptr_buffer_load_lds(rk, (lds_void_t *)(kt + 1024 * c), 16, off, 0, 0, 0);
+    }
+#pragma unroll
+    for (int c = 0; c < kCopies; ++c) {
+      const uint32_t off = src_off[c];
+      __builtin_amdgcn_raw_ptr_buffer_load_lds(rv, (lds_void_t *)(vt + 1024 * c), 16, off, 0, 0, 0);
+    }
+  };
+
+  // Lane-constant LDS offsets, as XORs of the chunk index: K row m32 (+ 32 per
+  // block), chunk 2 st + hh; V^T by two transposing reads per MFMA, where of a
+  // group of 16 lanes lane li reads 8 bytes of row 4 (group / 2) + li / 4 (the
+  // second: 8 rows on) at byte 64 n + 32 (group % 2) + 8 (li % 4).
+  const int koff0 = m32 * kRowB + ((hh ^ swizzle<D>(m32)) << 4);
+  const int grp = lane >> 4, li = lane & 15;
+  const int vrow = 4 * (grp >> 1) + (li >> 2), vbyte = 32 * (grp & 1) + 8 * (li & 3);
+  const int voff0 = vrow * kRowB + ((((vbyte >> 4) ^ swizzle<D>(vrow)) << 4) | (vbyte & 15));
+
+  f32x16_t acc[NB];
+#pragma unroll
+  for (int n = 0; n < NB; ++n) acc[n] = f32x16_t{};
+  float m = 0.f, l = 0.f;
+  float thr = -__FLT_MAX__;  // a tile's maximum above this moves m; m is unset so far
+
+  Ids next;
+  uint32_t bad = 0, bad_next = 0;
+  if (chunk > 0) {  // uniform: without keys the table is not read
+    next = ids_of(t_lo);
+    bad_next = bad_of(next);
+    copy(t_lo, next, ks0[half], vs0[half]);
+    next = ids_of(t_lo + 1);
+  }
+  // Tile i of the half from stage (kt, vt), with tile i + 1 on its way to the other.
+  auto step = [&](int i, const unsigned char *kt, const unsigned char *vt, unsigned char *kn,
+                  unsigned char *vn) __attribute__((always_inline)) {
+    // This wave's copies of tile i have landed; then everyone's have, and all
+    // reads of the other stage are done.
+    asm volatile("" ::: "memory");
+    __builtin_amdgcn_s_waitcnt(0);
+    __builtin_amdgcn_s_barrier();
+    asm volatile("" ::: "memory");
+    bad = bad_next;
+    if (i + 1 < chunk) copy(t_lo + i + 1, next, kn, vn);
+    bad_next = bad_of(next);
+    next = ids_of(t_lo + i + 2);
+    const int key0 = k_lo + (t_lo + i) * kTile;
+    if (t_lo + i >= t_hi || key0 >= any) return;  // uniform per wave
+
+    f32x16_t s[KB];
+#pragma unroll
+    for (int j = 0; j < KB; ++j) {
+      s[j] = f32x16_t{};
+#pragma unroll
+      for (int st = 0; st < QS; ++st) {
+        const v8 a = *reinterpret_cast<const v8 *>(kt + 32 * j * kRowB + (koff0 ^ (st << 5)));
+        s[j] = W::mfma(a, qf[st], s[j]);
+      }
+    }
+    const bool masked = key0 + kTile > all || key0 + kTile > k_hi || bad != 0;
+
+    // Scores relative to m.
+    if constexpr (kCap) {
+      float big = 0.f;
+#pragma unroll
+      for (int j = 0; j < KB; ++j)
+#pragma unroll
+        for (int e = 0; e < 16; e += 2) big = max3(big, fabsf(s[j][e]), fabsf(s[j][e + 1]));
+      if (__any(!(big <= near))) {
+#pragma unroll
+        for (int j = 0; j < KB; ++j)
+#pragma unroll
+          for (int e = 0; e < 16; ++e) {
+            const float x = __builtin_amdgcn_exp2f(s[j][e] * (2.f * kLog2e * c1));
+            s[j][e] = top * (1.f - 2.f * __builtin_amdgcn_rcpf(x + 1.f)) - m;
+          }
+      } else {
+#pragma unroll
+        for (int j = 0; j < KB; ++j)
+#pragma unroll
+          for (int e = 0; e < 16; ++e) {
+            const float x = s[j][e], u = x * x;
+            s[j][e] = fmaf(x, fmaf(u, fmaf(u, fmaf(u, b3, b2), b1), b0), -m);
+          }
+      }
+    } else {
+#pragma unroll
+      for (int j = 0; j < KB; ++j)
+#pragma unroll
+        for (int e = 0; e < 16; ++e) s[j][e] = fmaf(s[j][e], c2, -m);
+    }
+    if constexpr (kBias) {
+      const float d0 = static_cast<float>(pos - key0 - 4 * hh);
+#pragma unroll
+      for (int j = 0; j < KB; ++j)
+#pragma unroll
+        for (int e = 0; e < 16; ++e)
+          s[j][e] = fmaf(-slope, fabsf(d0 - static_cast<float>(32 * j + 8 * (e >> 2) + (e & 3))),
+                         s[j][e]);
+    }
+    if (masked) {
+      const int lim = min(limit, k_hi) - key0 - 4 * hh;
+#pragma unroll
+      for (int j = 0; j < KB; ++j)
+#pragma unroll
+        for (int e = 0; e < 16; ++e) {
+          const bool gone = bad >> (2 * j + (e >> 3)) & 1;
+          if (gone || 32 * j + 8 * (e >> 2) + (e & 3) >= lim) s[j][e] = -INFINITY;
+        }
+    }
+    float mc[4];
+#pragma unroll
+    for (int c = 0; c < 4; ++c) {
+      const f32x16_t &x = s[c >> 1];
+      const int b = 8 * (c & 1);
+      mc[c] = max3(max3(x[b], x[b + 1], x[b + 2]), x[b + 3], x[b + 4]);
+      mc[c] = __builtin_elementwise_maximum(max3(mc[c], x[b + 5], x[b + 6]), x[b + 7]);
+    }
+    const float rel = pair_max(__builtin_elementwise_maximum(
+        max3(mc[0], mc[1], mc[2]), mc[3]));
+    if (__any(rel > thr)) {
+      const bool move = rel > thr;
+      const float shift = move ? rel : 0.f;
+      const float fall = thr < 0.f ? 0.f : __builtin_amdgcn_exp2f(-shift);
+      // A row without a key so far has nothing to scale.
+      l = move ? l * fall : l;
+#pragma unroll
+      for (int n = 0; n < NB; ++n)
+#pragma unroll
+        for (int e = 0; e < 16; ++e) acc[n][e] = move ? acc[n][e] * fall : acc[n][e];
+      m += shift;
+      if (move) thr = kLazy;
+#pragma unroll
+      for (int j = 0; j < KB; ++j)
+#pragma unroll
+        for (int e = 0; e < 16; ++e) s[j][e] -= shift;
+    }
+    float lsum[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int j = 0; j < KB; ++j)
+#pragma unroll
+      for (int e = 0; e < 16; ++e) {
+        s[j][e] = __builtin_amdgcn_exp2f(s[j][e]);
+        lsum[e & 3] += s[j][e];
+      }
+    l += (lsum[0] + lsum[1]) + (lsum[2] + lsum[3]);
+
+    // Where some row does not see some key, a V that is not finite would reach
+    // it as 0 * V: such tiles are looked through, a lane per key.
+    uint64_t odd = 0;
+    if (masked) {
+      bool any_odd = false;
+#pragma unroll
+      for (int c = 0; c < kChunks; ++c) {
+        const uint4 x = *reinterpret_cast<const uint4 *>(vt + lane * kRowB +
+                                                         16 * ((c + lane) & (kChunks - 1)));
+        any_odd = any_odd || W::odd(x.x) || W::odd(x.y) || W::odd(x.z) || W::odd(x.w);
+      }
+      odd = __ballot(any_odd);
+    }
+    if (odd == 0) {
+#pragma unroll
+      for (int j = 0; j < KB; ++j)
+#pragma unroll
+        for (int h16 = 0; h16 < 2; ++h16) {
+          const int kb = 2 * j + h16;
+          const v8 pb = __builtin_bit_cast(
+              v8, make_uint4(pack2<T>(s[j][8 * h16], s[j][8 * h16 + 1]),
+                             pack2<T>(s[j][8 * h16 + 2], s[j][8 * h16 + 3]),
+                             pack2<T>(s[j][8 * h16 + 4], s[j][8 * h16 + 5]),
+                             pack2<T>(s[j][8 * h16 + 6], s[j][8 * h16 + 7])));
+#pragma unroll
+          for (int n = 0; n < NB; ++n) {
+            const unsigned char *at = vt + 16 * kb * kRowB + (voff0 ^ (n << 6));
+            const uint2 lo = __builtin_bit_cast(
+                uint2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4_t *)at));
+            const uint2 hi = __builtin_bit_cast(
+                uint2, __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+                           (lds_s16x4_t *)(vt + 16 * kb * kRowB +
+                                           ((voff0 ^ 16 ^ (n << 6)) + 8 * kRowB))));
+            acc[n] = W::mfma(__builtin_bit_cast(v8, make_uint4(lo.x, lo.y, hi.x, hi.y)), pb,
+                             acc[n]);
+          }
+        }
+    } else {
+      // Key by key, each row adding only what it sees. acc[n][4 g + e] is
+      // element 32 n + 8 g + 4 hh + e of the row.
+      const int lim = min(limit, k_hi) - key0;
+      for (int k = 0; k < kTile; ++k) {
+        float mine = 0.f;  // the lane's register for keys k and k ^ 4
+#pragma unroll
+        for (int j = 0; j < KB; ++j)
+#pragma unroll
+          for (int e = 0; e < 16; ++e)
+            if ((k & ~4) == 32 * j + 8 * (e >> 2) + (e & 3)) mine = s[j][e];
+        const float pk = __shfl(mine, m32 + 8 * (k & 4));
+        if (k >= lim) continue;
+#pragma unroll
+        for (int n = 0; n < NB; ++n)
+#pragma unroll
+          for (int g = 0; g < 4; ++g) {
+            const uint16_t *x = reinterpret_cast<const uint16_t *>(
+                vt + k * kRowB + 16 * ((4 * n + g) ^ swizzle<D>(k)) + 8 * hh);
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+              acc[n][4 * g + e] += pk * Elem<T>::to_f32(T{x[e]});
+          }
+      }
+    }
+  };
+  for (int i = 0; i < chunk; i += 2) {
+    step(i, ks0[half], vs0[half], ks1[half], vs1[half]);
+    if (i + 1 < chunk) step(i + 1, ks1[half], vs1[half], ks0[half], vs0[half]);
+  }
+  l = pair_sum(l);
+  if (thr < 0.f) m = -INFINITY;
+
+  // The second half hands (m, l, O^T) over through the stage buffers, word by
+  // word, lanes side by side.
+  constexpr int kWords = 16 * NB + 2;
+  static_assert(sizeof(ks0) >= kWords * 64 * sizeof(float), "hand-over buffer");
+  float *mine = reinterpret_cast<float *>(w == 0 ? &ks0[0][0] : w == 1 ? &ks1[0][0]
+                                          : w == 2 ? &vs0[0][0] : &vs1[0][0]);
+  auto word = [&](int a) __attribute__((always_inline)) -> float * {
+    return mine + a * 64 + lane;
+  };
+  __builtin_amdgcn_s_waitcnt(0);
+  __syncthreads();
+  if (half == 1) {
+    *word(0) = m;
+    *word(1) = l;
+#pragma unroll
+    for (int n = 0; n < NB; ++n)
+#pragma unroll
+      for (int e = 0; e < 16; ++e) *word(2 + 16 * n + e) = acc[n][e];
+  }
+  __syncthreads();
+  if (half == 1) return;
+  const float m1 = *word(0), l1 = *word(1);
+  const float all_m = fmaxf(m, m1), ref = all_m == -INFINITY ? 0.f : all_m;
+  const float f0 = __builtin_amdgcn_exp2f(m - ref), f1 = __builtin_amdgcn_exp2f(m1 - ref);
+  const float sum = l * f0 + l1 * f1;
+#pragma unroll
+  for (int n = 0; n < NB; ++n)
+#pragma unroll
+    for (int e = 0; e < 16; ++e) acc[n][e] = acc[n][e] * f0 + *word(2 + 16 * n + e) * f1;
+
+  if (!alone) {
+    const int64_t at = (item * p.hkv + kvh) * kTileRows + 32 * w + m32;
+    if (hh == 0) {
+      // Partial results are in units of the natural exponent.
+      p.ml[2 * at] = all_m * 0.6931471805599453f;
+      p.ml[2 * at + 1] = sum;
+    }
+#pragma unroll
+    for (int n = 0; n < NB; ++n)
+#pragma unroll
+      for (int g = 0; g < 4; ++g) {
+        const float4 x = make_float4(acc[n][4 * g], acc[n][4 * g + 1], acc[n][4 * g + 2],
+                                     acc[n][4 * g + 3]);
+        *reinterpret_cast<float4 *>(p.acc + at * D + 32 * n + 8 * g + 4 * hh) = x;
+      }
+    return;
+  }
+  if (!live) return;
+  const float inv = sum > 0.f ? 1.f / sum : sum == 0.f ? 0.f : sum;
+  uint16_t *o = static_cast<uint16_t *>(p.out) + row * p.o_st + head * p.o_sh;
+  const bool wide = p.o_st % 4 == 0 && p.o_sh % 4 == 0 && reinterpret_cast<uintptr_t>(p.out) % 8 == 0;
+#pragma unroll
+  for (int n = 0; n < NB; ++n)
+#pragma unroll
+    for (int g = 0; g < 4; ++g) {
+      const int e0 = 32 * n + 8 * g + 4 * hh;
+      if (e0 >= p.d) continue;
+      uint16_t x[4];
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+        x[e] = __builtin_bit_cast(uint16_t, Elem<T>::from_f32(acc[n][4 * g + e] * inv));
+      if (wide) {
+        *reinterpret_cast<uint2 *>(o + e0) =
+            make_uint2(x[0] | static_cast<uint32_t>(x[1]) << 16,
+                       x[2] | static_cast<uint32_t>(x[3]) << 16);
+      } else {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) o[e0 + e] = x[e];
+      }
+    }
+}
+
+template <typename T, int D>
+int launch_tiles(const ScoredParams &p, unsigned grid, hipStream_t stream) {
+#define MLR_TILES(C, B) scored_tiles_kernel<T, D, C, B><<<grid, kThreads, 0, stream>>>(p)
+  if (p.cap > 0) {
+    if (p.slopes) MLR_TILES(true, true); else MLR_TILES(true, false);
+  } else {
+    if (p.slopes) MLR_TILES(false, true); else MLR_TILES(false, false);
+  }
+#undef MLR_TILES
+  return check_launch("scored_tiles");
+}
+
+}  // namespace
+
+int launch_scored_tiles(const ScoredParams &p, int dtype, unsigned grid, hipStream_t stream) {
+  if (dtype == MLR_DTYPE_F16)
+    return p.d > 64 ? launch_tiles<f16_t, 128>(p, grid, stream)
+                    : launch_tiles<f16_t, 64>(p, grid, stream);
+  return p.d > 64 ? launch_tiles<bf16_t, 128>(p, grid, stream)
+                  : launch_tiles<bf16_t, 64>(p, grid, stream);
+}
+
+}  // namespace mlr

@@ -133,14 +133,14 @@ _PROTOTYPES = {
          _c_i64, _c_ptr, _c_i64, _c_i64, _c_f64, _c_f64, _c_ptr, _c_int, _c_ptr, _c_size, _c_ptr,
          _c_i64, _c_i64, _c_ptr],
     ),
-    "mlr_paged_prefill_scored_workspace_size": (_c_size, [_c_i64] * 6 + [_c_int]),
+    "mlr_paged_prefill_scored_workspace_size": (_c_size, [_c_i64] * 7 + [_c_int]),
     "mlr_paged_prefill_scored": (
         _c_int,
         [_c_ptr, _c_i64, _c_i64, _c_ptr, _c_ptr, _c_i64, _c_i64, _c_i64, _c_i64, _c_ptr, _c_i64,
          _c_i64, _c_ptr, _c_ptr, _c_ptr, _c_i64, _c_i64, _c_i64, _c_i64, _c_f64, _c_f64, _c_ptr,
          _c_int, _c_ptr, _c_size, _c_ptr, _c_i64, _c_i64, _c_ptr],
     ),
-    "mlr_paged_decode_shared_prefix_workspace_size": (_c_size, [_c_i64] * 6 + [_c_int]),
+    "mlr_paged_decode_shared_prefix_workspace_size": (_c_size, [_c_i64] * 7 + [_c_int]),
     "mlr_paged_decode_shared_prefix": (
         _c_int,
         [_c_ptr, _c_i64, _c_i64, _c_ptr, _c_ptr, _c_i64, _c_i64, _c_i64, _c_i64, _c_ptr, _c_i64,

@@ -221,7 +221,7 @@ def paged_attention_prefill_scored(
     lib = _lib.load()
     with _lib.on(device):
         nbytes = lib.mlr_paged_prefill_scored_workspace_size(
-            seqs, max_query_len, width * block_size, num_q_heads, num_kv_heads, head_dim, dcode)
+            seqs, max_query_len, width, block_size, num_q_heads, num_kv_heads, head_dim, dcode)
         ws = _workspace(nbytes, device)
         status = lib.mlr_paged_prefill_scored(
             q.data_ptr(), q.stride(0), q.stride(1), k_cache.data_ptr(), v_cache.data_ptr(),
@@ -306,7 +306,7 @@ def paged_attention_decode_shared_prefix(
     lib = _lib.load()
     with _lib.on(device):
         nbytes = lib.mlr_paged_decode_shared_prefix_workspace_size(
-            batch, num_q_heads, num_kv_heads, head_dim, prefix_len, width * block_size, dcode)
+            batch, num_q_heads, num_kv_heads, head_dim, prefix_len, width, block_size, dcode)
         ws = _workspace(nbytes, device)
         status = lib.mlr_paged_decode_shared_prefix(
             q.data_ptr(), q.stride(0), q.stride(1), k_cache.data_ptr(), v_cache.data_ptr(),
