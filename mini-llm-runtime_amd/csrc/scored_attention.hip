@@ -129,10 +129,12 @@ int64_t prefix_units(int64_t batch, int64_t group, int64_t rows) {
 
 // Whether a call with `rows` query rows per sequence and KV head goes to the
 // kernel of 128 rows a unit: more than two of the other kernel's units.
-bool takes_tiles(int64_t rows, int64_t block_size, int dtype) {
-  return dtype != MLR_DTYPE_F32 && rows > 2 * kRows && block_size >= 16 &&
-         log2_if_pow2(block_size) >= 4;
+bool takes_tiles(int64_t rows, int64_t block_size, int64_t hkv, int64_t d, int dtype) {
+  return dtype != MLR_DTYPE_F32 && rows > 2 * kRows && log2_if_pow2(block_size) >= 4 &&
+         block_size < (int64_t(1) << 30) / (hkv * d);  // 32-bit offsets inside a block
 }
+
+int64_t prefix_target(int64_t rows) { return rows == kTileRows ? cus() : target_items(); }
 
 // A prefill's rows per unit, units, items, and whether units stay whole: with a
 // unit for every CU there is nothing to gain from splits, which cost a pass over
@@ -142,10 +144,10 @@ struct PrefillPlan {
   bool whole, parts;
 };
 PrefillPlan plan_prefill(int64_t seqs, int64_t max_q, int64_t max_keys, int64_t block_size,
-                         int64_t hq, int64_t hkv, int dtype) {
+                         int64_t hq, int64_t hkv, int64_t d, int dtype) {
   const int64_t group = hq / hkv;
   PrefillPlan n;
-  const bool tiles = takes_tiles(max_q * group, block_size, dtype);
+  const bool tiles = takes_tiles(max_q * group, block_size, hkv, d, dtype);
   n.rows = tiles ? kTileRows : kRows;
   n.units = prefill_units(seqs, max_q, group, n.rows);
   n.whole = tiles && (n.units * hkv >= cus() || max_keys <= kMinSplit);
@@ -285,9 +287,11 @@ extern "C" size_t mlr_paged_prefill_scored_workspace_size(int64_t num_seqs, int6
                                                           int64_t num_q_heads,
                                                           int64_t num_kv_heads, int64_t head_dim,
                                                           int dtype) {
-  if (num_seqs <= 0 || max_query_len <= 0 || num_kv_heads <= 0 || num_q_heads <= 0) return 0;
+  if (num_seqs <= 0 || max_query_len <= 0 || num_kv_heads <= 0 || num_q_heads <= 0 ||
+      head_dim <= 0 || block_size <= 0)
+    return 0;
   const PrefillPlan n = plan_prefill(num_seqs, max_query_len, max_blocks * block_size, block_size,
-                                     num_q_heads, num_kv_heads, dtype);
+                                     num_q_heads, num_kv_heads, head_dim, dtype);
   return n.parts ? part_bytes(n.units, n.items, n.rows, head_dim) : 0;
 }
 
@@ -319,7 +323,7 @@ extern "C" int mlr_paged_prefill_scored(
               "mlr_paged_prefill_scored: too many query rows");
   const int64_t max_keys = max_blocks * block_size;
   const PrefillPlan n = plan_prefill(num_seqs, max_query_len, max_keys, block_size, num_q_heads,
-                                     num_kv_heads, dtype);
+                                     num_kv_heads, head_dim, dtype);
   const size_t need = mlr_paged_prefill_scored_workspace_size(
       num_seqs, max_query_len, max_blocks, block_size, num_q_heads, num_kv_heads, head_dim, dtype);
   MLR_REQUIRE(need == 0 || (workspace && workspace_bytes >= need),
@@ -345,13 +349,16 @@ extern "C" int mlr_paged_prefill_scored(
 extern "C" size_t mlr_paged_decode_shared_prefix_workspace_size(
     int64_t batch, int64_t num_q_heads, int64_t num_kv_heads, int64_t head_dim, int64_t prefix_len,
     int64_t max_blocks, int64_t block_size, int dtype) {
-  if (batch <= 0 || num_kv_heads <= 0 || num_q_heads <= 0) return 0;
+  if (batch <= 0 || num_kv_heads <= 0 || num_q_heads <= 0 || head_dim <= 0 || block_size <= 0)
+    return 0;
   const int64_t group = num_q_heads / num_kv_heads, target = target_items();
-  const int64_t rows = takes_tiles(batch * group, block_size, dtype) ? kTileRows : kRows;
+  const int64_t rows =
+      takes_tiles(batch * group, block_size, num_kv_heads, head_dim, dtype) ? kTileRows : kRows;
   const int64_t own = decode_units(batch, group), over = prefix_units(batch, group, rows);
   return part_bytes(own, max_items(own, num_kv_heads, max_blocks * block_size, target), kRows,
                     head_dim) +
-         part_bytes(over, max_items(over, num_kv_heads, prefix_len, target), rows, head_dim);
+         part_bytes(over, max_items(over, num_kv_heads, prefix_len, prefix_target(rows)), rows,
+                    head_dim);
 }
 
 extern "C" int mlr_paged_decode_shared_prefix(
@@ -390,7 +397,7 @@ extern "C" int mlr_paged_decode_shared_prefix(
   const int64_t own_items = max_items(own.units, own.hkv, max_keys, own.target);
   char *ws = place_parts(own, static_cast<char *>(workspace), own_items, kRows);
   ScoredParams over = params_of(o, kModePrefix);
-  const bool tiles = takes_tiles(batch * over.group, block_size, dtype);
+  const bool tiles = takes_tiles(batch * over.group, block_size, over.hkv, over.d, dtype);
   const int rows = tiles ? kTileRows : kRows;
   over.bt = prefix_table;
   over.bt_st = 0;
@@ -398,6 +405,7 @@ extern "C" int mlr_paged_decode_shared_prefix(
   over.units = over.tiles = static_cast<int>(prefix_units(batch, over.group, rows));
   over.start = prefix_len;
   over.force_partial = true;
+  over.target = prefix_target(rows);
   const int64_t over_items = max_items(over.units, over.hkv, prefix_len, over.target);
   place_parts(over, ws, over_items, rows);
   hipStream_t s = static_cast<hipStream_t>(stream);

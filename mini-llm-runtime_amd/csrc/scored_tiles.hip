@@ -55,10 +55,8 @@ template <> struct Wide<bf16_t> {
   __device__ static f32x16_t mfma(v8 a, v8 b, f32x16_t c) {
     return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0);
   }
-  // Whether a half of w is an infinity or NaN.
-  __device__ static bool odd(uint32_t w) {
-    return ((w & 0x7f807f80u) + 0x00800080u) & 0x80008000u;
-  }
+  // Bits 15 and 31: whether that half of w is an infinity or NaN.
+  __device__ static uint32_t odd(uint32_t w) { return (w & 0x7f807f80u) + 0x00800080u; }
 };
 template <> struct Wide<f16_t> {
   using v8 = f16x8_t;
@@ -66,9 +64,7 @@ template <> struct Wide<f16_t> {
   __device__ static f32x16_t mfma(v8 a, v8 b, f32x16_t c) {
     return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0);
   }
-  __device__ static bool odd(uint32_t w) {
-    return ((w & 0x7c007c00u) + 0x04000400u) & 0x80008000u;
-  }
+  __device__ static uint32_t odd(uint32_t w) { return (w & 0x7c007c00u) + 0x04000400u; }
 };
 
 template <typename T>
@@ -112,8 +108,7 @@ __device__ __forceinline__ int units_past(const ScoredParams &p, int seq, int64_
 }
 
 template <typename T, int D, bool kCap, bool kBias>
-__global__ __launch_bounds__(kThreads)
-    __attribute__((amdgpu_waves_per_eu(2)))
+__global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(D == 64 ? 4 : 2)))
 void scored_tiles_kernel(ScoredParams p) {
   using W = Wide<T>;
   using v8 = typename W::v8;
@@ -298,54 +293,54 @@ void scored_tiles_kernel(ScoredParams p) {
   const uint32_t kv_bytes = static_cast<uint32_t>(kvh) * (2 * p.d);
   const int64_t block_bytes = static_cast<int64_t>(row_bytes) << bs_log2;
 
-  // The block ids of tile i's four runs of 16 keys, and which are out of range.
-  struct Ids {
-    int64_t id[4];
+  // Whether some block id of the item is out of range (then every tile asks).
+  bool strange = false;
+  for (int i = (k_lo >> bs_log2) + tid; k_hi > 0 && i <= (k_hi - 1) >> bs_log2; i += kThreads) {
+    const int64_t id = p.bt[(p.mode == kModePrefix ? 0 : static_cast<int64_t>(t.seq) * p.bt_st) + i];
+    strange = strange || id < 0 || id >= p.num_blocks;
+  }
+  strange = __syncthreads_or(strange);
+
+  // The wave's 16 rows of tile i: where they start, and how many bytes from there
+  // on may be read (rows past k_hi and of blocks out of range arrive as zeros).
+  struct Span {
+    uint64_t at;
+    uint32_t bytes;
   };
-  auto ids_of = [&](int i) __attribute__((always_inline)) -> Ids {
-    Ids x;
-#pragma unroll
-    for (int b = 0; b < 4; ++b)
-      x.id[b] = table[min(k_lo + i * kTile + 16 * b, k_hi - 1) >> bs_log2];
+  auto id_of = [&](int i) __attribute__((always_inline)) -> int64_t {
+    return table[min(k_lo + i * kTile + 16 * w, k_hi - 1) >> bs_log2];
+  };
+  auto span_of = [&](int i, int64_t id) __attribute__((always_inline)) -> Span {
+    const int key = k_lo + i * kTile + 16 * w;
+    const bool ok = i < t_hi && key < k_hi && id >= 0 && id < p.num_blocks;
+    Span x;
+    x.bytes = ok ? static_cast<uint32_t>(min(k_hi - key, 16) - 1) * row_bytes + 2 * p.d : 0u;
+    x.at = ok ? static_cast<uint64_t>(id) * block_bytes +
+                    static_cast<uint32_t>(key & bs_mask) * row_bytes + kv_bytes
+              : 0u;
     return x;
   };
-  auto bad_of = [&](const Ids &x) __attribute__((always_inline)) -> uint32_t {
+  auto copy = [&](const Span &x, const void *cache, unsigned char *dst)
+      __attribute__((always_inline)) {
+    const __amdgpu_buffer_rsrc_t r = __builtin_amdgcn_make_buffer_rsrc(
+        const_cast<unsigned char *>(static_cast<const unsigned char *>(cache) + x.at), 0, x.bytes,
+        0x00020000);
+    dst += 16 * w * kRowB;
+#pragma unroll
+    for (int c = 0; c < kCopies; ++c) {
+      const uint32_t off = src_off[c];
+      __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (lds_void_t *)(dst + 1024 * c), 16, off, 0, 0, 0);
+    }
+  };
+  // One bit per run of 16 keys of tile i whose block is out of range.
+  auto bad_of = [&](int i) __attribute__((always_inline)) -> uint32_t {
     uint32_t bad = 0;
 #pragma unroll
-    for (int b = 0; b < 4; ++b)
-      if (x.id[b] < 0 || x.id[b] >= p.num_blocks) bad |= 1u << b;
+    for (int b = 0; b < 4; ++b) {
+      const int64_t id = table[min(k_lo + i * kTile + 16 * b, k_hi - 1) >> bs_log2];
+      if (id < 0 || id >= p.num_blocks) bad |= 1u << b;
+    }
     return bad;
-  };
-  // Copies the wave's 16 rows of tile i into a stage; rows past k_hi and of
-  // blocks out of range arrive as zeros.
-  auto copy = [&](int i, const Ids &x, unsigned char *kt, unsigned char *vt)
-      __attribute__((always_inline)) {
-    const int key = k_lo + i * kTile + 16 * w;
-    const int64_t id = w == 0 ? x.id[0] : w == 1 ? x.id[1] : w == 2 ? x.id[2] : x.id[3];
-    const bool ok = i < t_hi && key < k_hi && id >= 0 && id < p.num_blocks;
-    const uint32_t nrec =
-        ok ? static_cast<uint32_t>(min(k_hi - key, 16) - 1) * row_bytes + 2 * p.d : 0u;
-    const int64_t at = ok ? id * block_bytes +
-                                static_cast<int64_t>(key & bs_mask) * row_bytes + kv_bytes
-                          : 0;
-    const __amdgpu_buffer_rsrc_t rk = __builtin_amdgcn_make_buffer_rsrc(
-        const_cast<unsigned char *>(static_cast<const unsigned char *>(p.k) + at), 0, nrec,
-        0x00020000);
-    const __amdgpu_buffer_rsrc_t rv = __builtin_amdgcn_make_buffer_rsrc(
-        const_cast<unsigned char *>(static_cast<const unsigned char *>(p.v) + at), 0, nrec,
-        0x00020000);
-    kt += 16 * w * kRowB;
-    vt += 16 * w * kRowB;
-#pragma unroll
-    for (int c = 0; c < kCopies; ++c) {
-      const uint32_t off = src_off[c];
-      __builtin_amdgcn_raw_ptr_buffer_load_lds(rk, (lds_void_t *)(kt + 1024 * c), 16, off, 0, 0, 0);
-    }
-#pragma unroll
-    for (int c = 0; c < kCopies; ++c) {
-      const uint32_t off = src_off[c];
-      __builtin_amdgcn_raw_ptr_buffer_load_lds(rv, (lds_void_t *)(vt + 1024 * c), 16, off, 0, 0, 0);
-    }
   };
 
   // Lane-constant LDS offsets, as XORs of the chunk index: K row m32 (+ 32 per
@@ -363,41 +358,113 @@ void scored_tiles_kernel(ScoredParams p) {
   float m = 0.f, l = 0.f;
   float thr = -__FLT_MAX__;  // a tile's maximum above this moves m; m is unset so far
 
-  Ids next;
-  uint32_t bad = 0, bad_next = 0;
-  if (chunk > 0) {  // uniform: without keys the table is not read
-    next = ids_of(t_lo);
-    bad_next = bad_of(next);
-    copy(t_lo, next, ks0[half], vs0[half]);
-    next = ids_of(t_lo + 1);
-  }
-  // Tile i of the half from stage (kt, vt), with tile i + 1 on its way to the other.
-  auto step = [&](int i, const unsigned char *kt, const unsigned char *vt, unsigned char *kn,
-                  unsigned char *vn) __attribute__((always_inline)) {
-    // This wave's copies of tile i have landed; then everyone's have, and all
-    // reads of the other stage are done.
-    asm volatile("" ::: "memory");
-    __builtin_amdgcn_s_waitcnt(0);
-    __builtin_amdgcn_s_barrier();
-    asm volatile("" ::: "memory");
-    bad = bad_next;
-    if (i + 1 < chunk) copy(t_lo + i + 1, next, kn, vn);
-    bad_next = bad_of(next);
-    next = ids_of(t_lo + i + 2);
-    const int key0 = k_lo + (t_lo + i) * kTile;
-    if (t_lo + i >= t_hi || key0 >= any) return;  // uniform per wave
-
-    f32x16_t s[KB];
+  // Two phases per tile, a workgroup barrier after each, the halves one phase
+  // apart: on every SIMD one wave's matrix work meets the other's vector work.
+  //   M_i: O^T += V^T P^T of tile i - 1, S^T of tile i
+  //   V_i: copies of K_{i+2} and V_{i+1} into the stages that M_i has read,
+  //        then scores and probabilities of tile i, packed for M_{i+1}
+  // A wave waits for its own copies of the phase before, the barrier for all.
+  f32x16_t s[KB];
+  uint32_t pk[KB][8];
+  bool masked = false;  // whether some row of the wave does not see some key of the tile
+  auto active = [&](int i) __attribute__((always_inline)) {
+    return t_lo + i < t_hi && k_lo + (t_lo + i) * kTile < any;
+  };
+  auto add_values = [&](int i, const unsigned char *vt) __attribute__((always_inline)) {
+    // Where some row does not see some key, a V that is not finite would reach
+    // it as 0 * V: such tiles are looked through, a lane per key.
+    uint64_t odd = 0;
+    if (masked) {
+      uint32_t bits = 0;
+      int key = lane;
+      asm volatile("" : "+v"(key));
+#pragma unroll 2
+      for (int c = 0; c < kChunks; ++c) {
+        const uint4 x = *reinterpret_cast<const uint4 *>(vt + key * kRowB +
+                                                         16 * ((c + key) & (kChunks - 1)));
+        bits |= W::odd(x.x) | W::odd(x.y) | W::odd(x.z) | W::odd(x.w);
+      }
+      odd = __ballot((bits & 0x80008000u) != 0);
+    }
+    if (odd == 0) {
+      int vo = voff0;
+      asm volatile("" : "+v"(vo));
+#pragma unroll
+      for (int kb = 0; kb < 2 * KB; ++kb) {
+        const uint32_t *x = &pk[kb >> 1][4 * (kb & 1)];
+        const v8 pb = __builtin_bit_cast(v8, make_uint4(x[0], x[1], x[2], x[3]));
+#pragma unroll
+        for (int n = 0; n < NB; ++n) {
+          const uint2 lo = __builtin_bit_cast(
+              uint2, __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+                         (lds_s16x4_t *)(vt + 16 * kb * kRowB + (vo ^ (n << 6)))));
+          const uint2 hi = __builtin_bit_cast(
+              uint2, __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+                         (lds_s16x4_t *)(vt + 16 * kb * kRowB + ((vo ^ 16 ^ (n << 6)) + 8 * kRowB))));
+          acc[n] = W::mfma(__builtin_bit_cast(v8, make_uint4(lo.x, lo.y, hi.x, hi.y)), pb, acc[n]);
+        }
+      }
+      // Two MFMAs' V reads ahead of the MFMAs.
+      constexpr int kMfma = 2 * KB * NB;
+      __builtin_amdgcn_sched_group_barrier(0x100, 4, 0);
+#pragma unroll
+      for (int x = 0; x < kMfma - 2; ++x) {
+        __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+        __builtin_amdgcn_sched_group_barrier(0x100, 2, 0);
+      }
+      __builtin_amdgcn_sched_group_barrier(0x008, 2, 0);
+    } else {
+      // Key by key, each row adding only what it sees. acc[n][4 g + e] is
+      // element 32 n + 8 g + 4 hh + e of the row.
+      const int lim = min(limit, k_hi) - (k_lo + (t_lo + i) * kTile);
+      for (int k = 0; k < kTile; ++k) {
+        uint32_t mine = 0;  // the lane's pair of registers for keys k and k ^ 4
+#pragma unroll
+        for (int j = 0; j < KB; ++j)
+#pragma unroll
+          for (int x = 0; x < 8; ++x)
+            if ((k & ~5) == 32 * j + 8 * (x >> 1) + 2 * (x & 1)) mine = pk[j][x];
+        const uint32_t both = __shfl(mine, m32 + 8 * (k & 4));
+        const uint16_t one = static_cast<uint16_t>(k & 1 ? both >> 16 : both);
+        const float pr = Elem<T>::to_f32(T{one});
+        if (k >= lim) continue;
+#pragma unroll
+        for (int n = 0; n < NB; ++n)
+#pragma unroll
+          for (int g = 0; g < 4; ++g) {
+            const uint16_t *x = reinterpret_cast<const uint16_t *>(
+                vt + k * kRowB + 16 * ((4 * n + g) ^ swizzle<D>(k)) + 8 * hh);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) acc[n][4 * g + e] += pr * Elem<T>::to_f32(T{x[e]});
+          }
+      }
+    }
+  };
+  auto scores = [&](const unsigned char *kt) __attribute__((always_inline)) {
+    int ko = koff0;  // the offsets below are made here, not kept over the loop
+    asm volatile("" : "+v"(ko));
 #pragma unroll
     for (int j = 0; j < KB; ++j) {
       s[j] = f32x16_t{};
 #pragma unroll
       for (int st = 0; st < QS; ++st) {
-        const v8 a = *reinterpret_cast<const v8 *>(kt + 32 * j * kRowB + (koff0 ^ (st << 5)));
+        const v8 a = *reinterpret_cast<const v8 *>(kt + 32 * j * kRowB + (ko ^ (st << 5)));
         s[j] = W::mfma(a, qf[st], s[j]);
       }
     }
-    const bool masked = key0 + kTile > all || key0 + kTile > k_hi || bad != 0;
+    // Two K reads ahead of the MFMAs; more would only hold registers.
+    __builtin_amdgcn_sched_group_barrier(0x100, 2, 0);
+#pragma unroll
+    for (int x = 0; x < KB * QS - 2; ++x) {
+      __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+      __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
+    }
+    __builtin_amdgcn_sched_group_barrier(0x008, 2, 0);
+  };
+  auto weigh = [&](int i) __attribute__((always_inline)) {
+    const int key0 = k_lo + (t_lo + i) * kTile;
+    const uint32_t bad = strange ? bad_of(t_lo + i) : 0u;
+    masked = key0 + kTile > all || key0 + kTile > k_hi || bad != 0;
 
     // Scores relative to m.
     if constexpr (kCap) {
@@ -485,72 +552,78 @@ void scored_tiles_kernel(ScoredParams p) {
       }
     l += (lsum[0] + lsum[1]) + (lsum[2] + lsum[3]);
 
-    // Where some row does not see some key, a V that is not finite would reach
-    // it as 0 * V: such tiles are looked through, a lane per key.
-    uint64_t odd = 0;
-    if (masked) {
-      bool any_odd = false;
-#pragma unroll
-      for (int c = 0; c < kChunks; ++c) {
-        const uint4 x = *reinterpret_cast<const uint4 *>(vt + lane * kRowB +
-                                                         16 * ((c + lane) & (kChunks - 1)));
-        any_odd = any_odd || W::odd(x.x) || W::odd(x.y) || W::odd(x.z) || W::odd(x.w);
-      }
-      odd = __ballot(any_odd);
-    }
-    if (odd == 0) {
+    if constexpr (KB == 2) {
 #pragma unroll
       for (int j = 0; j < KB; ++j)
 #pragma unroll
-        for (int h16 = 0; h16 < 2; ++h16) {
-          const int kb = 2 * j + h16;
-          const v8 pb = __builtin_bit_cast(
-              v8, make_uint4(pack2<T>(s[j][8 * h16], s[j][8 * h16 + 1]),
-                             pack2<T>(s[j][8 * h16 + 2], s[j][8 * h16 + 3]),
-                             pack2<T>(s[j][8 * h16 + 4], s[j][8 * h16 + 5]),
-                             pack2<T>(s[j][8 * h16 + 6], s[j][8 * h16 + 7])));
-#pragma unroll
-          for (int n = 0; n < NB; ++n) {
-            const unsigned char *at = vt + 16 * kb * kRowB + (voff0 ^ (n << 6));
-            const uint2 lo = __builtin_bit_cast(
-                uint2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4_t *)at));
-            const uint2 hi = __builtin_bit_cast(
-                uint2, __builtin_amdgcn_ds_read_tr16_b64_v4i16(
-                           (lds_s16x4_t *)(vt + 16 * kb * kRowB +
-                                           ((voff0 ^ 16 ^ (n << 6)) + 8 * kRowB))));
-            acc[n] = W::mfma(__builtin_bit_cast(v8, make_uint4(lo.x, lo.y, hi.x, hi.y)), pb,
-                             acc[n]);
-          }
-        }
-    } else {
-      // Key by key, each row adding only what it sees. acc[n][4 g + e] is
-      // element 32 n + 8 g + 4 hh + e of the row.
-      const int lim = min(limit, k_hi) - key0;
-      for (int k = 0; k < kTile; ++k) {
-        float mine = 0.f;  // the lane's register for keys k and k ^ 4
-#pragma unroll
-        for (int j = 0; j < KB; ++j)
-#pragma unroll
-          for (int e = 0; e < 16; ++e)
-            if ((k & ~4) == 32 * j + 8 * (e >> 2) + (e & 3)) mine = s[j][e];
-        const float pk = __shfl(mine, m32 + 8 * (k & 4));
-        if (k >= lim) continue;
-#pragma unroll
-        for (int n = 0; n < NB; ++n)
-#pragma unroll
-          for (int g = 0; g < 4; ++g) {
-            const uint16_t *x = reinterpret_cast<const uint16_t *>(
-                vt + k * kRowB + 16 * ((4 * n + g) ^ swizzle<D>(k)) + 8 * hh);
-#pragma unroll
-            for (int e = 0; e < 4; ++e)
-              acc[n][4 * g + e] += pk * Elem<T>::to_f32(T{x[e]});
-          }
-      }
+        for (int x = 0; x < 8; ++x) pk[j][x] = pack2<T>(s[j][2 * x], s[j][2 * x + 1]);
     }
   };
-  for (int i = 0; i < chunk; i += 2) {
-    step(i, ks0[half], vs0[half], ks1[half], vs1[half]);
-    if (i + 1 < chunk) step(i + 1, ks1[half], vs1[half], ks0[half], vs0[half]);
+  // s_waitcnt: all but the newest batch of copies, and LDS; LDS and scalars alone.
+  constexpr int kBatch = 2 * kCopies;
+  constexpr int kWaitBatch = (kBatch & 15) | ((kBatch >> 4) << 14) | 0x70;
+  constexpr int kWaitLds = 0xC07F;
+  Span next_k{}, next_v{};
+  int64_t id = 0;
+  auto m_phase = [&](int i, const unsigned char *kt, const unsigned char *vt)
+      __attribute__((always_inline)) {
+    const int64_t id3 = id_of(t_lo + i + 3);
+    __builtin_amdgcn_s_setprio(3);
+    if (i >= 1 && active(i - 1)) add_values(i - 1, vt);
+    __builtin_amdgcn_sched_barrier(0);
+    if (active(i)) {
+      scores(kt);
+    } else {  // defined in every phase, so that it lives over none
+#pragma unroll
+      for (int j = 0; j < KB; ++j) s[j] = f32x16_t{};
+    }
+    __builtin_amdgcn_s_setprio(0);
+    next_v = next_k;
+    next_k = span_of(t_lo + i + 2, id);
+    id = id3;
+    asm volatile("" ::: "memory");
+    __builtin_amdgcn_s_waitcnt(kWaitLds);
+    __builtin_amdgcn_s_barrier();
+    asm volatile("" ::: "memory");
+  };
+  auto v_phase = [&](int i, unsigned char *kt, unsigned char *vt) __attribute__((always_inline)) {
+    copy(next_k, p.k, kt);
+    copy(next_v, p.v, vt);
+    if (active(i)) {
+      weigh(i);
+    } else {
+#pragma unroll
+      for (int j = 0; j < KB; ++j)
+#pragma unroll
+        for (int x = 0; x < 8; ++x) pk[j][x] = 0;
+    }
+    asm volatile("" ::: "memory");
+    __builtin_amdgcn_s_waitcnt(kWaitBatch);
+    __builtin_amdgcn_s_barrier();
+    asm volatile("" ::: "memory");
+  };
+  if (chunk > 0) {  // uniform: without keys the table is not read
+    const int64_t id0 = id_of(t_lo), id1 = id_of(t_lo + 1);
+    id = id_of(t_lo + 2);
+    const Span first = span_of(t_lo, id0);
+    next_k = span_of(t_lo + 1, id1);
+    copy(first, p.k, ks0[half]);
+    copy(first, p.v, vs0[half]);
+    copy(next_k, p.k, ks1[half]);
+    asm volatile("" ::: "memory");
+    __builtin_amdgcn_s_waitcnt(0);
+    __builtin_amdgcn_s_barrier();
+    if (half == 1) __builtin_amdgcn_s_barrier();
+    asm volatile("" ::: "memory");
+    for (int i = 0; i < chunk; i += 2) {
+      m_phase(i, ks0[half], vs1[half]);
+      v_phase(i, ks0[half], vs1[half]);
+      m_phase(i + 1, ks1[half], vs0[half]);
+      v_phase(i + 1, ks1[half], vs0[half]);
+    }
+    // The last tile's values; an odd count had them in the phase past its end.
+    if ((chunk & 1) == 0) m_phase(chunk, ks0[half], vs1[half]);
+    if (half == 0) __builtin_amdgcn_s_barrier();
   }
   l = pair_sum(l);
   if (thr < 0.f) m = -INFINITY;
@@ -602,9 +675,14 @@ void scored_tiles_kernel(ScoredParams p) {
       }
     return;
   }
-  if (!live) return;
+  // The row again, rather than kept over the loop.
+  int lane2 = m32;
+  asm volatile("" : "+v"(lane2));
+  const int r2 = t.r0 + 32 * w + lane2;
+  if (r2 >= t.rows) return;
+  const int tok2 = r2 / p.group, head2 = kvh * p.group + r2 - tok2 * p.group;
   const float inv = sum > 0.f ? 1.f / sum : sum == 0.f ? 0.f : sum;
-  uint16_t *o = static_cast<uint16_t *>(p.out) + row * p.o_st + head * p.o_sh;
+  uint16_t *o = static_cast<uint16_t *>(p.out) + (t.q0 + tok2) * p.o_st + head2 * p.o_sh;
   const bool wide = p.o_st % 4 == 0 && p.o_sh % 4 == 0 && reinterpret_cast<uintptr_t>(p.out) % 8 == 0;
 #pragma unroll
   for (int n = 0; n < NB; ++n)
