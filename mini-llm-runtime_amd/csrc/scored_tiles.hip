@@ -46,7 +46,7 @@ constexpr float kLazy = 8.f;
 constexpr int kTile = 64;    // keys
 constexpr int kHalves = 2;   // of the keys
 constexpr int kThreads = 256 * kHalves;
-constexpr int kRankUnits = 4096;  // most units that are ranked by their keys
+constexpr int kRankUnits = 4096, kRankSeqs = 512;  // most that are ranked by their keys
 
 template <typename T> struct Wide;
 template <> struct Wide<bf16_t> {
@@ -56,7 +56,9 @@ template <> struct Wide<bf16_t> {
     return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0);
   }
   // Bits 15 and 31: whether that half of w is an infinity or NaN.
-  __device__ static uint32_t odd(uint32_t w) { return (w & 0x7f807f80u) + 0x00800080u; }
+  __device__ static uint32_t odd(uint32_t w) {
+    return ((w & 0x7f807f80u) + 0x00800080u) & 0x80008000u;
+  }
 };
 template <> struct Wide<f16_t> {
   using v8 = f16x8_t;
@@ -64,7 +66,9 @@ template <> struct Wide<f16_t> {
   __device__ static f32x16_t mfma(v8 a, v8 b, f32x16_t c) {
     return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0);
   }
-  __device__ static uint32_t odd(uint32_t w) { return (w & 0x7c007c00u) + 0x04000400u; }
+  __device__ static uint32_t odd(uint32_t w) {
+    return ((w & 0x7c007c00u) + 0x04000400u) & 0x80008000u;
+  }
 };
 
 template <typename T>
@@ -94,17 +98,18 @@ __device__ __forceinline__ int swizzle(int r) {
   return ((r & 1) << 1) | (((r >> 1) & 3) << 2) | ((r >> 3) & 1);
 }
 
+// What the order of units needs of a sequence.
+struct Seq {
+  int rows, pos0, ahead;
+};
+
 // Units of a sequence that see more than `keys` keys: those whose last row
 // belongs to token keys - pos0 or a later one.
-__device__ __forceinline__ int units_past(const ScoredParams &p, int seq, int64_t keys) {
-  const Unit t = unit_of(p, seq * p.tiles, kTileRows);
-  if (t.rows == 0) return 0;
+__device__ __forceinline__ int units_past(const Seq &t, int group, int keys) {
   const int all = (t.rows + kTileRows - 1) / kTileRows;
-  if (t.ahead > keys) return all;
-  const int64_t tok = keys - t.pos0;
-  if (tok <= 0) return all;
-  const int64_t row = tok * p.group;
-  return row >= t.rows ? 0 : all - static_cast<int>(row / kTileRows);
+  const int tok = keys - t.pos0;
+  if (t.ahead > keys || tok <= 0) return all;
+  return tok > (t.rows - 1) / group ? 0 : all - tok * group / kTileRows;
 }
 
 template <typename T, int D, bool kCap, bool kBias>
@@ -121,7 +126,7 @@ void scored_tiles_kernel(ScoredParams p) {
   __shared__ __align__(1024) unsigned char ks0[kHalves][kTileB], ks1[kHalves][kTileB];
   __shared__ __align__(1024) unsigned char vs0[kHalves][kTileB], vs1[kHalves][kTileB];
   __shared__ int64_t s_keys[kThreads / 64];
-  __shared__ int s_count[kThreads / 64], s_unit, s_part, s_of;
+  __shared__ int s_count[kThreads / 64], s_unit, s_part, s_of, s_all, s_odd;
   const int tid = threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int w = wave & 3, half = wave >> 2;
@@ -140,19 +145,31 @@ void scored_tiles_kernel(ScoredParams p) {
     if (D == 64 && b >= p.ncu && b < 2 * p.ncu) b = min(n, 2 * p.ncu) - 1 - (b - p.ncu);
     const int rank = b / p.hkv;
     kvh = b - rank * p.hkv;
-    if (p.units > kRankUnits) {
+    if (p.units > kRankUnits || p.seqs > kRankSeqs) {
       const int seq = rank / p.tiles;
       if (tid == 0) s_unit = seq * p.tiles + p.tiles - 1 - (rank - seq * p.tiles);
     } else {
-      // By keys, then by sequence, then later rows first.
+      // By keys, then by sequence, then later rows first. The sequences' sizes
+      // are read once, into what will be the first stage.
+      Seq *seqs = reinterpret_cast<Seq *>(&ks0[0][0]);
+      static_assert(sizeof(ks0) >= kRankSeqs * sizeof(Seq), "the sizes fit a stage");
+      for (int q = tid; q < p.seqs; q += kThreads) {
+        const Unit t = unit_of(p, q * p.tiles, kTileRows);
+        seqs[q] = Seq{t.rows, static_cast<int>(t.pos0), static_cast<int>(t.ahead)};
+      }
       if (tid == 0) s_unit = -1;
       __syncthreads();
       for (int u = tid; u < p.units; u += kThreads) {
-        const Unit t = unit_of(p, u, kTileRows);
-        if (t.r0 >= t.rows) continue;
-        int r = (t.rows + kTileRows - 1) / kTileRows - 1 - t.r0 / kTileRows;
-        for (int q = 0; q < p.seqs; ++q)
-          if (q != t.seq) r += units_past(p, q, q < t.seq ? t.hi - 1 : t.hi);
+        const int seq = u / p.tiles, at = u - seq * p.tiles;
+        const Seq t = seqs[seq];
+        if (at * kTileRows >= t.rows) continue;
+        const int last = min(t.rows, (at + 1) * kTileRows) - 1;
+        const int hi = max(max(t.pos0 + last / p.group + 1, t.ahead), 0);
+        int r = (t.rows + kTileRows - 1) / kTileRows - 1 - at;
+        for (int q = 0; q < p.seqs; ++q) {
+          const Seq o = seqs[q];
+          if (q != seq && o.rows > 0) r += units_past(o, p.group, q < seq ? hi - 1 : hi);
+        }
         if (r == rank) s_unit = u;
       }
     }
@@ -205,6 +222,10 @@ void scored_tiles_kernel(ScoredParams p) {
     }
     if (blockIdx.x == 0 && tid == kThreads - 1) p.first[p.units] = items;
   }
+  if (tid == 0) {
+    s_all = 0x7fffffff;
+    s_odd = 0;
+  }
   __syncthreads();
   const int unit = __builtin_amdgcn_readfirstlane(s_unit);
   if (unit < 0) return;  // uniform: no item left for this workgroup
@@ -216,7 +237,9 @@ void scored_tiles_kernel(ScoredParams p) {
   const int k_hi = __builtin_amdgcn_readfirstlane(
       static_cast<int>(min(t.hi, static_cast<int64_t>(k_lo) + split)));
 
-  // This half's tiles [t_lo, t_hi) of the item's.
+  // This half's tiles [t_lo, t_hi) of the item's, taken from the last to the
+  // first: a bias by distance makes the last keys the heaviest, and the running
+  // maximum then stays where the first tile puts it.
   const int tiles = (k_hi - k_lo + kTile - 1) / kTile;
   const int chunk = (tiles + kHalves - 1) / kHalves;
   const int t_lo = half * chunk, t_hi = min(tiles, t_lo + chunk);
@@ -263,16 +286,22 @@ void scored_tiles_kernel(ScoredParams p) {
     q.w ^= flip;
     qf[s] = __builtin_bit_cast(v8, q);
   }
-  // Score in base 2: c2 s, or with the cap s (b0 + s^2 (b1 + ...)).
+  // Score in base 2: c2 s, or with the cap s (b0 + s^2 (b1 + ...)). Uniform, so
+  // held in scalar registers.
+  auto uniform = [](float x) {
+    return __int_as_float(__builtin_amdgcn_readfirstlane(__float_as_int(x)));
+  };
   const float scale = fabsf(p.scale);
-  const float c2 = scale * kLog2e;
-  const float c1 = kCap ? scale / p.cap : 0.f;     // y = c1 s
-  const float top = kCap ? p.cap * kLog2e : 0.f;   // the cap in base 2
-  const float b0 = 0.99999949f * c1 * top;
-  const float b1 = -0.33326618f * c1 * c1 * c1 * top;
-  const float b2 = 0.13193061f * c1 * c1 * c1 * c1 * c1 * top;
-  const float b3 = -0.044465f * c1 * c1 * c1 * c1 * c1 * c1 * c1 * top;
-  const float near = 0.5f / c1;                    // |s| up to which that holds
+  const float c2 = uniform(scale * kLog2e);
+  const float c1 = uniform(kCap ? scale / p.cap : 0.f);    // y = c1 s
+  const float top = uniform(kCap ? p.cap * kLog2e : 0.f);  // the cap in base 2
+  // tanh(y) / y up to |y| = 1/2 (relative error 5.1e-7) and 1/4 (4.0e-7).
+  const float c3 = c1 * c1 * c1 * top, c5 = c1 * c1 * c3;
+  const float near = uniform(0.5f / c1), near2 = uniform(0.25f / c1);
+  const float b0 = uniform(0.99999949f * c1 * top), b1 = uniform(-0.33326618f * c3);
+  const float b2 = uniform(0.13193061f * c5), b3 = uniform(-0.044465f * c1 * c1 * c5);
+  const float a0 = uniform(0.99999960f * c1 * top), a1 = uniform(-0.33321908f * c3);
+  const float a2 = uniform(0.12841613f * c5);
   const float slope = kBias ? p.slopes[head] * kLog2e : 0.f;
 
   // Copies: copy i of a wave's 16 rows moves chunk places [64 i, 64 i + 64);
@@ -299,7 +328,10 @@ void scored_tiles_kernel(ScoredParams p) {
     const int64_t id = p.bt[(p.mode == kModePrefix ? 0 : static_cast<int64_t>(t.seq) * p.bt_st) + i];
     strange = strange || id < 0 || id >= p.num_blocks;
   }
+  if (lane == 0) atomicMin(&s_all, all);
   strange = __syncthreads_or(strange);
+  // Tiles from this key on are hidden from some row of the unit in part.
+  const int unit_all = __builtin_amdgcn_readfirstlane(s_all);
 
   // The wave's 16 rows of tile i: where they start, and how many bytes from there
   // on may be read (rows past k_hi and of blocks out of range arrive as zeros).
@@ -307,12 +339,16 @@ void scored_tiles_kernel(ScoredParams p) {
     uint64_t at;
     uint32_t bytes;
   };
+  auto key_of = [&](int i) __attribute__((always_inline)) {  // first key of the i-th tile
+    return k_lo + (t_hi - 1 - i) * kTile;
+  };
+  const int first_key = k_lo + t_lo * kTile;
   auto id_of = [&](int i) __attribute__((always_inline)) -> int64_t {
-    return table[min(k_lo + i * kTile + 16 * w, k_hi - 1) >> bs_log2];
+    return table[min(max(key_of(i) + 16 * w, 0), k_hi - 1) >> bs_log2];
   };
   auto span_of = [&](int i, int64_t id) __attribute__((always_inline)) -> Span {
-    const int key = k_lo + i * kTile + 16 * w;
-    const bool ok = i < t_hi && key < k_hi && id >= 0 && id < p.num_blocks;
+    const int key = key_of(i) + 16 * w;
+    const bool ok = key >= first_key && key < k_hi && id >= 0 && id < p.num_blocks;
     Span x;
     x.bytes = ok ? static_cast<uint32_t>(min(k_hi - key, 16) - 1) * row_bytes + 2 * p.d : 0u;
     x.at = ok ? static_cast<uint64_t>(id) * block_bytes +
@@ -332,12 +368,12 @@ void scored_tiles_kernel(ScoredParams p) {
       __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (lds_void_t *)(dst + 1024 * c), 16, off, 0, 0, 0);
     }
   };
-  // One bit per run of 16 keys of tile i whose block is out of range.
-  auto bad_of = [&](int i) __attribute__((always_inline)) -> uint32_t {
+  // One bit per run of 16 keys from key0 on whose block is out of range.
+  auto bad_of = [&](int key0) __attribute__((always_inline)) -> uint32_t {
     uint32_t bad = 0;
 #pragma unroll
     for (int b = 0; b < 4; ++b) {
-      const int64_t id = table[min(k_lo + i * kTile + 16 * b, k_hi - 1) >> bs_log2];
+      const int64_t id = table[min(key0 + 16 * b, k_hi - 1) >> bs_log2];
       if (id < 0 || id >= p.num_blocks) bad |= 1u << b;
     }
     return bad;
@@ -366,77 +402,56 @@ void scored_tiles_kernel(ScoredParams p) {
   // A wave waits for its own copies of the phase before, the barrier for all.
   f32x16_t s[KB];
   uint32_t pk[KB][8];
-  bool masked = false;  // whether some row of the wave does not see some key of the tile
   auto active = [&](int i) __attribute__((always_inline)) {
-    return t_lo + i < t_hi && k_lo + (t_lo + i) * kTile < any;
+    const int key0 = key_of(i);
+    return key0 >= first_key && key0 < any;
   };
-  auto add_values = [&](int i, const unsigned char *vt) __attribute__((always_inline)) {
-    // Where some row does not see some key, a V that is not finite would reach
-    // it as 0 * V: such tiles are looked through, a lane per key.
-    uint64_t odd = 0;
-    if (masked) {
-      uint32_t bits = 0;
-      int key = lane;
-      asm volatile("" : "+v"(key));
-#pragma unroll 2
-      for (int c = 0; c < kChunks; ++c) {
-        const uint4 x = *reinterpret_cast<const uint4 *>(vt + key * kRowB +
-                                                         16 * ((c + key) & (kChunks - 1)));
-        bits |= W::odd(x.x) | W::odd(x.y) | W::odd(x.z) | W::odd(x.w);
+  auto add_values = [&](const unsigned char *vt) __attribute__((always_inline)) {
+    int vo = voff0;
+    asm volatile("" : "+v"(vo));
+#pragma unroll
+    for (int kb = 0; kb < 2 * KB; ++kb) {
+      const uint32_t *x = &pk[kb >> 1][4 * (kb & 1)];
+      const v8 pb = __builtin_bit_cast(v8, make_uint4(x[0], x[1], x[2], x[3]));
+#pragma unroll
+      for (int n = 0; n < NB; ++n) {
+        const uint2 lo = __builtin_bit_cast(
+            uint2, __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+                       (lds_s16x4_t *)(vt + 16 * kb * kRowB + (vo ^ (n << 6)))));
+        const uint2 hi = __builtin_bit_cast(
+            uint2, __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+                       (lds_s16x4_t *)(vt + 16 * kb * kRowB + ((vo ^ 16 ^ (n << 6)) + 8 * kRowB))));
+        acc[n] = W::mfma(__builtin_bit_cast(v8, make_uint4(lo.x, lo.y, hi.x, hi.y)), pb, acc[n]);
       }
-      odd = __ballot((bits & 0x80008000u) != 0);
     }
-    if (odd == 0) {
-      int vo = voff0;
-      asm volatile("" : "+v"(vo));
+    // Two MFMAs' V reads ahead of the MFMAs.
+    constexpr int kMfma = 2 * KB * NB;
+    __builtin_amdgcn_sched_group_barrier(0x100, 4, 0);
 #pragma unroll
-      for (int kb = 0; kb < 2 * KB; ++kb) {
-        const uint32_t *x = &pk[kb >> 1][4 * (kb & 1)];
-        const v8 pb = __builtin_bit_cast(v8, make_uint4(x[0], x[1], x[2], x[3]));
-#pragma unroll
-        for (int n = 0; n < NB; ++n) {
-          const uint2 lo = __builtin_bit_cast(
-              uint2, __builtin_amdgcn_ds_read_tr16_b64_v4i16(
-                         (lds_s16x4_t *)(vt + 16 * kb * kRowB + (vo ^ (n << 6)))));
-          const uint2 hi = __builtin_bit_cast(
-              uint2, __builtin_amdgcn_ds_read_tr16_b64_v4i16(
-                         (lds_s16x4_t *)(vt + 16 * kb * kRowB + ((vo ^ 16 ^ (n << 6)) + 8 * kRowB))));
-          acc[n] = W::mfma(__builtin_bit_cast(v8, make_uint4(lo.x, lo.y, hi.x, hi.y)), pb, acc[n]);
-        }
-      }
-      // Two MFMAs' V reads ahead of the MFMAs.
-      constexpr int kMfma = 2 * KB * NB;
-      __builtin_amdgcn_sched_group_barrier(0x100, 4, 0);
-#pragma unroll
-      for (int x = 0; x < kMfma - 2; ++x) {
-        __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
-        __builtin_amdgcn_sched_group_barrier(0x100, 2, 0);
-      }
-      __builtin_amdgcn_sched_group_barrier(0x008, 2, 0);
-    } else {
-      // Key by key, each row adding only what it sees. acc[n][4 g + e] is
-      // element 32 n + 8 g + 4 hh + e of the row.
-      const int lim = min(limit, k_hi) - (k_lo + (t_lo + i) * kTile);
-      for (int k = 0; k < kTile; ++k) {
-        uint32_t mine = 0;  // the lane's pair of registers for keys k and k ^ 4
-#pragma unroll
-        for (int j = 0; j < KB; ++j)
-#pragma unroll
-          for (int x = 0; x < 8; ++x)
-            if ((k & ~5) == 32 * j + 8 * (x >> 1) + 2 * (x & 1)) mine = pk[j][x];
-        const uint32_t both = __shfl(mine, m32 + 8 * (k & 4));
-        const uint16_t one = static_cast<uint16_t>(k & 1 ? both >> 16 : both);
-        const float pr = Elem<T>::to_f32(T{one});
-        if (k >= lim) continue;
-#pragma unroll
-        for (int n = 0; n < NB; ++n)
-#pragma unroll
-          for (int g = 0; g < 4; ++g) {
-            const uint16_t *x = reinterpret_cast<const uint16_t *>(
-                vt + k * kRowB + 16 * ((4 * n + g) ^ swizzle<D>(k)) + 8 * hh);
-#pragma unroll
-            for (int e = 0; e < 4; ++e) acc[n][4 * g + e] += pr * Elem<T>::to_f32(T{x[e]});
-          }
+    for (int x = 0; x < kMfma - 2; ++x) {
+      __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+      __builtin_amdgcn_sched_group_barrier(0x100, 2, 0);
+    }
+    __builtin_amdgcn_sched_group_barrier(0x008, 2, 0);
+  };
+  // Where some row does not see some key, a V that is not finite would reach
+  // it as 0 * V. So in such tiles each wave looks through the 16 rows that it has
+  // copied, turns what is not finite to zeros, and notes that the item has met
+  // such values; they are given to the rows that see them after the loop.
+  auto clean = [&](unsigned char *vt) __attribute__((always_inline)) {
+#pragma unroll 1
+    for (int c = 0; c < kCopies; ++c) {
+      uint4 *at = reinterpret_cast<uint4 *>(vt + 16 * w * kRowB + 1024 * c) + lane;
+      uint4 x = *at;
+      const uint4 o = make_uint4(W::odd(x.x), W::odd(x.y), W::odd(x.z), W::odd(x.w));
+      if ((o.x | o.y | o.z | o.w) != 0) {
+        // A flag in bit 15 of a half to ones all over that half.
+        x.x &= ~((o.x >> 15) * 0xffffu);
+        x.y &= ~((o.y >> 15) * 0xffffu);
+        x.z &= ~((o.z >> 15) * 0xffffu);
+        x.w &= ~((o.w >> 15) * 0xffffu);
+        *at = x;
+        s_odd = 1;
       }
     }
   };
@@ -462,9 +477,9 @@ void scored_tiles_kernel(ScoredParams p) {
     __builtin_amdgcn_sched_group_barrier(0x008, 2, 0);
   };
   auto weigh = [&](int i) __attribute__((always_inline)) {
-    const int key0 = k_lo + (t_lo + i) * kTile;
-    const uint32_t bad = strange ? bad_of(t_lo + i) : 0u;
-    masked = key0 + kTile > all || key0 + kTile > k_hi || bad != 0;
+    const int key0 = key_of(i);
+    const uint32_t bad = strange ? bad_of(key0) : 0u;
+    const bool masked = key0 + kTile > all || key0 + kTile > k_hi || bad != 0;
 
     // Scores relative to m.
     if constexpr (kCap) {
@@ -473,7 +488,15 @@ void scored_tiles_kernel(ScoredParams p) {
       for (int j = 0; j < KB; ++j)
 #pragma unroll
         for (int e = 0; e < 16; e += 2) big = max3(big, fabsf(s[j][e]), fabsf(s[j][e + 1]));
-      if (__any(!(big <= near))) {
+      if (!__any(!(big <= near2))) {
+#pragma unroll
+        for (int j = 0; j < KB; ++j)
+#pragma unroll
+          for (int e = 0; e < 16; ++e) {
+            const float x = s[j][e], u = x * x;
+            s[j][e] = fmaf(x, fmaf(u, fmaf(u, a2, a1), a0), -m);
+          }
+      } else if (__any(!(big <= near))) {
 #pragma unroll
         for (int j = 0; j < KB; ++j)
 #pragma unroll
@@ -526,15 +549,14 @@ void scored_tiles_kernel(ScoredParams p) {
     const float rel = pair_max(__builtin_elementwise_maximum(
         max3(mc[0], mc[1], mc[2]), mc[3]));
     if (__any(rel > thr)) {
+      // Rows below their threshold keep m: a factor of 1. A row without a key so
+      // far has sums of 0, whatever the factor.
       const bool move = rel > thr;
       const float shift = move ? rel : 0.f;
-      const float fall = thr < 0.f ? 0.f : __builtin_amdgcn_exp2f(-shift);
-      // A row without a key so far has nothing to scale.
-      l = move ? l * fall : l;
+      const float fall = move && thr > 0.f ? __builtin_amdgcn_exp2f(-shift) : 1.f;
+      l *= fall;
 #pragma unroll
-      for (int n = 0; n < NB; ++n)
-#pragma unroll
-        for (int e = 0; e < 16; ++e) acc[n][e] = move ? acc[n][e] * fall : acc[n][e];
+      for (int n = 0; n < NB; ++n) acc[n] *= fall;
       m += shift;
       if (move) thr = kLazy;
 #pragma unroll
@@ -552,12 +574,10 @@ void scored_tiles_kernel(ScoredParams p) {
       }
     l += (lsum[0] + lsum[1]) + (lsum[2] + lsum[3]);
 
-    if constexpr (KB == 2) {
 #pragma unroll
-      for (int j = 0; j < KB; ++j)
+    for (int j = 0; j < KB; ++j)
 #pragma unroll
-        for (int x = 0; x < 8; ++x) pk[j][x] = pack2<T>(s[j][2 * x], s[j][2 * x + 1]);
-    }
+      for (int x = 0; x < 8; ++x) pk[j][x] = pack2<T>(s[j][2 * x], s[j][2 * x + 1]);
   };
   // s_waitcnt: all but the newest batch of copies, and LDS; LDS and scalars alone.
   constexpr int kBatch = 2 * kCopies;
@@ -567,26 +587,29 @@ void scored_tiles_kernel(ScoredParams p) {
   int64_t id = 0;
   auto m_phase = [&](int i, const unsigned char *kt, const unsigned char *vt)
       __attribute__((always_inline)) {
-    const int64_t id3 = id_of(t_lo + i + 3);
+    const int64_t id3 = id_of(i + 3);
     __builtin_amdgcn_s_setprio(3);
-    if (i >= 1 && active(i - 1)) add_values(i - 1, vt);
+    if (i >= 1 && active(i - 1)) add_values(vt);
     __builtin_amdgcn_sched_barrier(0);
     if (active(i)) {
       scores(kt);
     } else {  // defined in every phase, so that it lives over none
 #pragma unroll
-      for (int j = 0; j < KB; ++j) s[j] = f32x16_t{};
+      for (int j = 0; j < KB; ++j) asm volatile("" : "=v"(s[j]));
     }
     __builtin_amdgcn_s_setprio(0);
     next_v = next_k;
-    next_k = span_of(t_lo + i + 2, id);
+    next_k = span_of(i + 2, id);
     id = id3;
     asm volatile("" ::: "memory");
     __builtin_amdgcn_s_waitcnt(kWaitLds);
     __builtin_amdgcn_s_barrier();
     asm volatile("" ::: "memory");
   };
-  auto v_phase = [&](int i, unsigned char *kt, unsigned char *vt) __attribute__((always_inline)) {
+  // vt: the stage of V_{i+1}; vi: that of V_i, which has landed when the copies
+  // of this phase are the only ones left.
+  auto v_phase = [&](int i, unsigned char *kt, unsigned char *vt, unsigned char *vi)
+      __attribute__((always_inline)) {
     copy(next_k, p.k, kt);
     copy(next_v, p.v, vt);
     if (active(i)) {
@@ -595,18 +618,22 @@ void scored_tiles_kernel(ScoredParams p) {
 #pragma unroll
       for (int j = 0; j < KB; ++j)
 #pragma unroll
-        for (int x = 0; x < 8; ++x) pk[j][x] = 0;
+        for (int x = 0; x < 8; ++x) asm volatile("" : "=v"(pk[j][x]));
     }
     asm volatile("" ::: "memory");
     __builtin_amdgcn_s_waitcnt(kWaitBatch);
+    if (key_of(i) + kTile > unit_all) {  // uniform
+      clean(vi);
+      __builtin_amdgcn_s_waitcnt(kWaitBatch);
+    }
     __builtin_amdgcn_s_barrier();
     asm volatile("" ::: "memory");
   };
   if (chunk > 0) {  // uniform: without keys the table is not read
-    const int64_t id0 = id_of(t_lo), id1 = id_of(t_lo + 1);
-    id = id_of(t_lo + 2);
-    const Span first = span_of(t_lo, id0);
-    next_k = span_of(t_lo + 1, id1);
+    const int64_t id0 = id_of(0), id1 = id_of(1);
+    id = id_of(2);
+    const Span first = span_of(0, id0);
+    next_k = span_of(1, id1);
     copy(first, p.k, ks0[half]);
     copy(first, p.v, vs0[half]);
     copy(next_k, p.k, ks1[half]);
@@ -617,13 +644,31 @@ void scored_tiles_kernel(ScoredParams p) {
     asm volatile("" ::: "memory");
     for (int i = 0; i < chunk; i += 2) {
       m_phase(i, ks0[half], vs1[half]);
-      v_phase(i, ks0[half], vs1[half]);
+      v_phase(i, ks0[half], vs1[half], vs0[half]);
       m_phase(i + 1, ks1[half], vs0[half]);
-      v_phase(i + 1, ks1[half], vs0[half]);
+      v_phase(i + 1, ks1[half], vs0[half], vs1[half]);
     }
     // The last tile's values; an odd count had them in the phase past its end.
     if ((chunk & 1) == 0) m_phase(chunk, ks0[half], vs1[half]);
     if (half == 0) __builtin_amdgcn_s_barrier();
+    __syncthreads();
+    if (s_odd) {  // rare: values that are not finite, for the rows that see them
+      const int end = min(k_hi, k_lo + t_hi * kTile);
+      for (int k = max(first_key, (unit_all - k_lo) / kTile * kTile + k_lo); k < end; ++k) {
+        const int64_t block = table[k >> bs_log2];
+        if (block < 0 || block >= p.num_blocks || k >= limit) continue;
+        const uint16_t *v = static_cast<const uint16_t *>(p.v) +
+                            ((block << bs_log2) + (k & bs_mask)) * (row_bytes / 2) + kv_bytes / 2;
+#pragma unroll
+        for (int n = 0; n < NB; ++n)
+#pragma unroll
+          for (int e = 0; e < 16; ++e) {
+            const int dim = 32 * n + 8 * (e >> 2) + 4 * hh + (e & 3);
+            const float x = dim < p.d ? Elem<T>::to_f32(T{v[dim]}) : 0.f;
+            if (!__builtin_isfinite(x)) acc[n][e] += x;
+          }
+      }
+    }
   }
   l = pair_sum(l);
   if (thr < 0.f) m = -INFINITY;
