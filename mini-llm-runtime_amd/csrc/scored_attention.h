@@ -18,6 +18,7 @@ enum ScoredMode {
   kModePrefill = 0,  // packed chunks, causal, prefixes seen ahead
   kModeDecode = 1,   // one token a sequence
   kModePrefix = 2,   // one token a sequence, the keys [0, prefix) of one table
+  kModeShared = 3,   // units of kModePrefix, then one unit per sequence of kModeDecode
 };
 
 constexpr int kMinSplit = 128;  // keys of the shortest split
@@ -31,7 +32,10 @@ struct ScoredParams {
   int64_t bt_st, bt_width;
   int seqs, tiles;         // sequences; units of a sequence (kModePrefix: of the call)
   int64_t total_q;         // rows of q
-  int64_t start;           // first key (kModeDecode), number of keys (kModePrefix)
+  int64_t start;           // first key (kModeDecode), number of keys (kModePrefix), both
+  const int64_t *prefix;   // kModePrefix, kModeShared: the prefix's table
+  int64_t prefix_width;
+  int prefix_units;        // kModeShared: units over the prefix
   float scale, cap;
   const float *slopes;
   void *out;
@@ -54,7 +58,12 @@ struct Unit {
   int64_t lo, hi;  // keys [lo, hi) that some row sees
   int rows, r0;    // rows of the sequence; first of the unit
   int seq;
+  bool prefix;     // over the shared prefix: keys by its table, rows of all sequences
 };
+
+__device__ __forceinline__ const int64_t *table_of(const ScoredParams &p, const Unit &t) {
+  return t.prefix ? p.prefix : p.bt + t.seq * p.bt_st;
+}
 
 __device__ __forceinline__ int64_t clamp64(int64_t x, int64_t lo, int64_t hi) {
   return x < lo ? lo : x > hi ? hi : x;
@@ -62,7 +71,11 @@ __device__ __forceinline__ int64_t clamp64(int64_t x, int64_t lo, int64_t hi) {
 
 __device__ __forceinline__ Unit unit_of(const ScoredParams &p, int u, int kRows) {
   Unit t;
-  t.seq = p.mode == kModePrefix ? 0 : u / p.tiles;
+  const bool prefix =
+      p.mode == kModePrefix || (p.mode == kModeShared && u < p.prefix_units);
+  t.prefix = prefix;
+  if (p.mode == kModeShared && !prefix) u -= p.prefix_units;
+  t.seq = prefix ? 0 : u / p.tiles;
   t.r0 = (u - t.seq * p.tiles) * kRows;
   const int64_t covered = p.bt_width * p.block_size;
   t.pos0 = t.ahead = 0;
@@ -83,7 +96,7 @@ __device__ __forceinline__ Unit unit_of(const ScoredParams &p, int u, int kRows)
       if (t.hi < t.ahead) t.hi = t.ahead;
       if (t.hi < 0) t.hi = 0;
     }
-  } else if (p.mode == kModeDecode) {
+  } else if (!prefix) {
     t.q0 = t.seq;
     t.ctx = clamp64(p.ctx[t.seq], 0, covered);
     t.rows = p.group;
@@ -93,7 +106,8 @@ __device__ __forceinline__ Unit unit_of(const ScoredParams &p, int u, int kRows)
     t.q0 = 0;
     t.ctx = 0;
     t.rows = p.seqs * p.group;
-    t.hi = p.start < covered ? p.start : covered;
+    const int64_t most = p.prefix_width * p.block_size;
+    t.hi = p.start < most ? p.start : most;
   }
   return t;
 }

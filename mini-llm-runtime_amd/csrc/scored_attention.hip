@@ -10,25 +10,31 @@ namespace {
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr int kRows = 16;
 
-// out = sum_i 2^{m_i - M} O_i / sum_i 2^{m_i - M} l_i over a row's items, those
-// of `p` and, for a shared prefix, of `x` too. One workgroup per 16 rows of a
-// (unit of p, KV head), 16 threads per row; items are added in their order. A
-// unit that has written its result itself is left alone.
+// out = sum_i e^{m_i - M} O_i / sum_i e^{m_i - M} l_i over a row's items: those
+// of its unit u0 + u of `p` and, over a shared prefix, those of `x` too. One wave
+// per row, 16 lanes side by side over its elements, four groups of lanes dealing
+// the items among them, the groups' sums joined in a fixed order. A unit that has
+// written its result itself is left alone. Rows from `used` on of a unit do not exist. Bound by latency: the row's m and l,
+// then its sums, are each read in a few rounds.
 template <typename T, int D>
-__global__ __launch_bounds__(256) void scored_merge(ScoredParams p, int p_rows, ScoredParams x,
-                                                    int x_rows, bool prefixed) {
+__global__ __launch_bounds__(256) void scored_merge(ScoredParams p, int u0, int p_rows, int used,
+                                                    ScoredParams x, int x_rows, bool prefixed) {
   constexpr int kVe = D / 16;
-  const int slices = p_rows / kRows, slice = blockIdx.x % slices, uk = blockIdx.x / slices;
-  const int u = uk / p.hkv, kvh = uk - u * p.hkv;
+  const int lane = threadIdx.x & 63;
+  const int slot = blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int uk = slot / used, rr = slot - uk * used;
+  const int u = u0 + uk / p.hkv, kvh = uk - uk / p.hkv * p.hkv;
+  if (u >= p.units) return;
   const int first = p.first[u], count = p.first[u + 1] - first;
   if (count == 0 || (count == 1 && !p.force_partial)) return;
   const Unit t = unit_of(p, u, p_rows);
-  const int rr = slice * kRows + (threadIdx.x >> 4), d0 = (threadIdx.x & 15) * kVe;
   const int r = t.r0 + rr;
   if (r >= t.rows) return;
+  const int d0 = (lane & 15) * kVe, group = lane >> 4;
   const int tok = r / p.group, g = r - tok * p.group;
   // Items of the row: `count` from p, then `more` from x.
-  int64_t at = (static_cast<int64_t>(first) * p.hkv + kvh) * p_rows + rr, x_at = 0;
+  const int64_t at = (static_cast<int64_t>(first) * p.hkv + kvh) * p_rows + rr;
+  int64_t x_at = 0;
   int more = 0;
   if (prefixed) {
     const int xr = t.seq * p.group + g;
@@ -40,10 +46,9 @@ __global__ __launch_bounds__(256) void scored_merge(ScoredParams p, int p_rows, 
   const int64_t step = static_cast<int64_t>(p.hkv) * p_rows;
   const int64_t x_step = static_cast<int64_t>(p.hkv) * x_rows;
   float m = -INFINITY;
-  for (int i = threadIdx.x & 15; i < count; i += 16) m = fmaxf(m, p.ml[2 * (at + i * step)]);
-  for (int i = threadIdx.x & 15; i < more; i += 16) m = fmaxf(m, x.ml[2 * (x_at + i * x_step)]);
-#pragma unroll
-  for (int o = 8; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor(m, o));
+  for (int i = lane; i < count; i += 64) m = fmaxf(m, p.ml[2 * (at + i * step)]);
+  for (int i = lane; i < more; i += 64) m = fmaxf(m, x.ml[2 * (x_at + i * x_step)]);
+  m = wave_max(m);
   const float ref = m == -INFINITY ? 0.f : m;
   float sum = 0.f, acc[kVe];
 #pragma unroll
@@ -60,10 +65,18 @@ __global__ __launch_bounds__(256) void scored_merge(ScoredParams p, int p_rows, 
       acc[n + 3] += v.w * f;
     }
   };
-#pragma unroll 4
-  for (int i = 0; i < count; ++i) add(p, at + i * step);
-#pragma unroll 4
-  for (int i = 0; i < more; ++i) add(x, x_at + i * x_step);
+#pragma unroll 8
+  for (int i = group; i < count; i += 4) add(p, at + i * step);
+#pragma unroll 8
+  for (int i = group; i < more; i += 4) add(x, x_at + i * x_step);
+  auto join = [](float v) {
+    v += __shfl_xor(v, 16);
+    return v + __shfl_xor(v, 32);
+  };
+  sum = join(sum);
+#pragma unroll
+  for (int n = 0; n < kVe; ++n) acc[n] = join(acc[n]);
+  if (group != 0) return;
   const float inv = sum > 0.f ? 1.f / sum : sum == 0.f ? 0.f : sum;
   T *dst = static_cast<T *>(p.out) + (t.q0 + tok) * p.o_st + (kvh * p.group + g) * p.o_sh;
 #pragma unroll
@@ -71,12 +84,16 @@ __global__ __launch_bounds__(256) void scored_merge(ScoredParams p, int p_rows, 
     if (d0 + n < p.d) dst[d0 + n] = Elem<T>::from_f32(acc[n] * inv);
 }
 
-int launch_merge(const ScoredParams &p, int p_rows, const ScoredParams &x, int x_rows,
+int launch_merge(const ScoredParams &p, int u0, int p_rows, const ScoredParams &x, int x_rows,
                  bool prefixed, int dtype, hipStream_t stream) {
-  const unsigned grid = static_cast<unsigned>(p.units) * p.hkv * (p_rows / kRows);
-#define MLR_MERGE(T)                                                                            \
-  if (p.d > 64) scored_merge<T, 128><<<grid, 256, 0, stream>>>(p, p_rows, x, x_rows, prefixed); \
-  else scored_merge<T, 64><<<grid, 256, 0, stream>>>(p, p_rows, x, x_rows, prefixed)
+  const int used = p.mode == kModePrefill ? p_rows : std::min(p_rows, p.group);
+  const unsigned grid =
+      static_cast<unsigned>(ceil_div(static_cast<int64_t>(p.units - u0) * p.hkv * used, 4));
+#define MLR_MERGE(T)                                                                         \
+  if (p.d > 64)                                                                              \
+    scored_merge<T, 128><<<grid, 256, 0, stream>>>(p, u0, p_rows, used, x, x_rows, prefixed);      \
+  else                                                                                       \
+    scored_merge<T, 64><<<grid, 256, 0, stream>>>(p, u0, p_rows, used, x, x_rows, prefixed)
   if (dtype == MLR_DTYPE_F32) {
     MLR_MERGE(float);
   } else if (dtype == MLR_DTYPE_F16) {
@@ -134,7 +151,24 @@ bool takes_tiles(int64_t rows, int64_t block_size, int64_t hkv, int64_t d, int d
          block_size < (int64_t(1) << 30) / (hkv * d);  // 32-bit offsets inside a block
 }
 
-int64_t prefix_target(int64_t rows) { return rows == kTileRows ? cus() : target_items(); }
+// A shared prefix on the kernel of 128 rows a unit, with each request's own keys
+// (all heads of a group in one unit) in the same launch. At head sizes above 64
+// that kernel's stages take a whole CU, so a request's few keys would hold one
+// each; there the requests' own keys go to the other kernel.
+bool shares_tiles(int64_t batch, int64_t group, int64_t block_size, int64_t hkv, int64_t d,
+                  int dtype) {
+  return d <= 64 && group <= kTileRows && takes_tiles(batch * group, block_size, hkv, d, dtype);
+}
+// Two workgroups fit a CU; the last split of each unit is half full on average, and
+// a second round of workgroups would cost more than longer splits.
+int64_t shared_target(int64_t units, int64_t hkv) {
+  const int64_t slots = 2 * static_cast<int64_t>(cus());
+  return std::max(slots / 2, slots - units * hkv / 2);
+}
+// For a prefix alone: items of equal length, one for each CU at most.
+int64_t prefix_target(int64_t units, int64_t hkv) {
+  return std::max<int64_t>(1, cus() / (units * hkv)) * units * hkv;
+}
 
 // A prefill's rows per unit, units, items, and whether units stay whole: with a
 // unit for every CU there is nothing to gain from splits, which cost a pass over
@@ -187,8 +221,8 @@ int check_operands(const Operands &o) {
   MLR_REQUIRE(head_dim_ok(o.d, o.dtype),
               "%s: head_dim must be a multiple of %d up to 128, got %lld", w,
               o.dtype == MLR_DTYPE_F32 ? 4 : 8, static_cast<long long>(o.d));
-  MLR_REQUIRE(o.num_blocks > 0 && o.block_size > 0 && o.bt_width >= 0,
-              "%s: the cache needs blocks of a positive size", w);
+  MLR_REQUIRE(o.num_blocks > 0 && o.num_blocks < (int64_t(1) << 31) && o.block_size > 0 && o.bt_width >= 0,
+              "%s: the cache needs fewer than 2^31 blocks of a positive size", w);
   MLR_REQUIRE(o.bt_width < (int64_t(1) << 31) / o.block_size,
               "%s: a block table must cover fewer than 2^31 positions", w);
   // A cap so small that its inverse is infinite would make NaN of scores of 0.
@@ -279,7 +313,7 @@ extern "C" int mlr_paged_decode_scored(
   if (need) place_parts(p, static_cast<char *>(workspace), items, kRows);
   hipStream_t s = static_cast<hipStream_t>(stream);
   if (const int rc = launch_scored_rows(p, dtype, grid_of(items), s)) return rc;
-  return need ? launch_merge(p, kRows, p, kRows, false, dtype, s) : MLR_OK;
+  return need ? launch_merge(p, 0, kRows, p, kRows, false, dtype, s) : MLR_OK;
 }
 
 extern "C" size_t mlr_paged_prefill_scored_workspace_size(int64_t num_seqs, int64_t max_query_len,
@@ -343,7 +377,7 @@ extern "C" int mlr_paged_prefill_scored(
                      ? launch_scored_tiles(p, dtype, static_cast<unsigned>(n.items), s)
                      : launch_scored_rows(p, dtype, grid_of(n.items), s);
   if (rc) return rc;
-  return n.parts ? launch_merge(p, rows, p, rows, false, dtype, s) : MLR_OK;
+  return n.parts ? launch_merge(p, 0, rows, p, rows, false, dtype, s) : MLR_OK;
 }
 
 extern "C" size_t mlr_paged_decode_shared_prefix_workspace_size(
@@ -351,14 +385,19 @@ extern "C" size_t mlr_paged_decode_shared_prefix_workspace_size(
     int64_t max_blocks, int64_t block_size, int dtype) {
   if (batch <= 0 || num_kv_heads <= 0 || num_q_heads <= 0 || head_dim <= 0 || block_size <= 0)
     return 0;
-  const int64_t group = num_q_heads / num_kv_heads, target = target_items();
+  const int64_t group = num_q_heads / num_kv_heads, max_keys = max_blocks * block_size;
+  if (shares_tiles(batch, group, block_size, num_kv_heads, head_dim, dtype)) {
+    const int64_t units = prefix_units(batch, group, kTileRows) + batch;
+    return part_bytes(units, max_items(units, num_kv_heads, std::max(prefix_len, max_keys),
+                                       shared_target(units, num_kv_heads)), kTileRows, head_dim);
+  }
   const int64_t rows =
       takes_tiles(batch * group, block_size, num_kv_heads, head_dim, dtype) ? kTileRows : kRows;
   const int64_t own = decode_units(batch, group), over = prefix_units(batch, group, rows);
-  return part_bytes(own, max_items(own, num_kv_heads, max_blocks * block_size, target), kRows,
-                    head_dim) +
-         part_bytes(over, max_items(over, num_kv_heads, prefix_len, prefix_target(rows)), rows,
-                    head_dim);
+  const int64_t target =
+      rows == kTileRows ? prefix_target(over, num_kv_heads) : target_items();
+  return part_bytes(own, max_items(own, num_kv_heads, max_keys, target_items()), kRows, head_dim) +
+         part_bytes(over, max_items(over, num_kv_heads, prefix_len, target), rows, head_dim);
 }
 
 extern "C" int mlr_paged_decode_shared_prefix(
@@ -389,29 +428,44 @@ extern "C" int mlr_paged_decode_shared_prefix(
   MLR_REQUIRE(workspace && workspace_bytes >= need,
               "mlr_paged_decode_shared_prefix: workspace of %zu bytes, %zu needed",
               workspace_bytes, need);
+  hipStream_t s = static_cast<hipStream_t>(stream);
+  const int64_t group = num_q_heads / num_kv_heads;
+  if (shares_tiles(batch, group, block_size, num_kv_heads, head_dim, dtype)) {
+    ScoredParams p = params_of(o, kModeShared);
+    p.prefix = prefix_table;
+    p.prefix_width = prefix_blocks;
+    p.prefix_units = static_cast<int>(prefix_units(batch, group, kTileRows));
+    p.tiles = 1;
+    p.units = static_cast<int>(p.prefix_units + batch);
+    p.start = prefix_len;
+    p.force_partial = true;
+    p.target = shared_target(p.units, p.hkv);
+    const int64_t items = max_items(p.units, p.hkv, std::max(prefix_len, max_keys), p.target);
+    place_parts(p, static_cast<char *>(workspace), items, kTileRows);
+    if (const int rc = launch_scored_tiles(p, dtype, static_cast<unsigned>(items), s)) return rc;
+    return launch_merge(p, p.prefix_units, kTileRows, p, kTileRows, true, dtype, s);
+  }
   ScoredParams own = params_of(o, kModeDecode);
-  own.tiles = static_cast<int>(ceil_div(own.group, kRows));
-  own.units = static_cast<int>(decode_units(batch, own.group));
+  own.tiles = static_cast<int>(ceil_div(group, kRows));
+  own.units = static_cast<int>(decode_units(batch, group));
   own.start = prefix_len;
   own.force_partial = true;
   const int64_t own_items = max_items(own.units, own.hkv, max_keys, own.target);
   char *ws = place_parts(own, static_cast<char *>(workspace), own_items, kRows);
   ScoredParams over = params_of(o, kModePrefix);
-  const bool tiles = takes_tiles(batch * over.group, block_size, over.hkv, over.d, dtype);
+  over.prefix = prefix_table;
+  over.prefix_width = prefix_blocks;
+  const bool tiles = takes_tiles(batch * group, block_size, over.hkv, over.d, dtype);
   const int rows = tiles ? kTileRows : kRows;
-  over.bt = prefix_table;
-  over.bt_st = 0;
-  over.bt_width = prefix_blocks;
-  over.units = over.tiles = static_cast<int>(prefix_units(batch, over.group, rows));
+  over.units = over.tiles = static_cast<int>(prefix_units(batch, group, rows));
   over.start = prefix_len;
   over.force_partial = true;
-  over.target = prefix_target(rows);
+  if (tiles) over.target = prefix_target(over.units, over.hkv);
   const int64_t over_items = max_items(over.units, over.hkv, prefix_len, over.target);
   place_parts(over, ws, over_items, rows);
-  hipStream_t s = static_cast<hipStream_t>(stream);
   const int rc = tiles ? launch_scored_tiles(over, dtype, static_cast<unsigned>(over_items), s)
                        : launch_scored_rows(over, dtype, grid_of(over_items), s);
   if (rc) return rc;
   if (const int rc2 = launch_scored_rows(own, dtype, grid_of(own_items), s)) return rc2;
-  return launch_merge(own, kRows, over, rows, true, dtype, s);
+  return launch_merge(own, 0, kRows, over, rows, true, dtype, s);
 }

@@ -278,7 +278,7 @@ __global__ __launch_bounds__(256) void scored_rows_kernel(ScoredParams p) {
     if (kPrefill) {
       pos = t.pos0 + tok;
       limit = max(pos + 1, t.ahead);
-    } else if (p.mode == kModePrefix) {
+    } else if (t.prefix) {
       // A request shorter than the prefix sees its own first positions.
       pos = p.ctx[row] - 1;
       limit = min(limit, pos + 1);
@@ -295,8 +295,8 @@ __global__ __launch_bounds__(256) void scored_rows_kernel(ScoredParams p) {
     }
 
     Rows<T, D, kPaged16> src{p, static_cast<const T *>(p.k), static_cast<const T *>(p.v),
-                             p.bt + (p.mode == kModePrefix ? 0 : t.seq * p.bt_st),
-                             p.bt_width * p.block_size, m16, g, kvh};
+                             table_of(p, t),
+                             (t.prefix ? p.prefix_width : p.bt_width) * p.block_size, m16, g, kvh};
     f32x4_t acc[kVe];
 #pragma unroll
     for (int n = 0; n < kVe; ++n) acc[n] = f32x4_t{0, 0, 0, 0};

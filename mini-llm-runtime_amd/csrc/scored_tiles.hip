@@ -233,7 +233,9 @@ void scored_tiles_kernel(ScoredParams p) {
   const bool alone = s_of == 1 && !p.force_partial;
   const Unit t = unit_of(p, unit, kTileRows);
   if (t.r0 >= t.rows) return;
-  const int k_lo = __builtin_amdgcn_readfirstlane(static_cast<int>(p.whole ? 0 : part * split));
+  const int k_lo =
+      __builtin_amdgcn_readfirstlane(static_cast<int>(unit_base(t) + (p.whole ? 0 : part * split)));
+  const int low = __builtin_amdgcn_readfirstlane(static_cast<int>(t.lo));  // first key seen
   const int k_hi = __builtin_amdgcn_readfirstlane(
       static_cast<int>(min(t.hi, static_cast<int64_t>(k_lo) + split)));
 
@@ -245,8 +247,10 @@ void scored_tiles_kernel(ScoredParams p) {
   const int t_lo = half * chunk, t_hi = min(tiles, t_lo + chunk);
 
   // The lane's row: token, head, position, first key that it does not see.
-  const int r = t.r0 + 32 * w + m32;
-  const bool live = r < t.rows;
+  const int r_first = t.r0 + 32 * w, unit_rows = t.rows;
+  const int64_t q_first = t.q0;
+  const int r = r_first + m32;
+  const bool live = r < unit_rows;
   const int rc = live ? r : t.rows - 1;
   const int tok = rc / p.group, head = kvh * p.group + rc - tok * p.group;
   const int64_t row = t.q0 + tok;
@@ -255,6 +259,7 @@ void scored_tiles_kernel(ScoredParams p) {
     pos = static_cast<int>(t.pos0) + tok;
     limit = max(pos + 1, static_cast<int>(t.ahead));
   } else {
+    // A request shorter than the prefix sees its own first positions.
     const int64_t ctx = clamp64(p.ctx[row], 0, 0x7fffffff);
     pos = static_cast<int>(ctx) - 1;
     limit = static_cast<int>(min(t.hi, ctx));
@@ -316,22 +321,28 @@ void scored_tiles_kernel(ScoredParams p) {
     src_off[i] = 8 * c < p.d ? rr * row_bytes + 16 * c : 0x7fffffffu;
   }
   typedef __attribute__((address_space(4))) const int64_t const_i64;
-  const const_i64 *table =
-      (const const_i64 *)p.bt + (p.mode == kModePrefix ? 0 : static_cast<int64_t>(t.seq) * p.bt_st);
+  const const_i64 *table = (const const_i64 *)table_of(p, t);
   const int bs_log2 = p.bs_log2, bs_mask = (1 << bs_log2) - 1;
-  const uint32_t kv_bytes = static_cast<uint32_t>(kvh) * (2 * p.d);
-  const int64_t block_bytes = static_cast<int64_t>(row_bytes) << bs_log2;
+  const uint32_t head_bytes = 2 * p.d, kv_bytes = static_cast<uint32_t>(kvh) * head_bytes;
+  // Fewer than 2^31 blocks of fewer than 2^31 bytes.
+  const uint32_t block_bytes = row_bytes << bs_log2, blocks = static_cast<uint32_t>(p.num_blocks);
+  auto known = [&](int64_t id) __attribute__((always_inline)) {
+    return static_cast<uint32_t>(static_cast<uint64_t>(id) >> 32) == 0u &&
+           static_cast<uint32_t>(id) < blocks;
+  };
 
   // Whether some block id of the item is out of range (then every tile asks).
   bool strange = false;
   for (int i = (k_lo >> bs_log2) + tid; k_hi > 0 && i <= (k_hi - 1) >> bs_log2; i += kThreads) {
-    const int64_t id = p.bt[(p.mode == kModePrefix ? 0 : static_cast<int64_t>(t.seq) * p.bt_st) + i];
-    strange = strange || id < 0 || id >= p.num_blocks;
+    const int64_t id = table_of(p, t)[i];
+    strange = strange || !known(id);
   }
   if (lane == 0) atomicMin(&s_all, all);
   strange = __syncthreads_or(strange);
-  // Tiles from this key on are hidden from some row of the unit in part.
-  const int unit_all = __builtin_amdgcn_readfirstlane(s_all);
+  // Tiles that start in [low, whole_to] are seen whole by all rows of the wave,
+  // those in [low, unit_to] by all rows of the unit.
+  const int whole_to = min(all, k_hi) - kTile;
+  const int unit_to = __builtin_amdgcn_readfirstlane(s_all) - kTile;
 
   // The wave's 16 rows of tile i: where they start, and how many bytes from there
   // on may be read (rows past k_hi and of blocks out of range arrive as zeros).
@@ -339,21 +350,20 @@ void scored_tiles_kernel(ScoredParams p) {
     uint64_t at;
     uint32_t bytes;
   };
+  const int first_key = k_lo + t_lo * kTile, last_key = k_lo + (t_hi - 1) * kTile;
   auto key_of = [&](int i) __attribute__((always_inline)) {  // first key of the i-th tile
-    return k_lo + (t_hi - 1 - i) * kTile;
+    return last_key - i * kTile;
   };
-  const int first_key = k_lo + t_lo * kTile;
   auto id_of = [&](int i) __attribute__((always_inline)) -> int64_t {
     return table[min(max(key_of(i) + 16 * w, 0), k_hi - 1) >> bs_log2];
   };
   auto span_of = [&](int i, int64_t id) __attribute__((always_inline)) -> Span {
     const int key = key_of(i) + 16 * w;
-    const bool ok = key >= first_key && key < k_hi && id >= 0 && id < p.num_blocks;
+    const bool ok = key >= first_key && key < k_hi && known(id);
     Span x;
-    x.bytes = ok ? static_cast<uint32_t>(min(k_hi - key, 16) - 1) * row_bytes + 2 * p.d : 0u;
-    x.at = ok ? static_cast<uint64_t>(id) * block_bytes +
-                    static_cast<uint32_t>(key & bs_mask) * row_bytes + kv_bytes
-              : 0u;
+    x.bytes = ok ? static_cast<uint32_t>(min(k_hi - key, 16) - 1) * row_bytes + head_bytes : 0u;
+    x.at = static_cast<uint64_t>(ok ? static_cast<uint32_t>(id) : 0u) * block_bytes +
+           (static_cast<uint32_t>(key & bs_mask) * row_bytes + kv_bytes);
     return x;
   };
   auto copy = [&](const Span &x, const void *cache, unsigned char *dst)
@@ -373,8 +383,7 @@ void scored_tiles_kernel(ScoredParams p) {
     uint32_t bad = 0;
 #pragma unroll
     for (int b = 0; b < 4; ++b) {
-      const int64_t id = table[min(key0 + 16 * b, k_hi - 1) >> bs_log2];
-      if (id < 0 || id >= p.num_blocks) bad |= 1u << b;
+      if (!known(table[min(key0 + 16 * b, k_hi - 1) >> bs_log2])) bad |= 1u << b;
     }
     return bad;
   };
@@ -479,7 +488,7 @@ void scored_tiles_kernel(ScoredParams p) {
   auto weigh = [&](int i) __attribute__((always_inline)) {
     const int key0 = key_of(i);
     const uint32_t bad = strange ? bad_of(key0) : 0u;
-    const bool masked = key0 + kTile > all || key0 + kTile > k_hi || bad != 0;
+    const bool masked = key0 > whole_to || key0 < low || bad != 0;
 
     // Scores relative to m.
     if constexpr (kCap) {
@@ -529,14 +538,33 @@ void scored_tiles_kernel(ScoredParams p) {
                          s[j][e]);
     }
     if (masked) {
-      const int lim = min(limit, k_hi) - key0 - 4 * hh;
+      // Key `at` of the tile is seen if at - from < lim - from, unsigned. One
+      // compare and select at a time: 32 compares side by side would take 64
+      // scalar registers, and every uniform value of the loop would be spilled.
+      const int from = max(low - key0 - 4 * hh, -128);
+      const int lim = min(min(limit, k_hi) - key0 - 4 * hh, 128);
+      const uint32_t span = static_cast<uint32_t>(max(lim - from, 0));
+      const float hidden = -INFINITY;
 #pragma unroll
       for (int j = 0; j < KB; ++j)
 #pragma unroll
         for (int e = 0; e < 16; ++e) {
-          const bool gone = bad >> (2 * j + (e >> 3)) & 1;
-          if (gone || 32 * j + 8 * (e >> 2) + (e & 3) >= lim) s[j][e] = -INFINITY;
+          const uint32_t at = 32 * j + 8 * (e >> 2) + (e & 3) - from;
+          float x = s[j][e];
+          asm volatile("v_cmp_lt_u32 vcc, %1, %2\n\tv_cndmask_b32 %0, %3, %0, vcc"
+                       : "+v"(x)
+                       : "v"(at), "v"(span), "v"(hidden)
+                       : "vcc");
+          s[j][e] = x;
         }
+      if (bad != 0) {
+#pragma unroll
+        for (int r = 0; r < 4; ++r)
+          if (bad >> r & 1) {
+#pragma unroll
+            for (int e = 0; e < 8; ++e) s[r >> 1][8 * (r & 1) + e] = hidden;
+          }
+      }
     }
     float mc[4];
 #pragma unroll
@@ -622,7 +650,7 @@ void scored_tiles_kernel(ScoredParams p) {
     }
     asm volatile("" ::: "memory");
     __builtin_amdgcn_s_waitcnt(kWaitBatch);
-    if (key_of(i) + kTile > unit_all) {  // uniform
+    if (key_of(i) > unit_to || key_of(i) < low) {  // uniform
       clean(vi);
       __builtin_amdgcn_s_waitcnt(kWaitBatch);
     }
@@ -654,9 +682,12 @@ void scored_tiles_kernel(ScoredParams p) {
     __syncthreads();
     if (s_odd) {  // rare: values that are not finite, for the rows that see them
       const int end = min(k_hi, k_lo + t_hi * kTile);
-      for (int k = max(first_key, (unit_all - k_lo) / kTile * kTile + k_lo); k < end; ++k) {
+      for (int k = max(first_key, low); k < end; ++k) {
+        // Only tiles that were looked through.
+        const int key0 = k_lo + (k - k_lo) / kTile * kTile;
+        if (key0 <= unit_to && key0 >= low) continue;
         const int64_t block = table[k >> bs_log2];
-        if (block < 0 || block >= p.num_blocks || k >= limit) continue;
+        if (!known(block) || k >= limit) continue;
         const uint16_t *v = static_cast<const uint16_t *>(p.v) +
                             ((block << bs_log2) + (k & bs_mask)) * (row_bytes / 2) + kv_bytes / 2;
 #pragma unroll
@@ -703,12 +734,21 @@ void scored_tiles_kernel(ScoredParams p) {
 #pragma unroll
     for (int e = 0; e < 16; ++e) acc[n][e] = acc[n][e] * f0 + *word(2 + 16 * n + e) * f1;
 
+  // What the end needs of the arguments is read again here, and the row made
+  // again, rather than kept over the loop.
+  typedef const __attribute__((address_space(4))) ScoredParams const_params;
+  const_params *late = (const_params *)__builtin_amdgcn_kernarg_segment_ptr();
+  asm volatile("" : "+s"(late));
+  int lane2 = m32;
+  asm volatile("" : "+v"(lane2));
+  const int r2 = r_first + lane2;
+  if (r2 >= unit_rows) return;
   if (!alone) {
-    const int64_t at = (item * p.hkv + kvh) * kTileRows + 32 * w + m32;
+    const int64_t at = (item * late->hkv + kvh) * kTileRows + 32 * w + lane2;
     if (hh == 0) {
       // Partial results are in units of the natural exponent.
-      p.ml[2 * at] = all_m * 0.6931471805599453f;
-      p.ml[2 * at + 1] = sum;
+      late->ml[2 * at] = all_m * 0.6931471805599453f;
+      late->ml[2 * at + 1] = sum;
     }
 #pragma unroll
     for (int n = 0; n < NB; ++n)
@@ -716,25 +756,23 @@ void scored_tiles_kernel(ScoredParams p) {
       for (int g = 0; g < 4; ++g) {
         const float4 x = make_float4(acc[n][4 * g], acc[n][4 * g + 1], acc[n][4 * g + 2],
                                      acc[n][4 * g + 3]);
-        *reinterpret_cast<float4 *>(p.acc + at * D + 32 * n + 8 * g + 4 * hh) = x;
+        *reinterpret_cast<float4 *>(late->acc + at * D + 32 * n + 8 * g + 4 * hh) = x;
       }
     return;
   }
-  // The row again, rather than kept over the loop.
-  int lane2 = m32;
-  asm volatile("" : "+v"(lane2));
-  const int r2 = t.r0 + 32 * w + lane2;
-  if (r2 >= t.rows) return;
-  const int tok2 = r2 / p.group, head2 = kvh * p.group + r2 - tok2 * p.group;
+  const int group = late->group, tok2 = r2 / group, head2 = kvh * group + r2 - tok2 * group;
   const float inv = sum > 0.f ? 1.f / sum : sum == 0.f ? 0.f : sum;
-  uint16_t *o = static_cast<uint16_t *>(p.out) + (t.q0 + tok2) * p.o_st + head2 * p.o_sh;
-  const bool wide = p.o_st % 4 == 0 && p.o_sh % 4 == 0 && reinterpret_cast<uintptr_t>(p.out) % 8 == 0;
+  const int64_t o_st = late->o_st, o_sh = late->o_sh;
+  uint16_t *o = static_cast<uint16_t *>(late->out) + (q_first + tok2) * o_st + head2 * o_sh;
+  const bool wide =
+      o_st % 4 == 0 && o_sh % 4 == 0 && reinterpret_cast<uintptr_t>(late->out) % 8 == 0;
+  const int d = late->d;
 #pragma unroll
   for (int n = 0; n < NB; ++n)
 #pragma unroll
     for (int g = 0; g < 4; ++g) {
       const int e0 = 32 * n + 8 * g + 4 * hh;
-      if (e0 >= p.d) continue;
+      if (e0 >= d) continue;
       uint16_t x[4];
 #pragma unroll
       for (int e = 0; e < 4; ++e)
