@@ -707,15 +707,17 @@ int mlr_paged_decode_shared_prefix(const void *q, int64_t q_stride_b, int64_t q_
  *   and logprobs[r] (may be null) is log(w / S).
  * temperature <= 0 (or NaN), or an infinite maximum: the first of the order,
  * logprob 0. A row without a value above -inf, or a row id out of range: -1 and
- * -inf. NaN logits are never drawn. vocab <= 2^23.
+ * -inf. NaN logits are never drawn. vocab <= 2^23. The workspace (0 bytes where a
+ * batch fills the GPU by itself) needs no preparation.
  */
+size_t mlr_sample_tokens_workspace_size(int64_t num_rows, int64_t vocab);
 int mlr_sample_tokens(const void *logits, int64_t row_stride, int64_t num_logit_rows, int dtype,
                       const int64_t *row_ids, const void *uniforms, int uniforms_f64,
                       const float *temperature, double temperature_value, const void *top_k,
                       int top_k_dtype, int64_t top_k_value, const float *top_p,
                       double top_p_value, const float *min_p, double min_p_value,
                       int64_t *tokens, float *logprobs, int64_t num_rows, int64_t vocab,
-                      void *stream);
+                      void *workspace, size_t workspace_bytes, void *stream);
 
 #ifdef __cplusplus
 }

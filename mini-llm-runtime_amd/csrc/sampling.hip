@@ -22,11 +22,14 @@
 // the same token always, and a token differs from the formula's in exact
 // arithmetic only where u S is within about 1e-11 S of a border.
 //
-// One workgroup of 1,024 threads per row: a row is read three times (maximum,
-// bins, collecting the bin), the later times from the caches.
+// One workgroup of 1,024 threads per row, which reads it three times (maximum,
+// bins, collecting), the later times from the caches. What bounds a large batch is
+// the 64-bit arithmetic of the weights, once per element. With few rows one CU
+// each would be the bound; then a row is cut over several workgroups and the
+// steps are launches of their own, the bins summed by integer atomics.
 #include "mlr_common.h"
 
-#include <cfloat>
+#include <algorithm>
 
 namespace mlr {
 namespace {
@@ -36,7 +39,10 @@ constexpr int kWavesWg = kThreads / 64;
 constexpr int kBins = 4096;  // 4 per thread; the last holds what weighs nothing
 constexpr int kList = 2048;  // 2 per thread
 constexpr int kTable = 1024;
+constexpr int kMaxParts = 64, kPartMin = 2048;
 constexpr int64_t kMaxVocab = int64_t(1) << 23;  // a segment of 1 / kBins of it fits the list
+
+struct RowSpace;
 
 struct SampleParams {
   const void *logits;
@@ -51,6 +57,8 @@ struct SampleParams {
   float *logprobs;
   int vocab, shift;
   bool uniforms_f64, top_k_i64;
+  int parts;        // workgroups a row is cut over
+  RowSpace *space;  // [rows], if parts > 1
 };
 
 template <typename T>
@@ -110,8 +118,8 @@ __device__ __forceinline__ void each(const T *row, int n, F f) {
 
 // What turns a logit into its weight and its bin.
 struct Scale {
-  float mx, bins;  // the row's maximum; bins per unit of distance
-  double mxd, c;   // c: 1024ths of a halving per unit of distance
+  float mx, bins;        // the row's maximum; bins per unit of distance
+  double mxd, c, far;    // c: 1024ths of a halving per unit of distance; far: 60 halvings
   int shift;
 
   __device__ __forceinline__ int bin(float x) const {
@@ -121,10 +129,10 @@ struct Scale {
     constexpr double kMagic = 6755399441055744.0;  // 1.5 * 2^52: rounds to integer
     constexpr double kStep = 0.69314718055994530942 / kTable;
     // Past 60 halvings every weight rounds to 0; fmin also takes a NaN there.
-    const double t = fmin((mxd - static_cast<double>(x)) * c, 60.0 * kTable);
-    const double whole = t + kMagic;
+    const double d = fmin(mxd - static_cast<double>(x), far);
+    const double whole = fma(d, c, kMagic);
     const int k = __double2loint(whole);
-    const double r = t - (whole - kMagic);
+    const double r = fma(d, c, kMagic - whole);
     const double series = fma(r, fma(r, 0.5 * kStep * kStep, -kStep), 1.0);
     const double w = ldexp(series * table[k & (kTable - 1)], shift - (k >> 10));
     return __double_as_longlong(w + 4503599627370496.0) & 0xFFFFFFFFFFFFFull;
@@ -182,6 +190,25 @@ __device__ void scan_block(Scan<N> &s, Shared &sh) {
   s.total_w = tw;
 }
 
+// Sum and largest of the threads' values, the same in all of them.
+__device__ uint64_t total_of(uint64_t w, Shared &sh) {
+  Scan<1> s;
+  s.c[0] = 0;
+  s.w[0] = w;
+  scan_block(s, sh);
+  return s.total_w;
+}
+__device__ uint64_t max_of(uint64_t w, Shared &sh) {
+#pragma unroll
+  for (int o = 32; o > 0; o >>= 1)
+    w = max(w, static_cast<uint64_t>(__shfl_xor(static_cast<unsigned long long>(w), o)));
+  __syncthreads();
+  if ((threadIdx.x & 63) == 0) sh.scan_w[threadIdx.x >> 6] = w;
+  __syncthreads();
+  for (int i = 0; i < kWavesWg; ++i) w = max(w, sh.scan_w[i]);
+  return w;
+}
+
 // A place in the order: the array's entry at which the running count (kCount)
 // or weight reaches `target` (1 <= target <= total), what lies before it and
 // the entry itself. The same in all threads.
@@ -234,22 +261,17 @@ __device__ __forceinline__ void clear_bins(Shared &sh) {
   __syncthreads();
 }
 
-// Collects the elements that `take` accepts (at most kList) and sorts them;
-// the result holds the list's entries two to a thread, with `base` before them.
-template <typename T, typename F>
-__device__ Scan<2> collect(const T *row, int n, const Scale &sc, Shared &sh, uint32_t base_c,
-                           uint64_t base_w, F take) {
-  __syncthreads();
-  if (threadIdx.x == 0) sh.fill = 0;
-  __syncthreads();
-  each(row, n, [&](float x, int i) {
-    if (take(x, i)) {
-      const uint32_t at = atomicAdd(&sh.fill, 1u);
-      if (at < kList) sh.list[at] = (static_cast<uint64_t>(~key_of(x)) << 32) | static_cast<uint32_t>(i);
-    }
-  });
-  __syncthreads();
-  const int count = min(static_cast<int>(sh.fill), kList);
+__device__ __forceinline__ uint64_t entry_of(float x, int i) {
+  return (static_cast<uint64_t>(~key_of(x)) << 32) | static_cast<uint32_t>(i);
+}
+__device__ __forceinline__ float value_of(uint64_t entry) {
+  return of_key(~static_cast<uint32_t>(entry >> 32));
+}
+
+// Sorts the first `count` entries of the list; the result holds them two to a
+// thread, with `base` before them.
+__device__ Scan<2> sort_list(const Scale &sc, Shared &sh, int count, uint32_t base_c,
+                             uint64_t base_w) {
   int size = 128;
   while (size < count) size *= 2;
   for (int i = threadIdx.x + count; i < size; i += kThreads) sh.list[i] = ~uint64_t(0);
@@ -272,7 +294,7 @@ __device__ Scan<2> collect(const T *row, int n, const Scale &sc, Shared &sh, uin
   for (int i = 0; i < 2; ++i) {
     const int at = threadIdx.x * 2 + i;
     s.c[i] = at < count;
-    s.w[i] = at < count ? sc.weight(of_key(~static_cast<uint32_t>(sh.list[at] >> 32)), sh.table) : 0;
+    s.w[i] = at < count ? sc.weight(value_of(sh.list[at]), sh.table) : 0;
   }
   scan_block(s, sh);
   s.before_c += base_c;
@@ -280,6 +302,30 @@ __device__ Scan<2> collect(const T *row, int n, const Scale &sc, Shared &sh, uin
   s.total_c += base_c;
   s.total_w += base_w;
   return s;
+}
+
+// Collects the elements that `take` accepts, as many as the list holds; how many
+// there were.
+template <typename T, typename F>
+__device__ int gather(const T *row, int n, Shared &sh, F take) {
+  __syncthreads();
+  if (threadIdx.x == 0) sh.fill = 0;
+  __syncthreads();
+  each(row, n, [&](float x, int i) {
+    if (take(x, i)) {
+      const uint32_t at = atomicAdd(&sh.fill, 1u);
+      if (at < kList) sh.list[at] = entry_of(x, i);
+    }
+  });
+  __syncthreads();
+  return static_cast<int>(sh.fill);
+}
+
+template <typename T, typename F>
+__device__ Scan<2> collect(const T *row, int n, const Scale &sc, Shared &sh, uint32_t base_c,
+                           uint64_t base_w, F take) {
+  const int count = min(gather(row, n, sh, take), kList);
+  return sort_list(sc, sh, count, base_c, base_w);
 }
 
 // The element of the row at which the running count or weight reaches target.
@@ -293,15 +339,28 @@ struct Element {
 template <bool kCount, typename T>
 __device__ Element find_crowded(const T *row, int n, const Scale &sc, Shared &sh, const Place &bin,
                                 uint64_t target) {
+  // 16-bit logits crowd a bin with one value alone: then there is nothing to
+  // narrow down.
+  uint64_t low = ~uint64_t(0), high = 0;
+  each(row, n, [&](float x, int) {
+    if (sc.bin(x) == bin.at) {
+      const uint64_t k = key_of(x);
+      low = min(low, k);
+      high = max(high, k);
+    }
+  });
+  high = max_of(high, sh);
+  low = ~max_of(~low, sh);
   uint32_t key = 0, mask = 0;
   Place at = bin;
-  for (int shift = 20; shift >= 0; shift = shift > 8 ? shift - 12 : shift - 8) {
+  if (low == high) key = static_cast<uint32_t>(low);
+  for (int shift = low == high ? -1 : 20; shift >= 0; shift = shift > 8 ? shift - 12 : shift - 8) {
     // 12, 12 and 8 bits of the key, in descending order.
     const int bits = shift == 0 ? 8 : 12;
     clear_bins(sh);
     each(row, n, [&](float x, int) {
       const uint32_t k = key_of(x);
-      if (x == x && sc.bin(x) == bin.at && (k & mask) == key) {
+      if (sc.bin(x) == bin.at && (k & mask) == key) {
         const int digit = (1 << bits) - 1 - ((k >> shift) & ((1 << bits) - 1));
         atomicAdd(&sh.cnt[digit], 1u);
         atomicAdd(reinterpret_cast<unsigned long long *>(&sh.wsum[digit]),
@@ -340,208 +399,578 @@ template <bool kCount>
 __device__ Element find_listed(const Scan<2> &l, uint64_t target, Shared &sh) {
   const Place e = find<kCount>(l, target, sh);
   const uint64_t v = sh.list[e.at];
-  return {of_key(~static_cast<uint32_t>(v >> 32)), static_cast<int>(static_cast<uint32_t>(v)),
-          e.before_w + e.w};
+  return {value_of(v), static_cast<int>(static_cast<uint32_t>(v)), e.before_w + e.w};
+}
+
+// A row's source and parameters.
+template <typename T>
+struct Row {
+  const T *x;
+  double temp, top_p, min_p, u;
+  int64_t top_k;
+};
+
+template <typename T>
+__device__ __forceinline__ bool row_of(const SampleParams &p, int64_t out, Row<T> &r) {
+  const int64_t src = p.row_ids ? p.row_ids[out] : out;
+  if (src < 0 || src >= p.num_logit_rows) return false;
+  r.x = static_cast<const T *>(p.logits) + src * p.row_st;
+  r.temp = p.temperature ? static_cast<double>(p.temperature[out]) : p.temperature_v;
+  r.top_p = p.top_p ? static_cast<double>(p.top_p[out]) : p.top_p_v;
+  r.min_p = p.min_p ? static_cast<double>(p.min_p[out]) : p.min_p_v;
+  r.top_k = !p.top_k       ? p.top_k_v
+            : p.top_k_i64 ? static_cast<const int64_t *>(p.top_k)[out]
+                          : static_cast<const int32_t *>(p.top_k)[out];
+  r.u = p.uniforms_f64 ? static_cast<const double *>(p.uniforms)[out]
+                       : static_cast<const float *>(p.uniforms)[out];
+  return true;
+}
+
+__device__ __forceinline__ void put(const SampleParams &p, int64_t out, int token, float logprob) {
+  if (threadIdx.x == 0) {
+    p.tokens[out] = token;
+    if (p.logprobs) p.logprobs[out] = logprob;
+  }
+}
+
+// The largest value and its first index; index 0x7fffffff where there is none.
+struct Top {
+  float x;
+  int i;
+};
+__device__ __forceinline__ Top larger(Top a, Top b) {
+  return b.x > a.x || (b.x == a.x && b.i < a.i) ? b : a;
+}
+__device__ __forceinline__ Top wave_top(Top t) {
+#pragma unroll
+  for (int o = 32; o > 0; o >>= 1) t = larger(t, Top{__shfl_xor(t.x, o), __shfl_xor(t.i, o)});
+  return t;
+}
+template <typename T>
+__device__ Top top_of(const T *row, int n, Shared &sh) {
+  Top t{-INFINITY, 0x7fffffff};
+  each(row, n, [&](float x, int i) {
+    if (x > t.x) t = Top{x, i};  // a thread's indices ascend
+  });
+  t = wave_top(t);
+  if ((threadIdx.x & 63) == 0) {
+    sh.red_x[threadIdx.x >> 6] = t.x;
+    sh.red_i[threadIdx.x >> 6] = t.i;
+  }
+  __syncthreads();
+  t = Top{sh.red_x[0], sh.red_i[0]};
+  for (int i = 1; i < kWavesWg; ++i) t = larger(t, Top{sh.red_x[i], sh.red_i[i]});
+  return t;
+}
+
+// Rows whose token is the first of the order whatever the random number: no
+// temperature, the first kept only, or an infinite logit.
+template <typename T>
+__device__ __forceinline__ bool only_first(const Row<T> &r, const Top &t) {
+  return t.i == 0x7fffffff || !(r.temp > 0) || r.top_k == 1 || r.top_p <= 0 || r.min_p > 1 ||
+         t.x == INFINITY;
+}
+__device__ __forceinline__ void put_first(const SampleParams &p, int64_t out, const Top &t) {
+  const bool none = t.i == 0x7fffffff;
+  put(p, out, none ? -1 : t.i, none ? -INFINITY : 0.f);
+}
+
+__device__ __forceinline__ Scale scale_of(float top, double temp, int shift) {
+  Scale sc;
+  sc.mx = top;
+  sc.mxd = top;
+  sc.shift = shift;
+  sc.c = kTable / (temp * 0.69314718055994530942);
+  sc.far = 60.0 * kTable / sc.c;
+  // The last bin starts past 46 halvings, where every weight rounds to 0.
+  sc.bins = static_cast<float>(fmin((kBins - 1) / (46.0 * 0.69314718055994530942 * temp), 1e30));
+  return sc;
+}
+
+__device__ __forceinline__ void make_table(Shared &sh) {
+  for (int i = threadIdx.x; i < kTable; i += kThreads)
+    sh.table[i] = exp2(-static_cast<double>(i) / kTable);
+}
+
+// Counts, and weights if asked for, of a row's (or a part's) bins into LDS.
+template <typename T>
+__device__ void fill_bins(const T *row, int n, const Scale &sc, Shared &sh, bool weights) {
+  clear_bins(sh);
+  each(row, n, [&](float x, int) {
+    const int b = sc.bin(x);  // a NaN goes to the last bin
+    if (b < kBins - 1) {
+      atomicAdd(&sh.cnt[b], 1u);
+      if (weights)
+        atomicAdd(reinterpret_cast<unsigned long long *>(&sh.wsum[b]),
+                  static_cast<unsigned long long>(sc.weight(x, sh.table)));
+    }
+  });
+  __syncthreads();
+}
+
+__device__ __forceinline__ uint64_t whole(double x) {  // 0 for a NaN
+  return x >= 1 ? (x < 9.0e18 ? static_cast<uint64_t>(x) : static_cast<uint64_t>(9.0e18)) : 0;
+}
+__device__ __forceinline__ uint64_t top_p_target(double top_p, uint64_t kept) {
+  return min(max(whole(ceil(top_p * static_cast<double>(kept))), uint64_t(1)), kept);
+}
+// In integers "exceeds u S" is "reaches floor(u S) + 1" (not added in 64-bit
+// floating point, which has no such neighbour past 2^53).
+__device__ __forceinline__ uint64_t draw_target(double u, uint64_t kept) {
+  return min(whole(u * static_cast<double>(kept)) + 1, kept);
+}
+
+// Up to which distance from the maximum min-p keeps, and the bin of that.
+struct Far {
+  double far;
+  int bin;
+};
+__device__ __forceinline__ Far far_of(double min_p, double temp, const Scale &sc) {
+  const double far = -temp * log(min_p);
+  return {far, static_cast<int>(fmin(far * static_cast<double>(sc.bins), kBins - 1.0))};
+}
+
+// Elements of the row before bin b and their weight.
+struct Before {
+  uint32_t c;
+  uint64_t w;
+};
+__device__ Before before_bin(const Scan<4> &h, int b, Shared &sh) {
+  __syncthreads();
+  if (b / 4 == static_cast<int>(threadIdx.x)) {
+    Before x{h.before_c, h.before_w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      if (i < (b & 3)) {
+        x.c += h.c[i];
+        x.w += h.w[i];
+      }
+    sh.found_c = x.c;
+    sh.found_w = x.w;
+  }
+  __syncthreads();
+  return {sh.found_c, sh.found_w};
+}
+
+__device__ __forceinline__ void put_drawn(const SampleParams &p, int64_t out, double temp,
+                                          const Scale &sc, const Element &e, uint64_t kept) {
+  put(p, out, e.index,
+      static_cast<float>(-(sc.mxd - e.x) / temp - log(ldexp(static_cast<double>(kept), -p.shift))));
+}
+
+// A row step by step, each border by a pass of its own: for top-k past the list
+// and rows whose borders lie in crowded bins. h: the row's bins, if `weighed`.
+template <typename T>
+__device__ void sample_stepwise(const SampleParams &p, int64_t out, const Row<T> &r,
+                                const Scale &sc, Shared &sh, Scan<4> h, bool weighed) {
+  const int n = p.vocab;
+  if (!weighed) {
+    fill_bins(r.x, n, sc, sh, true);
+    h = scan_bins(sh, true);
+  }
+  auto only = [&](const Place &b) {
+    return collect(r.x, n, sc, sh, b.before_c, b.before_w,
+                   [&](float x, int) { return sc.bin(x) == b.at; });
+  };
+  auto reach = [&](uint64_t target) {  // a weight's place in the order
+    const Place b = find<false>(h, target, sh);
+    if (b.c > kList) return find_crowded<false>(r.x, n, sc, sh, b, target);
+    return find_listed<false>(only(b), target, sh);
+  };
+  uint64_t kept = h.total_w;
+  if (r.top_k > 0 && r.top_k < h.total_c) {
+    const Place b = find<true>(h, r.top_k, sh);
+    kept = b.c > kList ? find_crowded<true>(r.x, n, sc, sh, b, r.top_k).through_w
+                       : find_listed<true>(only(b), r.top_k, sh).through_w;
+  }
+  if (r.top_p < 1) kept = reach(top_p_target(r.top_p, kept)).through_w;
+  if (r.min_p > 0) {
+    // What the bins next to the border hold of such elements is added one by one.
+    const Far f = far_of(r.min_p, r.temp, sc);
+    uint64_t w = 0;
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      if (static_cast<int>(threadIdx.x) * 4 + i < f.bin - 1) w += h.w[i];
+    each(r.x, n, [&](float x, int) {
+      const int bx = sc.bin(x);
+      if (bx >= f.bin - 1 && bx <= f.bin + 1 && bx < kBins - 1 && sc.mxd - x <= f.far)
+        w += sc.weight(x, sh.table);
+    });
+    kept = min(kept, total_of(w, sh));
+  }
+  const Element e = reach(draw_target(r.u, kept));
+  put_drawn(p, out, r.temp, sc, e, kept);
+}
+
+// Which elements decide a row, from its bins alone: a head of the order (top-k),
+// or up to three runs of bins: those of the borders of top-p and min-p, and those
+// in which the draw can fall given what the borders' bins leave open.
+struct Plan {
+  bool listed;  // whether there is such a plan at all
+  bool head;
+  int lo[3], hi[3];       // ascending, apart from each other; kBins: none
+  uint64_t before_w[3];   // weight of the row before each run
+
+  __device__ __forceinline__ bool takes(int b) const {
+    return (b >= lo[0] && b <= hi[0]) || (b >= lo[1] && b <= hi[1]) || (b >= lo[2] && b <= hi[2]);
+  }
+};
+
+template <typename T>
+__device__ Plan plan_of(const Row<T> &r, int n, const Scale &sc, const Scan<4> &h, Shared &sh) {
+  Plan pl;
+  pl.listed = true;
+#pragma unroll
+  for (int i = 0; i < 3; ++i) {
+    pl.lo[i] = pl.hi[i] = kBins;
+    pl.before_w[i] = 0;
+  }
+  pl.head = r.top_k > 0 && r.top_k < n;
+  if (pl.head) {
+    pl.lo[0] = 0;
+    pl.hi[0] = kBins - 2;
+    uint32_t through = h.total_c;
+    if (r.top_k < h.total_c) {
+      const Place b = find<true>(h, r.top_k, sh);
+      pl.hi[0] = b.at;
+      through = b.before_c + b.c;
+    }
+    pl.listed = through <= kList;
+    return pl;
+  }
+  uint64_t least = h.total_w, most = h.total_w;
+  if (r.top_p < 1) {
+    const uint64_t target = top_p_target(r.top_p, h.total_w);
+    const Place b = find<false>(h, target, sh);
+    least = target;
+    most = b.before_w + b.w;
+    pl.lo[0] = pl.hi[0] = b.at;
+  }
+  if (r.min_p > 0) {
+    const int b = far_of(r.min_p, r.temp, sc).bin;
+    const int lo = min(max(b - 1, 0), kBins - 2), hi = min(b + 1, kBins - 2);
+    least = min(least, max(before_bin(h, lo, sh).w, uint64_t(1)));
+    most = min(most, max(before_bin(h, hi + 1, sh).w, uint64_t(1)));
+    pl.lo[1] = lo;
+    pl.hi[1] = hi;
+  }
+  pl.lo[2] = find<false>(h, draw_target(r.u, least), sh).at;
+  pl.hi[2] = find<false>(h, draw_target(r.u, most), sh).at;
+  // Ascending, then joined where they meet.
+  auto order = [&](int i, int j) {
+    if (pl.lo[j] < pl.lo[i]) {
+      const int lo = pl.lo[i], hi = pl.hi[i];
+      pl.lo[i] = pl.lo[j];
+      pl.hi[i] = pl.hi[j];
+      pl.lo[j] = lo;
+      pl.hi[j] = hi;
+    }
+  };
+  auto join = [&](int i, int j) {
+    if (pl.lo[j] < kBins && pl.lo[j] <= pl.hi[i] + 1) {
+      pl.hi[i] = max(pl.hi[i], pl.hi[j]);
+      pl.lo[j] = pl.hi[j] = kBins;
+    }
+  };
+  order(0, 1);
+  order(1, 2);
+  order(0, 1);
+  join(0, 1);
+  join(pl.lo[1] < kBins ? 1 : 0, 2);
+  uint32_t count = 0;
+#pragma unroll
+  for (int i = 0; i < 3; ++i)
+    if (pl.lo[i] < kBins) {
+      const Before x = before_bin(h, pl.lo[i], sh);
+      pl.before_w[i] = x.w;
+      count += before_bin(h, pl.hi[i] + 1, sh).c - x.c;
+    }
+  pl.listed = count <= kList;
+  return pl;
+}
+
+// Ends a row whose plan's elements, `count` of them, are in the list.
+template <typename T>
+__device__ void sample_listed(const SampleParams &p, int64_t out, const Row<T> &r, const Scale &sc,
+                              const Plan &pl, int count, uint64_t total_w, Shared &sh) {
+  Scan<2> l = sort_list(sc, sh, count, 0, 0);
+  uint64_t kept = total_w;
+  uint64_t before[2] = {l.before_w, l.before_w + l.w[0]};
+  if (pl.head) {
+    kept = l.total_w;
+    if (r.top_k > 0 && r.top_k < l.total_c) kept = find_listed<true>(l, r.top_k, sh).through_w;
+  } else {
+    // An entry's place in the row: its place in its run, after what precedes the
+    // run. Runs are in the list whole.
+    uint64_t in_list[3] = {0, 0, 0};  // weight of the list before each run
+#pragma unroll
+    for (int i = 1; i < 3; ++i) {
+      if (pl.lo[i] >= kBins) continue;  // uniform
+      uint64_t w = 0;
+#pragma unroll
+      for (int e = 0; e < 2; ++e)
+        if (l.c[e] && sc.bin(value_of(sh.list[threadIdx.x * 2 + e])) < pl.lo[i]) w += l.w[e];
+      in_list[i] = total_of(w, sh);
+    }
+#pragma unroll
+    for (int e = 0; e < 2; ++e) {
+      if (!l.c[e]) continue;
+      const int b = sc.bin(value_of(sh.list[threadIdx.x * 2 + e]));
+      const int i = b >= pl.lo[2] ? 2 : b >= pl.lo[1] ? 1 : 0;
+      before[e] = before[e] - in_list[i] + pl.before_w[i];
+    }
+  }
+  // The entry at which the running weight reaches target.
+  auto reach = [&](uint64_t target) {
+    __syncthreads();
+#pragma unroll
+    for (int e = 0; e < 2; ++e)
+      if (before[e] < target && target <= before[e] + l.w[e]) {
+        sh.found_at = threadIdx.x * 2 + e;
+        sh.found_w = before[e] + l.w[e];
+      }
+    __syncthreads();
+    const uint64_t v = sh.list[sh.found_at];
+    return Element{value_of(v), static_cast<int>(static_cast<uint32_t>(v)), sh.found_w};
+  };
+  if (r.top_p < 1) kept = reach(top_p_target(r.top_p, kept)).through_w;
+  if (r.min_p > 0) {
+    // Weight up to the last entry within the distance. Where the list is a head it
+    // holds all that is kept; else the bins about the distance are a part of it.
+    const Far f = far_of(r.min_p, r.temp, sc);
+    uint64_t w = 0;
+#pragma unroll
+    for (int e = 0; e < 2; ++e)
+      if (l.c[e] && sc.mxd - value_of(sh.list[threadIdx.x * 2 + e]) <= f.far)
+        w = max(w, before[e] + l.w[e]);
+    w = max_of(w, sh);
+    // At least all that lies before the run of those bins.
+    if (!pl.head) {
+      const int lo = min(max(f.bin - 1, 0), kBins - 2);
+      w = max(w, pl.before_w[lo >= pl.lo[2] ? 2 : lo >= pl.lo[1] ? 1 : 0]);
+    }
+    kept = min(kept, w);
+  }
+  put_drawn(p, out, r.temp, sc, reach(draw_target(r.u, kept)), kept);
+}
+
+// Whether a row is ended in steps by one workgroup from the start.
+template <typename T>
+__device__ __forceinline__ bool stepwise(const Row<T> &r, int n) {
+  return r.top_k > kList && r.top_k < n;
 }
 
 template <typename T>
 __global__ __launch_bounds__(kThreads) void sample_kernel(SampleParams p) {
   __shared__ Shared sh;
-  const int tid = threadIdx.x, lane = tid & 63, wv = tid >> 6;
   const int64_t out = blockIdx.x;
   const int n = p.vocab;
-  const int64_t src = p.row_ids ? p.row_ids[out] : out;
-  if (src < 0 || src >= p.num_logit_rows) {
-    if (tid == 0) {
-      p.tokens[out] = -1;
-      if (p.logprobs) p.logprobs[out] = -INFINITY;
-    }
+  Row<T> r;
+  if (!row_of(p, out, r)) {
+    put(p, out, -1, -INFINITY);
     return;
   }
-  const T *row = static_cast<const T *>(p.logits) + src * p.row_st;
-  const double temp = p.temperature ? static_cast<double>(p.temperature[out]) : p.temperature_v;
-  const double top_p = p.top_p ? static_cast<double>(p.top_p[out]) : p.top_p_v;
-  const double min_p = p.min_p ? static_cast<double>(p.min_p[out]) : p.min_p_v;
-  const int64_t top_k = !p.top_k       ? p.top_k_v
-                        : p.top_k_i64 ? static_cast<const int64_t *>(p.top_k)[out]
-                                      : static_cast<const int32_t *>(p.top_k)[out];
-  const double u = p.uniforms_f64 ? static_cast<const double *>(p.uniforms)[out]
-                                  : static_cast<const float *>(p.uniforms)[out];
-  for (int i = tid; i < kTable; i += kThreads)
-    sh.table[i] = exp2(-static_cast<double>(i) / kTable);
+  make_table(sh);
+  const Top t = top_of(r.x, n, sh);
+  if (only_first(r, t)) {
+    put_first(p, out, t);
+    return;
+  }
+  const Scale sc = scale_of(t.x, r.temp, p.shift);
+  if (n <= kList) {  // all of it
+    Plan pl{};
+    pl.head = true;
+    const int count = gather(r.x, n, sh, [&](float x, int) { return sc.bin(x) < kBins - 1; });
+    sample_listed(p, out, r, sc, pl, count, 0, sh);
+    return;
+  }
+  const bool weights = !(r.top_k > 0 && r.top_k < n);
+  Scan<4> h{};
+  if (!stepwise(r, n)) {
+    fill_bins(r.x, n, sc, sh, weights);
+    h = scan_bins(sh, weights);
+    const Plan pl = plan_of(r, n, sc, h, sh);
+    if (pl.listed) {
+      const int count = gather(r.x, n, sh, [&](float x, int) { return pl.takes(sc.bin(x)); });
+      sample_listed(p, out, r, sc, pl, count, h.total_w, sh);
+      return;
+    }
+  }
+  sample_stepwise(p, out, r, sc, sh, h, weights);
+}
 
-  // The maximum and its first index.
-  float best = -INFINITY;
-  int best_i = 0x7fffffff;
-  each(row, n, [&](float x, int i) {
-    if (x > best) {  // a thread's indices ascend
-      best = x;
-      best_i = i;
+// A row cut over workgroups. What they share of it; every entry is written before
+// it is read, the bins and the counter by split_top.
+struct RowSpace {
+  uint64_t wsum[kBins];
+  uint64_t list[kList];
+  uint32_t cnt[kBins];
+  float top_x[kMaxParts];
+  int top_i[kMaxParts];
+  uint32_t fill;
+};
+
+// The part of a row that workgroup `part` reads: [from, from + count).
+struct Part {
+  int64_t out;
+  int part, from, count;
+};
+__device__ __forceinline__ Part part_of(const SampleParams &p) {
+  Part t;
+  t.out = blockIdx.x / p.parts;
+  t.part = static_cast<int>(blockIdx.x - t.out * p.parts);
+  const int size = ((p.vocab + p.parts - 1) / p.parts + 7) & ~7;
+  t.from = min(t.part * size, p.vocab);
+  t.count = min(size, p.vocab - t.from);
+  return t;
+}
+
+template <typename T>
+__global__ __launch_bounds__(kThreads) void split_top(SampleParams p) {
+  __shared__ Shared sh;
+  const Part t = part_of(p);
+  RowSpace &sp = p.space[t.out];
+  for (int i = t.part * kThreads + threadIdx.x; i < kBins; i += p.parts * kThreads) {
+    sp.wsum[i] = 0;
+    sp.cnt[i] = 0;
+  }
+  if (t.part == 0 && threadIdx.x == 0) sp.fill = 0;
+  Row<T> r;
+  if (!row_of(p, t.out, r)) return;
+  const Top top = top_of(r.x + t.from, t.count, sh);
+  if (threadIdx.x == 0) {
+    sp.top_x[t.part] = top.x;
+    sp.top_i[t.part] = top.i == 0x7fffffff ? top.i : top.i + t.from;
+  }
+}
+
+// A lane per part.
+__device__ __forceinline__ Top top_of_parts(const SampleParams &p, const RowSpace &sp) {
+  static_assert(kMaxParts <= 64, "a lane per part");
+  const int lane = threadIdx.x & 63;
+  return wave_top(lane < p.parts ? Top{sp.top_x[lane], sp.top_i[lane]}
+                                 : Top{-INFINITY, 0x7fffffff});
+}
+
+template <typename T>
+__global__ __launch_bounds__(kThreads) void split_bins(SampleParams p) {
+  __shared__ Shared sh;
+  const Part t = part_of(p);
+  RowSpace &sp = p.space[t.out];
+  Row<T> r;
+  if (!row_of(p, t.out, r)) return;
+  const Top top = top_of_parts(p, sp);
+  if (only_first(r, top) || stepwise(r, p.vocab)) return;
+  make_table(sh);
+  const Scale sc = scale_of(top.x, r.temp, p.shift);
+  const bool weights = !(r.top_k > 0 && r.top_k < p.vocab);
+  fill_bins(r.x + t.from, t.count, sc, sh, weights);
+  for (int i = threadIdx.x; i < kBins; i += kThreads)
+    if (sh.cnt[i] != 0) {
+      atomicAdd(&sp.cnt[i], sh.cnt[i]);
+      if (weights)
+        atomicAdd(reinterpret_cast<unsigned long long *>(&sp.wsum[i]),
+                  static_cast<unsigned long long>(sh.wsum[i]));
     }
-  });
+}
+
+__device__ __forceinline__ Scan<4> bins_of(const RowSpace &sp, Shared &sh) {
+  Scan<4> s;
 #pragma unroll
-  for (int o = 32; o > 0; o >>= 1) {
-    const float x = __shfl_xor(best, o);
-    const int i = __shfl_xor(best_i, o);
-    if (x > best || (x == best && i < best_i)) {
-      best = x;
-      best_i = i;
-    }
+  for (int i = 0; i < 4; ++i) {
+    s.c[i] = sp.cnt[threadIdx.x * 4 + i];
+    s.w[i] = sp.wsum[threadIdx.x * 4 + i];
   }
-  if (lane == 0) {
-    sh.red_x[wv] = best;
-    sh.red_i[wv] = best_i;
-  }
+  scan_block(s, sh);
+  return s;
+}
+
+template <typename T>
+__global__ __launch_bounds__(kThreads) void split_gather(SampleParams p) {
+  __shared__ Shared sh;
+  const Part t = part_of(p);
+  RowSpace &sp = p.space[t.out];
+  Row<T> r;
+  if (!row_of(p, t.out, r)) return;
+  const Top top = top_of_parts(p, sp);
+  if (only_first(r, top) || stepwise(r, p.vocab)) return;
+  const Scale sc = scale_of(top.x, r.temp, p.shift);
+  const Scan<4> h = bins_of(sp, sh);
+  const Plan pl = plan_of(r, p.vocab, sc, h, sh);
+  if (!pl.listed) return;
+  const int count = gather(r.x + t.from, t.count, sh,
+                           [&](float x, int) { return pl.takes(sc.bin(x)); });
+  if (threadIdx.x == 0) sh.found_n = atomicAdd(&sp.fill, static_cast<uint32_t>(count));
   __syncthreads();
-  best = sh.red_x[0];
-  best_i = sh.red_i[0];
-  for (int i = 1; i < kWavesWg; ++i)
-    if (sh.red_x[i] > best || (sh.red_x[i] == best && sh.red_i[i] < best_i)) {
-      best = sh.red_x[i];
-      best_i = sh.red_i[i];
-    }
-  // One token alone: no temperature, the first kept only, or an infinite logit.
-  if (best_i == 0x7fffffff || !(temp > 0) || top_k == 1 || top_p <= 0 || min_p > 1 ||
-      best == INFINITY) {
-    if (tid == 0) {
-      const bool none = best_i == 0x7fffffff;
-      p.tokens[out] = none ? -1 : best_i;
-      if (p.logprobs) p.logprobs[out] = none ? -INFINITY : 0.f;
-    }
+  const int base = static_cast<int>(sh.found_n);
+  for (int i = threadIdx.x; i < min(count, kList); i += kThreads)
+    if (base + i < kList) sp.list[base + i] = sh.list[i] + static_cast<uint64_t>(t.from);
+}
+
+template <typename T>
+__global__ __launch_bounds__(kThreads) void split_end(SampleParams p) {
+  __shared__ Shared sh;
+  const int64_t out = blockIdx.x;
+  const RowSpace &sp = p.space[out];
+  Row<T> r;
+  if (!row_of(p, out, r)) {
+    put(p, out, -1, -INFINITY);
     return;
   }
+  const Top top = top_of_parts(p, sp);
+  if (only_first(r, top)) {
+    put_first(p, out, top);
+    return;
+  }
+  make_table(sh);
+  const Scale sc = scale_of(top.x, r.temp, p.shift);
+  Scan<4> h{};
+  if (!stepwise(r, p.vocab)) {
+    h = bins_of(sp, sh);
+    const Plan pl = plan_of(r, p.vocab, sc, h, sh);
+    if (pl.listed) {
+      const int count = static_cast<int>(sp.fill);
+      for (int i = threadIdx.x; i < count; i += kThreads) sh.list[i] = sp.list[i];
+      __syncthreads();
+      sample_listed(p, out, r, sc, pl, count, h.total_w, sh);
+      return;
+    }
+  }
+  __syncthreads();  // the table
+  sample_stepwise(p, out, r, sc, sh, h, !(r.top_k > 0 && r.top_k < p.vocab));
+}
 
-  Scale sc;
-  sc.mx = best;
-  sc.mxd = best;
-  sc.shift = p.shift;
-  sc.c = kTable / (temp * 0.69314718055994530942);
-  // The last bin starts past 46 halvings, where every weight rounds to 0.
-  sc.bins = static_cast<float>(fmin((kBins - 1) / (46.0 * 0.69314718055994530942 * temp), 1e30));
-  auto bins = [&](bool weights) {
-    clear_bins(sh);
-    each(row, n, [&](float x, int) {
-      const int b = sc.bin(x);  // a NaN goes to the last bin
-      if (b < kBins - 1) {
-        atomicAdd(&sh.cnt[b], 1u);
-        if (weights)
-          atomicAdd(reinterpret_cast<unsigned long long *>(&sh.wsum[b]),
-                    static_cast<unsigned long long>(sc.weight(x, sh.table)));
-      }
-    });
-    __syncthreads();
-    return scan_bins(sh, weights);
-  };
-  auto up_to = [&](int b) {
-    return collect(row, n, sc, sh, 0, 0, [&](float x, int) { return sc.bin(x) <= b; });
-  };
-  auto only = [&](const Place &b) {
-    return collect(row, n, sc, sh, b.before_c, b.before_w,
-                   [&](float x, int) { return sc.bin(x) == b.at; });
-  };
+template <typename T>
+int launch_sample(const SampleParams &p, unsigned rows, hipStream_t stream) {
+  if (p.parts == 1) {
+    sample_kernel<T><<<rows, kThreads, 0, stream>>>(p);
+    return check_launch("mlr_sample_tokens");
+  }
+  const unsigned grid = rows * p.parts;
+  split_top<T><<<grid, kThreads, 0, stream>>>(p);
+  split_bins<T><<<grid, kThreads, 0, stream>>>(p);
+  split_gather<T><<<grid, kThreads, 0, stream>>>(p);
+  split_end<T><<<rows, kThreads, 0, stream>>>(p);
+  return check_launch("mlr_sample_tokens");
+}
 
-  Scan<4> h;        // the bins
-  Scan<2> l;        // the list
-  bool listed = false;  // whether the list holds all that can be kept
-  uint64_t kept;    // weight of what is kept
-  bool need_k = top_k > 0 && top_k < n;
-  if (n <= kList) {
-    l = up_to(kBins - 2);
-    listed = true;
-    kept = l.total_w;
-    if (need_k && top_k < l.total_c) kept = find_listed<true>(l, top_k, sh).through_w;
-  } else if (need_k && top_k <= kList) {
-    h = bins(false);
-    Place b{kBins - 2, 0, 0, 0, 0};
-    uint32_t through = h.total_c;
-    if (top_k < h.total_c) {
-      b = find<true>(h, top_k, sh);
-      through = b.before_c + b.c;
-    }
-    if (through <= kList) {
-      l = up_to(b.at);
-      listed = true;
-      kept = top_k < l.total_c ? find_listed<true>(l, top_k, sh).through_w : l.total_w;
-    }
-  }
-  auto reach = [&](uint64_t target) {  // a weight's place in the order
-    if (listed) return find_listed<false>(l, target, sh);
-    const Place b = find<false>(h, target, sh);
-    if (b.c > kList) return find_crowded<false>(row, n, sc, sh, b, target);
-    l = only(b);
-    return find_listed<false>(l, target, sh);
-  };
-  if (!listed) {
-    h = bins(true);
-    kept = h.total_w;
-    if (need_k && top_k < h.total_c) {
-      const Place b = find<true>(h, top_k, sh);
-      if (b.c > kList) {
-        kept = find_crowded<true>(row, n, sc, sh, b, top_k).through_w;
-      } else {
-        l = only(b);
-        kept = find_listed<true>(l, top_k, sh).through_w;
-      }
-    }
-  }
-  auto whole = [&](double x) {  // 0 for a NaN
-    return x >= 1 ? (x < 9.0e18 ? static_cast<uint64_t>(x) : static_cast<uint64_t>(9.0e18)) : 0;
-  };
-  if (top_p < 1) {
-    const uint64_t target =
-        min(max(whole(ceil(top_p * static_cast<double>(kept))), uint64_t(1)), kept);
-    if (!listed) {
-      const Place b = find<false>(h, target, sh);
-      if (b.before_c + b.c <= kList) {
-        l = up_to(b.at);
-        listed = true;
-      }
-    }
-    kept = reach(target).through_w;
-  }
-  if (min_p > 0) {
-    // Up to this distance from the maximum; what the bins next to it hold of
-    // such elements is added one by one.
-    const double far = -temp * log(min_p);
-    const int b = static_cast<int>(fmin(far * static_cast<double>(sc.bins), kBins - 1.0));
-    uint64_t w = 0;
-    if (listed) {
-#pragma unroll
-      for (int i = 0; i < 2; ++i)
-        if (l.c[i]) {
-          const float x = of_key(~static_cast<uint32_t>(sh.list[tid * 2 + i] >> 32));
-          if (sc.mxd - x <= far) w += l.w[i];
-        }
-    } else {
-#pragma unroll
-      for (int i = 0; i < 4; ++i)
-        if (tid * 4 + i < b - 1) w += h.w[i];
-      each(row, n, [&](float x, int) {
-        const int bx = sc.bin(x);
-        if (bx >= b - 1 && bx <= b + 1 && bx < kBins - 1 && sc.mxd - x <= far)
-          w += sc.weight(x, sh.table);
-      });
-    }
-    Scan<1> s;
-    s.c[0] = 0;
-    s.w[0] = w;
-    scan_block(s, sh);
-    if (s.total_w < kept) kept = s.total_w;
-  }
-  // In integers "exceeds u S" is "reaches floor(u S) + 1" (not added in 64-bit
-  // floating point, which has no such neighbour past 2^53).
-  const uint64_t target = min(whole(u * static_cast<double>(kept)) + 1, kept);
-  const Element e = reach(target);
-  if (tid == 0) {
-    p.tokens[out] = e.index;
-    if (p.logprobs)
-      p.logprobs[out] = static_cast<float>(-(sc.mxd - e.x) / temp -
-                                           log(ldexp(static_cast<double>(kept), -p.shift)));
-  }
+// Workgroups a row is cut over: so many that the batch has one for every CU, each
+// with at least kPartMin elements; two parts would save less than the further
+// launches take.
+int parts_of(int64_t rows, int64_t vocab) {
+  const int cus = current_device_cus() > 0 ? current_device_cus() : 256;
+  const int64_t n = std::min({cus / std::max<int64_t>(rows, 1), vocab / kPartMin,
+                              static_cast<int64_t>(kMaxParts)});
+  return n >= 3 ? static_cast<int>(n) : 1;
 }
 
 }  // namespace
 }  // namespace mlr
+
+extern "C" size_t mlr_sample_tokens_workspace_size(int64_t num_rows, int64_t vocab) {
+  if (num_rows <= 0 || vocab <= 0 || mlr::parts_of(num_rows, vocab) == 1) return 0;
+  return static_cast<size_t>(num_rows) * sizeof(mlr::RowSpace);
+}
 
 extern "C" int mlr_sample_tokens(const void *logits, int64_t row_stride, int64_t num_logit_rows,
                                  int dtype, const int64_t *row_ids, const void *uniforms,
@@ -549,7 +978,8 @@ extern "C" int mlr_sample_tokens(const void *logits, int64_t row_stride, int64_t
                                  double temperature_value, const void *top_k, int top_k_dtype,
                                  int64_t top_k_value, const float *top_p, double top_p_value,
                                  const float *min_p, double min_p_value, int64_t *tokens,
-                                 float *logprobs, int64_t num_rows, int64_t vocab, void *stream) {
+                                 float *logprobs, int64_t num_rows, int64_t vocab,
+                                 void *workspace, size_t workspace_bytes, void *stream) {
   using namespace mlr;
   clear_error();
   MLR_REQUIRE(num_rows >= 0 && num_rows < (int64_t(1) << 31),
@@ -566,7 +996,14 @@ extern "C" int mlr_sample_tokens(const void *logits, int64_t row_stride, int64_t
               "mlr_sample_tokens: unsupported dtype %d", dtype);
   if (num_rows == 0) return MLR_OK;
   MLR_REQUIRE(logits && uniforms && tokens, "mlr_sample_tokens: null pointer");
+  const size_t need = mlr_sample_tokens_workspace_size(num_rows, vocab);
+  MLR_REQUIRE(need == 0 || (workspace && workspace_bytes >= need &&
+                            reinterpret_cast<uintptr_t>(workspace) % 8 == 0),
+              "mlr_sample_tokens: workspace of %zu bytes, %zu needed, 8-byte aligned",
+              workspace_bytes, need);
   SampleParams p;
+  p.parts = parts_of(num_rows, vocab);
+  p.space = static_cast<RowSpace *>(workspace);
   p.logits = logits;
   p.row_st = row_stride;
   p.num_logit_rows = num_logit_rows;
@@ -591,9 +1028,8 @@ extern "C" int mlr_sample_tokens(const void *logits, int64_t row_stride, int64_t
   hipStream_t s = static_cast<hipStream_t>(stream);
   const unsigned grid = static_cast<unsigned>(num_rows);
   switch (dtype) {
-    case MLR_DTYPE_F32: sample_kernel<float><<<grid, kThreads, 0, s>>>(p); break;
-    case MLR_DTYPE_F16: sample_kernel<f16_t><<<grid, kThreads, 0, s>>>(p); break;
-    default: sample_kernel<bf16_t><<<grid, kThreads, 0, s>>>(p); break;
+    case MLR_DTYPE_F32: return launch_sample<float>(p, grid, s);
+    case MLR_DTYPE_F16: return launch_sample<f16_t>(p, grid, s);
+    default: return launch_sample<bf16_t>(p, grid, s);
   }
-  return check_launch("mlr_sample_tokens");
 }

@@ -124,8 +124,10 @@ _PROTOTYPES = {
     "mlr_sample_tokens": (
         _c_int,
         [_c_ptr, _c_i64, _c_i64, _c_int, _c_ptr, _c_ptr, _c_int, _c_ptr, _c_f64, _c_ptr, _c_int,
-         _c_i64, _c_ptr, _c_f64, _c_ptr, _c_f64, _c_ptr, _c_ptr, _c_i64, _c_i64, _c_ptr],
+         _c_i64, _c_ptr, _c_f64, _c_ptr, _c_f64, _c_ptr, _c_ptr, _c_i64, _c_i64, _c_ptr, _c_size,
+         _c_ptr],
     ),
+    "mlr_sample_tokens_workspace_size": (_c_size, [_c_i64, _c_i64]),
     "mlr_paged_decode_scored_workspace_size": (_c_size, [_c_i64] * 5),
     "mlr_paged_decode_scored": (
         _c_int,

@@ -1,6 +1,6 @@
 """Sampling with temperature, top-k, top-p and min-p on the HIP library
-(csrc/sampling.hip): one launch, one given random number a row, the same token
-for the same logits and numbers always. No reference counterpart: the
+(csrc/sampling.hip): one given random number a row, the same token for the same
+logits and numbers always; one launch, or four over a few long rows. No reference counterpart: the
 reference decodes greedily (runtime/model_runner.py:287-322)."""
 
 from __future__ import annotations
@@ -78,13 +78,16 @@ def sample_tokens(logits: torch.Tensor, uniforms: torch.Tensor, *,
     logprobs = torch.empty(count, dtype=torch.float32, device=device) if return_logprobs else None
     if count:
         index = _lib.INDEX_CODES[top_k.dtype] if args["top_k"][0] is not None else 1
+        lib = _lib.load()
         with _lib.on(device):
-            status = _lib.load().mlr_sample_tokens(
+            nbytes = lib.mlr_sample_tokens_workspace_size(count, vocab)
+            ws = torch.empty(nbytes, dtype=torch.uint8, device=device) if nbytes else None
+            status = lib.mlr_sample_tokens(
                 logits.data_ptr(), stride, total, _lib.DTYPE_CODES[logits.dtype],
                 None if rows is None else rows.data_ptr(), uniforms.data_ptr(),
                 uniforms.dtype == torch.float64, *args["temperature"], args["top_k"][0], index,
                 args["top_k"][1], *args["top_p"], *args["min_p"], tokens.data_ptr(),
                 None if logprobs is None else logprobs.data_ptr(), count, vocab,
-                _lib.stream_handle(device))
+                None if ws is None else ws.data_ptr(), nbytes, _lib.stream_handle(device))
         _lib.check(status, "mlr_sample_tokens")
     return (tokens, logprobs) if return_logprobs else tokens
