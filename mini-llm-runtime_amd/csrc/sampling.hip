@@ -68,16 +68,15 @@ struct alignas(16) Row16 {
 
 struct Shared {
   double table[kTable];
-  uint64_t wsum[kBins];
+  uint64_t wsum[kBins + 64];  // from kBins on: a slot per lane for what has no bin
   uint64_t list[kList];  // sorted: ~key in the upper half, index in the lower
-  uint32_t cnt[kBins];
+  uint32_t cnt[kBins + 64];
   uint64_t scan_w[kWavesWg];
   uint32_t scan_c[kWavesWg];
   uint64_t found_w;
   uint32_t found_c, found_at, found_n;
   uint32_t fill;
   float red_x[kWavesWg];
-  int red_i[kWavesWg];
 };
 
 // FP32 values in unsigned order; both zeros alike.
@@ -89,14 +88,19 @@ __device__ __forceinline__ float of_key(uint32_t k) {
   return __uint_as_float(k ^ (k & 0x80000000u ? 0x80000000u : 0xffffffffu));
 }
 
-// f(x, index) over a row, 16 bytes a load, four loads of a thread in flight.
+// f(x, first index, count) over a row in runs of count <= N neighbours: 16 bytes
+// a load, four loads of a thread in flight. A thread's indices ascend.
 template <typename T, typename F>
-__device__ __forceinline__ void each(const T *row, int n, F f) {
+__device__ __forceinline__ void each_run(const T *row, int n, F f) {
   constexpr int kVec = 16 / sizeof(T), kDeep = 4;
   const int tid = threadIdx.x;
   const int head = min(n, static_cast<int>(((16 - (reinterpret_cast<uintptr_t>(row) & 15)) & 15) /
                                            sizeof(T)));
-  if (tid < head) f(Elem<T>::to_f32(row[tid]), tid);
+  float x[kVec] = {};
+  if (tid < head) {
+    x[0] = Elem<T>::to_f32(row[tid]);
+    f(x, tid, std::integral_constant<int, 1>{});
+  }
   const int nv = (n - head) / kVec;
   const Row16<T> *vec = reinterpret_cast<const Row16<T> *>(row + head);
   for (int v0 = tid; v0 < nv; v0 += kDeep * kThreads) {
@@ -108,12 +112,24 @@ __device__ __forceinline__ void each(const T *row, int n, F f) {
       const int v = v0 + k * kThreads;
       if (v < nv) {
 #pragma unroll
-        for (int j = 0; j < kVec; ++j) f(Elem<T>::to_f32(r[k].v[j]), head + v * kVec + j);
+        for (int j = 0; j < kVec; ++j) x[j] = Elem<T>::to_f32(r[k].v[j]);
+        f(x, head + v * kVec, std::integral_constant<int, kVec>{});
       }
     }
   }
   const int rest = head + nv * kVec + tid;
-  if (rest < n) f(Elem<T>::to_f32(row[rest]), rest);
+  if (rest < n) {
+    x[0] = Elem<T>::to_f32(row[rest]);
+    f(x, rest, std::integral_constant<int, 1>{});
+  }
+}
+// f(x, index) over a row.
+template <typename T, typename F>
+__device__ __forceinline__ void each(const T *row, int n, F f) {
+  each_run(row, n, [&](const float *x, int i, auto count) {
+#pragma unroll
+    for (int j = 0; j < decltype(count)::value; ++j) f(x[j], i + j);
+  });
 }
 
 // What turns a logit into its weight and its bin.
@@ -274,21 +290,42 @@ __device__ Scan<2> sort_list(const Scale &sc, Shared &sh, int count, uint32_t ba
                              uint64_t base_w) {
   int size = 128;
   while (size < count) size *= 2;
-  for (int i = threadIdx.x + count; i < size; i += kThreads) sh.list[i] = ~uint64_t(0);
-  __syncthreads();
-  // Bitonic sort: every thread compares one pair a step.
-  for (int k = 2; k <= size; k *= 2)
-    for (int j = k / 2; j > 0; j /= 2) {
-      for (int t = threadIdx.x; t < size / 2; t += kThreads) {
-        const int a = 2 * t - (t & (j - 1)), b = a + j;
-        const uint64_t x = sh.list[a], y = sh.list[b];
-        if ((x > y) == ((a & k) == 0)) {
-          sh.list[a] = y;
-          sh.list[b] = x;
-        }
+  // Bitonic sort, two neighbours a thread in registers: partners within 128
+  // entries are lanes of one wave; further ones meet in LDS.
+  const int at0 = threadIdx.x * 2;
+  uint64_t e[2];
+#pragma unroll
+  for (int i = 0; i < 2; ++i) e[i] = at0 + i < count ? sh.list[at0 + i] : ~uint64_t(0);
+  for (int k = 2; k <= size; k *= 2) {
+    const bool up = (at0 & k) == 0;
+    for (int j = k / 2; j > 1; j /= 2) {
+      uint64_t o[2];
+      if (j < 128) {
+#pragma unroll
+        for (int i = 0; i < 2; ++i)
+          o[i] = __shfl_xor(static_cast<unsigned long long>(e[i]), j / 2);
+      } else {
+        __syncthreads();
+#pragma unroll
+        for (int i = 0; i < 2; ++i) sh.list[at0 + i] = e[i];
+        __syncthreads();
+#pragma unroll
+        for (int i = 0; i < 2; ++i) o[i] = sh.list[(at0 + i) ^ j];
       }
-      __syncthreads();
+      const bool least = ((at0 & j) == 0) == up;
+#pragma unroll
+      for (int i = 0; i < 2; ++i) e[i] = (o[i] < e[i]) == least ? o[i] : e[i];
     }
+    if ((e[1] < e[0]) == up) {
+      const uint64_t x = e[0];
+      e[0] = e[1];
+      e[1] = x;
+    }
+  }
+  __syncthreads();
+#pragma unroll
+  for (int i = 0; i < 2; ++i) sh.list[at0 + i] = e[i];
+  __syncthreads();
   Scan<2> s;
 #pragma unroll
   for (int i = 0; i < 2; ++i) {
@@ -311,11 +348,18 @@ __device__ int gather(const T *row, int n, Shared &sh, F take) {
   __syncthreads();
   if (threadIdx.x == 0) sh.fill = 0;
   __syncthreads();
-  each(row, n, [&](float x, int i) {
-    if (take(x, i)) {
-      const uint32_t at = atomicAdd(&sh.fill, 1u);
-      if (at < kList) sh.list[at] = entry_of(x, i);
-    }
+  each_run(row, n, [&](const float *x, int i, auto count) {
+    // One branch for a run of neighbours, most of which take no part.
+    uint32_t taken = 0;
+#pragma unroll
+    for (int j = 0; j < decltype(count)::value; ++j) taken |= (take(x[j], i + j) ? 1u : 0u) << j;
+    if (taken == 0) return;
+#pragma unroll
+    for (int j = 0; j < decltype(count)::value; ++j)
+      if (taken >> j & 1) {
+        const uint32_t at = atomicAdd(&sh.fill, 1u);
+        if (at < kList) sh.list[at] = entry_of(x[j], i + j);
+      }
   });
   __syncthreads();
   return static_cast<int>(sh.fill);
@@ -335,26 +379,32 @@ struct Element {
   uint64_t through_w;  // weight up to and with it
 };
 
-// An element among those of `bin`, which hold it; more than kList of them.
-template <bool kCount, typename T>
+// An element among those of `bin`, which hold it; more than kList of them. Its
+// index only if kIndex: a border needs the weight up to it alone.
+template <bool kCount, bool kIndex, typename T>
 __device__ Element find_crowded(const T *row, int n, const Scale &sc, Shared &sh, const Place &bin,
                                 uint64_t target) {
   // 16-bit logits crowd a bin with one value alone: then there is nothing to
-  // narrow down.
+  // narrow down, and the same pass has counted the value by runs of 2^seg indices.
+  int seg = 0;
+  while ((n - 1) >> seg >= kBins) ++seg;
   uint64_t low = ~uint64_t(0), high = 0;
-  each(row, n, [&](float x, int) {
+  if (kIndex) clear_bins(sh);
+  each(row, n, [&](float x, int i) {
     if (sc.bin(x) == bin.at) {
       const uint64_t k = key_of(x);
       low = min(low, k);
       high = max(high, k);
+      if (kIndex) atomicAdd(&sh.cnt[i >> seg], 1u);
     }
   });
   high = max_of(high, sh);
   low = ~max_of(~low, sh);
+  const bool one = low == high;
   uint32_t key = 0, mask = 0;
   Place at = bin;
-  if (low == high) key = static_cast<uint32_t>(low);
-  for (int shift = low == high ? -1 : 20; shift >= 0; shift = shift > 8 ? shift - 12 : shift - 8) {
+  if (one) key = static_cast<uint32_t>(low);
+  for (int shift = one ? -1 : 20; shift >= 0; shift = shift > 8 ? shift - 12 : shift - 8) {
     // 12, 12 and 8 bits of the key, in descending order.
     const int bits = shift == 0 ? 8 : 12;
     clear_bins(sh);
@@ -380,19 +430,23 @@ __device__ Element find_crowded(const T *row, int n, const Scale &sc, Shared &sh
   const uint64_t each_w = at.w / at.c;
   const uint64_t m = kCount ? target - at.before_c
                             : (target - at.before_w + each_w - 1) / each_w;
-  int seg = 0;  // segments of 2^seg indices
-  while ((n - 1) >> seg >= kBins) ++seg;
-  clear_bins(sh);
-  each(row, n, [&](float y, int i) {
-    if (y == x) atomicAdd(&sh.cnt[i >> seg], 1u);
-  });
-  __syncthreads();
+  Element e{x, -1, at.before_w + m * each_w};
+  if (!kIndex) return e;
+  if (!one) {
+    clear_bins(sh);
+    each(row, n, [&](float y, int i) {
+      if (y == x) atomicAdd(&sh.cnt[i >> seg], 1u);
+    });
+    __syncthreads();
+  }
   const Scan<4> s = scan_bins(sh, false);
   const Place part = find<true>(s, m, sh);
-  const Scan<2> l = collect(row, n, sc, sh, part.before_c, 0,
-                            [&](float y, int i) { return y == x && i >> seg == part.at; });
-  const Place e = find<true>(l, m, sh);
-  return {x, static_cast<int>(static_cast<uint32_t>(sh.list[e.at])), at.before_w + m * each_w};
+  const int from = part.at << seg;
+  const Scan<2> l = collect(row + from, min(1 << seg, n - from), sc, sh, part.before_c, 0,
+                            [&](float y, int) { return y == x; });
+  const Place found = find<true>(l, m, sh);
+  e.index = from + static_cast<int>(static_cast<uint32_t>(sh.list[found.at]));
+  return e;
 }
 
 template <bool kCount>
@@ -433,46 +487,45 @@ __device__ __forceinline__ void put(const SampleParams &p, int64_t out, int toke
   }
 }
 
-// The largest value and its first index; index 0x7fffffff where there is none.
-struct Top {
-  float x;
-  int i;
-};
-__device__ __forceinline__ Top larger(Top a, Top b) {
-  return b.x > a.x || (b.x == a.x && b.i < a.i) ? b : a;
-}
-__device__ __forceinline__ Top wave_top(Top t) {
+__device__ __forceinline__ float wave_top(float x) {
 #pragma unroll
-  for (int o = 32; o > 0; o >>= 1) t = larger(t, Top{__shfl_xor(t.x, o), __shfl_xor(t.i, o)});
+  for (int o = 32; o > 0; o >>= 1) x = fmaxf(x, __shfl_xor(x, o));
+  return x;
+}
+// The largest value (NaNs aside; -inf where there is none) and the index of the
+// first that equals it, which only some rows need.
+template <typename T>
+__device__ float top_of(const T *row, int n, Shared &sh) {
+  float t = -INFINITY;
+  each(row, n, [&](float x, int) { t = fmaxf(t, x); });
+  t = wave_top(t);
+  __syncthreads();
+  if ((threadIdx.x & 63) == 0) sh.red_x[threadIdx.x >> 6] = t;
+  __syncthreads();
+  for (int i = 0; i < kWavesWg; ++i) t = fmaxf(t, sh.red_x[i]);
   return t;
 }
 template <typename T>
-__device__ Top top_of(const T *row, int n, Shared &sh) {
-  Top t{-INFINITY, 0x7fffffff};
+__device__ int index_of(const T *row, int n, float top, Shared &sh) {
+  uint64_t first = 0x7fffffff;
   each(row, n, [&](float x, int i) {
-    if (x > t.x) t = Top{x, i};  // a thread's indices ascend
+    if (x == top) first = min(first, static_cast<uint64_t>(i));
   });
-  t = wave_top(t);
-  if ((threadIdx.x & 63) == 0) {
-    sh.red_x[threadIdx.x >> 6] = t.x;
-    sh.red_i[threadIdx.x >> 6] = t.i;
-  }
-  __syncthreads();
-  t = Top{sh.red_x[0], sh.red_i[0]};
-  for (int i = 1; i < kWavesWg; ++i) t = larger(t, Top{sh.red_x[i], sh.red_i[i]});
-  return t;
+  return static_cast<int>(~max_of(~first, sh));
 }
 
 // Rows whose token is the first of the order whatever the random number: no
 // temperature, the first kept only, or an infinite logit.
 template <typename T>
-__device__ __forceinline__ bool only_first(const Row<T> &r, const Top &t) {
-  return t.i == 0x7fffffff || !(r.temp > 0) || r.top_k == 1 || r.top_p <= 0 || r.min_p > 1 ||
-         t.x == INFINITY;
+__device__ __forceinline__ bool only_first(const Row<T> &r, float top) {
+  return top == -INFINITY || !(r.temp > 0) || r.top_k == 1 || r.top_p <= 0 || r.min_p > 1 ||
+         top == INFINITY;
 }
-__device__ __forceinline__ void put_first(const SampleParams &p, int64_t out, const Top &t) {
-  const bool none = t.i == 0x7fffffff;
-  put(p, out, none ? -1 : t.i, none ? -INFINITY : 0.f);
+template <typename T>
+__device__ __forceinline__ void put_first(const SampleParams &p, int64_t out, const Row<T> &r,
+                                          float top, Shared &sh) {
+  if (top == -INFINITY) put(p, out, -1, -INFINITY);
+  else put(p, out, index_of(r.x, p.vocab, top, sh), 0.f);
 }
 
 __device__ __forceinline__ Scale scale_of(float top, double temp, int shift) {
@@ -496,15 +549,20 @@ __device__ __forceinline__ void make_table(Shared &sh) {
 template <typename T>
 __device__ void fill_bins(const T *row, int n, const Scale &sc, Shared &sh, bool weights) {
   clear_bins(sh);
-  each(row, n, [&](float x, int) {
-    const int b = sc.bin(x);  // a NaN goes to the last bin
-    if (b < kBins - 1) {
-      atomicAdd(&sh.cnt[b], 1u);
-      if (weights)
-        atomicAdd(reinterpret_cast<unsigned long long *>(&sh.wsum[b]),
+  const int spare = kBins + (threadIdx.x & 63);
+  auto fill = [&](auto weigh) {
+    each(row, n, [&](float x, int) {
+      // Without branches: what lies in the last bin (a NaN too) goes to the
+      // lane's spare slot.
+      const int b = sc.bin(x), slot = b < kBins - 1 ? b : spare;
+      atomicAdd(&sh.cnt[slot], 1u);
+      if constexpr (decltype(weigh)::value)
+        atomicAdd(reinterpret_cast<unsigned long long *>(&sh.wsum[slot]),
                   static_cast<unsigned long long>(sc.weight(x, sh.table)));
-    }
-  });
+    });
+  };
+  if (weights) fill(std::true_type{});
+  else fill(std::false_type{});
   __syncthreads();
 }
 
@@ -572,18 +630,20 @@ __device__ void sample_stepwise(const SampleParams &p, int64_t out, const Row<T>
     return collect(r.x, n, sc, sh, b.before_c, b.before_w,
                    [&](float x, int) { return sc.bin(x) == b.at; });
   };
-  auto reach = [&](uint64_t target) {  // a weight's place in the order
+  // A weight's place in the order; its index for the draw alone.
+  auto reach = [&](uint64_t target, auto index) {
     const Place b = find<false>(h, target, sh);
-    if (b.c > kList) return find_crowded<false>(r.x, n, sc, sh, b, target);
+    if (b.c > kList)
+      return find_crowded<false, decltype(index)::value>(r.x, n, sc, sh, b, target);
     return find_listed<false>(only(b), target, sh);
   };
   uint64_t kept = h.total_w;
   if (r.top_k > 0 && r.top_k < h.total_c) {
     const Place b = find<true>(h, r.top_k, sh);
-    kept = b.c > kList ? find_crowded<true>(r.x, n, sc, sh, b, r.top_k).through_w
+    kept = b.c > kList ? find_crowded<true, false>(r.x, n, sc, sh, b, r.top_k).through_w
                        : find_listed<true>(only(b), r.top_k, sh).through_w;
   }
-  if (r.top_p < 1) kept = reach(top_p_target(r.top_p, kept)).through_w;
+  if (r.top_p < 1) kept = reach(top_p_target(r.top_p, kept), std::false_type{}).through_w;
   if (r.min_p > 0) {
     // What the bins next to the border hold of such elements is added one by one.
     const Far f = far_of(r.min_p, r.temp, sc);
@@ -598,7 +658,7 @@ __device__ void sample_stepwise(const SampleParams &p, int64_t out, const Row<T>
     });
     kept = min(kept, total_of(w, sh));
   }
-  const Element e = reach(draw_target(r.u, kept));
+  const Element e = reach(draw_target(r.u, kept), std::true_type{});
   put_drawn(p, out, r.temp, sc, e, kept);
 }
 
@@ -612,7 +672,10 @@ struct Plan {
   uint64_t before_w[3];   // weight of the row before each run
 
   __device__ __forceinline__ bool takes(int b) const {
-    return (b >= lo[0] && b <= hi[0]) || (b >= lo[1] && b <= hi[1]) || (b >= lo[2] && b <= hi[2]);
+    auto in = [&](int i) {
+      return static_cast<uint32_t>(b - lo[i]) <= static_cast<uint32_t>(hi[i] - lo[i]);
+    };
+    return in(0) | in(1) | in(2);
   }
 };
 
@@ -771,12 +834,12 @@ __global__ __launch_bounds__(kThreads) void sample_kernel(SampleParams p) {
     return;
   }
   make_table(sh);
-  const Top t = top_of(r.x, n, sh);
-  if (only_first(r, t)) {
-    put_first(p, out, t);
+  const float top = top_of(r.x, n, sh);
+  if (only_first(r, top)) {
+    put_first(p, out, r, top, sh);
     return;
   }
-  const Scale sc = scale_of(t.x, r.temp, p.shift);
+  const Scale sc = scale_of(top, r.temp, p.shift);
   if (n <= kList) {  // all of it
     Plan pl{};
     pl.head = true;
@@ -805,9 +868,9 @@ struct RowSpace {
   uint64_t wsum[kBins];
   uint64_t list[kList];
   uint32_t cnt[kBins];
-  float top_x[kMaxParts];
-  int top_i[kMaxParts];
+  float top[kMaxParts];
   uint32_t fill;
+  uint32_t first;  // least index of the largest value, for rows that need it
 };
 
 // The part of a row that workgroup `part` reads: [from, from + count).
@@ -834,22 +897,21 @@ __global__ __launch_bounds__(kThreads) void split_top(SampleParams p) {
     sp.wsum[i] = 0;
     sp.cnt[i] = 0;
   }
-  if (t.part == 0 && threadIdx.x == 0) sp.fill = 0;
+  if (t.part == 0 && threadIdx.x == 0) {
+    sp.fill = 0;
+    sp.first = 0x7fffffff;
+  }
   Row<T> r;
   if (!row_of(p, t.out, r)) return;
-  const Top top = top_of(r.x + t.from, t.count, sh);
-  if (threadIdx.x == 0) {
-    sp.top_x[t.part] = top.x;
-    sp.top_i[t.part] = top.i == 0x7fffffff ? top.i : top.i + t.from;
-  }
+  const float top = top_of(r.x + t.from, t.count, sh);
+  if (threadIdx.x == 0) sp.top[t.part] = top;
 }
 
 // A lane per part.
-__device__ __forceinline__ Top top_of_parts(const SampleParams &p, const RowSpace &sp) {
+__device__ __forceinline__ float top_of_parts(const SampleParams &p, const RowSpace &sp) {
   static_assert(kMaxParts <= 64, "a lane per part");
   const int lane = threadIdx.x & 63;
-  return wave_top(lane < p.parts ? Top{sp.top_x[lane], sp.top_i[lane]}
-                                 : Top{-INFINITY, 0x7fffffff});
+  return wave_top(lane < p.parts ? sp.top[lane] : -INFINITY);
 }
 
 template <typename T>
@@ -859,10 +921,16 @@ __global__ __launch_bounds__(kThreads) void split_bins(SampleParams p) {
   RowSpace &sp = p.space[t.out];
   Row<T> r;
   if (!row_of(p, t.out, r)) return;
-  const Top top = top_of_parts(p, sp);
-  if (only_first(r, top) || stepwise(r, p.vocab)) return;
+  const float top = top_of_parts(p, sp);
+  if (only_first(r, top)) {
+    if (top == -INFINITY || sp.top[t.part] != top) return;  // uniform
+    const int at = index_of(r.x + t.from, t.count, top, sh);
+    if (threadIdx.x == 0) atomicMin(&sp.first, static_cast<uint32_t>(t.from + at));
+    return;
+  }
+  if (stepwise(r, p.vocab)) return;
   make_table(sh);
-  const Scale sc = scale_of(top.x, r.temp, p.shift);
+  const Scale sc = scale_of(top, r.temp, p.shift);
   const bool weights = !(r.top_k > 0 && r.top_k < p.vocab);
   fill_bins(r.x + t.from, t.count, sc, sh, weights);
   for (int i = threadIdx.x; i < kBins; i += kThreads)
@@ -892,9 +960,9 @@ __global__ __launch_bounds__(kThreads) void split_gather(SampleParams p) {
   RowSpace &sp = p.space[t.out];
   Row<T> r;
   if (!row_of(p, t.out, r)) return;
-  const Top top = top_of_parts(p, sp);
+  const float top = top_of_parts(p, sp);
   if (only_first(r, top) || stepwise(r, p.vocab)) return;
-  const Scale sc = scale_of(top.x, r.temp, p.shift);
+  const Scale sc = scale_of(top, r.temp, p.shift);
   const Scan<4> h = bins_of(sp, sh);
   const Plan pl = plan_of(r, p.vocab, sc, h, sh);
   if (!pl.listed) return;
@@ -917,13 +985,14 @@ __global__ __launch_bounds__(kThreads) void split_end(SampleParams p) {
     put(p, out, -1, -INFINITY);
     return;
   }
-  const Top top = top_of_parts(p, sp);
+  const float top = top_of_parts(p, sp);
   if (only_first(r, top)) {
-    put_first(p, out, top);
+    const bool none = top == -INFINITY;
+    put(p, out, none ? -1 : static_cast<int>(sp.first), none ? -INFINITY : 0.f);
     return;
   }
   make_table(sh);
-  const Scale sc = scale_of(top.x, r.temp, p.shift);
+  const Scale sc = scale_of(top, r.temp, p.shift);
   Scan<4> h{};
   if (!stepwise(r, p.vocab)) {
     h = bins_of(sp, sh);
