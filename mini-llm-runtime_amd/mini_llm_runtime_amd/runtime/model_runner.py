@@ -31,6 +31,11 @@ a packed prefill whose shape repeats replays its recorded forward.
 ``run_generation_step`` also checks the decode workspaces once per step: a
 split merge that gave up waiting (it only writes NaN) raises
 ``DecodeMergeError`` there instead of reaching the sampled tokens unnoticed.
+
+Tokens are the argmax (``greedy_sample``), as in the reference, or whatever the
+``sampler`` that a step is given picks: ``random_sample`` draws with temperature,
+top-k, top-p and min-p from given random numbers, and ``RandomSampler`` is a
+sampler that brings its own.
 """
 
 from __future__ import annotations
@@ -41,6 +46,7 @@ import torch
 
 from ..kernels import paged_attention as kpa
 from ..kernels import step_checks as kchk
+from ..kernels.sampling import sample_tokens
 from .paged_kv_cache import PagedKVCache
 from .request import Request, RequestStatus
 from .scheduler import Scheduler, SchedulerOutput
@@ -522,9 +528,63 @@ def greedy_sample(packed_logits: torch.Tensor, batch: ModelBatch) -> dict[str, i
     return dict(zip(batch.request_ids, picks))
 
 
+def random_sample(packed_logits: torch.Tensor, batch: ModelBatch, uniforms: torch.Tensor, *,
+                  temperature=1.0, top_k=0, top_p=1.0, min_p=0.0) -> dict[str, int]:
+    """A token drawn for each request from the logits of its last scheduled
+    token (no reference counterpart; the checks are greedy_sample's).
+
+    uniforms [num_requests] in [0, 1), in the batch's order; temperature, top_k,
+    top_p and min_p are numbers, or tensors of one value per request, with the
+    meaning of kernels.sampling.sample_tokens. bf16, fp16 and FP32 logits on a HIP
+    device."""
+    if packed_logits.ndim != 2:
+        raise ValueError("packed_logits must have shape [total_tokens, vocab_size]")
+    if packed_logits.shape[0] != batch.input_token_ids.shape[0]:
+        raise ValueError("packed_logits token dimension must match ModelBatch tokens")
+    n = len(batch.request_ids)
+    if n + 1 != batch.query_start_loc.numel():
+        raise ValueError("query_start_loc must contain one more entry than request_ids")
+    if uniforms.shape != (n,):
+        raise ValueError("uniforms must hold one number per request")
+    if not n:
+        return {}
+    qsl_dev = batch.query_start_loc
+    # A row that a malformed query_start_loc names outside the logits samples -1;
+    # the offsets come back with the tokens and are checked below.
+    picks_dev = sample_tokens(packed_logits, uniforms, temperature=temperature, top_k=top_k,
+                              top_p=top_p, min_p=min_p, rows=qsl_dev[1:] - 1)
+    host = torch.cat([qsl_dev, picks_dev]).tolist()
+    qsl, picks = host[:n + 1], host[n + 1:]
+    for i, request_id in enumerate(batch.request_ids):
+        if qsl[i + 1] <= qsl[i]:
+            raise ValueError(f"Request {request_id} must contain at least one query token")
+    for request_id, token in zip(batch.request_ids, picks):
+        if token < 0:
+            raise ValueError(f"Request {request_id} has no token with a logit above -inf")
+    return dict(zip(batch.request_ids, picks))
+
+
+class RandomSampler:
+    """A `sampler` for run_generation_step: random_sample with numbers from its
+    own seeded generator, one per request and step."""
+
+    def __init__(self, seed: int, *, temperature: float = 1.0, top_k: int = 0,
+                 top_p: float = 1.0, min_p: float = 0.0) -> None:
+        self.generator = torch.Generator().manual_seed(seed)
+        self.params = dict(temperature=temperature, top_k=top_k, top_p=top_p, min_p=min_p)
+
+    def __call__(self, packed_logits: torch.Tensor, batch: ModelBatch) -> dict[str, int]:
+        numbers = torch.rand(len(batch.request_ids), generator=self.generator)
+        return random_sample(packed_logits, batch, numbers.to(packed_logits.device),
+                             **self.params)
+
+
 def run_generation_step(model, scheduler: Scheduler,
                         eos_token_id: int | None = None,
-                        decode_graphs=None, prefill_graphs=None) -> GenerationStepResult:
+                        decode_graphs=None, prefill_graphs=None,
+                        sampler=None) -> GenerationStepResult:
+    """One step. `sampler`, if given, picks the tokens in greedy_sample's place:
+    sampler(packed_logits, batch) -> {request_id: token id}."""
     if not scheduler.waiting and not scheduler.running:
         raise ValueError("Cannot run generation step with no requests")
     scheduler_output = scheduler.schedule()
@@ -535,7 +595,7 @@ def run_generation_step(model, scheduler: Scheduler,
     packed_logits = execute_model_batch(model=model, batch=batch, kv_cache=scheduler.kv_cache,
                                         decode_graphs=decode_graphs,
                                         prefill_graphs=prefill_graphs)
-    sampled = greedy_sample(packed_logits, batch)
+    sampled = (greedy_sample if sampler is None else sampler)(packed_logits, batch)
     if batch.input_token_ids.device.type == "cuda":
         # Before any sampled token is committed to the scheduler.
         kpa.check_decode_workspaces(batch.input_token_ids.device)
