@@ -44,7 +44,7 @@ struct ScoredParams {
   bool force_partial;      // results go to the workspace even of a single split
   int64_t target;          // items the call is cut into, about
   bool whole;              // no splits: an item is a unit
-  int bs_log2, ncu;        // kernels that need them: log2 of block_size, CUs of the GPU
+  int bs_log2, ncu;        // log2 of block_size (-1: no power of two); CUs of the GPU
   int *first;              // [units + 1]: items before each unit (of one KV head)
   float *ml, *acc;         // [items][kRows][2], [items][kRows][D] of partial results
 };
@@ -118,14 +118,19 @@ __device__ __forceinline__ int64_t unit_len(const Unit &t) {
   return t.hi > t.lo && t.r0 < t.rows ? t.hi - unit_base(t) : 0;
 }
 // A unit with rows but no key has one item, which writes what an empty sum gives.
-__device__ __forceinline__ int unit_items(const Unit &t, int64_t split) {
-  if (t.r0 >= t.rows) return 0;
-  const int64_t n = (unit_len(t) + split - 1) / split;
+// Lengths are below 2^31 and the split at least kMinSplit.
+__device__ __forceinline__ int items_of(int64_t len, int split) {
+  const uint32_t n = (static_cast<uint32_t>(len) + split - 1) / static_cast<uint32_t>(split);
   return n > 0 ? static_cast<int>(n) : 1;
 }
-__device__ __forceinline__ int64_t split_of(int64_t total_keys, const ScoredParams &p) {
-  const int64_t s = (total_keys * p.hkv + p.target - 1) / p.target;
-  return ((s > kMinSplit ? s : kMinSplit) + 63) & ~int64_t(63);
+__device__ __forceinline__ int unit_items(const Unit &t, int split) {
+  return t.r0 < t.rows ? items_of(unit_len(t), split) : 0;
+}
+// In floating point, as the 64-bit division takes longer; the same everywhere.
+__device__ __forceinline__ int split_of(int64_t total_keys, const ScoredParams &p) {
+  const double s = static_cast<double>(total_keys) * p.hkv / static_cast<double>(p.target);
+  const int split = s < 2.0e9 ? static_cast<int>(s) + 1 : 2000000000;
+  return ((split > kMinSplit ? split : kMinSplit) + 63) & ~63;
 }
 
 int launch_scored_rows(const ScoredParams &p, int dtype, unsigned grid, hipStream_t stream);

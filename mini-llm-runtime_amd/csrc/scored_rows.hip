@@ -119,23 +119,22 @@ struct Rows {
   const ScoredParams &p;
   const T *k, *v;
   const int64_t *table;
-  int64_t covered;
+  int covered, bs;  // positions of the table, below 2^31; block_size, if it is less
   int m16, g, kvh;
 
-  __device__ __forceinline__ int64_t slot_of(int64_t key, bool &ok) const {
+  __device__ __forceinline__ int64_t slot_of(int key, bool &ok) const {
     ok = key < covered;
-    const int64_t at = ok ? key / p.block_size : 0;
+    const int at = !ok ? 0 : p.bs_log2 >= 0 ? key >> p.bs_log2 : key / bs;
     const int64_t blk = table[at];
     ok = ok && blk >= 0 && blk < p.num_blocks;
-    return ok ? blk * p.block_size + (key - at * p.block_size) : 0;
+    return ok ? blk * p.block_size + (key - at * bs) : 0;
   }
 
   // The tile of keys [key0, key0 + 16), key0 a multiple of 16; only keys in
-  // [lo, end) count. Absent K rows are read from slot 0 (their
-  // scores are masked), absent V rows are zeros. Returns, as
-  // bit i, whether the lane's key 4 g + i exists.
-  __device__ __forceinline__ uint32_t load(Tile<T, D> &t, int64_t key0, int64_t lo,
-                                               int64_t end) const {
+  // [lo, end) count. Absent K rows are read from slot 0 (their scores are
+  // masked), absent V rows are zeros. Returns, as bit i, whether the lane's key
+  // 4 g + i exists.
+  __device__ __forceinline__ uint32_t load(Tile<T, D> &t, int key0, int lo, int end) const {
     int64_t ks, vs[4];
     bool kok, vok[4];
     if constexpr (kPaged16) {
@@ -152,7 +151,7 @@ struct Rows {
       ks = slot_of(min(key0 + m16, end - 1), kok);
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        const int64_t key = key0 + 4 * g + i;
+        const int key = key0 + 4 * g + i;
         vs[i] = slot_of(min(key, end - 1), vok[i]);
         vok[i] = vok[i] && key >= lo && key < end;
       }
@@ -209,18 +208,27 @@ __global__ __launch_bounds__(256) void scored_rows_kernel(ScoredParams p) {
   const int m16 = lane & 15, g = lane >> 4;
 
   // The cut: all keys, hence the split length; this thread's units and the
-  // items before them.
+  // items before them. -1: a unit without rows.
   const int per = (p.units + 255) / 256;
   const int u_lo = min(tid * per, p.units), u_hi = min(u_lo + per, p.units);
-  int64_t keys = 0;
-  for (int u = u_lo; u < u_hi; ++u) keys += unit_len(unit_of(p, u, kRows));
+  auto len_of = [&](int u) -> int64_t {
+    const Unit t = unit_of(p, u, kRows);
+    return t.r0 < t.rows ? unit_len(t) : -1;
+  };
+  const int64_t len0 = u_lo < u_hi ? len_of(u_lo) : -1;  // mostly there is no other
+  auto items_at = [&](int u, int split) {
+    const int64_t len = u == u_lo ? len0 : len_of(u);
+    return len < 0 ? 0 : items_of(len, split);
+  };
+  int64_t keys = max(len0, int64_t(0));
+  for (int u = u_lo + 1; u < u_hi; ++u) keys += max(len_of(u), int64_t(0));
 #pragma unroll
   for (int o = 32; o > 0; o >>= 1) keys += __shfl_xor(keys, o);
   if (lane == 0) s_keys[wv] = keys;
   __syncthreads();
-  const int64_t split = split_of(s_keys[0] + s_keys[1] + s_keys[2] + s_keys[3], p);
+  const int split = split_of(s_keys[0] + s_keys[1] + s_keys[2] + s_keys[3], p);
   int own = 0;
-  for (int u = u_lo; u < u_hi; ++u) own += unit_items(unit_of(p, u, kRows), split);
+  for (int u = u_lo; u < u_hi; ++u) own += items_at(u, split);
   int before = own;
 #pragma unroll
   for (int o = 1; o < 64; o <<= 1) {
@@ -239,18 +247,18 @@ __global__ __launch_bounds__(256) void scored_rows_kernel(ScoredParams p) {
     int at = before;
     for (int u = u_lo; u < u_hi; ++u) {
       p.first[u] = at;
-      at += unit_items(unit_of(p, u, kRows), split);
+      at += items_at(u, split);
     }
     if (tid == 255) p.first[p.units] = items;
   }
 
   const float inv_cap = kCap ? 1.f / p.cap : 0.f;
-  for (int64_t w = blockIdx.x; w < static_cast<int64_t>(items) * p.hkv; w += gridDim.x) {
-    const int item = static_cast<int>(w / p.hkv), kvh = static_cast<int>(w - int64_t(item) * p.hkv);
+  for (int w = blockIdx.x; w < items * p.hkv; w += gridDim.x) {
+    const int item = w / p.hkv, kvh = w - item * p.hkv;
     if (item >= before && item < before + own) {
       int at = before;
       for (int u = u_lo; u < u_hi; ++u) {
-        const int n = unit_items(unit_of(p, u, kRows), split);
+        const int n = items_at(u, split);
         if (item < at + n) {
           s_unit = u;
           s_split = item - at;
@@ -265,8 +273,11 @@ __global__ __launch_bounds__(256) void scored_rows_kernel(ScoredParams p) {
     const int part = __builtin_amdgcn_readfirstlane(s_split);
     const bool alone = s_of == 1 && !p.force_partial;
     const Unit t = unit_of(p, unit, kRows);
-    const int64_t base = unit_base(t);
-    const int64_t k0 = base + part * split, k1 = min(t.hi, k0 + split);
+    // Keys are below 2^31.
+    const int64_t from = unit_base(t) + static_cast<int64_t>(part) * split;
+    const int k0 = __builtin_amdgcn_readfirstlane(static_cast<int>(min(from, int64_t(0x7fffff00))));
+    const int k1 = __builtin_amdgcn_readfirstlane(static_cast<int>(min(t.hi, from + split)));
+    const int lo = __builtin_amdgcn_readfirstlane(static_cast<int>(t.lo));
 
     // The lane's row: its query, its position and the keys that it sees.
     const int r = t.r0 + m16;
@@ -274,13 +285,13 @@ __global__ __launch_bounds__(256) void scored_rows_kernel(ScoredParams p) {
     const int tok = live ? r / p.group : 0;
     const int head = kvh * p.group + (live ? r - tok * p.group : 0);
     const int64_t row = t.q0 + tok;
-    int64_t pos = t.ctx - 1, limit = t.hi;
+    int pos = static_cast<int>(t.ctx) - 1, limit = static_cast<int>(t.hi);
     if (kPrefill) {
-      pos = t.pos0 + tok;
-      limit = max(pos + 1, t.ahead);
+      pos = static_cast<int>(t.pos0) + tok;
+      limit = max(pos + 1, static_cast<int>(t.ahead));
     } else if (t.prefix) {
       // A request shorter than the prefix sees its own first positions.
-      pos = p.ctx[row] - 1;
+      pos = static_cast<int>(clamp64(p.ctx[row], 0, 0x7fffffff)) - 1;
       limit = min(limit, pos + 1);
     }
     if (!live) limit = 0;
@@ -296,7 +307,9 @@ __global__ __launch_bounds__(256) void scored_rows_kernel(ScoredParams p) {
 
     Rows<T, D, kPaged16> src{p, static_cast<const T *>(p.k), static_cast<const T *>(p.v),
                              table_of(p, t),
-                             (t.prefix ? p.prefix_width : p.bt_width) * p.block_size, m16, g, kvh};
+                             static_cast<int>((t.prefix ? p.prefix_width : p.bt_width) *
+                                              p.block_size),
+                             static_cast<int>(min(p.block_size, int64_t(0x7fffffff))), m16, g, kvh};
     f32x4_t acc[kVe];
 #pragma unroll
     for (int n = 0; n < kVe; ++n) acc[n] = f32x4_t{0, 0, 0, 0};
@@ -304,20 +317,20 @@ __global__ __launch_bounds__(256) void scored_rows_kernel(ScoredParams p) {
 
     M tile[kBatch];
     uint32_t ok[kBatch];
-    const int64_t step = 16 * kWavesWg;
-    for (int64_t b0 = k0 + 16 * wv; b0 < k1; b0 += step * kBatch) {
+    constexpr int step = 16 * kWavesWg;
+    for (int b0 = k0 + 16 * wv; b0 < k1; b0 += step * kBatch) {
 #pragma unroll
       for (int b = 0; b < kBatch; ++b) {
-        const int64_t key0 = b0 + b * step;
+        const int key0 = b0 + b * step;
         ok[b] = 0;
-        if (key0 < k1) ok[b] = src.load(tile[b], key0, t.lo, k1);
+        if (key0 < k1) ok[b] = src.load(tile[b], key0, lo, k1);
       }
       // Scores of the batch and their maximum.
       float x[kBatch][4];
       float top = mx;
 #pragma unroll
       for (int b = 0; b < kBatch; ++b) {
-        const int64_t key0 = b0 + b * step;
+        const int key0 = b0 + b * step;
         if (key0 >= k1) {
 #pragma unroll
           for (int i = 0; i < 4; ++i) x[b][i] = -INFINITY;
@@ -338,10 +351,10 @@ __global__ __launch_bounds__(256) void scored_rows_kernel(ScoredParams p) {
         }
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-          const int64_t key = key0 + 4 * g + i;
-          const float dist = static_cast<float>(llabs(pos - key));
+          const int key = key0 + 4 * g + i;
+          const float dist = static_cast<float>(abs(pos - key));
           const float y = score<T, kCap>(s[i] * p.scale, p, inv_cap, slope, dist);
-          const bool seen = (ok[b] >> i & 1) && key >= t.lo && key < limit;
+          const bool seen = (ok[b] >> i & 1) && key >= lo && key < limit;
           x[b][i] = seen ? y : -INFINITY;
           top = fmaxf(top, x[b][i]);
         }
@@ -411,11 +424,11 @@ __global__ __launch_bounds__(256) void scored_rows_kernel(ScoredParams p) {
             const float p0 = __shfl(pr[0], from), p1 = __shfl(pr[1], from);
             const float p2 = __shfl(pr[2], from), p3 = __shfl(pr[3], from);
             const float pj = (j & 2) ? ((j & 1) ? p3 : p2) : ((j & 1) ? p1 : p0);
-            const int64_t key = b0 + b * step + j;
+            const int key = b0 + b * step + j;
             bool exists = key < k1;
             int64_t slot = 0;
             if (exists) slot = src.slot_of(key, exists);
-            if (!exists || key < t.lo || key >= limit) continue;
+            if (!exists || key < lo || key >= limit) continue;
             const T *vr = src.v + (slot * p.hkv + kvh) * p.d;
 #pragma unroll
             for (int n = 0; n < kVe; ++n)
@@ -460,7 +473,7 @@ __global__ __launch_bounds__(256) void scored_rows_kernel(ScoredParams p) {
     }
     const int orow = t.r0 + rr;
     if (!alone) {
-      const int64_t at = w * kRows + rr;
+      const int64_t at = static_cast<int64_t>(w) * kRows + rr;
       if ((tid & 15) == 0) {
         p.ml[2 * at] = m_all;
         p.ml[2 * at + 1] = sum;

@@ -133,7 +133,7 @@ void scored_tiles_kernel(ScoredParams p) {
   const int m32 = lane & 31, hh = lane >> 5;
 
   // Which item this workgroup takes.
-  int64_t split = int64_t(1) << 40;
+  int split = 0x7fffffc0;
   int64_t item;
   int kvh;
   if (p.whole) {
@@ -234,7 +234,7 @@ void scored_tiles_kernel(ScoredParams p) {
   const Unit t = unit_of(p, unit, kTileRows);
   if (t.r0 >= t.rows) return;
   const int k_lo =
-      __builtin_amdgcn_readfirstlane(static_cast<int>(unit_base(t) + (p.whole ? 0 : part * split)));
+      __builtin_amdgcn_readfirstlane(static_cast<int>(unit_base(t) + (p.whole ? 0 : static_cast<int64_t>(part) * split)));
   const int low = __builtin_amdgcn_readfirstlane(static_cast<int>(t.lo));  // first key seen
   const int k_hi = __builtin_amdgcn_readfirstlane(
       static_cast<int>(min(t.hi, static_cast<int64_t>(k_lo) + split)));
