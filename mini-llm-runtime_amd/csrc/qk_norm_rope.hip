@@ -22,11 +22,15 @@
 // over the head's lanes. A head's lanes keep their place from head to head,
 // so a lane reads its cosines, sines and weights once per token or once at all.
 // A wave takes a token, or a token's heads are dealt over several waves (few
-// tokens). The token's angles are computed one per lane and exchanged through
+// tokens); the next head is loaded while one is worked on. The token's angles are computed one per lane and exchanged through
 // the wave's own LDS rows.
 //
-// Bound by memory: each element is read and written once.
+// Bound by memory: each element is read and written once (bf16, 4,096 tokens of
+// 28/4 heads of 128: 75.6 MB in 14.6 us, 5.2 TB/s, the rate of a large copy; the
+// kernel that loaded two heads and then worked on both took 16.4 us).
 #include "mlr_common.h"
+
+#include <algorithm>
 
 namespace mlr {
 namespace {
@@ -71,7 +75,7 @@ __device__ __forceinline__ float sum_lanes(float x, int width) {
   return x;
 }
 
-template <typename T, typename I, int VEC, int K, bool kInter, bool kNorm>
+template <typename T, typename I, int VEC, bool kInter, bool kNorm>
 __global__ __launch_bounds__(256) void qk_norm_rope_kernel(NormRopeParams p, int width) {
   using V = Pack<T, VEC>;
   extern __shared__ float cs_all[];  // per wave: [half] cos, [half] sin
@@ -116,17 +120,13 @@ __global__ __launch_bounds__(256) void qk_norm_rope_kernel(NormRopeParams p, int
     const int64_t t = it / p.parts;
     const int part = static_cast<int>(it - t * p.parts);
     const T *row = static_cast<const T *>(p.qkv) + t * p.qkv_st;
-    V lo[K], hi[K];
+    V lo, hi;
     auto load = [&](int h0) {
-#pragma unroll
-      for (int k = 0; k < K; ++k) {
-        const int h = min(h0 + (k * p.parts + part) * hpw + hl, heads - 1);
-        const T *src = row + static_cast<int64_t>(h) * d;
-        lo[k] = *reinterpret_cast<const V *>(src + e_lo);
-        hi[k] = *reinterpret_cast<const V *>(src + e_hi);
-      }
+      const T *src = row + static_cast<int64_t>(min(h0 + hl, heads - 1)) * d;
+      lo = *reinterpret_cast<const V *>(src + e_lo);
+      hi = *reinterpret_cast<const V *>(src + e_hi);
     };
-    load(0);
+    load(part * hpw);
     const int64_t slot = static_cast<int64_t>(static_cast<const I *>(p.slots)[t]);
     const bool write_kv = slot >= 0 && slot < p.num_slots;
     const double pos = static_cast<double>(p.positions[t]);
@@ -145,70 +145,67 @@ __global__ __launch_bounds__(256) void qk_norm_rope_kernel(NormRopeParams p, int
       c[j] = rot ? cs[pair + j] : 1.f;
       s[j] = rot ? cs[half + pair + j] : 0.f;
     }
-    for (int h0 = 0;;) {
+    const int step = p.parts * hpw;
+    for (int h0 = part * hpw; h0 < heads; h0 += step) {
+      const int h = h0 + hl;
+      const V now_lo = lo, now_hi = hi;
+      if (h0 + step < heads) load(h0 + step);  // in flight while this head is worked on
+      const bool is_q = h < p.hq, is_v = h >= p.hq + p.hkv;
+      float a[VEC], b[VEC];  // lo and hi
 #pragma unroll
-      for (int k = 0; k < K; ++k) {
-        const int h = h0 + (k * p.parts + part) * hpw + hl;
-        const bool is_q = h < p.hq, is_v = h >= p.hq + p.hkv;
-        float a[VEC], b[VEC];  // lo and hi
-#pragma unroll
-        for (int j = 0; j < VEC; ++j) {
-          if constexpr (kInter) {
-            a[j] = Elem<T>::to_f32(2 * j < VEC ? lo[k].v[2 * j % VEC] : hi[k].v[2 * j % VEC]);
-            b[j] = Elem<T>::to_f32(2 * j + 1 < VEC ? lo[k].v[(2 * j + 1) % VEC]
-                                                   : hi[k].v[(2 * j + 1) % VEC]);
-          } else {
-            a[j] = Elem<T>::to_f32(lo[k].v[j]);
-            b[j] = Elem<T>::to_f32(hi[k].v[j]);
-          }
-        }
-        if constexpr (kNorm) {
-          float sq = 0.f;
-#pragma unroll
-          for (int j = 0; j < VEC; ++j) sq += a[j] * a[j] + b[j] * b[j];
-          sq = sum_lanes(live ? sq : 0.f, width);
-          const float r = rsqrtf(sq / static_cast<float>(d) + p.eps);
-#pragma unroll
-          for (int j = 0; j < VEC; ++j) {
-            const int lo_at = kInter ? 2 * j : j, hi_at = kInter ? 2 * j + 1 : j;
-            const V &wl = is_q ? qw_lo : kw_lo, &wh = is_q ? qw_hi : kw_hi;
-            const T w_a = kInter ? (lo_at < VEC ? wl.v[lo_at % VEC] : wh.v[lo_at % VEC])
-                                 : wl.v[j];
-            const T w_b = kInter ? (hi_at < VEC ? wl.v[hi_at % VEC] : wh.v[hi_at % VEC])
-                                 : wh.v[j];
-            a[j] = a[j] * r * Elem<T>::to_f32(w_a);
-            b[j] = b[j] * r * Elem<T>::to_f32(w_b);
-          }
-        }
-        V olo = lo[k], ohi = hi[k];
-        if (!is_v) {
-#pragma unroll
-          for (int j = 0; j < VEC; ++j) {
-            // Beyond the rotated part the values pass as they are, so that one
-            // that is not finite stays alone.
-            const T x = Elem<T>::from_f32(rot ? a[j] * c[j] - b[j] * s[j] : a[j]);
-            const T y = Elem<T>::from_f32(rot ? b[j] * c[j] + a[j] * s[j] : b[j]);
-            if constexpr (kInter) {
-              (2 * j < VEC ? olo : ohi).v[2 * j % VEC] = x;
-              (2 * j + 1 < VEC ? olo : ohi).v[(2 * j + 1) % VEC] = y;
-            } else {
-              olo.v[j] = x;
-              ohi.v[j] = y;
-            }
-          }
-        }
-        if (live && h < heads && (is_q || write_kv)) {
-          T *o = is_q ? static_cast<T *>(p.q_out) + t * p.q_st + static_cast<int64_t>(h) * d
-                 : is_v
-                     ? static_cast<T *>(p.vc) + (slot * p.hkv + (h - p.hq - p.hkv)) * d
-                     : static_cast<T *>(p.kc) + (slot * p.hkv + (h - p.hq)) * d;
-          *reinterpret_cast<V *>(o + e_lo) = olo;
-          *reinterpret_cast<V *>(o + e_hi) = ohi;
+      for (int j = 0; j < VEC; ++j) {
+        if constexpr (kInter) {
+          a[j] = Elem<T>::to_f32(2 * j < VEC ? now_lo.v[2 * j % VEC] : now_hi.v[2 * j % VEC]);
+          b[j] = Elem<T>::to_f32(2 * j + 1 < VEC ? now_lo.v[(2 * j + 1) % VEC]
+                                                 : now_hi.v[(2 * j + 1) % VEC]);
+        } else {
+          a[j] = Elem<T>::to_f32(now_lo.v[j]);
+          b[j] = Elem<T>::to_f32(now_hi.v[j]);
         }
       }
-      h0 += K * p.parts * hpw;
-      if (h0 + part * hpw >= heads) break;
-      load(h0);
+      if constexpr (kNorm) {
+        float sq = 0.f;
+#pragma unroll
+        for (int j = 0; j < VEC; ++j) sq += a[j] * a[j] + b[j] * b[j];
+        sq = sum_lanes(live ? sq : 0.f, width);
+        const float r = rsqrtf(sq / static_cast<float>(d) + p.eps);
+#pragma unroll
+        for (int j = 0; j < VEC; ++j) {
+          const int lo_at = kInter ? 2 * j : j, hi_at = kInter ? 2 * j + 1 : j;
+          const V &wl = is_q ? qw_lo : kw_lo, &wh = is_q ? qw_hi : kw_hi;
+          const T w_a = kInter ? (lo_at < VEC ? wl.v[lo_at % VEC] : wh.v[lo_at % VEC])
+                               : wl.v[j];
+          const T w_b = kInter ? (hi_at < VEC ? wl.v[hi_at % VEC] : wh.v[hi_at % VEC])
+                               : wh.v[j];
+          a[j] = a[j] * r * Elem<T>::to_f32(w_a);
+          b[j] = b[j] * r * Elem<T>::to_f32(w_b);
+        }
+      }
+      V olo = now_lo, ohi = now_hi;
+      if (!is_v) {
+#pragma unroll
+        for (int j = 0; j < VEC; ++j) {
+          // Beyond the rotated part the values pass as they are, so that one
+          // that is not finite stays alone.
+          const T x = Elem<T>::from_f32(rot ? a[j] * c[j] - b[j] * s[j] : a[j]);
+          const T y = Elem<T>::from_f32(rot ? b[j] * c[j] + a[j] * s[j] : b[j]);
+          if constexpr (kInter) {
+            (2 * j < VEC ? olo : ohi).v[2 * j % VEC] = x;
+            (2 * j + 1 < VEC ? olo : ohi).v[(2 * j + 1) % VEC] = y;
+          } else {
+            olo.v[j] = x;
+            ohi.v[j] = y;
+          }
+        }
+      }
+      if (live && h < heads && (is_q || write_kv)) {
+        T *o = is_q ? static_cast<T *>(p.q_out) + t * p.q_st + static_cast<int64_t>(h) * d
+               : is_v
+                   ? static_cast<T *>(p.vc) + (slot * p.hkv + (h - p.hq - p.hkv)) * d
+                   : static_cast<T *>(p.kc) + (slot * p.hkv + (h - p.hq)) * d;
+        *reinterpret_cast<V *>(o + e_lo) = olo;
+        *reinterpret_cast<V *>(o + e_hi) = ohi;
+      }
     }
     __builtin_amdgcn_wave_barrier();  // cs is rewritten for the next token
   }
@@ -223,16 +220,19 @@ int launch(NormRopeParams p, hipStream_t stream) {
               p.d, VEC);
   const int heads = p.hq + 2 * p.hkv;
   const int passes = (heads + 64 / width - 1) / (64 / width);
-  p.parts = p.num_tokens >= 1024 ? 1 : passes < 4 ? passes : 4;
-  const int per = (passes + p.parts - 1) / p.parts;
+  // Heads of a token are dealt over so many waves that the call has about sixteen
+  // for every CU, a pass of the heads at least each. 32/8 heads of 128, us, a wave per
+  // token and this rule: bf16, 1 token 7.0 and 3.9, 512 tokens 8.8 and 5.8, 2,048
+  // tokens 13.2 and 12.5; FP32 7.9 and 3.7, 10.9 and 7.0, 19.2 and 18.2. At 4,096
+  // tokens two waves each would take 22.1 in place of 19.9 (bf16).
+  const int cus = current_device_cus() > 0 ? current_device_cus() : 256;
+  p.parts = static_cast<int>(std::max<int64_t>(
+      1, std::min<int64_t>({16 * static_cast<int64_t>(cus) / p.num_tokens, passes, 16})));
   const int waves = 4;
   const int64_t wgs = ceil_div(p.num_tokens * p.parts, waves);
   const unsigned blocks = static_cast<unsigned>(wgs < 65536 ? wgs : 65536);
   const size_t lds = static_cast<size_t>(waves) * 2 * p.half * sizeof(float);
-  if (per == 1)
-    qk_norm_rope_kernel<T, I, VEC, 1, kInter, kNorm><<<blocks, 64 * waves, lds, stream>>>(p, width);
-  else
-    qk_norm_rope_kernel<T, I, VEC, 2, kInter, kNorm><<<blocks, 64 * waves, lds, stream>>>(p, width);
+  qk_norm_rope_kernel<T, I, VEC, kInter, kNorm><<<blocks, 64 * waves, lds, stream>>>(p, width);
   return check_launch("mlr_qk_norm_rope_write");
 }
 
