@@ -3,8 +3,8 @@
 //
 // A unit is a group of query rows that share their keys: kRows consecutive rows
 // of one sequence and KV head, a row being one (token, query head of the KV
-// head's group), tokens first. Its keys are cut into splits of equal length;
-// an item is one (unit, split, KV head). The split length is chosen on the
+// head's group), tokens first. Its keys are cut into splits, alike in length;
+// an item is one (unit, split, KV head). The longest split is chosen on the
 // device from the lengths themselves: the whole call makes about `target`
 // items whatever the table's width says, and the same lengths always give the
 // same splits.
@@ -126,11 +126,29 @@ __device__ __forceinline__ int items_of(int64_t len, int split) {
 __device__ __forceinline__ int unit_items(const Unit &t, int split) {
   return t.r0 < t.rows ? items_of(unit_len(t), split) : 0;
 }
+// Length of the n items of a unit: alike, up to `step` keys, a power of two that
+// divides the split length; so none is longer than that, and none is empty.
+__device__ __forceinline__ int item_len(const Unit &t, int n, int step) {
+  const uint32_t len = static_cast<uint32_t>(unit_len(t));
+  return static_cast<int>(((len + n - 1) / static_cast<uint32_t>(n) + step - 1) & -step);
+}
 // In floating point, as the 64-bit division takes longer; the same everywhere.
 __device__ __forceinline__ int split_of(int64_t total_keys, const ScoredParams &p) {
   const double s = static_cast<double>(total_keys) * p.hkv / static_cast<double>(p.target);
   const int split = s < 2.0e9 ? static_cast<int>(s) + 1 : 2000000000;
   return ((split > kMinSplit ? split : kMinSplit) + 63) & ~63;
+}
+
+// Whether a prefill of `units` units of 128 rows over all KV heads, the longest of
+// `keys` keys, gains from splits: whole it takes the time of its longest unit, split
+// the partial results of all units take theirs. bf16, whole and split, us:
+//   14 units of 1,024 and 4,096 keys, head size 64: 24 and 20, 65 and 24
+//   56 units of 1,024, 2,048 and 4,096 keys: 25 and 27, 38 and 31, 66 and 46
+//   32 units of 512, 1,024 and 2,048 keys, head size 128: 20 and 26, 28 and 28, 43 and 31
+//   128 units of 2,048, 4,096 and 16,384 keys: 45 and 53, 75 and 71, 260 and 183
+//   224 units of 4,096 and 16,384 keys, head size 64: 68 and 96, 250 and 245
+__host__ __device__ inline bool splits_pay(int64_t units, int64_t keys, int cus) {
+  return 2 * units <= cus && keys > 512 + units * units / 4;
 }
 
 int launch_scored_rows(const ScoredParams &p, int dtype, unsigned grid, hipStream_t stream);

@@ -112,7 +112,19 @@ int cus() {
   const int n = current_device_cus();
   return n > 0 ? n : 256;
 }
-int64_t target_items() { return 2 * static_cast<int64_t>(cus()); }
+// Items of the kernel of 16 rows a unit. `slots` workgroups run at once; units of
+// different lengths make half an item each more than their keys ask for, and items
+// past a full round cost a round. With too many units for one round, two rounds of
+// shorter items even out better. 64 requests of 128 to 4,096 keys, us, this rule and
+// two items for every CU: bf16, 14/2 heads of 64 25.1 and 27.6, 12/4 heads of 64 33.3
+// and 37.9, 32/8 heads of 128 96 and 113; FP32, 32/8 heads of 128 193 and 256. (64
+// requests of exactly 1,024 keys, 32/8 heads of 128: 51.5 and 44.9, as a unit for
+// each of the 512 slots is a perfect round.)
+int64_t rows_target(int64_t units, int64_t hkv, int64_t d) {
+  const int64_t slots = (d > 64 ? 2 : 3) * static_cast<int64_t>(cus());
+  const int64_t rounds = 3 * units * hkv <= 2 * slots ? 1 : 2;
+  return std::max(slots / 2, rounds * slots - units * hkv / 2);
+}
 
 // Items of a call at most, over its KV heads, cut into about `target`.
 int64_t max_items(int64_t units, int64_t hkv, int64_t max_keys, int64_t target) {
@@ -147,20 +159,28 @@ int64_t prefix_units(int64_t batch, int64_t group, int64_t rows) {
   return ceil_div(batch * group, rows);
 }
 
-// Whether a call with `rows` query rows per sequence and KV head goes to the
-// kernel of 128 rows a unit: more than two of the other kernel's units.
-bool takes_tiles(int64_t rows, int64_t block_size, int64_t hkv, int64_t d, int dtype) {
-  return dtype != MLR_DTYPE_F32 && rows > 2 * kRows && log2_if_pow2(block_size) >= 4 &&
+// What the kernel of 128 rows a unit can run.
+bool fits_tiles(int64_t block_size, int64_t hkv, int64_t d, int dtype) {
+  return dtype != MLR_DTYPE_F32 && log2_if_pow2(block_size) >= 4 &&
          block_size < (int64_t(1) << 30) / (hkv * d);  // 32-bit offsets inside a block
+}
+// Whether a call with `rows` query rows per sequence and KV head goes to it: more
+// than two of the other kernel's units (16 chunks after 4,096 keys, this kernel and
+// the other: 28 rows 28.3 and 26.4 us, 35 rows 29.9 and 49.9 us at head size 64;
+// 16 rows 81 and 65 us, 64 rows 87 and 175 us at 128).
+bool takes_tiles(int64_t rows, int64_t block_size, int64_t hkv, int64_t d, int dtype) {
+  return rows > 2 * kRows && fits_tiles(block_size, hkv, d, dtype);
 }
 
 // A shared prefix on the kernel of 128 rows a unit, with each request's own keys
-// (all heads of a group in one unit) in the same launch. At head sizes above 64
-// that kernel's stages take a whole CU, so a request's few keys would hold one
-// each; there the requests' own keys go to the other kernel.
-bool shares_tiles(int64_t batch, int64_t group, int64_t block_size, int64_t hkv, int64_t d,
-                  int dtype) {
-  return d <= 64 && group <= kTileRows && takes_tiles(batch * group, block_size, hkv, d, dtype);
+// (all heads of a group in one unit) in the same launch: a launch less, also for
+// few rows (8,192 keys shared by 2, 8 and 64 requests of 14/2 heads of 64: 16.4,
+// 17.3 and 26.9 us, against 19.6, 22.9 and 29.6 us). At head sizes above 64 that
+// kernel's stages take a whole CU, so a request's few keys would hold one each;
+// there the requests' own keys go to the other kernel (16 and 64 requests of 32/8
+// heads of 128: 33.9 and 45.1 us, in one launch 36.2 and 53.3 us).
+bool shares_tiles(int64_t group, int64_t block_size, int64_t hkv, int64_t d, int dtype) {
+  return d <= 64 && group <= kTileRows && fits_tiles(block_size, hkv, d, dtype);
 }
 // Two workgroups fit a CU; the last split of each unit is half full on average, and
 // a second round of workgroups would cost more than longer splits.
@@ -173,9 +193,16 @@ int64_t prefix_target(int64_t units, int64_t hkv) {
   return std::max<int64_t>(1, cus() / (units * hkv)) * units * hkv;
 }
 
-// A prefill's rows per unit, units, items, and whether units stay whole: with a
-// unit for every CU there is nothing to gain from splits, which cost a pass over
-// FP32 partial results.
+// Items of a prefill on that kernel: one for each CU, less the last splits of the
+// units, half full on average.
+int64_t tiles_target(int64_t units, int64_t hkv) {
+  return std::max<int64_t>(cus() / 2, cus() - units * hkv / 2);
+}
+
+// A prefill's rows per unit, units, items, and whether units stay whole. Splits on
+// the kernel of 128 rows cost a pass over FP32 partial results of every unit, so
+// they pay only where units are few and their keys many (see splits_pay); the kernel
+// decides that from the lengths, and what no lengths could change is decided here.
 struct PrefillPlan {
   int64_t rows, units, items;
   bool whole, parts;
@@ -187,8 +214,10 @@ PrefillPlan plan_prefill(int64_t seqs, int64_t max_q, int64_t max_keys, int64_t 
   const bool tiles = takes_tiles(max_q * group, block_size, hkv, d, dtype);
   n.rows = tiles ? kTileRows : kRows;
   n.units = prefill_units(seqs, max_q, group, n.rows);
-  n.whole = tiles && (n.units * hkv >= cus() || max_keys <= kMinSplit);
-  n.items = n.whole ? n.units * hkv : max_items(n.units, hkv, max_keys, target_items());
+  n.whole = tiles && !splits_pay(n.units * hkv, max_keys, cus());
+  n.items = n.whole   ? n.units * hkv
+            : tiles ? max_items(n.units, hkv, max_keys, tiles_target(n.units, hkv))
+                    : max_items(n.units, hkv, max_keys, rows_target(n.units, hkv, d));
   n.parts = !n.whole && max_keys > kMinSplit;
   return n;
 }
@@ -272,7 +301,6 @@ ScoredParams params_of(const Operands &o, int mode) {
   p.o_st = o.o_st;
   p.o_sh = o.o_sh;
   p.mode = mode;
-  p.target = target_items();
   p.ncu = cus();
   p.bs_log2 = log2_if_pow2(o.block_size);
   return p;
@@ -290,8 +318,9 @@ extern "C" size_t mlr_paged_decode_scored_workspace_size(int64_t batch, int64_t 
                                                          int64_t max_context) {
   if (batch <= 0 || num_kv_heads <= 0 || num_q_heads <= 0 || max_context <= kMinSplit) return 0;
   const int64_t units = decode_units(batch, num_q_heads / num_kv_heads);
-  return part_bytes(units, max_items(units, num_kv_heads, max_context, target_items()), kRows,
-                    head_dim);
+  return part_bytes(units, max_items(units, num_kv_heads, max_context,
+                                     rows_target(units, num_kv_heads, head_dim)),
+                    kRows, head_dim);
 }
 
 extern "C" int mlr_paged_decode_scored(
@@ -319,6 +348,7 @@ extern "C" int mlr_paged_decode_scored(
   ScoredParams p = params_of(o, kModeDecode);
   p.tiles = static_cast<int>(ceil_div(p.group, kRows));
   p.units = static_cast<int>(decode_units(batch, p.group));
+  p.target = rows_target(p.units, p.hkv, p.d);
   const int64_t items = max_items(p.units, p.hkv, max_keys, p.target);
   if (need) place_parts(p, static_cast<char *>(workspace), items, kRows);
   hipStream_t s = static_cast<hipStream_t>(stream);
@@ -380,6 +410,7 @@ extern "C" int mlr_paged_prefill_scored(
   p.units = static_cast<int>(n.units);
   p.tiles = static_cast<int>(n.units / num_seqs);
   p.whole = n.whole;
+  p.target = n.rows == kTileRows ? tiles_target(n.units, p.hkv) : rows_target(n.units, p.hkv, p.d);
   const int rows = static_cast<int>(n.rows);
   if (n.parts) place_parts(p, static_cast<char *>(workspace), n.items, rows);
   hipStream_t s = static_cast<hipStream_t>(stream);
@@ -396,7 +427,7 @@ extern "C" size_t mlr_paged_decode_shared_prefix_workspace_size(
   if (batch <= 0 || num_kv_heads <= 0 || num_q_heads <= 0 || head_dim <= 0 || block_size <= 0)
     return 0;
   const int64_t group = num_q_heads / num_kv_heads, max_keys = max_blocks * block_size;
-  if (shares_tiles(batch, group, block_size, num_kv_heads, head_dim, dtype)) {
+  if (shares_tiles(group, block_size, num_kv_heads, head_dim, dtype)) {
     const int64_t units = prefix_units(batch, group, kTileRows) + batch;
     return part_bytes(units, max_items(units, num_kv_heads, std::max(prefix_len, max_keys),
                                        shared_target(units, num_kv_heads)), kTileRows, head_dim);
@@ -404,9 +435,10 @@ extern "C" size_t mlr_paged_decode_shared_prefix_workspace_size(
   const int64_t rows =
       takes_tiles(batch * group, block_size, num_kv_heads, head_dim, dtype) ? kTileRows : kRows;
   const int64_t own = decode_units(batch, group), over = prefix_units(batch, group, rows);
-  const int64_t target =
-      rows == kTileRows ? prefix_target(over, num_kv_heads) : target_items();
-  return part_bytes(own, max_items(own, num_kv_heads, max_keys, target_items()), kRows, head_dim) +
+  const int64_t target = rows == kTileRows ? prefix_target(over, num_kv_heads)
+                                           : rows_target(over, num_kv_heads, head_dim);
+  return part_bytes(own, max_items(own, num_kv_heads, max_keys,
+                                   rows_target(own, num_kv_heads, head_dim)), kRows, head_dim) +
          part_bytes(over, max_items(over, num_kv_heads, prefix_len, target), rows, head_dim);
 }
 
@@ -441,7 +473,7 @@ extern "C" int mlr_paged_decode_shared_prefix(
               workspace_bytes, need);
   hipStream_t s = static_cast<hipStream_t>(stream);
   const int64_t group = num_q_heads / num_kv_heads;
-  if (shares_tiles(batch, group, block_size, num_kv_heads, head_dim, dtype)) {
+  if (shares_tiles(group, block_size, num_kv_heads, head_dim, dtype)) {
     ScoredParams p = params_of(o, kModeShared);
     p.prefix = prefix_table;
     p.prefix_width = prefix_blocks;
@@ -459,6 +491,7 @@ extern "C" int mlr_paged_decode_shared_prefix(
   ScoredParams own = params_of(o, kModeDecode);
   own.tiles = static_cast<int>(ceil_div(group, kRows));
   own.units = static_cast<int>(decode_units(batch, group));
+  own.target = rows_target(own.units, own.hkv, own.d);
   own.start = prefix_len;
   own.force_partial = true;
   const int64_t own_items = max_items(own.units, own.hkv, max_keys, own.target);
@@ -471,7 +504,8 @@ extern "C" int mlr_paged_decode_shared_prefix(
   over.units = over.tiles = static_cast<int>(prefix_units(batch, group, rows));
   over.start = prefix_len;
   over.force_partial = true;
-  if (tiles) over.target = prefix_target(over.units, over.hkv);
+  over.target = tiles ? prefix_target(over.units, over.hkv)
+                      : rows_target(over.units, over.hkv, over.d);
   const int64_t over_items = max_items(over.units, over.hkv, prefix_len, over.target);
   place_parts(over, ws, over_items, rows);
   const int rc = tiles ? launch_scored_tiles(over, dtype, static_cast<unsigned>(over_items), s)

@@ -271,12 +271,14 @@ __global__ __launch_bounds__(256) void scored_rows_kernel(ScoredParams p) {
     __syncthreads();
     const int unit = __builtin_amdgcn_readfirstlane(s_unit);
     const int part = __builtin_amdgcn_readfirstlane(s_split);
-    const bool alone = s_of == 1 && !p.force_partial;
+    const int parts = __builtin_amdgcn_readfirstlane(s_of);
+    const bool alone = parts == 1 && !p.force_partial;
     const Unit t = unit_of(p, unit, kRows);
+    const int len = item_len(t, parts, 16);
     // Keys are below 2^31.
-    const int64_t from = unit_base(t) + static_cast<int64_t>(part) * split;
+    const int64_t from = unit_base(t) + static_cast<int64_t>(part) * len;
     const int k0 = __builtin_amdgcn_readfirstlane(static_cast<int>(min(from, int64_t(0x7fffff00))));
-    const int k1 = __builtin_amdgcn_readfirstlane(static_cast<int>(min(t.hi, from + split)));
+    const int k1 = __builtin_amdgcn_readfirstlane(static_cast<int>(min(t.hi, from + len)));
     const int lo = __builtin_amdgcn_readfirstlane(static_cast<int>(t.lo));
 
     // The lane's row: its query, its position and the keys that it sees.

@@ -126,7 +126,7 @@ void scored_tiles_kernel(ScoredParams p) {
   __shared__ __align__(1024) unsigned char ks0[kHalves][kTileB], ks1[kHalves][kTileB];
   __shared__ __align__(1024) unsigned char vs0[kHalves][kTileB], vs1[kHalves][kTileB];
   __shared__ int64_t s_keys[kThreads / 64];
-  __shared__ int s_count[kThreads / 64], s_unit, s_part, s_of, s_all, s_odd;
+  __shared__ int s_count[kThreads / 64], s_most[kThreads / 64], s_unit, s_part, s_of, s_all, s_odd;
   const int tid = threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int w = wave & 3, half = wave >> 2;
@@ -182,14 +182,30 @@ void scored_tiles_kernel(ScoredParams p) {
     const int per = (p.units + kThreads - 1) / kThreads;
     const int u_lo = min(tid * per, p.units), u_hi = min(u_lo + per, p.units);
     int64_t keys = 0;
-    for (int u = u_lo; u < u_hi; ++u) keys += unit_len(unit_of(p, u, kTileRows));
+    int most = 0;
+    for (int u = u_lo; u < u_hi; ++u) {
+      const int64_t len = unit_len(unit_of(p, u, kTileRows));
+      keys += len;
+      most = max(most, static_cast<int>(len));
+    }
 #pragma unroll
-    for (int o = 32; o > 0; o >>= 1) keys += __shfl_xor(keys, o);
-    if (lane == 0) s_keys[wave] = keys;
+    for (int o = 32; o > 0; o >>= 1) {
+      keys += __shfl_xor(keys, o);
+      most = max(most, __shfl_xor(most, o));
+    }
+    if (lane == 0) {
+      s_keys[wave] = keys;
+      s_most[wave] = most;
+    }
     __syncthreads();
     keys = 0;
-    for (int i = 0; i < kThreads / 64; ++i) keys += s_keys[i];
-    split = split_of(keys, p);
+    for (int i = 0; i < kThreads / 64; ++i) {
+      keys += s_keys[i];
+      most = max(most, s_most[i]);
+    }
+    // A prefill's units stay whole unless splits pay.
+    if (p.mode != kModePrefill || splits_pay(static_cast<int64_t>(p.units) * p.hkv, most, p.ncu))
+      split = split_of(keys, p);
     int own = 0;
     for (int u = u_lo; u < u_hi; ++u) own += unit_items(unit_of(p, u, kTileRows), split);
     int before = own;
@@ -230,14 +246,16 @@ void scored_tiles_kernel(ScoredParams p) {
   const int unit = __builtin_amdgcn_readfirstlane(s_unit);
   if (unit < 0) return;  // uniform: no item left for this workgroup
   const int part = __builtin_amdgcn_readfirstlane(s_part);
-  const bool alone = s_of == 1 && !p.force_partial;
+  const int parts = __builtin_amdgcn_readfirstlane(s_of);
+  const bool alone = parts == 1 && !p.force_partial;
   const Unit t = unit_of(p, unit, kTileRows);
   if (t.r0 >= t.rows) return;
+  const int len = item_len(t, parts, kTile);
   const int k_lo =
-      __builtin_amdgcn_readfirstlane(static_cast<int>(unit_base(t) + (p.whole ? 0 : static_cast<int64_t>(part) * split)));
+      __builtin_amdgcn_readfirstlane(static_cast<int>(unit_base(t) + static_cast<int64_t>(part) * len));
   const int low = __builtin_amdgcn_readfirstlane(static_cast<int>(t.lo));  // first key seen
   const int k_hi = __builtin_amdgcn_readfirstlane(
-      static_cast<int>(min(t.hi, static_cast<int64_t>(k_lo) + split)));
+      static_cast<int>(min(t.hi, static_cast<int64_t>(k_lo) + len)));
 
   // This half's tiles [t_lo, t_hi) of the item's, taken from the last to the
   // first: a bias by distance makes the last keys the heaviest, and the running
