@@ -262,8 +262,8 @@ def rotary_frequencies(rotary_dim: int, base: float = 10000.0, *, scaling: str |
     - "ntk": base * factor ** (rotary_dim / (rotary_dim - 2)) in place of base;
     - "yarn": f_i where a pair turns more than beta_fast times over
       original_max_position positions, f_i / factor where fewer than beta_slow
-      times, and between the two a mix linear in the pair's index; attention_factor
-      is 0.1 ln(factor) + 1 (1 otherwise).
+      times, and between the two (rounded outwards to whole pairs) a mix linear in
+      the pair's index; attention_factor is 0.1 ln(factor) + 1 (1 otherwise).
     """
     if rotary_dim <= 0 or rotary_dim % 2:
         raise ValueError("rotary_dim must be a positive even number")

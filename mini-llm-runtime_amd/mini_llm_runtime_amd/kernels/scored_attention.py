@@ -1,6 +1,6 @@
 """Paged attention with capped or biased scores, with prefixes that are seen
 whole, and over a prefix that a decode batch shares (csrc/scored_rows.hip,
-csrc/scored_attention.hip). No reference counterpart; beside the plain calls of
+csrc/scored_tiles.hip, csrc/scored_attention.hip). No reference counterpart; beside the plain calls of
 ``paged_attention``, with the same caches, tables and packed batches.
 
 For the query at position i of head h and a key at j:
