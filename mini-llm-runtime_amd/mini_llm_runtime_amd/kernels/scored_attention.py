@@ -136,7 +136,7 @@ def paged_attention_decode_scored(
 
 
 def _validate_prefill(block_tables, query_start_loc, context_lens, prefix_lens, block_size,
-                      num_blocks, total_q) -> None:
+                      num_blocks, total_q, max_query_len=None) -> None:
     """One host sync for all metadata checks of a packed batch."""
     width = block_tables.shape[1]
     lens = query_start_loc[1:] - query_start_loc[:-1]
@@ -145,6 +145,7 @@ def _validate_prefill(block_tables, query_start_loc, context_lens, prefix_lens, 
     bad = used & ((block_tables < 0) | (block_tables >= num_blocks))
     flags = [query_start_loc[0] != 0, (lens < 0).any(), query_start_loc[-1] != total_q,
              (context_lens < lens).any(), (required > width).any(), bad.any()]
+    flags.append((lens > (total_q if max_query_len is None else max_query_len)).any())
     if prefix_lens is not None:
         flags.append(((prefix_lens < 0) | (prefix_lens > context_lens)).any())
     flags = torch.stack(flags).tolist()
@@ -157,7 +158,9 @@ def _validate_prefill(block_tables, query_start_loc, context_lens, prefix_lens, 
     if flags[3]:
         raise ValueError("context_lens must cover each request's tokens")
     _raise_table_errors(False, flags[4], flags[5])
-    if prefix_lens is not None and flags[6]:
+    if flags[6]:
+        raise ValueError("max_query_len must cover the longest chunk")
+    if prefix_lens is not None and flags[7]:
         raise ValueError("prefix_lens must lie between 0 and context_lens")
 
 
@@ -209,7 +212,7 @@ def paged_attention_prefill_scored(
     num_blocks, _, num_kv_heads, _ = k_cache.shape
     if validate:
         _validate_prefill(block_tables, query_start_loc, context_lens, prefix_lens, block_size,
-                          num_blocks, total_q)
+                          num_blocks, total_q, max_query_len)
     if max_query_len is None:
         max_query_len = int((query_start_loc[1:] - query_start_loc[:-1]).max().item())
     elif max_query_len < 0:
