@@ -595,10 +595,13 @@ def run_generation_step(model, scheduler: Scheduler,
     packed_logits = execute_model_batch(model=model, batch=batch, kv_cache=scheduler.kv_cache,
                                         decode_graphs=decode_graphs,
                                         prefill_graphs=prefill_graphs)
-    sampled = (greedy_sample if sampler is None else sampler)(packed_logits, batch)
-    if batch.input_token_ids.device.type == "cuda":
-        # Before any sampled token is committed to the scheduler.
-        kpa.check_decode_workspaces(batch.input_token_ids.device)
+    try:
+        sampled = (greedy_sample if sampler is None else sampler)(packed_logits, batch)
+    finally:
+        if batch.input_token_ids.device.type == "cuda":
+            # Before any sampled token is committed to the scheduler, and also where
+            # the sampler raised: what it refuses may be the NaN of a failed merge.
+            kpa.check_decode_workspaces(batch.input_token_ids.device)
     eos = ({rid for rid, tok in sampled.items() if tok == eos_token_id}
            if eos_token_id is not None else set())
     finished = scheduler.update_after_model(scheduler_output=scheduler_output,
