@@ -23,6 +23,11 @@ enum ScoredMode {
 
 constexpr int kMinSplit = 128;  // keys of the shortest split
 
+// tanh(y) = y (kTanh0 + kTanh1 y^2 + kTanh2 y^4 + kTanh3 y^6) for |y| <= 1/2, with a
+// relative error of 5.1e-7.
+constexpr float kTanh0 = 0.99999949f, kTanh1 = -0.33326618f;
+constexpr float kTanh2 = 0.13193061f, kTanh3 = -0.044465f;
+
 struct ScoredParams {
   const void *q, *k, *v;
   int64_t q_st, q_sh;
