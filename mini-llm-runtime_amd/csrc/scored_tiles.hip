@@ -324,14 +324,19 @@ void scored_tiles_kernel(ScoredParams p) {
   };
   const float scale = fabsf(p.scale);
   const float c2 = uniform(scale * kLog2e);
-  const float c1 = uniform(kCap ? scale / p.cap : 0.f);    // y = c1 s
+  const float c1 = uniform(kCap ? fminf(scale / p.cap, 1e37f) : 0.f);  // y = c1 s
   const float top = uniform(kCap ? p.cap * kLog2e : 0.f);  // the cap in base 2
-  // tanh(y) / y up to |y| = 1/2 (relative error 5.1e-7) and 1/4 (4.0e-7).
-  const float c3 = c1 * c1 * c1 * top, c5 = c1 * c1 * c3;
-  const float near = uniform(0.5f / c1), near2 = uniform(0.25f / c1);
-  const float b0 = uniform(0.99999949f * c1 * top), b1 = uniform(-0.33326618f * c3);
-  const float b2 = uniform(0.13193061f * c5), b3 = uniform(-0.044465f * c1 * c1 * c5);
-  const float a0 = uniform(0.99999960f * c1 * top), a1 = uniform(-0.33321908f * c3);
+  // tanh(y) / y up to |y| = 1/2 (relative error 5.1e-7) and 1/4 (4.0e-7), the powers
+  // of c1 in the factors. Scores whose square has no finite value take the
+  // exponential; under a cap so small (some 1e-7 of the scale) that the factors
+  // have none, all do, as a score of 0 times such a factor would be NaN.
+  const float c3 = c1 * c1 * c2, c5 = c1 * c1 * c3, c7 = c1 * c1 * c5;
+  const bool held = c7 < __FLT_MAX__;
+  const float near = uniform(held ? fminf(0.5f / c1, 1.8e19f) : -1.f);
+  const float near2 = uniform(held ? fminf(0.25f / c1, 1.8e19f) : -1.f);
+  const float b0 = uniform(kTanh0 * c2), b1 = uniform(kTanh1 * c3);
+  const float b2 = uniform(kTanh2 * c5), b3 = uniform(kTanh3 * c7);
+  const float a0 = uniform(0.99999960f * c2), a1 = uniform(-0.33321908f * c3);
   const float a2 = uniform(0.12841613f * c5);
   const float slope = kBias ? p.slopes[head] * kLog2e : 0.f;
 

@@ -23,7 +23,7 @@ from test_gpu_scored_attention import padded, pool, queries
 pytestmark = pytest.mark.gpu
 
 DTYPES = [torch.bfloat16, torch.float16, torch.float32]
-CAPS = [1e-8, 1e-4, 1e3, 1e5, 1e6, 1e8, 1e12, 1e20, 1e30]
+CAPS = [1e-30, 1e-20, 1e-12, 1e-8, 1e-4, 1e3, 1e5, 1e6, 1e8, 1e12, 1e20, 1e30]
 
 
 def attend(q, k, v, limit, scale, cap, dtype):
@@ -80,3 +80,21 @@ def test_caps(device, dtype, hq, hkv, d, bs, cap, size):
         qd[rows.to(device)], kd, vd, bt[0], prefix, bt.expand(len(rows), -1),
         (rows + 1).to(device), bs, softcap=cap)
     assert_within(got, want[rows], bound[rows], "a shared prefix")
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("scale", [1e12, -1e12, 1e-12])
+@pytest.mark.parametrize("d", [64, 128])
+def test_zero_scores_at_the_ends_of_cap_and_scale(device, dtype, scale, d):
+    """Queries of zero: every visible key weighs the same, on the kernel of many rows."""
+    n, bs = 200, 16
+    k, v, (table,) = pool([n], 2, d, bs, dtype, 73)
+    q = torch.zeros(n, 6, d, dtype=dtype)
+    for cap in (1e-30, 1e30):
+        want, bound = attend(q, gather(k, table, n, bs), gather(v, table, n, bs),
+                             torch.arange(1, n + 1), abs(scale), cap, dtype)
+        got = paged_attention_prefill_scored(
+            q.to(device), k.to(device), v.to(device), padded([table]).to(device),
+            torch.tensor([0, n], device=device), torch.tensor([n], device=device), bs, softcap=cap,
+            scale=scale)
+        assert_within(got, want, bound, f"cap {cap}")
