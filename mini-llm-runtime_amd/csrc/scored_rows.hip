@@ -180,28 +180,41 @@ struct Rows {
   }
 };
 
-// x in units of the natural exponent -> capped and biased.
-template <typename T, bool kCap>
-__device__ __forceinline__ float score(float x, const ScoredParams &p, float inv_cap, float slope,
-                                       float dist) {
-  if constexpr (kCap) {
-    if constexpr (sizeof(T) == 4) {
-      x = p.cap * tanhf(x * inv_cap);
-    } else {
-      // y P(y^2) near 0, which keeps scores that lie far below the cap; from 1/2 on
-      // 1 - 2 / (exp(2 y) + 1), an absolute error of 4e-7. Either is within 9e-7 of
-      // the score, whatever the cap.
-      const float y = x * inv_cap, u = y * y;
-      const float near = y * fmaf(u, fmaf(u, fmaf(u, kTanh3, kTanh2), kTanh1), kTanh0);
-      const float e = __builtin_amdgcn_exp2f(y * (2.f * kLog2e));
-      const float far = 1.f - 2.f * __builtin_amdgcn_rcpf(e + 1.f);
-      x = p.cap * (fabsf(y) <= 0.5f ? near : far);
+// Caps four scores of a lane, in units of the natural exponent. In 16-bit types y P(y^2)
+// near 0, which keeps scores that lie far below the cap, and from 1/2 on 1 - 2 /
+// (exp(2 y) + 1), an absolute error of 4e-7. Either is within 9e-7 of the score,
+// whatever the cap. The wave leaves out the second where no score needs it.
+template <typename T>
+__device__ __forceinline__ void cap_scores(float (&x)[4], float cap, float inv_cap) {
+  if constexpr (sizeof(T) == 4) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) x[i] = cap * tanhf(x[i] * inv_cap);
+  } else {
+    float y[4], t[4];
+    bool near = true;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      y[i] = x[i] * inv_cap;
+      near = near && fabsf(y[i]) <= 0.5f;
+      const float u = y[i] * y[i];
+      t[i] = y[i] * fmaf(u, fmaf(u, fmaf(u, kTanh3, kTanh2), kTanh1), kTanh0);
     }
+    if (__any(!near)) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const float e = __builtin_amdgcn_exp2f(y[i] * (2.f * kLog2e));
+        const float far = 1.f - 2.f * __builtin_amdgcn_rcpf(e + 1.f);
+        t[i] = fabsf(y[i]) <= 0.5f ? t[i] : far;
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i) x[i] = cap * t[i];
   }
-  return x - slope * dist;
 }
 
-template <typename T, int D, bool kCap, bool kPaged16, bool kPrefill>
+// kPrefill: the rows are tokens of chunks, not requests. kUnlike: rows of a unit may
+// see different keys (chunks, and requests shorter than the prefix that they share).
+template <typename T, int D, bool kCap, bool kPaged16, bool kPrefill, bool kUnlike>
 __global__ __launch_bounds__(256) void scored_rows_kernel(ScoredParams p) {
   constexpr int kVe = D / 16;  // elements of a row that a lane of P V holds
   constexpr int kE = 16 / sizeof(T);
@@ -304,6 +317,7 @@ __global__ __launch_bounds__(256) void scored_rows_kernel(ScoredParams p) {
       pos = static_cast<int>(clamp64(p.ctx[row], 0, 0x7fffffff)) - 1;
       limit = min(limit, pos + 1);
     }
+    const int own_end = live ? limit : 0x7fffffff;  // first key that the row does not see
     if (!live) limit = 0;
     const float slope = p.slopes ? p.slopes[head] : 0.f;
     uint4 q[M::kK];
@@ -359,13 +373,16 @@ __global__ __launch_bounds__(256) void scored_rows_kernel(ScoredParams p) {
               s = __builtin_amdgcn_mfma_f32_16x16x4f32(a[e], c[e], s, 0, 0, 0);
           }
         }
+        float y[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) y[i] = s[i] * p.scale;
+        if constexpr (kCap) cap_scores<T>(y, p.cap, inv_cap);
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
           const int key = key0 + 4 * g + i;
-          const float dist = static_cast<float>(abs(pos - key));
-          const float y = score<T, kCap>(s[i] * p.scale, p, inv_cap, slope, dist);
+          y[i] -= slope * static_cast<float>(abs(pos - key));
           const bool seen = (ok[b] >> i & 1) && key >= lo && key < limit;
-          x[b][i] = seen ? y : -INFINITY;
+          x[b][i] = seen ? y[i] : -INFINITY;
           top = fmaxf(top, x[b][i]);
         }
       }
@@ -387,7 +404,7 @@ __global__ __launch_bounds__(256) void scored_rows_kernel(ScoredParams p) {
           l += pr[i];
         }
         bool plain = true;
-        if constexpr (kPrefill) {
+        if (kUnlike && __builtin_expect(__any(own_end < min(b0 + b * step + 16, k1)), 0)) {
           // Keys that some row does not see: a V that is not finite must not
           // reach that row as 0 * V.
           bool bad = false;
@@ -403,7 +420,7 @@ __global__ __launch_bounds__(256) void scored_rows_kernel(ScoredParams p) {
             }
           plain = __builtin_amdgcn_ballot_w64(bad) == 0;
         }
-        if (plain) {
+        if (__builtin_expect(plain, 1)) {
 #pragma unroll
           for (int n = 0; n < kVe; ++n) {
             if constexpr (sizeof(T) == 2) {
@@ -505,10 +522,12 @@ __global__ __launch_bounds__(256) void scored_rows_kernel(ScoredParams p) {
 
 template <typename T, int D>
 int launch_rows(const ScoredParams &p, unsigned grid, hipStream_t stream) {
-  const bool paged16 = p.block_size % 16 == 0, prefill = p.mode == kModePrefill;
-#define MLR_ROWS(C, B, F) scored_rows_kernel<T, D, C, B, F><<<grid, 256, 0, stream>>>(p)
-#define MLR_ROWS_B(C, B) \
-  if (prefill) MLR_ROWS(C, B, true); else MLR_ROWS(C, B, false);
+  const bool paged16 = p.block_size % 16 == 0;
+#define MLR_ROWS(C, B, F, U) scored_rows_kernel<T, D, C, B, F, U><<<grid, 256, 0, stream>>>(p)
+#define MLR_ROWS_B(C, B)                                        \
+  if (p.mode == kModePrefill) MLR_ROWS(C, B, true, true);       \
+  else if (p.mode == kModePrefix) MLR_ROWS(C, B, false, true);  \
+  else MLR_ROWS(C, B, false, false);
   if (p.cap > 0) {
     if (paged16) { MLR_ROWS_B(true, true) } else { MLR_ROWS_B(true, false) }
   } else {
