@@ -541,8 +541,12 @@ void scored_tiles_kernel(ScoredParams p) {
         for (int j = 0; j < KB; ++j)
 #pragma unroll
           for (int e = 0; e < 16; ++e) {
-            const float x = __builtin_amdgcn_exp2f(s[j][e] * (2.f * kLog2e * c1));
-            s[j][e] = top * (1.f - 2.f * __builtin_amdgcn_rcpf(x + 1.f)) - m;
+            // Score by score: the exponential's error is some 4e-7 of the cap.
+            const float x = s[j][e], u = x * x;
+            const float w = __builtin_amdgcn_exp2f(x * (2.f * kLog2e * c1));
+            const float far = top * (1.f - 2.f * __builtin_amdgcn_rcpf(w + 1.f));
+            const float low = x * fmaf(u, fmaf(u, fmaf(u, b3, b2), b1), b0);
+            s[j][e] = (fabsf(x) <= near ? low : far) - m;
           }
       } else {
 #pragma unroll

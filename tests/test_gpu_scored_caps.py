@@ -98,3 +98,26 @@ def test_zero_scores_at_the_ends_of_cap_and_scale(device, dtype, scale, d):
             torch.tensor([0, n], device=device), torch.tensor([n], device=device), bs, softcap=cap,
             scale=scale)
         assert_within(got, want, bound, f"cap {cap}")
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("hq,hkv,d", [(14, 2, 64), (8, 2, 128)])
+def test_one_score_near_a_large_cap(device, dtype, hq, hkv, d):
+    """A key whose score with one query is most of the cap, among ordinary ones: the
+    other queries keep the accuracy of theirs."""
+    n, bs, cap = 200, 16, 1e6
+    k, v, (table,) = pool([n], hkv, d, bs, dtype, 74)
+    q = queries(n, hq, d, dtype, 75, 2.0)
+    q[:, :, 0] = 0.0
+    q[90, :, 0] = 400.0
+    k[table[20 // bs], 20 % bs, :, 0] = 7e5 * d ** 0.5 / 400.0
+    want, bound = attend(q, gather(k, table, n, bs), gather(v, table, n, bs),
+                         torch.arange(1, n + 1), d ** -0.5, cap, dtype)
+    qd, kd, vd, bt = q.to(device), k.to(device), v.to(device), padded([table]).to(device)
+    for first in (0, 88):  # a chunk of many rows, and its last rows
+        rows = slice(first, min(n, first + (5 if first else n)))
+        ctx = rows.stop
+        got = paged_attention_prefill_scored(
+            qd[rows], kd, vd, bt, torch.tensor([0, ctx - first], device=device),
+            torch.tensor([ctx], device=device), bs, softcap=cap)
+        assert_within(got, want[rows], bound[rows], f"rows from {first}")
