@@ -179,8 +179,18 @@ bool takes_tiles(int64_t rows, int64_t block_size, int64_t hkv, int64_t d, int d
 // kernel's stages take a whole CU, so a request's few keys would hold one each;
 // there the requests' own keys go to the other kernel (16 and 64 requests of 32/8
 // heads of 128: 33.9 and 45.1 us, in one launch 36.2 and 53.3 us).
-bool shares_tiles(int64_t group, int64_t block_size, int64_t hkv, int64_t d, int dtype) {
-  return d <= 64 && group <= kTileRows && fits_tiles(block_size, hkv, d, dtype);
+// So they do where there are many of them: a unit's 128 rows of partial results hold
+// one group only, 32 KB for each request and KV head, and from some four for every CU
+// on reading and writing them takes longer than the launch saved. 4,096 shared and
+// up to 300 own keys, one launch and two, us: 12/12 heads of 64, 64, 128 and 256
+// requests 36.0 and 38.2, 53.7 and 47.4, 97.1 and 77.1; 32/32 heads, 32 and 128
+// requests 42.6 and 52.2, 123.5 and 93.1; 8,192 shared and up to 1,000 own: 14/2 heads,
+// 512 requests 83.0 and 86.1; 32/8 heads, 128 requests 65.0 and 69.5; but 2,000 shared
+// and up to 100 own, 16/4 heads, 256 requests: 44.6 and 37.4.
+bool shares_tiles(int64_t batch, int64_t group, int64_t block_size, int64_t hkv, int64_t d,
+                  int dtype) {
+  return d <= 64 && group <= kTileRows && batch * hkv <= 4 * static_cast<int64_t>(cus()) &&
+         fits_tiles(block_size, hkv, d, dtype);
 }
 // Two workgroups fit a CU; the last split of each unit is half full on average, and
 // a second round of workgroups would cost more than longer splits.
@@ -427,7 +437,7 @@ extern "C" size_t mlr_paged_decode_shared_prefix_workspace_size(
   if (batch <= 0 || num_kv_heads <= 0 || num_q_heads <= 0 || head_dim <= 0 || block_size <= 0)
     return 0;
   const int64_t group = num_q_heads / num_kv_heads, max_keys = max_blocks * block_size;
-  if (shares_tiles(group, block_size, num_kv_heads, head_dim, dtype)) {
+  if (shares_tiles(batch, group, block_size, num_kv_heads, head_dim, dtype)) {
     const int64_t units = prefix_units(batch, group, kTileRows) + batch;
     return part_bytes(units, max_items(units, num_kv_heads, std::max(prefix_len, max_keys),
                                        shared_target(units, num_kv_heads)), kTileRows, head_dim);
@@ -473,7 +483,7 @@ extern "C" int mlr_paged_decode_shared_prefix(
               workspace_bytes, need);
   hipStream_t s = static_cast<hipStream_t>(stream);
   const int64_t group = num_q_heads / num_kv_heads;
-  if (shares_tiles(group, block_size, num_kv_heads, head_dim, dtype)) {
+  if (shares_tiles(batch, group, block_size, num_kv_heads, head_dim, dtype)) {
     ScoredParams p = params_of(o, kModeShared);
     p.prefix = prefix_table;
     p.prefix_width = prefix_blocks;
