@@ -140,7 +140,7 @@ __device__ __forceinline__ int item_len(const Unit &t, int n, int step) {
 // In floating point, as the 64-bit division takes longer; the same everywhere.
 __device__ __forceinline__ int split_of(int64_t total_keys, const ScoredParams &p) {
   const double s = static_cast<double>(total_keys) * p.hkv / static_cast<double>(p.target);
-  const int split = s < 2.0e9 ? static_cast<int>(s) + 1 : 2000000000;
+  const int split = s < 2.0e9 ? static_cast<int>(s) + 1 : 0x7fffff80;  // past every length
   return ((split > kMinSplit ? split : kMinSplit) + 63) & ~63;
 }
 

@@ -213,8 +213,12 @@ int64_t tiles_target(int64_t units, int64_t hkv) {
 // the kernel of 128 rows cost a pass over FP32 partial results of every unit, so
 // they pay only where units are few and their keys many (see splits_pay); the kernel
 // decides that from the lengths, and what no lengths could change is decided here.
+// On the other kernel a call of so many units that their partial results would pass
+// kMostParts (a batch of one long prompt and many short ones has room for as many
+// long ones) has enough items without splits.
+constexpr size_t kMostParts = size_t(256) << 20;
 struct PrefillPlan {
-  int64_t rows, units, items;
+  int64_t rows, units, items, target;
   bool whole, parts;
 };
 PrefillPlan plan_prefill(int64_t seqs, int64_t max_q, int64_t max_keys, int64_t block_size,
@@ -224,10 +228,14 @@ PrefillPlan plan_prefill(int64_t seqs, int64_t max_q, int64_t max_keys, int64_t 
   const bool tiles = takes_tiles(max_q * group, block_size, hkv, d, dtype);
   n.rows = tiles ? kTileRows : kRows;
   n.units = prefill_units(seqs, max_q, group, n.rows);
-  n.whole = tiles && !splits_pay(n.units * hkv, max_keys, cus());
-  n.items = n.whole   ? n.units * hkv
-            : tiles ? max_items(n.units, hkv, max_keys, tiles_target(n.units, hkv))
-                    : max_items(n.units, hkv, max_keys, rows_target(n.units, hkv, d));
+  n.target = tiles ? tiles_target(n.units, hkv) : rows_target(n.units, hkv, d);
+  n.items = max_items(n.units, hkv, max_keys, n.target);
+  n.whole = tiles ? !splits_pay(n.units * hkv, max_keys, cus())
+                  : part_bytes(n.units, n.items, kRows, d) > kMostParts;
+  if (n.whole) {
+    n.target = 1;  // a split as long as all keys
+    n.items = n.units * hkv;
+  }
   n.parts = !n.whole && max_keys > kMinSplit;
   return n;
 }
@@ -420,7 +428,7 @@ extern "C" int mlr_paged_prefill_scored(
   p.units = static_cast<int>(n.units);
   p.tiles = static_cast<int>(n.units / num_seqs);
   p.whole = n.whole;
-  p.target = n.rows == kTileRows ? tiles_target(n.units, p.hkv) : rows_target(n.units, p.hkv, p.d);
+  p.target = n.target;
   const int rows = static_cast<int>(n.rows);
   if (n.parts) place_parts(p, static_cast<char *>(workspace), n.items, rows);
   hipStream_t s = static_cast<hipStream_t>(stream);

@@ -20,3 +20,16 @@ def test_shared_prefix_workspace(batch, hq, hkv, most, dtype):
     size = _lib.load().mlr_paged_decode_shared_prefix_workspace_size(
         batch, hq, hkv, 64, 8192, 576, 16, _lib.DTYPE_CODES[dtype])
     assert 0 < size <= most * MB
+
+
+@pytest.mark.parametrize("dtype,block_size", [(torch.float32, 16), (torch.bfloat16, 24)])
+@pytest.mark.parametrize("hq,hkv,d", [(14, 2, 64), (32, 8, 128)])
+def test_prefill_workspace(dtype, block_size, hq, hkv, d):
+    """One long prompt in a batch of many sequences does not reserve partial results
+    for as many long ones."""
+    size = _lib.load().mlr_paged_prefill_scored_workspace_size
+    code = _lib.DTYPE_CODES[dtype]
+    for seqs in (1, 8, 64, 1000):
+        for longest in (1, 16, 512, 4096, 32768):
+            assert size(seqs, longest, 4096, block_size, hq, hkv, d, code) <= 256 * MB
+    assert size(8, 512, 4096, block_size, hq, hkv, d, code) > 0
