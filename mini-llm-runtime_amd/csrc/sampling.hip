@@ -459,6 +459,11 @@ __device__ Element find_listed(const Scan<2> &l, uint64_t target, Shared &sh) {
   return {value_of(v), static_cast<int>(static_cast<uint32_t>(v)), e.before_w + e.w};
 }
 
+// Temperatures are held between these: below the least, every FP32 logit but those
+// equal to the largest weighs 0, and above the most all weigh the same, while the
+// 64-bit arithmetic stays clear of infinities.
+constexpr double kLeastTemp = 1e-290, kMostTemp = 1e290;
+
 // A row's source and parameters.
 template <typename T>
 struct Row {
@@ -473,6 +478,7 @@ __device__ __forceinline__ bool row_of(const SampleParams &p, int64_t out, Row<T
   if (src < 0 || src >= p.num_logit_rows) return false;
   r.x = static_cast<const T *>(p.logits) + src * p.row_st;
   r.temp = p.temperature ? static_cast<double>(p.temperature[out]) : p.temperature_v;
+  if (r.temp > 0) r.temp = fmin(fmax(r.temp, kLeastTemp), kMostTemp);
   r.top_p = p.top_p ? static_cast<double>(p.top_p[out]) : p.top_p_v;
   r.min_p = p.min_p ? static_cast<double>(p.min_p[out]) : p.min_p_v;
   r.top_k = !p.top_k       ? p.top_k_v
@@ -587,7 +593,7 @@ struct Far {
   int bin;
 };
 __device__ __forceinline__ Far far_of(double min_p, double temp, const Scale &sc) {
-  const double far = -temp * log(min_p);
+  const double far = temp < kMostTemp ? -temp * log(min_p) : INFINITY;
   return {far, static_cast<int>(fmin(far * static_cast<double>(sc.bins), kBins - 1.0))};
 }
 
