@@ -1079,7 +1079,8 @@ extern "C" int mlr_sample_tokens(const void *logits, int64_t row_stride, int64_t
   MLR_REQUIRE(dtype == MLR_DTYPE_F32 || dtype == MLR_DTYPE_F16 || dtype == MLR_DTYPE_BF16,
               "mlr_sample_tokens: unsupported dtype %d", dtype);
   if (num_rows == 0) return MLR_OK;
-  MLR_REQUIRE(logits && uniforms && tokens, "mlr_sample_tokens: null pointer");
+  MLR_REQUIRE((logits || num_logit_rows == 0) && uniforms && tokens,
+              "mlr_sample_tokens: null pointer");
   const size_t need = mlr_sample_tokens_workspace_size(num_rows, vocab);
   MLR_REQUIRE(need == 0 || (workspace && workspace_bytes >= need &&
                             reinterpret_cast<uintptr_t>(workspace) % 8 == 0),

@@ -8,6 +8,7 @@ import math
 import pytest
 import torch
 
+from mini_llm_runtime_amd.kernels.sampling import sample_tokens
 from test_gpu_sampling import check, logits_of, uniforms_of
 
 pytestmark = pytest.mark.gpu
@@ -26,3 +27,12 @@ def test_temperatures(device, dtype, vocab, temperature, params):
     x[:, 17] = x[:, 900] = top  # a draw between equal ones where all else weighs 0
     x[4:, 30] = top[4:].float().abs().to(dtype) * 2
     check(x, uniforms_of(6, 92), temperature=temperature, **params)
+
+
+@pytest.mark.parametrize("vocab", [1000, 130003])
+def test_no_logits_rows_at_all(device, vocab):
+    """Every row id is out of range then."""
+    tokens, logprobs = sample_tokens(torch.empty(0, vocab, device=device),
+                                     torch.full((3,), 0.5, device=device), return_logprobs=True,
+                                     rows=torch.tensor([0, -1, 7], device=device))
+    assert tokens.tolist() == [-1] * 3 and logprobs.tolist() == [-math.inf] * 3
