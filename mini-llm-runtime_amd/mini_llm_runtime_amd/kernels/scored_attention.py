@@ -207,12 +207,12 @@ def paged_attention_prefill_scored(
         if prefix_lens.shape != (seqs,):
             raise ValueError("prefix_lens must hold one length per sequence")
     out = _out(q, out, device)
-    if seqs == 0 or total_q == 0:
-        return out
     num_blocks, _, num_kv_heads, _ = k_cache.shape
     if validate:
         _validate_prefill(block_tables, query_start_loc, context_lens, prefix_lens, block_size,
                           num_blocks, total_q, max_query_len)
+    if seqs == 0 or total_q == 0:
+        return out
     if max_query_len is None:
         max_query_len = int((query_start_loc[1:] - query_start_loc[:-1]).max().item())
     elif max_query_len < 0:
