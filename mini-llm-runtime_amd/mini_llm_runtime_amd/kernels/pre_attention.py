@@ -269,8 +269,8 @@ def rotary_frequencies(rotary_dim: int, base: float = 10000.0, *, scaling: str |
         raise ValueError("rotary_dim must be a positive even number")
     if not base > 0:
         raise ValueError("base must be positive")
-    if not factor >= 1:
-        raise ValueError("factor must be at least 1")
+    if not 1 <= factor < math.inf:
+        raise ValueError("factor must be at least 1, and finite")
     if scaling not in (None, "linear", "ntk", "yarn"):
         raise ValueError(f"unknown rotary scaling {scaling!r}")
     half = rotary_dim // 2
@@ -284,6 +284,8 @@ def rotary_frequencies(rotary_dim: int, base: float = 10000.0, *, scaling: str |
     if scaling == "linear":
         freq = freq / factor
     elif scaling == "yarn":
+        if not base > 1:  # the pairs turn ever slower
+            raise ValueError("yarn scaling needs a base above 1")
         if original_max_position <= 0:
             raise ValueError("yarn scaling needs original_max_position")
         if not beta_fast > beta_slow > 0:

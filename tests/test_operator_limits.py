@@ -3,10 +3,13 @@ here reaches a GPU."""
 
 from __future__ import annotations
 
+import math
+
 import pytest
 import torch
 
 from mini_llm_runtime_amd import _lib
+from mini_llm_runtime_amd.kernels.pre_attention import rotary_frequencies
 
 MB = 1 << 20
 
@@ -33,3 +36,17 @@ def test_prefill_workspace(dtype, block_size, hq, hkv, d):
         for longest in (1, 16, 512, 4096, 32768):
             assert size(seqs, longest, 4096, block_size, hq, hkv, d, code) <= 256 * MB
     assert size(8, 512, 4096, block_size, hq, hkv, d, code) > 0
+
+
+@pytest.mark.parametrize("base", [1.0, 0.5])
+def test_yarn_needs_falling_frequencies(base):
+    with pytest.raises(ValueError, match="base above 1"):
+        rotary_frequencies(8, base, scaling="yarn", factor=2.0, original_max_position=64)
+    freq, m = rotary_frequencies(8, 1.0, scaling="ntk", factor=8.0)
+    assert m == 1.0 and abs(float(freq[-1]) * 8.0 - 1.0) < 1e-6
+
+
+@pytest.mark.parametrize("scaling", ["linear", "ntk", "yarn"])
+def test_factor_must_be_finite(scaling):
+    with pytest.raises(ValueError, match="factor"):
+        rotary_frequencies(8, scaling=scaling, factor=math.inf, original_max_position=64)
