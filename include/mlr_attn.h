@@ -628,8 +628,9 @@ int mlr_qk_norm_rope_write(const void *qkv, int64_t qkv_stride_t, const void *q_
  * no key (or none with a score above -inf) gets zeros. FP32, fp16 and bf16,
  * head_dim a multiple of 8 (FP32: 4) up to 128, any block_size, fewer than 2^31
  * positions per table; q rows, the cache and the row strides are 16-byte
- * aligned, out rows have unit stride. FP32 scores and sums; 16-bit types round the
- * probabilities once as operands of the matrix cores and the result once.
+ * aligned, out rows have unit stride. softcap is 0 or in [1e-30, 1e30]. FP32 scores
+ * and sums; 16-bit types round the probabilities once as operands of the matrix cores
+ * and the result once, and a capped score is within 9e-7 of its own size.
  * Block ids out of range mask their keys, whose K and V are not read; V rows of
  * keys that no query of the call sees may hold anything. Workspaces (sizes by
  * the functions beside each call, 0 where none is needed) need no preparation
@@ -707,7 +708,8 @@ int mlr_paged_decode_shared_prefix(const void *q, int64_t q_stride_b, int64_t q_
  *   and logprobs[r] (may be null) is log(w / S).
  * temperature <= 0 (or NaN), or an infinite maximum: the first of the order,
  * logprob 0. A row without a value above -inf, or a row id out of range: -1 and
- * -inf. NaN logits are never drawn. vocab <= 2^23. The workspace (0 bytes where a
+ * -inf. NaN logits are never drawn, nor tokens that weigh less than 2^-45 of the
+ * first (past 2^18 tokens: of 2^(log2 vocab - 63)). vocab <= 2^23. The workspace (0 bytes where a
  * batch fills the GPU by itself) needs no preparation.
  */
 size_t mlr_sample_tokens_workspace_size(int64_t num_rows, int64_t vocab);

@@ -46,11 +46,11 @@
 // (kernels/reference/paged_attention.py:346-434): FP32 softmax statistics,
 // FP32 accumulation of P@V and one rounding of the output. Three roundings
 // differ from the reference and stay far inside the 2e-2 tolerance of its
-// bf16 tests: q*scale*log2(e) is rounded to bf16 (relative 2^-9 per element,
+// bf16 tests: q*scale*log2(e) is rounded to bf16 (relative 2^-8 per element,
 // the size of the reference's own bf16 rounding of q.k at :411-413, which is
 // not done here), and P is rounded to bf16 as the MFMA operand. fp16 runs the
 // same kernel with fp16 operands (the same two roundings, to fp16: relative
-// 2^-12), round-to-nearest-even throughout.
+// 2^-11), round-to-nearest-even throughout.
 //
 // A call whose work items leave CUs idle (one sequence's chunk over a long
 // context, few heads) cuts the key range of each item over several workgroups

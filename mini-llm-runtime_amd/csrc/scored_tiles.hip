@@ -17,7 +17,8 @@
 //     the running maximum only when a tile exceeds it by 2^kLazy: probabilities
 //     stay below 2^kLazy, numerator and sum share m, and most tiles rescale nothing.
 //   O^T[D x 32 rows] += V^T P^T: B = P^T straight from the S^T registers, rounded
-//     to the 16-bit type (relative 2^-9, 2^-12), A = V^T by transposing LDS reads.
+//     to the 16-bit type (by at most 2^-8 of it in bf16, 2^-11 in fp16; see
+//     scored_rows.hip), A = V^T by transposing LDS reads.
 //
 // Tiles are taken from the last to the first, as a bias by distance makes the last
 // keys the heaviest, and the two key halves run their vector and matrix phases in
@@ -29,10 +30,11 @@
 // tanh(y) = y P(y^2) with three terms beyond the first (relative error 5.1e-7
 // for |y| <= 1/2) adds 16 and with two (4.0e-7 for |y| <= 1/4) 12, so a tile takes
 // the shortest form that holds for all of its scores (with the order of the keys,
-// 101 -> 92 us on the first of these). Measured: capped bf16, 8 chunks of 512 tokens
-// after up to 3,584, 14/2 heads of 64: 36.0 GF in 78 us, 460 TF/s; biased fp16 prompts
-// at head size 128: 52.7 GF in 92 us, 570 TF/s; 64 requests over 8,192 shared keys
-// with their own: 20 us of the kernel; 32 over 24,576, head size 128: 30 us.
+// 101 -> 92 us on the first of these); where none does, the exponential or the
+// polynomial score by score. Measured: capped bf16, 8 chunks of 512 tokens after up to
+// 3,584, 14/2 heads of 64: 36.0 GF in 76 us, 470 TF/s; biased fp16 prompts at head size
+// 128: 52.7 GF in 89 us, 590 TF/s; 64 requests over 8,192 shared keys with their own:
+// 20 us of the kernel; 32 over 24,000, head size 128: 29 us.
 //
 // LDS rows are unpadded; the 16-byte chunk c of row r lies at c ^ swizzle(r),
 // which keeps the row reads of K and the transposing reads of V free of bank
@@ -158,7 +160,10 @@ void scored_tiles_kernel(ScoredParams p) {
       if (tid == 0) s_unit = seq * p.tiles + p.tiles - 1 - (rank - seq * p.tiles);
     } else {
       // By keys, then by sequence, then later rows first. The sequences' sizes
-      // are read once, into what will be the first stage.
+      // are read once, into what will be the first stage. Every workgroup does this,
+      // in time units * sequences, which pays for some chunks but not for many short
+      // ones: 32, 64 and 256 prompts of 128 tokens at 14/2 heads of 64 take 22, 63 and
+      // 1,668 us, the plain prefill, whose units have no order, 16, 30 and 128 us.
       Seq *seqs = reinterpret_cast<Seq *>(&ks0[0][0]);
       static_assert(sizeof(ks0) >= kRankSeqs * sizeof(Seq), "the sizes fit a stage");
       for (int q = tid; q < p.seqs; q += kThreads) {

@@ -31,7 +31,9 @@ def sample_tokens(logits: torch.Tensor, uniforms: torch.Tensor, *,
 
     A temperature of 0 or an infinite largest logit gives the first of the order
     (logprob 0); a row without a logit above -inf, or a rows[b] out of range, -1
-    (-inf). Logits of -inf or NaN are never drawn.
+    (-inf). Logits of -inf or NaN are never drawn. Weights are held to 2^-44 of the
+    largest (less finely past 2^18 tokens), so a token of less than half of that is
+    not drawn either.
     """
     if logits.ndim != 2 or logits.shape[1] == 0:
         raise ValueError("logits must have shape [num_rows, vocab]")

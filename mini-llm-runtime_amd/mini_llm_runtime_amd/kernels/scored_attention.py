@@ -11,7 +11,9 @@ For the query at position i of head h and a key at j:
 
 and the result is the softmax of x over the visible keys, times V. bf16, fp16
 and FP32; head_dim a multiple of 8 (FP32: 4) up to 128; any block size. Scores,
-statistics and sums are FP32, whatever the type.
+statistics and sums are FP32, whatever the type. In bf16 and fp16 the probabilities
+are rounded to the type before they meet V, at every head size, and a capped score is
+within 9e-7 of its own size.
 
 Workspaces come from torch's allocator on the current stream, call by call, so
 calls on different streams, or captured into different graphs, never share one.
