@@ -175,7 +175,9 @@ bool takes_tiles(int64_t rows, int64_t block_size, int64_t hkv, int64_t d, int d
 // A shared prefix on the kernel of 128 rows a unit, with each request's own keys
 // (all heads of a group in one unit) in the same launch: a launch less, also for
 // few rows (8,192 keys shared by 2, 8 and 64 requests of 14/2 heads of 64: 16.4,
-// 17.3 and 26.9 us, against 19.6, 22.9 and 29.6 us). At head sizes above 64 that
+// 17.3 and 26.9 us, against 19.6, 22.9 and 29.6 us), and for long keys of the
+// requests' own (2,000 shared and up to 4,000 own: 64 requests of 14/2 heads 29.1 and
+// 38.3 us, 32 of 12/12 heads 65.8 and 75.3 us). At head sizes above 64 that
 // kernel's stages take a whole CU, so a request's few keys would hold one each;
 // there the requests' own keys go to the other kernel (16 and 64 requests of 32/8
 // heads of 128: 33.9 and 45.1 us, in one launch 36.2 and 53.3 us).
