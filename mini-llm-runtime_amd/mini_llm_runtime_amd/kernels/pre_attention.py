@@ -319,7 +319,8 @@ def qk_norm_rope_write(qkv: torch.Tensor, positions: torch.Tensor, inv_freq: tor
     (normalised) values. The arithmetic is FP32 (angles in 64 bits: exact
     positions up to 2^53) with one rounding at the end.
 
-    positions int64 [T]; inv_freq [R / 2], used as FP32; k_cache and v_cache one
+    positions int64 [T]; inv_freq [R / 2], used as FP32 (converted in each call from
+    another type); k_cache and v_cache one
     contiguous layer [num_blocks, block_size, Hkv, D] in qkv's dtype;
     slot_mapping int32/int64 [T]: a token whose slot lies outside the cache
     (-1 in a padded batch) writes no k and v, and no two tokens may share a slot.
@@ -369,7 +370,7 @@ def qk_norm_rope_write(qkv: torch.Tensor, positions: torch.Tensor, inv_freq: tor
         raise ValueError("KV cache layers must be contiguous")
     if tokens == 0:
         return out
-    freq = _freq_fp32(inv_freq)
+    freq = inv_freq.to(torch.float32).contiguous()
     positions, slot_mapping = positions.contiguous(), slot_mapping.contiguous()
     many = tokens > 1
     lib = _lib.load()
