@@ -38,20 +38,31 @@ _SUPPORTED = (torch.float32, torch.float16, torch.bfloat16)
 # to bf16 casts its buffers), so that a call does not launch a conversion.
 # An entry keeps its source tensor alive, so the source's storage cannot be
 # reused while cached, and records the source's version counter, so an
-# in-place change of the buffer is seen.
+# in-place change of the buffer is seen. Copies that leave the cache stay
+# alive (head_dim / 2 numbers each): a graph may have recorded their address.
 _FREQ32: dict = {}
 _FREQ32_MAX = 64
+_FREQ32_PAST: list = []
 
 
 def _freq_fp32(inv_freq: torch.Tensor) -> torch.Tensor:
     if inv_freq.dtype == torch.float32 and inv_freq.is_contiguous():
         return inv_freq
+    if inv_freq.is_inference():  # no version counter
+        return inv_freq.to(torch.float32).contiguous()
     key = (inv_freq.data_ptr(), inv_freq.dtype, inv_freq.device, inv_freq.stride())
     hit = _FREQ32.get(key)
     if hit is not None and hit[0] is inv_freq and hit[1] == inv_freq._version:
         return hit[2]
     freq = inv_freq.to(torch.float32).contiguous()
+    if inv_freq.is_cuda:
+        if torch.cuda.is_current_stream_capturing():
+            return freq  # made by the graph's replays, for the graph alone
+        torch.cuda.current_stream(inv_freq.device).synchronize()  # any stream may use it
+    if hit is not None:
+        _FREQ32_PAST.append(hit[2])
     if len(_FREQ32) >= _FREQ32_MAX:
+        _FREQ32_PAST.extend(entry[2] for entry in _FREQ32.values())
         _FREQ32.clear()
     _FREQ32[key] = (inv_freq, inv_freq._version, freq)
     return freq
