@@ -570,11 +570,12 @@ class RandomSampler:
 
     def __init__(self, seed: int, *, temperature: float = 1.0, top_k: int = 0,
                  top_p: float = 1.0, min_p: float = 0.0) -> None:
-        self.generator = torch.Generator().manual_seed(seed)
+        self.generator = torch.Generator("cpu").manual_seed(seed)
         self.params = dict(temperature=temperature, top_k=top_k, top_p=top_p, min_p=min_p)
 
     def __call__(self, packed_logits: torch.Tensor, batch: ModelBatch) -> dict[str, int]:
-        numbers = torch.rand(len(batch.request_ids), generator=self.generator)
+        numbers = torch.rand(len(batch.request_ids), generator=self.generator,
+                             dtype=torch.float32, device="cpu")
         return random_sample(packed_logits, batch, numbers.to(packed_logits.device),
                              **self.params)
 

@@ -49,3 +49,21 @@ def test_an_error_of_the_sampler_passes_where_the_merge_was_sound(device):
 
     with torch.no_grad(), pytest.raises(KeyError, match="no such request"):
         run_generation_step(model, scheduler, sampler=broken)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float64])
+def test_random_sampler_under_other_defaults(device, dtype):
+    """The same tokens whatever the default device and dtype are."""
+    outs = []
+    for default in ("cpu", "cuda"):
+        model, scheduler = serving(device, torch.bfloat16)
+        before = torch.get_default_dtype()
+        with torch.device(default), torch.no_grad():
+            try:
+                torch.set_default_dtype(before if default == "cpu" else dtype)
+                sampler = RandomSampler(11, temperature=1.3)
+                outs.append([run_generation_step(model, scheduler, sampler=sampler)
+                             .sampled_token_ids for _ in range(4)])
+            finally:
+                torch.set_default_dtype(before)
+    assert outs[0] == outs[1]
