@@ -721,6 +721,117 @@ int mlr_sample_tokens(const void *logits, int64_t row_stride, int64_t num_logit_
                       int64_t *tokens, float *logprobs, int64_t num_rows, int64_t vocab,
                       void *workspace, size_t workspace_bytes, void *stream);
 
+/*
+ * Which keys of a paged cache a token sees, and which it holds. All of these take
+ * bf16, fp16 and FP32, any block_size, fewer than 2^31 positions per table and 16-byte
+ * aligned operands and row starts; the attention calls are over the operands of
+ * mlr_paged_decode_scored and mlr_paged_prefill_scored (head_dim, softcap, lengths of 0,
+ * block ids out of range, workspaces and roundings as there). No counterpart in the
+ * reference.
+ *
+ * mlr_tree_ancestors: parents [total_q] holds for each token of sequence s, at the rows
+ * [query_start_loc[s], query_start_loc[s+1]), the place of its parent among them (out of
+ * range: none). ancestors [total_q, words]: bit j % 64 of word j / 64 of a row says
+ * whether token j of the sequence is that token or one of its ancestors (tokens past
+ * 64 * words have no bit).
+ *
+ * mlr_paged_attention_tree: packed sequences as for mlr_paged_prefill_scored, whose last
+ * n keys of context_lens[s] are those of its n rows. A row sees every key before
+ * them, and of them those whose bit its row of ancestors (any bits, not only a tree's)
+ * has set; one that sees none gets zeros.
+ */
+int mlr_tree_ancestors(const int64_t *parents, const int64_t *query_start_loc, int64_t num_seqs,
+                       int64_t total_q, int64_t words, int64_t *ancestors, void *stream);
+size_t mlr_paged_attention_tree_workspace_size(int64_t num_seqs, int64_t max_query_len,
+                                               int64_t max_blocks, int64_t block_size,
+                                               int64_t num_q_heads, int64_t num_kv_heads,
+                                               int64_t head_dim, int dtype);
+int mlr_paged_attention_tree(const void *q, int64_t q_stride_t, int64_t q_stride_h,
+                             const void *k_cache, const void *v_cache, int64_t num_blocks,
+                             int64_t block_size, int64_t num_kv_heads, int64_t head_dim,
+                             const int64_t *block_tables, int64_t bt_stride, int64_t max_blocks,
+                             const int64_t *query_start_loc, const int64_t *context_lens,
+                             const int64_t *ancestors, int64_t words, int64_t num_seqs,
+                             int64_t total_q, int64_t max_query_len, int64_t num_q_heads,
+                             double scale, double softcap, int dtype, void *workspace,
+                             size_t workspace_bytes, void *out, int64_t out_stride_t,
+                             int64_t out_stride_h, void *stream);
+
+/*
+ * mlr_paged_decode_weighted: mlr_paged_decode_scored (without a bias) that also adds to
+ * key_weights, FP32 [num_blocks, num_kv_heads, block_size], each key's attention weight,
+ * summed over the query heads of the KV head; the entry of a sequence's newest key is
+ * set to it. Requests that share a block add to the same entries, in any order.
+ *
+ * mlr_evict_keys: of each sequence and KV head the first `sinks` keys, the last `recent` and
+ * of the others the heaviest by key_weights stay, `budget` in all (ties: the lower
+ * position; NaN counts as -infinity), in order: kept [batch, num_kv_heads, budget] gets
+ * their positions, -1 past the end, new_lens [batch] their number, and the rows of both
+ * caches and key_weights move to the positions 0, 1, ... of the sequence. What lies behind
+ * them is left as it is. The sequences' blocks must be their own.
+ *
+ * mlr_compact_keys: the move alone: the rows at positions kept[b, h, i] (row strides
+ * kept_stride_b and kept_stride_h, 0 where all KV heads share a list) go to positions
+ * start[b] + i (start null: i); a list ascends, with kept[b, h, i] >= start[b] + i, and
+ * entries below 0 move nothing. key_weights may be null.
+ */
+size_t mlr_paged_decode_weighted_workspace_size(int64_t batch, int64_t num_q_heads,
+                                                int64_t num_kv_heads, int64_t head_dim,
+                                                int64_t max_context);
+int mlr_paged_decode_weighted(const void *q, int64_t q_stride_b, int64_t q_stride_h,
+                              const void *k_cache, const void *v_cache, float *key_weights,
+                              int64_t num_blocks, int64_t block_size, int64_t num_kv_heads,
+                              int64_t head_dim, const int64_t *block_tables, int64_t bt_stride,
+                              int64_t max_blocks, const int64_t *seq_lens, int64_t batch,
+                              int64_t num_q_heads, double scale, double softcap, int dtype,
+                              void *workspace, size_t workspace_bytes, void *out,
+                              int64_t out_stride_b, int64_t out_stride_h, void *stream);
+int mlr_evict_keys(void *k_cache, void *v_cache, float *key_weights, int64_t num_blocks,
+                   int64_t block_size, int64_t num_kv_heads, int64_t head_dim,
+                   const int64_t *block_tables, int64_t bt_stride, int64_t max_blocks,
+                   const int64_t *seq_lens, int64_t batch, int64_t budget, int64_t sinks,
+                   int64_t recent, int dtype, int64_t *kept, int64_t *new_lens, void *stream);
+int mlr_compact_keys(void *k_cache, void *v_cache, float *key_weights, int64_t num_blocks,
+                     int64_t block_size, int64_t num_kv_heads, int64_t head_dim,
+                     const int64_t *block_tables, int64_t bt_stride, int64_t max_blocks,
+                     const int64_t *kept, int64_t kept_stride_b, int64_t kept_stride_h,
+                     int64_t num_kept, const int64_t *start, int64_t batch, int dtype,
+                     void *stream);
+
+/*
+ * mlr_update_key_bounds: key_bounds [num_blocks, 2, num_kv_heads, head_dim], in the cache's
+ * type: the elementwise minimum and maximum of a block's keys that exist, NaN where one
+ * is. Every block that holds a position of [starts[b], seq_lens[b]) (starts null: of all
+ * blocks) is written anew; max_new is at least the longest such range.
+ *
+ * mlr_paged_decode_sparse: mlr_paged_decode_scored (without a bias) over some blocks of each
+ * sequence, chosen for each KV head: the first `sinks`, the last `recent` (at least 1, so
+ * that the last block, whose bounds may lag behind, is always read), and of the others
+ * those of the largest score, `budget` in all (ties: the lower one), where
+ *   score = max over the heads h of the group of sum_d max(q_hd min_d, q_hd max_d)
+ * in 64 bits, of -q where scale is negative; a head's sum that is NaN does not count, and a
+ * block id out of range scores -infinity. chosen [batch, num_kv_heads, budget] (may be
+ * null): their places in order, -1 past the end.
+ */
+int mlr_update_key_bounds(const void *k_cache, void *key_bounds, int64_t num_blocks,
+                          int64_t block_size, int64_t num_kv_heads, int64_t head_dim,
+                          const int64_t *block_tables, int64_t bt_stride, int64_t max_blocks,
+                          const int64_t *seq_lens, const int64_t *starts, int64_t max_new,
+                          int64_t batch, int dtype, void *stream);
+size_t mlr_paged_decode_sparse_workspace_size(int64_t batch, int64_t num_q_heads,
+                                              int64_t num_kv_heads, int64_t head_dim,
+                                              int64_t max_blocks, int64_t block_size,
+                                              int64_t budget);
+int mlr_paged_decode_sparse(const void *q, int64_t q_stride_b, int64_t q_stride_h,
+                            const void *k_cache, const void *v_cache, const void *key_bounds,
+                            int64_t num_blocks, int64_t block_size, int64_t num_kv_heads,
+                            int64_t head_dim, const int64_t *block_tables, int64_t bt_stride,
+                            int64_t max_blocks, const int64_t *seq_lens, int64_t batch,
+                            int64_t num_q_heads, int64_t budget, int64_t sinks, int64_t recent,
+                            double scale, double softcap, int dtype, int64_t *chosen,
+                            void *workspace, size_t workspace_bytes, void *out,
+                            int64_t out_stride_b, int64_t out_stride_h, void *stream);
+
 #ifdef __cplusplus
 }
 #endif

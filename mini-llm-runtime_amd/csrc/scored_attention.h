@@ -35,6 +35,7 @@ struct ScoredParams {
   int hkv, group, d, hq;
   const int64_t *bt, *ctx, *qsl, *ahead;
   int64_t bt_st, bt_width;
+  int64_t bt_sh;           // from one KV head's table to the next's; 0: one table for all
   int seqs, tiles;         // sequences; units of a sequence (kModePrefix: of the call)
   int64_t total_q;         // rows of q
   int64_t start;           // first key (kModeDecode), number of keys (kModePrefix), both
@@ -43,6 +44,10 @@ struct ScoredParams {
   int prefix_units;        // kModeShared: units over the prefix
   float scale, cap;
   const float *slopes;
+  const int64_t *bits;     // kModePrefill: what each row sees of its sequence's last tokens,
+  int words;               // `words` words a row (null: causal)
+  float *scores;           // kModeDecode: where to leave the scores (null: nowhere),
+  int64_t scores_st;       // [seqs * hq][scores_st]
   void *out;
   int64_t o_st, o_sh;
   int mode, units;
@@ -70,6 +75,12 @@ __device__ __forceinline__ const int64_t *table_of(const ScoredParams &p, const 
   return t.prefix ? p.prefix : p.bt + t.seq * p.bt_st;
 }
 
+// Whether row `row` sees the key at place `node` >= 0 of its sequence's last tokens.
+__device__ __forceinline__ bool bit_of(const ScoredParams &p, int64_t row, int node) {
+  const int word = node >> 6;
+  return word < p.words && (static_cast<uint64_t>(p.bits[row * p.words + word]) >> (node & 63) & 1);
+}
+
 __device__ __forceinline__ int64_t clamp64(int64_t x, int64_t lo, int64_t hi) {
   return x < lo ? lo : x > hi ? hi : x;
 }
@@ -90,7 +101,8 @@ __device__ __forceinline__ Unit unit_of(const ScoredParams &p, int u, int kRows)
     const int64_t end = clamp64(p.qsl[t.seq + 1], t.q0, p.total_q);
     t.ctx = clamp64(p.ctx[t.seq], 0, covered);
     t.pos0 = t.ctx - (end - t.q0);
-    t.ahead = p.ahead ? clamp64(p.ahead[t.seq], 0, t.ctx) : 0;
+    // With bits, which keys a row sees of the last ones is up to them.
+    t.ahead = p.bits ? t.ctx : p.ahead ? clamp64(p.ahead[t.seq], 0, t.ctx) : 0;
     // Rows past the declared longest chunk have no unit.
     const int64_t rows = (end - t.q0) * p.group, most = static_cast<int64_t>(p.tiles) * kRows;
     t.rows = static_cast<int>(rows < most ? rows : most);
@@ -157,6 +169,34 @@ __host__ __device__ inline bool splits_pay(int64_t units, int64_t keys, int cus)
 }
 
 int launch_scored_rows(const ScoredParams &p, int dtype, unsigned grid, hipStream_t stream);
+
+// Rows of a unit of that kernel, and a call of it over single tokens: its operands, the
+// checks that all entry points share, its cut into items and its workspace.
+constexpr int kRows = 16;
+struct Operands {
+  const char *what;
+  const void *q;
+  int64_t q_st, q_sh;
+  const void *k, *v;
+  int64_t num_blocks, block_size, hkv, d;
+  const int64_t *bt;
+  int64_t bt_st, bt_width;
+  const int64_t *ctx;
+  int64_t seqs, hq;
+  double scale, cap;
+  const float *slopes;
+  int dtype;
+  const void *out;
+  int64_t o_st, o_sh;
+};
+int check_operands(const Operands &o);
+ScoredParams params_of(const Operands &o, int mode);
+size_t decode_workspace(int64_t batch, int64_t hq, int64_t hkv, int64_t d, int64_t max_keys);
+// Plans a decode and places its partial results; the number of its items.
+int64_t plan_decode(ScoredParams &p, int64_t max_keys, char *workspace);
+unsigned grid_of(int64_t items);
+int merge_decode(const ScoredParams &p, int dtype, hipStream_t stream);
+size_t align256(size_t n);
 
 // Units of 128 rows; bf16 and fp16, block_size a power of two from 16 on.
 constexpr int kTileRows = 128;

@@ -5,10 +5,12 @@
 #include <algorithm>
 
 namespace mlr {
+
+size_t align256(size_t n) { return (n + 255) & ~size_t(255); }
+
 namespace {
 
 constexpr float kLog2e = 1.4426950408889634f;
-constexpr int kRows = 16;
 
 // out = sum_i e^{m_i - M} O_i / sum_i e^{m_i - M} l_i over a row's items: those
 // of its unit u0 + u of `p` and, over a shared prefix, those of `x` too. One wave
@@ -132,8 +134,6 @@ int64_t max_items(int64_t units, int64_t hkv, int64_t max_keys, int64_t target) 
   return std::min(by_len, units + ceil_div(target, hkv) + 1) * hkv;
 }
 
-size_t align256(size_t n) { return (n + 255) & ~size_t(255); }
-
 // Workspace of one kernel's partial results: [first | ml | acc].
 size_t part_bytes(int64_t units, int64_t items, int64_t rows, int64_t d) {
   const int64_t wide = d > 64 ? 128 : 64;
@@ -252,22 +252,7 @@ bool covers_less(int64_t blocks, int64_t block_size) {
          blocks * block_size <= (int64_t(1) << 31) - 4096;
 }
 
-struct Operands {
-  const char *what;
-  const void *q;
-  int64_t q_st, q_sh;
-  const void *k, *v;
-  int64_t num_blocks, block_size, hkv, d;
-  const int64_t *bt;
-  int64_t bt_st, bt_width;
-  const int64_t *ctx;
-  int64_t seqs, hq;
-  double scale, cap;
-  const float *slopes;
-  int dtype;
-  const void *out;
-  int64_t o_st, o_sh;
-};
+}  // namespace
 
 int check_operands(const Operands &o) {
   const char *w = o.what;
@@ -328,7 +313,24 @@ ScoredParams params_of(const Operands &o, int mode) {
 
 unsigned grid_of(int64_t items) { return static_cast<unsigned>(std::min<int64_t>(items, 1024)); }
 
-}  // namespace
+size_t decode_workspace(int64_t batch, int64_t hq, int64_t hkv, int64_t d, int64_t max_keys) {
+  const int64_t units = decode_units(batch, hq / hkv);
+  return part_bytes(units, max_items(units, hkv, max_keys, rows_target(units, hkv, d)), kRows, d);
+}
+
+int64_t plan_decode(ScoredParams &p, int64_t max_keys, char *workspace) {
+  p.tiles = static_cast<int>(ceil_div(p.group, kRows));
+  p.units = static_cast<int>(decode_units(p.seqs, p.group));
+  p.target = rows_target(p.units, p.hkv, p.d);
+  const int64_t items = max_items(p.units, p.hkv, max_keys, p.target);
+  if (workspace) place_parts(p, workspace, items, kRows);
+  return items;
+}
+
+int merge_decode(const ScoredParams &p, int dtype, hipStream_t stream) {
+  return launch_merge(p, 0, kRows, p, kRows, false, dtype, stream);
+}
+
 }  // namespace mlr
 
 using namespace mlr;
@@ -337,10 +339,7 @@ extern "C" size_t mlr_paged_decode_scored_workspace_size(int64_t batch, int64_t 
                                                          int64_t num_kv_heads, int64_t head_dim,
                                                          int64_t max_context) {
   if (batch <= 0 || num_kv_heads <= 0 || num_q_heads <= 0 || max_context <= kMinSplit) return 0;
-  const int64_t units = decode_units(batch, num_q_heads / num_kv_heads);
-  return part_bytes(units, max_items(units, num_kv_heads, max_context,
-                                     rows_target(units, num_kv_heads, head_dim)),
-                    kRows, head_dim);
+  return decode_workspace(batch, num_q_heads, num_kv_heads, head_dim, max_context);
 }
 
 extern "C" int mlr_paged_decode_scored(
@@ -366,14 +365,10 @@ extern "C" int mlr_paged_decode_scored(
   MLR_REQUIRE(need == 0 || (workspace && workspace_bytes >= need),
               "mlr_paged_decode_scored: workspace of %zu bytes, %zu needed", workspace_bytes, need);
   ScoredParams p = params_of(o, kModeDecode);
-  p.tiles = static_cast<int>(ceil_div(p.group, kRows));
-  p.units = static_cast<int>(decode_units(batch, p.group));
-  p.target = rows_target(p.units, p.hkv, p.d);
-  const int64_t items = max_items(p.units, p.hkv, max_keys, p.target);
-  if (need) place_parts(p, static_cast<char *>(workspace), items, kRows);
+  const int64_t items = plan_decode(p, max_keys, need ? static_cast<char *>(workspace) : nullptr);
   hipStream_t s = static_cast<hipStream_t>(stream);
   if (const int rc = launch_scored_rows(p, dtype, grid_of(items), s)) return rc;
-  return need ? launch_merge(p, 0, kRows, p, kRows, false, dtype, s) : MLR_OK;
+  return need ? merge_decode(p, dtype, s) : MLR_OK;
 }
 
 extern "C" size_t mlr_paged_prefill_scored_workspace_size(int64_t num_seqs, int64_t max_query_len,
@@ -389,6 +384,45 @@ extern "C" size_t mlr_paged_prefill_scored_workspace_size(int64_t num_seqs, int6
   return n.parts ? part_bytes(n.units, n.items, n.rows, head_dim) : 0;
 }
 
+// Packed sequences: chunks with `ahead` or, with bits, drafted tokens.
+static int run_packed(const Operands &o, const int64_t *query_start_loc, const int64_t *ahead,
+                      const int64_t *bits, int64_t words, int64_t total_q, int64_t max_query_len,
+                      void *workspace, size_t workspace_bytes, void *stream) {
+  if (const int rc = check_operands(o)) return rc;
+  MLR_REQUIRE(total_q >= 0 && max_query_len >= 0, "%s: token counts must be >= 0", o.what);
+  if (o.seqs == 0 || total_q == 0 || max_query_len == 0) return MLR_OK;
+  MLR_REQUIRE(o.q && o.k && o.v && (o.bt || o.bt_width == 0) && query_start_loc && o.ctx && o.out,
+              "%s: null pointer", o.what);
+  max_query_len = std::min(max_query_len, total_q);
+  const int64_t group = o.hq / o.hkv;
+  MLR_REQUIRE(max_query_len < (int64_t(1) << 31) / group &&
+                  prefill_units(o.seqs, max_query_len, group, kRows) * o.hkv < (int64_t(1) << 25),
+              "%s: too many query rows", o.what);
+  const PrefillPlan n = plan_prefill(o.seqs, max_query_len, o.bt_width * o.block_size,
+                                     o.block_size, o.hq, o.hkv, o.d, o.dtype);
+  const size_t need = n.parts ? part_bytes(n.units, n.items, n.rows, o.d) : 0;
+  MLR_REQUIRE(need == 0 || (workspace && workspace_bytes >= need),
+              "%s: workspace of %zu bytes, %zu needed", o.what, workspace_bytes, need);
+  ScoredParams p = params_of(o, kModePrefill);
+  p.qsl = query_start_loc;
+  p.ahead = ahead;
+  p.bits = bits;
+  p.words = static_cast<int>(words);
+  p.total_q = total_q;
+  p.units = static_cast<int>(n.units);
+  p.tiles = static_cast<int>(n.units / o.seqs);
+  p.whole = n.whole;
+  p.target = n.target;
+  const int rows = static_cast<int>(n.rows);
+  if (n.parts) place_parts(p, static_cast<char *>(workspace), n.items, rows);
+  hipStream_t s = static_cast<hipStream_t>(stream);
+  const int rc = rows == kTileRows
+                     ? launch_scored_tiles(p, o.dtype, static_cast<unsigned>(n.items), s)
+                     : launch_scored_rows(p, o.dtype, grid_of(n.items), s);
+  if (rc) return rc;
+  return n.parts ? launch_merge(p, 0, rows, p, rows, false, o.dtype, s) : MLR_OK;
+}
+
 extern "C" int mlr_paged_prefill_scored(
     const void *q, int64_t q_stride_t, int64_t q_stride_h, const void *k_cache,
     const void *v_cache, int64_t num_blocks, int64_t block_size, int64_t num_kv_heads,
@@ -402,43 +436,37 @@ extern "C" int mlr_paged_prefill_scored(
                    num_blocks, block_size, num_kv_heads, head_dim, block_tables, bt_stride,
                    max_blocks, context_lens, num_seqs, num_q_heads, scale, softcap, alibi_slopes,
                    dtype, out, out_stride_t, out_stride_h};
-  if (const int rc = check_operands(o)) return rc;
-  MLR_REQUIRE(total_q >= 0 && max_query_len >= 0,
-              "mlr_paged_prefill_scored: token counts must be >= 0");
-  if (num_seqs == 0 || total_q == 0 || max_query_len == 0) return MLR_OK;
-  MLR_REQUIRE(q && k_cache && v_cache && (block_tables || max_blocks == 0) && query_start_loc &&
-                  context_lens && out,
-              "mlr_paged_prefill_scored: null pointer");
-  max_query_len = std::min(max_query_len, total_q);
-  const int64_t group = num_q_heads / num_kv_heads;
-  MLR_REQUIRE(max_query_len < (int64_t(1) << 31) / group &&
-                  prefill_units(num_seqs, max_query_len, group, kRows) * num_kv_heads <
-                      (int64_t(1) << 25),
-              "mlr_paged_prefill_scored: too many query rows");
-  const int64_t max_keys = max_blocks * block_size;
-  const PrefillPlan n = plan_prefill(num_seqs, max_query_len, max_keys, block_size, num_q_heads,
-                                     num_kv_heads, head_dim, dtype);
-  const size_t need = mlr_paged_prefill_scored_workspace_size(
-      num_seqs, max_query_len, max_blocks, block_size, num_q_heads, num_kv_heads, head_dim, dtype);
-  MLR_REQUIRE(need == 0 || (workspace && workspace_bytes >= need),
-              "mlr_paged_prefill_scored: workspace of %zu bytes, %zu needed", workspace_bytes,
-              need);
-  ScoredParams p = params_of(o, kModePrefill);
-  p.qsl = query_start_loc;
-  p.ahead = prefix_lens;
-  p.total_q = total_q;
-  p.units = static_cast<int>(n.units);
-  p.tiles = static_cast<int>(n.units / num_seqs);
-  p.whole = n.whole;
-  p.target = n.target;
-  const int rows = static_cast<int>(n.rows);
-  if (n.parts) place_parts(p, static_cast<char *>(workspace), n.items, rows);
-  hipStream_t s = static_cast<hipStream_t>(stream);
-  const int rc = rows == kTileRows
-                     ? launch_scored_tiles(p, dtype, static_cast<unsigned>(n.items), s)
-                     : launch_scored_rows(p, dtype, grid_of(n.items), s);
-  if (rc) return rc;
-  return n.parts ? launch_merge(p, 0, rows, p, rows, false, dtype, s) : MLR_OK;
+  return run_packed(o, query_start_loc, prefix_lens, nullptr, 0, total_q, max_query_len, workspace,
+                    workspace_bytes, stream);
+}
+
+extern "C" size_t mlr_paged_attention_tree_workspace_size(int64_t num_seqs, int64_t max_query_len,
+                                                          int64_t max_blocks, int64_t block_size,
+                                                          int64_t num_q_heads,
+                                                          int64_t num_kv_heads, int64_t head_dim,
+                                                          int dtype) {
+  return mlr_paged_prefill_scored_workspace_size(num_seqs, max_query_len, max_blocks, block_size,
+                                                 num_q_heads, num_kv_heads, head_dim, dtype);
+}
+
+extern "C" int mlr_paged_attention_tree(
+    const void *q, int64_t q_stride_t, int64_t q_stride_h, const void *k_cache,
+    const void *v_cache, int64_t num_blocks, int64_t block_size, int64_t num_kv_heads,
+    int64_t head_dim, const int64_t *block_tables, int64_t bt_stride, int64_t max_blocks,
+    const int64_t *query_start_loc, const int64_t *context_lens, const int64_t *ancestors,
+    int64_t words, int64_t num_seqs, int64_t total_q, int64_t max_query_len, int64_t num_q_heads,
+    double scale, double softcap, int dtype, void *workspace, size_t workspace_bytes, void *out,
+    int64_t out_stride_t, int64_t out_stride_h, void *stream) {
+  clear_error();
+  const Operands o{"mlr_paged_attention_tree", q, q_stride_t, q_stride_h, k_cache, v_cache,
+                   num_blocks, block_size, num_kv_heads, head_dim, block_tables, bt_stride,
+                   max_blocks, context_lens, num_seqs, num_q_heads, scale, softcap, nullptr,
+                   dtype, out, out_stride_t, out_stride_h};
+  MLR_REQUIRE(words > 0 && words < (1 << 24),
+              "mlr_paged_attention_tree: a row of ancestors needs 1 to 2^24 - 1 words");
+  MLR_REQUIRE(ancestors || num_seqs == 0 || total_q == 0, "mlr_paged_attention_tree: null pointer");
+  return run_packed(o, query_start_loc, nullptr, ancestors, words, total_q, max_query_len,
+                    workspace, workspace_bytes, stream);
 }
 
 extern "C" size_t mlr_paged_decode_shared_prefix_workspace_size(

@@ -37,7 +37,6 @@ typedef _Float16 f16x4_t __attribute__((ext_vector_type(4)));
 typedef short s16x4_t __attribute__((ext_vector_type(4)));
 typedef float f32x4_t __attribute__((ext_vector_type(4)));
 
-constexpr int kRows = 16;
 constexpr int kWavesWg = 4;
 constexpr float kLog2e = 1.4426950408889634f;
 
@@ -217,7 +216,10 @@ __device__ __forceinline__ void cap_scores(float (&x)[4], float cap, float inv_c
 
 // kPrefill: the rows are tokens of chunks, not requests. kUnlike: rows of a unit may
 // see different keys (chunks, and requests shorter than the prefix that they share).
-template <typename T, int D, bool kCap, bool kPaged16, bool kPrefill, bool kUnlike>
+// kTree: of its sequence's last tokens a row sees those that its bits name. kKeep: the
+// scores stay for a pass that weighs the keys.
+template <typename T, int D, bool kCap, bool kPaged16, bool kPrefill, bool kUnlike, bool kTree,
+          bool kKeep>
 __global__ __launch_bounds__(256) void scored_rows_kernel(ScoredParams p) {
   constexpr int kVe = D / 16;  // elements of a row that a lane of P V holds
   constexpr int kE = 16 / sizeof(T);
@@ -320,7 +322,9 @@ __global__ __launch_bounds__(256) void scored_rows_kernel(ScoredParams p) {
       pos = static_cast<int>(clamp64(p.ctx[row], 0, 0x7fffffff)) - 1;
       limit = min(limit, pos + 1);
     }
-    const int own_end = live ? limit : 0x7fffffff;  // first key that the row does not see
+    // The first key that the row does not see (kTree: may not see).
+    const int tree0 = static_cast<int>(t.pos0);
+    const int own_end = !live ? 0x7fffffff : kTree ? tree0 : limit;
     if (!live) limit = 0;
     const float slope = p.slopes ? p.slopes[head] : 0.f;
     uint4 q[M::kK];
@@ -333,7 +337,7 @@ __global__ __launch_bounds__(256) void scored_rows_kernel(ScoredParams p) {
     }
 
     Rows<T, D, kPaged16> src{p, static_cast<const T *>(p.k), static_cast<const T *>(p.v),
-                             table_of(p, t),
+                             table_of(p, t) + kvh * p.bt_sh,
                              static_cast<int>((t.prefix ? p.prefix_width : p.bt_width) *
                                               p.block_size),
                              static_cast<int>(min(p.block_size, int64_t(0x7fffffff))), m16, g, kvh};
@@ -384,10 +388,14 @@ __global__ __launch_bounds__(256) void scored_rows_kernel(ScoredParams p) {
         for (int i = 0; i < 4; ++i) {
           const int key = key0 + 4 * g + i;
           y[i] -= slope * static_cast<float>(abs(pos - key));
-          const bool seen = (ok[b] >> i & 1) && key >= lo && key < limit;
+          bool seen = (ok[b] >> i & 1) && key >= lo && key < limit;
+          if (kTree && seen && key >= tree0) seen = bit_of(p, row, key - tree0);
           x[b][i] = seen ? y[i] : -INFINITY;
           top = fmaxf(top, x[b][i]);
         }
+        if (kKeep && live)
+          *reinterpret_cast<float4 *>(p.scores + (row * p.hq + head) * p.scores_st + key0 + 4 * g) =
+              make_float4(x[b][0], x[b][1], x[b][2], x[b][3]);
       }
       top = max_groups(top);
       // A row that has seen no key yet keeps its reference point at 0.
@@ -459,6 +467,7 @@ __global__ __launch_bounds__(256) void scored_rows_kernel(ScoredParams p) {
             int64_t slot = 0;
             if (exists) slot = src.slot_of(key, exists);
             if (!exists || key < lo || key >= limit) continue;
+            if (kTree && key >= tree0 && !bit_of(p, row, key - tree0)) continue;
             const T *vr = src.v + (slot * p.hkv + kvh) * p.d;
 #pragma unroll
             for (int n = 0; n < kVe; ++n)
@@ -526,11 +535,14 @@ __global__ __launch_bounds__(256) void scored_rows_kernel(ScoredParams p) {
 template <typename T, int D>
 int launch_rows(const ScoredParams &p, unsigned grid, hipStream_t stream) {
   const bool paged16 = p.block_size % 16 == 0;
-#define MLR_ROWS(C, B, F, U) scored_rows_kernel<T, D, C, B, F, U><<<grid, 256, 0, stream>>>(p)
-#define MLR_ROWS_B(C, B)                                        \
-  if (p.mode == kModePrefill) MLR_ROWS(C, B, true, true);       \
-  else if (p.mode == kModePrefix) MLR_ROWS(C, B, false, true);  \
-  else MLR_ROWS(C, B, false, false);
+#define MLR_ROWS(C, B, F, U, R, K) \
+  scored_rows_kernel<T, D, C, B, F, U, R, K><<<grid, 256, 0, stream>>>(p)
+#define MLR_ROWS_B(C, B)                                                             \
+  if (p.mode == kModePrefill && p.bits) MLR_ROWS(C, B, true, true, true, false);     \
+  else if (p.mode == kModePrefill) MLR_ROWS(C, B, true, true, false, false);         \
+  else if (p.mode == kModePrefix) MLR_ROWS(C, B, false, true, false, false);         \
+  else if (p.scores) MLR_ROWS(C, B, false, false, false, true);                      \
+  else MLR_ROWS(C, B, false, false, false, false);
   if (p.cap > 0) {
     if (paged16) { MLR_ROWS_B(true, true) } else { MLR_ROWS_B(true, false) }
   } else {

@@ -122,7 +122,8 @@ __device__ __forceinline__ int units_past(const Seq &t, int group, int keys) {
   return tok > (t.rows - 1) / group ? 0 : all - tok * group / kTileRows;
 }
 
-template <typename T, int D, bool kCap, bool kBias>
+// kTree: of its sequence's last tokens a row sees those that its bits name.
+template <typename T, int D, bool kCap, bool kBias, bool kTree>
 __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(D == 64 ? 4 : 2)))
 void scored_tiles_kernel(ScoredParams p) {
   using W = Wide<T>;
@@ -297,7 +298,8 @@ void scored_tiles_kernel(ScoredParams p) {
   }
   if (!live) limit = 0;
   // Keys that all of the wave's rows see, and that any does.
-  int all = live ? limit : 0x7fffffff, any = limit;
+  const int tree0 = static_cast<int>(t.pos0);
+  int all = !live ? 0x7fffffff : kTree ? tree0 : limit, any = limit;
 #pragma unroll
   for (int o = 32; o > 0; o >>= 1) {
     all = min(all, __shfl_xor(all, o));
@@ -578,25 +580,55 @@ void scored_tiles_kernel(ScoredParams p) {
                          s[j][e]);
     }
     if (masked) {
-      // Key `at` of the tile is seen if at - from < lim - from, unsigned. One
-      // compare and select at a time: 32 compares side by side would take 64
-      // scalar registers, and every uniform value of the loop would be spilled.
-      const int from = max(low - key0 - 4 * hh, -128);
-      const int lim = min(min(limit, k_hi) - key0 - 4 * hh, 128);
-      const uint32_t span = static_cast<uint32_t>(max(lim - from, 0));
       const float hidden = -INFINITY;
-#pragma unroll
-      for (int j = 0; j < KB; ++j)
-#pragma unroll
-        for (int e = 0; e < 16; ++e) {
-          const uint32_t at = 32 * j + 8 * (e >> 2) + (e & 3) - from;
-          float x = s[j][e];
-          asm volatile("v_cmp_lt_u32 vcc, %1, %2\n\tv_cndmask_b32 %0, %3, %0, vcc"
-                       : "+v"(x)
-                       : "v"(at), "v"(span), "v"(hidden)
-                       : "vcc");
-          s[j][e] = x;
+      if constexpr (kTree) {
+        // Bit x: whether the row sees key key0 + x. The bits of place `from` on
+        // of the drafted tokens, below which every key is seen, up to the end.
+        const int from = key0 - tree0, left = min(limit, k_hi) - key0;
+        auto word = [&](int i) __attribute__((always_inline)) -> uint64_t {
+          return live && i < p.words ? static_cast<uint64_t>(p.bits[row * p.words + i]) : 0u;
+        };
+        uint64_t sees = ~uint64_t(0);
+        if (from >= 0) {
+          const int shift = from & 63;
+          sees = word(from >> 6) >> shift;
+          if (shift > 0) sees |= word((from >> 6) + 1) << (64 - shift);
+        } else if (from > -64) {
+          sees = (sees >> (64 + from)) | word(0) << -from;
         }
+        if (left < 64) sees = left > 0 ? sees & ~uint64_t(0) >> (64 - left) : 0u;
+        sees >>= 4 * hh;
+#pragma unroll
+        for (int j = 0; j < KB; ++j) {
+          const uint32_t half = static_cast<uint32_t>(sees >> (32 * j));
+#pragma unroll
+          for (int e = 0; e < 16; ++e) {
+            // All ones where the key is seen.
+            const int keep = static_cast<int>(half << (31 - 8 * (e >> 2) - (e & 3))) >> 31;
+            s[j][e] = __int_as_float((__float_as_int(s[j][e]) & keep) |
+                                     (__float_as_int(hidden) & ~keep));
+          }
+        }
+      } else {
+        // Key `at` of the tile is seen if at - from < lim - from, unsigned. One
+        // compare and select at a time: 32 compares side by side would take 64
+        // scalar registers, and every uniform value of the loop would be spilled.
+        const int from = max(low - key0 - 4 * hh, -128);
+        const int lim = min(min(limit, k_hi) - key0 - 4 * hh, 128);
+        const uint32_t span = static_cast<uint32_t>(max(lim - from, 0));
+#pragma unroll
+        for (int j = 0; j < KB; ++j)
+#pragma unroll
+          for (int e = 0; e < 16; ++e) {
+            const uint32_t at = 32 * j + 8 * (e >> 2) + (e & 3) - from;
+            float x = s[j][e];
+            asm volatile("v_cmp_lt_u32 vcc, %1, %2\n\tv_cndmask_b32 %0, %3, %0, vcc"
+                         : "+v"(x)
+                         : "v"(at), "v"(span), "v"(hidden)
+                         : "vcc");
+            s[j][e] = x;
+          }
+      }
       if (bad != 0) {
 #pragma unroll
         for (int r = 0; r < 4; ++r)
@@ -728,6 +760,7 @@ void scored_tiles_kernel(ScoredParams p) {
         if (key0 <= unit_to && key0 >= low) continue;
         const int64_t block = table[k >> bs_log2];
         if (!known(block) || k >= limit) continue;
+        if (kTree && k >= tree0 && !bit_of(p, row, k - tree0)) continue;
         const uint16_t *v = static_cast<const uint16_t *>(p.v) +
                             ((block << bs_log2) + (k & bs_mask)) * (row_bytes / 2) + kv_bytes / 2;
 #pragma unroll
@@ -830,11 +863,13 @@ void scored_tiles_kernel(ScoredParams p) {
 
 template <typename T, int D>
 int launch_tiles(const ScoredParams &p, unsigned grid, hipStream_t stream) {
-#define MLR_TILES(C, B) scored_tiles_kernel<T, D, C, B><<<grid, kThreads, 0, stream>>>(p)
-  if (p.cap > 0) {
-    if (p.slopes) MLR_TILES(true, true); else MLR_TILES(true, false);
+#define MLR_TILES(C, B, R) scored_tiles_kernel<T, D, C, B, R><<<grid, kThreads, 0, stream>>>(p)
+  if (p.bits) {
+    if (p.cap > 0) MLR_TILES(true, false, true); else MLR_TILES(false, false, true);
+  } else if (p.cap > 0) {
+    if (p.slopes) MLR_TILES(true, true, false); else MLR_TILES(true, false, false);
   } else {
-    if (p.slopes) MLR_TILES(false, true); else MLR_TILES(false, false);
+    if (p.slopes) MLR_TILES(false, true, false); else MLR_TILES(false, false, false);
   }
 #undef MLR_TILES
   return check_launch("scored_tiles");

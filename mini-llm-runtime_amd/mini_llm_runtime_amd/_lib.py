@@ -149,6 +149,44 @@ _PROTOTYPES = {
          _c_i64, _c_ptr, _c_i64, _c_i64, _c_ptr, _c_i64, _c_i64, _c_f64, _c_f64, _c_ptr, _c_int,
          _c_ptr, _c_size, _c_ptr, _c_i64, _c_i64, _c_ptr],
     ),
+    "mlr_tree_ancestors": (
+        _c_int, [_c_ptr, _c_ptr, _c_i64, _c_i64, _c_i64, _c_ptr, _c_ptr]),
+    "mlr_paged_attention_tree_workspace_size": (_c_size, [_c_i64] * 7 + [_c_int]),
+    "mlr_paged_attention_tree": (
+        _c_int,
+        [_c_ptr, _c_i64, _c_i64, _c_ptr, _c_ptr, _c_i64, _c_i64, _c_i64, _c_i64, _c_ptr, _c_i64,
+         _c_i64, _c_ptr, _c_ptr, _c_ptr, _c_i64, _c_i64, _c_i64, _c_i64, _c_i64, _c_f64, _c_f64,
+         _c_int, _c_ptr, _c_size, _c_ptr, _c_i64, _c_i64, _c_ptr],
+    ),
+    "mlr_paged_decode_weighted_workspace_size": (_c_size, [_c_i64] * 5),
+    "mlr_paged_decode_weighted": (
+        _c_int,
+        [_c_ptr, _c_i64, _c_i64, _c_ptr, _c_ptr, _c_ptr, _c_i64, _c_i64, _c_i64, _c_i64, _c_ptr,
+         _c_i64, _c_i64, _c_ptr, _c_i64, _c_i64, _c_f64, _c_f64, _c_int, _c_ptr, _c_size, _c_ptr,
+         _c_i64, _c_i64, _c_ptr],
+    ),
+    "mlr_evict_keys": (
+        _c_int,
+        [_c_ptr, _c_ptr, _c_ptr, _c_i64, _c_i64, _c_i64, _c_i64, _c_ptr, _c_i64, _c_i64, _c_ptr,
+         _c_i64, _c_i64, _c_i64, _c_i64, _c_int, _c_ptr, _c_ptr, _c_ptr],
+    ),
+    "mlr_compact_keys": (
+        _c_int,
+        [_c_ptr, _c_ptr, _c_ptr, _c_i64, _c_i64, _c_i64, _c_i64, _c_ptr, _c_i64, _c_i64, _c_ptr,
+         _c_i64, _c_i64, _c_i64, _c_ptr, _c_i64, _c_int, _c_ptr],
+    ),
+    "mlr_update_key_bounds": (
+        _c_int,
+        [_c_ptr, _c_ptr, _c_i64, _c_i64, _c_i64, _c_i64, _c_ptr, _c_i64, _c_i64, _c_ptr, _c_ptr,
+         _c_i64, _c_i64, _c_int, _c_ptr],
+    ),
+    "mlr_paged_decode_sparse_workspace_size": (_c_size, [_c_i64] * 7),
+    "mlr_paged_decode_sparse": (
+        _c_int,
+        [_c_ptr, _c_i64, _c_i64, _c_ptr, _c_ptr, _c_ptr, _c_i64, _c_i64, _c_i64, _c_i64, _c_ptr,
+         _c_i64, _c_i64, _c_ptr, _c_i64, _c_i64, _c_i64, _c_i64, _c_i64, _c_f64, _c_f64, _c_int,
+         _c_ptr, _c_ptr, _c_size, _c_ptr, _c_i64, _c_i64, _c_ptr],
+    ),
     "mlr_pa_accumulate": (_c_int, [_c_ptr, _c_ptr, _c_ptr, _c_i64, _c_ptr]),
     "mlr_build_step_metadata": (
         _c_int,

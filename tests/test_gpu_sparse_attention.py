@@ -1,0 +1,245 @@
+"""Key bounds and sparse decode against 64 bits."""
+
+from __future__ import annotations
+
+import pytest
+import torch
+
+from mini_llm_runtime_amd.kernels.scored_attention import paged_attention_decode_scored
+from mini_llm_runtime_amd.kernels.sparse_attention import (paged_attention_decode_sparse,
+                                                           update_key_bounds)
+
+import selection_oracle as so
+
+pytestmark = pytest.mark.gpu
+
+BF, FP, F32 = torch.bfloat16, torch.float16, torch.float32
+
+
+def bounds_of(k, tables, lens, starts, bs, before):
+    out = before.clone()
+    for i, n in enumerate(lens):
+        first = 0 if starts is None else starts[i] // bs
+        if starts is not None and starts[i] >= n:
+            continue
+        for j in range(first, -(-n // bs)):
+            keys = k[tables[i, j], :min(bs, n - j * bs)]
+            out[tables[i, j], 0], out[tables[i, j], 1] = keys.amin(0), keys.amax(0)
+    return out
+
+
+@pytest.mark.parametrize("dtype", [BF, FP, F32])
+@pytest.mark.parametrize("heads", [(2, 64), (1, 128), (3, 8), (4, 80), (2, 256)])
+@pytest.mark.parametrize("block_size", [16, 1, 7, 64])
+def test_bounds(device, dtype, heads, block_size):
+    lens = [1, 15, 16, 17, 200]
+    k, _, tables = so.pool(lens, block_size, *heads, dtype, 3)
+    before = torch.full((k.shape[0], 2, *heads), 3.0).to(dtype)
+    for starts, new in ((None, None), ([0, 14, 15, 16, 199], 1), ([1, 3, 0, 17, 150], 50),
+                        ([0, 14, 15, 16, 199], None)):
+        got = before.to(device)
+        update_key_bounds(k.to(device), got, tables.to(device), torch.tensor(lens).to(device),
+                          block_size,
+                          starts=None if starts is None else torch.tensor(starts).to(device),
+                          max_new=new)
+        assert torch.equal(got.cpu(), bounds_of(k, tables, lens, starts, block_size, before))
+
+
+@pytest.mark.parametrize("dtype", [BF, FP, F32])
+def test_bounds_of_odd_values(device, dtype):
+    """A NaN stays, infinities bound, and what lies behind the last key is not read."""
+    k, _, tables = so.pool([40], 16, 2, 64, dtype, 3)
+    k[tables[0, 0], 3, 0, 5] = float("nan")
+    k[tables[0, 1], 2, 1, 7] = float("inf")
+    k[tables[0, 1], 9, 1, 7] = -float("inf")
+    k[tables[0, 2], 8:] = float("nan")
+    got = torch.zeros(k.shape[0], 2, 2, 64, dtype=dtype, device=device)
+    update_key_bounds(k.to(device), got, tables.to(device), torch.tensor([40]).to(device), 16)
+    want = bounds_of(k, tables, [40], None, 16, torch.zeros(k.shape[0], 2, 2, 64, dtype=dtype))
+    torch.testing.assert_close(got.cpu(), want, rtol=0, atol=0, equal_nan=True)
+    assert want[tables[0, 0], :, 0, 5].isnan().all()
+    assert want[tables[0, 2]].isfinite().all()
+
+
+def test_bounds_padded_rows_and_bad_blocks(device):
+    k, _, tables = so.pool([40, 40], 16, 2, 64, BF, 3)
+    want = bounds_of(k, tables[1:], [40], None, 16, torch.zeros(k.shape[0], 2, 2, 64, dtype=BF))
+    want[tables[1, 1]] = 0
+    tables[1, 1] = 1 << 33
+    got = torch.zeros(k.shape[0], 2, 2, 64, dtype=BF, device=device)
+    update_key_bounds(k.to(device), got, tables.to(device), torch.tensor([0, 40]).to(device), 16,
+                      validate=False)
+    assert torch.equal(got.cpu(), want)
+
+
+def run_case(device, dtype, heads, lens, budget, sinks=1, recent=1, block_size=16, cap=0.0,
+             scale=None, seed=0, validate=True, change=None, width=None):
+    hq, hkv, d = heads
+    k, v, tables = so.pool(lens, block_size, hkv, d, dtype, seed, width=width)
+    gen = torch.Generator().manual_seed(seed + 1)
+    q = torch.randn(len(lens), hq, d, generator=gen).to(dtype)
+    bounds = torch.zeros(k.shape[0], 2, hkv, d, dtype=dtype)
+    bounds = bounds_of(k, tables, lens, None, block_size, bounds)
+    if change is not None:
+        change(q, k, v, bounds, tables)
+    scale = d ** -0.5 if scale is None else scale
+    got, blocks = paged_attention_decode_sparse(
+        q.to(device), k.to(device), v.to(device), bounds.to(device), tables.to(device),
+        torch.tensor(lens).to(device), block_size, budget, sinks=sinks, recent=recent,
+        softcap=cap, scale=scale, return_blocks=True, validate=validate)
+    for i, n in enumerate(lens):
+        count = -(-n // block_size)
+        used = tables[i, :count].clamp(0, k.shape[0] - 1)
+        x = -q[i] if scale < 0 else q[i]
+        score = so.block_scores(x, bounds[used, 0], bounds[used, 1])
+        seen = torch.zeros(1, hkv, n, dtype=torch.bool)
+        for h in range(hkv):
+            stay = so.choose(score[h], sinks, recent, budget)
+            assert blocks[i, h].tolist() == stay + [-1] * (budget - len(stay)), (i, h)
+            for j in stay:
+                seen[0, h, j * block_size:(j + 1) * block_size] = True
+        slot = so.slots(tables[i], n, block_size).clamp(min=0)
+        want, bound, _, _ = so.attend(q[i:i + 1], k.view(-1, hkv, d)[slot],
+                                      v.view(-1, hkv, d)[slot], seen, scale, cap, dtype)
+        so.assert_within(got[i:i + 1], want, bound, f"request {i}")
+    return got, blocks
+
+
+@pytest.mark.parametrize("dtype", [BF, FP, F32])
+@pytest.mark.parametrize("heads", [(14, 2, 64), (8, 2, 128), (4, 4, 96), (6, 2, 40), (16, 1, 16),
+                                   (80, 1, 32), (3, 1, 8)])
+def test_sparse(device, dtype, heads):
+    run_case(device, dtype, heads, [1, 16, 17, 100, 500, 513], 8, sinks=1, recent=2)
+
+
+@pytest.mark.parametrize("dtype", [BF, F32])
+@pytest.mark.parametrize("block_size", [1, 5, 8, 32, 24])
+def test_block_sizes(device, dtype, block_size):
+    run_case(device, dtype, (4, 2, 64), [1, 31, 330], 6, block_size=block_size)
+
+
+@pytest.mark.parametrize("budget,sinks,recent", [(1, 0, 1), (2, 1, 1), (5, 0, 5), (5, 4, 1),
+                                                 (9, 0, 1), (100, 3, 3)])
+def test_budgets(device, budget, sinks, recent):
+    run_case(device, BF, (14, 2, 64), [1, 80, 81, 400, 1000], budget, sinks, recent)
+
+
+@pytest.mark.parametrize("dtype", [BF, F32])
+def test_long_contexts(device, dtype):
+    run_case(device, dtype, (4, 2, 64), [20000, 7], 100, recent=3)
+    run_case(device, dtype, (2, 2, 8), [150000], 700, recent=3)
+
+
+@pytest.mark.parametrize("dtype", [BF, FP, F32])
+def test_capped_and_negative_scale(device, dtype):
+    run_case(device, dtype, (14, 2, 64), [300, 200], 5, cap=10.0)
+    run_case(device, dtype, (14, 2, 64), [300, 200], 5, scale=-0.1)
+
+
+def test_ties_go_to_the_lower_block(device):
+    def change(q, k, v, bounds, tables):
+        bounds[:, 0] = -1.0
+        bounds[:, 1] = 1.0
+        bounds[tables[0, 20], 1] = 2.0
+
+    _, blocks = run_case(device, BF, (14, 2, 64), [600], 6, change=change)
+    assert blocks[0, 0].tolist() == [0, 1, 2, 3, 20, 37]
+
+
+def test_scores_apart_by_less_than_32_bits_hold(device):
+    """Sums of terms of unlike size, whose 32-bit sums would be equal."""
+    def change(q, k, v, bounds, tables):
+        q[:] = 1.0
+        q[0, :, 1] = 2.0 ** -10
+        bounds[:] = 1.0
+        bounds[:, :, :, 0] = 2.0 ** 14
+        for j in (9, 5, 30):
+            bounds[tables[0, j], 1, :, 1] = 1.0 + 2.0 ** -7
+
+    _, blocks = run_case(device, F32, (2, 1, 64), [600], 5, change=change)
+    assert blocks[0, 0].tolist() == [0, 5, 9, 30, 37]
+
+
+@pytest.mark.parametrize("dtype", [BF, F32])
+def test_bounds_that_are_not_finite(device, dtype):
+    """A head's NaN does not count, and a block of NaN scores lowest; infinities score."""
+    def change(q, k, v, bounds, tables):
+        bounds[tables[0, 3]] = float("nan")
+        bounds[tables[0, 5], 1, 0, 2] = float("inf")
+        bounds[tables[0, 6], 0, 0, 2] = -float("inf")
+        q[0, 0, 2] = 0.0
+
+    run_case(device, dtype, (4, 2, 64), [400], 6, change=change)
+
+
+@pytest.mark.parametrize("dtype", [BF, F32])
+def test_hidden_rows_are_not_read(device, dtype):
+    """Blocks that are not chosen, and rows behind the last key, may hold anything."""
+    def change(q, k, v, bounds, tables):
+        for j in range(2, 24):
+            bounds[tables[0, j]] = 0.0 if j != 7 else bounds[tables[0, j]].abs() + 5
+            if j != 7:
+                k[tables[0, j]] = float("nan")
+                v[tables[0, j]] = float("nan")
+        bounds[tables[0, 1]] = 0.0
+        bounds[tables[0, 1], 1] = 100.0
+        bounds[tables[0, 1], 0] = -100.0
+        bounds[tables[0, 7], 0] = -50.0
+        bounds[tables[0, 7], 1] = 50.0
+        k[tables[0, 24], 9:] = float("nan")
+        v[tables[0, 24], 9:] = float("nan")
+
+    got, _ = run_case(device, dtype, (14, 2, 64), [393], 4, change=change)
+    assert got.isfinite().all()
+
+
+def test_padded_rows_and_wide_tables(device):
+    got, blocks = run_case(device, BF, (14, 2, 64), [0, 400, 0], 5, validate=False, width=64)
+    assert (got[0] == 0).all() and (got[2] == 0).all() and (blocks[0] == -1).all()
+
+
+def test_bad_blocks_score_lowest_and_are_masked(device):
+    k, v, tables = so.pool([160], 16, 2, 64, BF, 0)
+    bounds = bounds_of(k, tables, [160], None, 16, torch.zeros(k.shape[0], 2, 2, 64, dtype=BF))
+    q = torch.randn(1, 14, 64, generator=torch.Generator().manual_seed(1)).to(BF)
+    tables[0, 4] = 1 << 40
+    got, blocks = paged_attention_decode_sparse(
+        q.to(device), k.to(device), v.to(device), bounds.to(device), tables.to(device),
+        torch.tensor([160]).to(device), 16, 9, return_blocks=True, validate=False)
+    assert blocks[0].tolist() == [[0, 1, 2, 3, 5, 6, 7, 8, 9]] * 2
+    tables[0, 4] = 0
+    seen = torch.ones(1, 160, dtype=torch.bool)
+    seen[:, 64:80] = False
+    slot = so.slots(tables[0], 160, 16)
+    want, bound, _, _ = so.attend(q, k.view(-1, 2, 64)[slot], v.view(-1, 2, 64)[slot], seen,
+                                  0.125, 0.0, BF)
+    so.assert_within(got, want, bound)
+
+
+@pytest.mark.parametrize("dtype", [BF, FP, F32])
+def test_whole_requests_are_the_scored_decode(device, dtype):
+    """A budget of all blocks: no bounds are read, and the result is the decode's."""
+    k, v, tables = so.pool([100, 1, 333], 16, 2, 64, dtype, 0)
+    q = torch.randn(3, 14, 64, generator=torch.Generator().manual_seed(1)).to(dtype)
+    bounds = torch.full((k.shape[0], 2, 2, 64), float("nan"), dtype=dtype)
+    lens = torch.tensor([100, 1, 333]).to(device)
+    q, k, v, tables = (x.to(device) for x in (q, k, v, tables))
+    got = paged_attention_decode_sparse(q, k, v, bounds.to(device), tables, lens, 16, 21)
+    want = paged_attention_decode_scored(q, k, v, tables, lens, 16)
+    torch.testing.assert_close(got, want, rtol=0, atol=0)
+
+
+def test_strides(device):
+    """q as a view of packed rows, an out with wide rows, int32 metadata."""
+    k, v, tables = so.pool([300, 100], 16, 2, 64, BF, 0)
+    wide = torch.randn(2, 18 * 64, generator=torch.Generator().manual_seed(1)).to(BF).to(device)
+    q = wide[:, :14 * 64].view(2, 14, 64)
+    bounds = torch.stack([k.amin(1), k.amax(1)], 1).to(device)
+    k, v, tables = k.to(device), v.to(device), tables.to(device)
+    lens = torch.tensor([300, 100]).to(device)
+    want = paged_attention_decode_sparse(q.contiguous(), k, v, bounds, tables, lens, 16, 5)
+    out = torch.zeros(2, 14, 100, dtype=BF, device=device)
+    got = paged_attention_decode_sparse(q, k, v, bounds, tables.int(), lens.int(), 16, 5,
+                                        out=out[..., :64])
+    torch.testing.assert_close(got, want, rtol=0, atol=0)
+    assert (out[..., 64:] == 0).all()
