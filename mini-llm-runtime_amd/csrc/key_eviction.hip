@@ -91,116 +91,250 @@ struct CacheParams {
   int bs_log2;  // log2 of block_size, -1 if it is no power of two
 
   __device__ __forceinline__ int64_t covered() const { return bt_width * block_size; }
+  // Positions and block sizes are below 2^31.
+  __device__ __forceinline__ uint32_t block_of(uint32_t at) const {
+    return bs_log2 >= 0 ? at >> bs_log2 : at / static_cast<uint32_t>(block_size);
+  }
   // Slot of a position of a request, -1 if there is none.
   __device__ __forceinline__ int64_t slot(int64_t seq, int64_t pos) const {
     if (pos < 0 || pos >= covered()) return -1;
-    const int64_t at = bs_log2 >= 0 ? pos >> bs_log2 : pos / block_size;
+    const int64_t at = block_of(static_cast<uint32_t>(pos));
     const int64_t block = bt[seq * bt_st + at];
     return block < 0 || block >= num_blocks ? -1 : block * block_size + (pos - at * block_size);
   }
 };
 
-// A workgroup chooses the places of one request and KV head.
-__global__ __launch_bounds__(kSelectThreads) void choose_keys(CacheParams c, const int64_t *ctx,
-                                                              int sinks, int recent, int budget,
-                                                              int64_t *kept, int64_t *lens) {
+// A workgroup chooses the places of one request and KV head. Bound by latency: the keys'
+// two loads (a table, then four neighbouring weights where a block holds a multiple of
+// four), two digits of the selection, the list.
+template <int kThreads, int kHeld>
+__global__ __launch_bounds__(kThreads) void choose_keys(CacheParams c, const int64_t *ctx,
+                                                        int sinks, int recent, int budget,
+                                                        int64_t *kept, int64_t *lens) {
   __shared__ SelectShared s;
   const int64_t seq = blockIdx.x % c.seqs, kvh = blockIdx.x / c.seqs;
   const int n = static_cast<int>(clamp64(ctx[seq], 0, c.covered()));
   int64_t *list = kept + (seq * c.hkv + kvh) * budget;
-  const int chosen = select_places<uint32_t, 16>(
+  const int64_t *table = c.bt + seq * c.bt_st;
+  const bool fours = c.block_size % 4 == 0 && reinterpret_cast<uintptr_t>(c.weights) % 16 == 0;
+  // A weight's place; block ids out of range count as -infinity.
+  auto entry = [&](int64_t block, uint32_t i) __attribute__((always_inline)) {
+    return c.weights + (block * c.hkv + kvh) * c.block_size + i;
+  };
+  const uint32_t bs = static_cast<uint32_t>(c.block_size);
+  const int chosen = select_places<uint32_t, kThreads, kHeld>(
       s, n, sinks, recent, budget,
-      [&](int i) __attribute__((always_inline)) {
-        const int64_t at = c.slot(seq, i);
-        if (at < 0) return order_key(-INFINITY);
-        const int64_t block = c.bs_log2 >= 0 ? at >> c.bs_log2 : at / c.block_size;
-        return order_key(
-            c.weights[(block * c.hkv + kvh) * c.block_size + (at - block * c.block_size)]);
+      [&](auto &keys, auto place) __attribute__((always_inline)) {
+        constexpr int kMany = sizeof(keys) / sizeof(keys[0]);
+        int64_t block[kMany];
+        if (fours) {
+#pragma unroll
+          for (int j = 0; j < kMany; ++j) block[j] = table[c.block_of(min(place(j), n - 1))];
+#pragma unroll
+          for (int j = 0; j < kMany; ++j) {
+            const bool ok = block[j] >= 0 && block[j] < c.num_blocks;
+            const uint32_t at = min(place(j), n - 1), in = at - c.block_of(at) * bs;
+            const float4 w = *reinterpret_cast<const float4 *>(entry(ok ? block[j] : 0, in & ~3u));
+            keys[j][0] = order_key(ok ? w.x : -INFINITY);
+            keys[j][1] = order_key(ok ? w.y : -INFINITY);
+            keys[j][2] = order_key(ok ? w.z : -INFINITY);
+            keys[j][3] = order_key(ok ? w.w : -INFINITY);
+          }
+        } else {
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+#pragma unroll
+            for (int j = 0; j < kMany; ++j) block[j] = table[c.block_of(min(place(j) + e, n - 1))];
+#pragma unroll
+            for (int j = 0; j < kMany; ++j) {
+              const bool ok = block[j] >= 0 && block[j] < c.num_blocks;
+              const uint32_t at = min(place(j) + e, n - 1), in = at - c.block_of(at) * bs;
+              const float w = *entry(ok ? block[j] : 0, in);
+              keys[j][e] = order_key(ok ? w : -INFINITY);
+            }
+          }
+        }
       },
       [&](int r, int i) __attribute__((always_inline)) { list[r] = i; });
-  for (int i = chosen + threadIdx.x; i < budget; i += kSelectThreads) list[i] = -1;
+  for (int i = chosen + threadIdx.x; i < budget; i += kThreads) list[i] = -1;
   if (kvh == 0 && threadIdx.x == 0) lens[seq] = chosen;
 }
 
-// Rows start + i <- row kept[i]. Lists ascend and kept[i] >= start + i, so a row is
-// written only after, or together with, the reading of the row that lay there, if a
-// list is gone through in order: a wave takes 64 bytes of every row of a list, of K or of
-// V, 16 rows at a time and kBatch of those between their reads and their writes.
-// Columns never meet, so nothing but the wave's own wait orders them.
-constexpr int kBatch = 8;
+// Rows start + i <- row kept[i]. Lists ascend and kept[i] >= start + i: what is written
+// in place i lies at or before the row that is read for it, so a row is overwritten by
+// its own place in the list or a later one. A workgroup that goes through a list in
+// order, a batch of rows at a time, may therefore read the next batch before it has
+// written this one; it only has to have read all of a batch before it writes any of it:
+// one barrier a batch. Columns of 64 bytes of K and of V never meet, so each is a
+// workgroup of its own and nothing else orders them.
+//
+// Bound by what is in flight: each wave has two batches of 16 loads, one landing while the
+// other is written. The rows' places are made a batch ahead, from the list, which is read
+// two ahead, and the request's block table, which lies in LDS.
+constexpr int kLanes = 4;    // of 16 bytes, of a row of a column
+constexpr int kLoads = 16;   // of a wave and batch
+constexpr int kWaveRows = 64 / kLanes * kLoads;
+constexpr int kTable = 4096;  // block ids that lie in LDS; the others are read again
 struct Lists {
   const int64_t *kept, *start;
   int64_t st_b, st_h, n;
 };
 
-__global__ __launch_bounds__(256) void move_rows(CacheParams c, Lists l, int columns) {
-  const int lane = threadIdx.x & 63;
-  const int64_t task =
-      blockIdx.x * 4 + static_cast<int64_t>(__builtin_amdgcn_readfirstlane(threadIdx.x >> 6));
-  // Columns of K, of V, then the weights.
-  const int per = 2 * columns + (c.weights ? 1 : 0);
-  const int64_t pair = task / per;
-  if (pair >= c.seqs * c.hkv) return;
-  const int column = static_cast<int>(task - pair * per);
-  const int64_t seq = pair / c.hkv, kvh = pair - seq * c.hkv;
-  const int64_t *list = l.kept + seq * l.st_b + kvh * l.st_h;
-  const int64_t start = l.start ? l.start[seq] : 0;
-  if (column == 2 * columns) {
-    for (int64_t i0 = 0; i0 < l.n; i0 += 64 * kBatch) {
-      float x[kBatch];
-      int64_t to[kBatch];
+// What a row of a column is: `step` bytes apart from `base` on, row(block, i) of them for
+// place i of a block.
+template <typename Unit, int kPer, int kWaves, class Row>
+__device__ __forceinline__ void move_list(const CacheParams &c, const int64_t *list, int64_t n,
+                                          int64_t start, int64_t seq, bool mine,
+                                          int64_t (*places)[2][kWaveRows], uint32_t *table,
+                                          unsigned char *base, int64_t step, Row row) {
+  constexpr int kRowsLoad = 64 / kPer;            // rows of a load
+  constexpr int kCount = kWaveRows / kRowsLoad;   // loads
+  constexpr int kBatch = kWaveRows * kWaves;      // rows of the workgroup's batch
+  const int lane = threadIdx.x & 63, sub = lane / kPer;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int64_t *ids = c.bt + seq * c.bt_st;
+  constexpr uint32_t kNone = ~0u;  // block ids are below 2^31
+  auto known = [&](int64_t id) __attribute__((always_inline)) {
+    return id >= 0 && id < c.num_blocks ? static_cast<uint32_t>(id) : kNone;
+  };
+  auto id_of = [&](uint32_t at) __attribute__((always_inline)) {
+    return at < kTable ? table[at] : known(ids[at]);
+  };
+  int from[kWaveRows / 64];  // positions are below 2^31; -1: nothing to move
+  auto read_list = [&](int64_t batch) __attribute__((always_inline)) {
 #pragma unroll
-      for (int u = 0; u < kBatch; ++u) {
-        const int64_t i = i0 + 64 * u + lane;
-        to[u] = -1;
-        const int64_t from = i < l.n ? list[i] : -1;
-        if (from < 0 || from == start + i) continue;
-        const int64_t src = c.slot(seq, from), dst = c.slot(seq, start + i);
-        if (src < 0 || dst < 0) continue;
-        const int64_t sb = src / c.block_size, db = dst / c.block_size;
-        x[u] = c.weights[(sb * c.hkv + kvh) * c.block_size + (src - sb * c.block_size)];
-        to[u] = (db * c.hkv + kvh) * c.block_size + (dst - db * c.block_size);
-      }
-      asm volatile("" ::: "memory");
-      __builtin_amdgcn_s_waitcnt(0);
-      asm volatile("" ::: "memory");
-#pragma unroll
-      for (int u = 0; u < kBatch; ++u)
-        if (to[u] >= 0) c.weights[to[u]] = x[u];
+    for (int j = 0; j < kWaveRows / 64; ++j) {
+      const int64_t i = batch * kBatch + wave * kWaveRows + 64 * j + lane;
+      const int64_t x = list[min(i, n - 1)];
+      from[j] = i < n && x >= 0 && x < c.covered() ? static_cast<int>(x) : -1;
     }
-    return;
-  }
-  unsigned char *cache = column < columns ? c.k : c.v;
-  const int64_t byte = 64 * (column < columns ? column : column - columns) + 16 * (lane & 3);
-  const bool mine = byte < c.row_bytes;
-  for (int64_t i0 = 0; i0 < l.n; i0 += 16 * kBatch) {
-    uint4 x[kBatch];
-    int64_t to[kBatch];
+  };
+  // Byte offsets of a batch's rows: a source of 0 and a target of -1 where nothing moves.
+  auto make_places = [&](int64_t batch) __attribute__((always_inline)) {
+    const uint32_t bs = static_cast<uint32_t>(c.block_size);
 #pragma unroll
-    for (int u = 0; u < kBatch; ++u) {
-      const int64_t i = i0 + 16 * u + (lane >> 2);
-      to[u] = -1;
-      const int64_t from = i < l.n && mine ? list[i] : -1;
-      if (from < 0 || from == start + i) continue;
-      const int64_t src = c.slot(seq, from), dst = c.slot(seq, start + i);
-      if (src < 0 || dst < 0) continue;
-      x[u] = *reinterpret_cast<const uint4 *>(cache + (src * c.hkv + kvh) * c.row_bytes + byte);
-      to[u] = (dst * c.hkv + kvh) * c.row_bytes + byte;
+    for (int j = 0; j < kWaveRows / 64; ++j) {
+      const int64_t to = start + batch * kBatch + wave * kWaveRows + 64 * j + lane;
+      bool ok = from[j] >= 0 && from[j] != to && to >= 0 && to < c.covered();
+      const uint32_t src = ok ? from[j] : 0, dst = ok ? static_cast<uint32_t>(to) : 0;
+      const uint32_t sa = c.block_of(src), da = c.block_of(dst);
+      const uint32_t sb = id_of(sa), db = id_of(da);
+      ok = ok && sb != kNone && db != kNone;
+      places[batch & 1][0][64 * j + lane] = ok ? row(sb, src - sa * bs) * step : 0;
+      places[batch & 1][1][64 * j + lane] = ok ? row(db, dst - da * bs) * step : -1;
     }
-    asm volatile("" ::: "memory");
-    __builtin_amdgcn_s_waitcnt(0);
-    asm volatile("" ::: "memory");
+  };
+  // Batches are whole: rows past the list read row 0 and are not written.
+  Unit x0[kCount], x1[kCount];
+  auto read = [&](Unit (&to)[kCount], int64_t batch) __attribute__((always_inline)) {
+    int64_t at[kCount];
 #pragma unroll
-    for (int u = 0; u < kBatch; ++u)
-      if (to[u] >= 0) *reinterpret_cast<uint4 *>(cache + to[u]) = x[u];
+    for (int u = 0; u < kCount; ++u) at[u] = places[batch & 1][0][u * kRowsLoad + sub];
+#pragma unroll
+    for (int u = 0; u < kCount; ++u) to[u] = *reinterpret_cast<const Unit *>(base + at[u]);
+  };
+  auto write = [&](const Unit (&of)[kCount], int64_t batch) __attribute__((always_inline)) {
+    int64_t at[kCount];
+#pragma unroll
+    for (int u = 0; u < kCount; ++u) at[u] = places[batch & 1][1][u * kRowsLoad + sub];
+#pragma unroll
+    for (int u = 0; u < kCount; ++u)
+      if (at[u] >= 0 && mine) *reinterpret_cast<Unit *>(base + at[u]) = of[u];
+  };
+  read_list(0);
+  const int held = static_cast<int>(min(c.bt_width, int64_t(kTable)));
+#pragma unroll 4
+  for (int i = threadIdx.x; i < held; i += 64 * kWaves) table[i] = known(ids[i]);
+  __syncthreads();
+  make_places(0);
+  const int64_t batches = (n + kBatch - 1) / kBatch;
+  read(x0, 0);
+  if (batches > 1) read_list(1);
+  // Writes batch b, which `of` holds, with the next one on its way to `to`.
+  auto step_of = [&](Unit (&of)[kCount], Unit (&to)[kCount], int64_t b)
+      __attribute__((always_inline)) {
+    if (b + 1 < batches) {
+      make_places(b + 1);
+      if (b + 2 < batches) read_list(b + 2);
+      asm volatile("" ::: "memory");
+      read(to, b + 1);
+      asm volatile("" ::: "memory");
+      __builtin_amdgcn_s_waitcnt(0x0f70 | (kCount & 15) | (kCount >> 4) << 14);
+    } else {
+      asm volatile("" ::: "memory");
+      __builtin_amdgcn_s_waitcnt(0x0f70);
+    }
+    if (kWaves > 1) __builtin_amdgcn_s_barrier();
+    asm volatile("" ::: "memory");
+    write(of, b);
+    asm volatile("" ::: "memory");
+  };
+  for (int64_t b = 0; b < batches; b += 2) {
+    step_of(x0, x1, b);
+    if (b + 1 < batches) step_of(x1, x0, b + 1);
   }
 }
 
+// A workgroup's task: a column of K, of V, or the weights, of one request and KV head.
+template <int kWaves>
+__global__ __launch_bounds__(64 * kWaves) void move_rows(CacheParams c, Lists l, int columns) {
+  __shared__ int64_t places[kWaves][2][2][kWaveRows];
+  __shared__ uint32_t table[kTable];
+  // The columns of a line of 128 bytes on one XCD, and on each lines of all heads.
+  constexpr int kPerLine = 8 / kLanes;
+  const int64_t pairs = c.seqs * c.hkv;
+  const int lines = (columns + kPerLine - 1) / kPerLine;
+  const int64_t i = blockIdx.x / 8, k = i / kPerLine;
+  const int64_t at = 8 * k + ((blockIdx.x - k - k / 8) & 7);
+  const int64_t line = at / pairs, pair = at - line * pairs;
+  if (line > 2 * lines || (line == 2 * lines && (!c.weights || i % kPerLine != 0))) return;
+  const int64_t column = (line % lines) * kPerLine + i % kPerLine;
+  if (line < 2 * lines && column >= columns) return;
+  const int64_t seq = pair / c.hkv, kvh = pair - seq * c.hkv;
+  const int64_t *list = l.kept + seq * l.st_b + kvh * l.st_h;
+  const int64_t start = l.start ? l.start[seq] : 0;
+  int64_t(*mine)[2][kWaveRows] = places[threadIdx.x >> 6];
+  if (line == 2 * lines) {
+    move_list<float, 1, kWaves>(c, list, l.n, start, seq, true, mine, table,
+                                reinterpret_cast<unsigned char *>(c.weights), sizeof(float),
+                                [&](int64_t block, int64_t i) __attribute__((always_inline)) {
+                                  return (block * c.hkv + kvh) * c.block_size + i;
+                                });
+    return;
+  }
+  typedef uint32_t u32x4_t __attribute__((ext_vector_type(4)));
+  unsigned char *cache = line < lines ? c.k : c.v;
+  const int64_t byte = 16 * kLanes * column + 16 * (threadIdx.x % kLanes);
+  const bool in_row = byte < c.row_bytes;
+  move_list<u32x4_t, kLanes, kWaves>(
+      c, list, l.n, start, seq, in_row, mine, table,
+      cache + kvh * c.row_bytes + (in_row ? byte : 0), c.hkv * c.row_bytes,
+      [&](int64_t block, int64_t i) __attribute__((always_inline)) {
+        return block * c.block_size + i;
+      });
+}
+
+int64_t cus() {
+  const int n = current_device_cus();
+  return n > 0 ? n : 256;
+}
+
 int launch_move(const CacheParams &c, const Lists &l, hipStream_t stream) {
-  if (l.n == 0) return MLR_OK;
-  const int columns = static_cast<int>(ceil_div(c.row_bytes, 64));
-  const int64_t waves = c.seqs * c.hkv * (2 * columns + (c.weights ? 1 : 0));
-  move_rows<<<static_cast<unsigned>(ceil_div(waves, 4)), 256, 0, stream>>>(c, l, columns);
+  if (l.n == 0 || c.bt_width == 0) return MLR_OK;
+  const int columns = static_cast<int>(ceil_div(c.row_bytes, 16 * kLanes));
+  const int64_t lines = 2 * ceil_div(columns, 8 / kLanes) + (c.weights ? 1 : 0);
+  const int64_t groups = ceil_div(c.seqs * c.hkv * lines, 8) * 8 * (8 / kLanes);
+  MLR_REQUIRE(groups < (int64_t(1) << 31), "move_rows: too many rows");
+  const unsigned grid = static_cast<unsigned>(groups);
+  // As many waves a column as the list fills, up to some nine for every CU: more would run
+  // one after the other. us by 2, 4 and 8: 4 lists of 6,144 rows for each of 8 heads of 128
+  // (256 columns) 69, 59, 55; 64 of 1,024 for 2 heads of 64 (640 columns) 15, 17, 24.
+  const int64_t active = c.seqs * c.hkv * (2 * columns + (c.weights ? 1 : 0));
+  const int64_t most = std::min(ceil_div(l.n, kWaveRows), 9 * cus() / active);
+  if (most >= 8) move_rows<8><<<grid, 512, 0, stream>>>(c, l, columns);
+  else if (most >= 4) move_rows<4><<<grid, 256, 0, stream>>>(c, l, columns);
+  else if (most >= 2) move_rows<2><<<grid, 128, 0, stream>>>(c, l, columns);
+  else move_rows<1><<<grid, 64, 0, stream>>>(c, l, columns);
   return check_launch("move_rows");
 }
 
@@ -311,9 +445,17 @@ extern "C" int mlr_evict_keys(void *k_cache, void *v_cache, float *key_weights,
                                  num_kv_heads, head_dim, block_tables, bt_stride, max_blocks,
                                  batch, dtype);
   hipStream_t s = static_cast<hipStream_t>(stream);
-  choose_keys<<<static_cast<unsigned>(batch * num_kv_heads), kSelectThreads, 0, s>>>(
-      c, seq_lens, static_cast<int>(sinks), static_cast<int>(recent), static_cast<int>(budget),
-      kept, new_lens);
+  const unsigned lists = static_cast<unsigned>(batch * num_kv_heads);
+#define MLR_CHOOSE(T, H)                                                                   \
+  choose_keys<T, H><<<lists, T, 0, s>>>(c, seq_lens, static_cast<int>(sinks),              \
+                                        static_cast<int>(recent), static_cast<int>(budget), \
+                                        kept, new_lens)
+  // As many waves as hold the longest row's keys in registers: fewer meet sooner.
+  const int64_t most = max_blocks * block_size;
+  if (most <= 2048) MLR_CHOOSE(256, 2);
+  else if (most <= 16384) MLR_CHOOSE(1024, 4);
+  else MLR_CHOOSE(1024, 8);
+#undef MLR_CHOOSE
   if (const int rc = check_launch("choose_keys")) return rc;
   return launch_move(c, Lists{kept, nullptr, num_kv_heads * budget, budget,
                               std::min(budget, max_blocks * block_size)}, s);

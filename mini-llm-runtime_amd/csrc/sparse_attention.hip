@@ -110,97 +110,200 @@ struct SparseParams {
   int64_t seqs;
   bool flip;  // a negative scale: the largest score is that of -q
   int sinks, recent, budget, list;  // list: columns of `table`, min(budget, bt_width)
-  uint64_t *keys;                   // [seqs, hkv, bt_width] scores as ordered keys
+  uint64_t *keys;                   // [seqs, hkv, keys_st] scores as ordered keys
+  int64_t keys_st;                  // bt_width, in whole fours
   int64_t *table;                   // [seqs, hkv, list] physical blocks of the chosen
   int64_t *lens;                    // [seqs] keys of the chosen blocks
   int64_t *chosen;                  // [seqs, hkv, budget] their places, may be null
 };
 
-// Scores. kL lanes side by side hold the two bound rows of a block, 16 bytes each; a
-// wave takes 64 / kL blocks at a time, and head by head adds up its products in 64
-// bits.
-constexpr int kScoreBlocks = 64;  // blocks of a workgroup
-constexpr int kHeldHeads = 64;    // heads of a group whose q lies in LDS; the rest is read again
-template <typename T, int kL>
-__global__ __launch_bounds__(256) void score_blocks(SparseParams p) {
+typedef double f64x4_t __attribute__((ext_vector_type(4)));
+
+// Whether a 32-bit word of a row holds an infinity or NaN.
+template <typename T>
+__device__ __forceinline__ bool odd(uint32_t w) {
+  if constexpr (sizeof(T) == 4) return (w & 0x7f800000u) == 0x7f800000u;
+  else if constexpr (std::is_same_v<T, bf16_t>)
+    return (((w & 0x7f807f80u) + 0x00800080u) & 0x80008000u) != 0;
+  else return (((w & 0x7c007c00u) + 0x04000400u) & 0x80008000u) != 0;
+}
+template <typename T>
+__device__ __forceinline__ bool odd(uint4 w) {
+  return odd<T>(w.x) || odd<T>(w.y) || odd<T>(w.z) || odd<T>(w.w);
+}
+
+// Scores on v_mfma_f64_16x16x4: sum_d max(q low, q high) = [q-, q+].[low, high] with q- =
+// min(q, 0) and q+ = max(q, 0), 16 heads times 16 blocks. Operand A is q (lane l: head
+// l % 16), B the bounds (lane l: block l % 16); of a row lane group l / 16 has every
+// fourth piece of 16 bytes, so that its k-th elements are those of A and B alike. A
+// group of fewer heads repeats its last one, and the maximum over heads needs no mask.
+// Where a bound or q is not finite, 0 times it would be NaN where the larger of both
+// products is not: such tiles are added up product by product.
+//
+// Bound by the matrix unit where the heads of a group are many, by the reads of the bounds
+// where they are few: 8 requests of 2,048 blocks, 28/4 heads of 128, bf16, 33 MB in 26 us.
+template <typename T, int kT>
+__global__ __launch_bounds__(256) void score_blocks(SparseParams p, int tiles) {
   constexpr int kE = 16 / sizeof(T);
-  constexpr int kPer = 64 / kL;
-  extern __shared__ float s_q[];  // [min(group, kHeldHeads)][kL * kE]
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  const int tid = threadIdx.x, lane = tid & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int col = lane & 15, g = lane >> 4;
   const int64_t b = blockIdx.x;
   const int64_t seq = b % p.seqs, kvh = b / p.seqs % p.hkv;
-  const int64_t first = b / p.seqs / p.hkv * kScoreBlocks;
+  // A wave's tiles of 16 blocks: the workgroup's in turn.
+  const int64_t first = (b / p.seqs / p.hkv * 4 * tiles + wave) * 16;
   const int64_t ctx = clamp64(p.ctx[seq], 0, p.bt_width * p.block_size);
   const int64_t n = (ctx + p.block_size - 1) / p.block_size;
-  if (first >= n || n <= p.budget) return;  // uniform: nothing there, or nothing to choose
+  if (first >= n || n <= p.budget) return;  // nothing there, or nothing to choose
+  const int64_t *table = p.bt + seq * p.bt_st;
+  const T *bounds = static_cast<const T *>(p.bounds) + kvh * p.d;
+  const int64_t row = p.hkv * p.d;
   const T *q = static_cast<const T *>(p.q) + seq * p.q_st + kvh * p.group * p.q_sh;
-  auto query = [&](int h, int e) __attribute__((always_inline)) {
-    const float x = e < p.d ? Elem<T>::to_f32(q[h * p.q_sh + e]) : 0.f;
-    return p.flip ? -x : x;
+  auto id_of = [&](int i) __attribute__((always_inline)) {
+    return table[min(first + 64 * i + col, n - 1)];
   };
-  const int heads = static_cast<int>(p.group), held = min(heads, kHeldHeads);
-  for (int i = tid; i < held * kL * kE; i += 256)
-    s_q[i] = query(i / (kL * kE), i % (kL * kE));
-  __syncthreads();
-  const int part = lane % kL, sub = lane / kL;
-  const int64_t last = min(first + kScoreBlocks, n);
-  for (int64_t j0 = first + wave * kPer; j0 < last; j0 += 4 * kPer) {
-    const int64_t j = j0 + sub;
-    const int64_t id = j < last ? p.bt[seq * p.bt_st + j] : -1;
-    const bool there = id >= 0 && id < p.num_blocks;
-    double low[kE], high[kE];
-    float x[kE], y[kE];
-    uint4 lw = make_uint4(0, 0, 0, 0), hw = lw;
-    if (there && part * kE < p.d) {
-      const T *at = static_cast<const T *>(p.bounds) + (id * 2 * p.hkv + kvh) * p.d + part * kE;
-      lw = *reinterpret_cast<const uint4 *>(at);
-      hw = *reinterpret_cast<const uint4 *>(at + p.hkv * p.d);
-    }
-    unpack<T>(lw, x);
-    unpack<T>(hw, y);
+  struct Tile {
+    uint4 low[kT], high[kT];
+    bool there;
+  };
+  auto read = [&](Tile &x, int i, int64_t id) __attribute__((always_inline)) {
+    x.there = first + 64 * i + col < n && id >= 0 && id < p.num_blocks;
+    const T *at = bounds + (x.there ? id : 0) * 2 * row;
 #pragma unroll
-    for (int e = 0; e < kE; ++e) {
-      low[e] = x[e];
-      high[e] = y[e];
+    for (int t = 0; t < kT; ++t) {
+      const int e = (g + 4 * t) * kE;
+      x.low[t] = x.high[t] = make_uint4(0, 0, 0, 0);
+      if (e < p.d && x.there) {
+        x.low[t] = *reinterpret_cast<const uint4 *>(at + e);
+        x.high[t] = *reinterpret_cast<const uint4 *>(at + row + e);
+      }
     }
-    double best = -INFINITY;
-    for (int h = 0; h < heads; ++h) {
-      double sum = 0.;
+  };
+  const int heads = static_cast<int>(p.group);
+  const bool many = heads > 16;
+  // q of heads h0 ..: its negative and its positive part, in 64 bits.
+  double below[kT][kE], above[kT][kE];
+  bool q_odd = false;
+  auto read_q = [&](int h0) __attribute__((always_inline)) {
+    const T *mine = q + min(h0 + col, heads - 1) * p.q_sh;
+    q_odd = false;
+#pragma unroll
+    for (int t = 0; t < kT; ++t) {
+      const int e0 = (g + 4 * t) * kE;
+      uint4 x = make_uint4(0, 0, 0, 0);
+      if (e0 < p.d) x = *reinterpret_cast<const uint4 *>(mine + e0);
+      q_odd = q_odd || odd<T>(x);
+      float f[kE];
+      unpack<T>(x, f);
 #pragma unroll
       for (int e = 0; e < kE; ++e) {
-        const float f =
-            h < held ? s_q[h * (kL * kE) + part * kE + e] : query(h, part * kE + e);
-        sum = fma(static_cast<double>(f), f >= 0.f ? high[e] : low[e], sum);
+        const float v = p.flip ? -f[e] : f[e];
+        below[t][e] = fminf(v, 0.f);
+        above[t][e] = fmaxf(v, 0.f);
       }
-#pragma unroll
-      for (int o = 1; o < kL; o <<= 1) sum += __shfl_xor(sum, o);
-      best = sum > best ? sum : best;  // a sum that is NaN counts for nothing
     }
-    if (part == 0 && j < last)
-      p.keys[(seq * p.hkv + kvh) * p.bt_width + j] = order_key(there ? best : -INFINITY);
+  };
+  auto score = [&](const Tile &x, int i) __attribute__((always_inline)) {
+    bool bound_odd = false;
+#pragma unroll
+    for (int t = 0; t < kT; ++t)
+      bound_odd = bound_odd || odd<T>(x.low[t]) || odd<T>(x.high[t]);
+    double best = -INFINITY;
+    for (int h0 = 0; h0 < heads; h0 += 16) {
+      if (many) read_q(h0);
+      if (__builtin_expect(!__any(bound_odd || q_odd), 1)) {
+        f64x4_t sum0 = {0., 0., 0., 0.}, sum1 = {0., 0., 0., 0.};
+#pragma unroll
+        for (int t = 0; t < kT; ++t) {
+          float l[kE], u[kE];
+          unpack<T>(x.low[t], l);
+          unpack<T>(x.high[t], u);
+#pragma unroll
+          for (int e = 0; e < kE; ++e) {
+            sum0 = __builtin_amdgcn_mfma_f64_16x16x4f64(below[t][e], l[e], sum0, 0, 0, 0);
+            sum1 = __builtin_amdgcn_mfma_f64_16x16x4f64(above[t][e], u[e], sum1, 0, 0, 0);
+          }
+        }
+#pragma unroll
+        for (int r = 0; r < 4; ++r) best = fmax(best, sum0[r] + sum1[r]);
+      } else {
+        for (int h = h0; h < min(h0 + 16, heads); ++h) {
+          double sum = 0.;
+#pragma unroll
+          for (int t = 0; t < kT; ++t) {
+            float l[kE], u[kE];
+            unpack<T>(x.low[t], l);
+            unpack<T>(x.high[t], u);
+#pragma unroll
+            for (int e = 0; e < kE; ++e) {
+              const int at = (g + 4 * t) * kE + e;
+              if (at >= p.d) continue;
+              const float f = Elem<T>::to_f32(q[h * p.q_sh + at]);
+              const double v = p.flip ? -f : f;
+              sum = fma(v, v >= 0. ? u[e] : l[e], sum);
+            }
+          }
+          sum += __shfl_xor(sum, 16);
+          sum += __shfl_xor(sum, 32);
+          best = sum > best ? sum : best;  // a sum that is NaN does not count
+        }
+      }
+    }
+    best = fmax(best, __shfl_xor(best, 16));
+    best = fmax(best, __shfl_xor(best, 32));
+    const int64_t j = first + 64 * i + col;
+    if (g == 0 && j < n)
+      p.keys[(seq * p.hkv + kvh) * p.keys_st + j] = order_key(x.there ? best : -INFINITY);
+  };
+  Tile even, other;
+  const int count = static_cast<int>(min(int64_t(tiles), (n - first + 63) / 64));
+  read(even, 0, id_of(0));
+  int64_t id = id_of(1);
+  if (!many) read_q(0);
+  for (int i = 0; i < count; i += 2) {
+    if (i + 1 < count) read(other, i + 1, id);
+    id = id_of(i + 2);
+    score(even, i);
+    if (i + 1 >= count) break;
+    if (i + 2 < count) read(even, i + 2, id);
+    id = id_of(i + 3);
+    score(other, i + 1);
   }
 }
 
 // A workgroup chooses the blocks of one request and KV head.
-__global__ __launch_bounds__(kSelectThreads) void choose_blocks(SparseParams p) {
+template <int kThreads, int kHeld>
+__global__ __launch_bounds__(kThreads) void choose_blocks(SparseParams p) {
   __shared__ SelectShared s;
   const int64_t seq = blockIdx.x % p.seqs, kvh = blockIdx.x / p.seqs;
   const int64_t pair = seq * p.hkv + kvh;
   const int64_t ctx = clamp64(p.ctx[seq], 0, p.bt_width * p.block_size);
   const int n = static_cast<int>((ctx + p.block_size - 1) / p.block_size);
-  const uint64_t *keys = p.keys + pair * p.bt_width;
+  const uint64_t *keys = p.keys + pair * p.keys_st;
   const int64_t *row = p.bt + seq * p.bt_st;
   int64_t *table = p.table + pair * p.list;
   int64_t *chosen = p.chosen ? p.chosen + pair * p.budget : nullptr;
-  const int count = select_places<uint64_t, 8>(
+  const int count = select_places<uint64_t, kThreads, kHeld>(
       s, n, p.sinks, p.recent, p.budget,
-      [&](int i) __attribute__((always_inline)) { return keys[i]; },
+      [&](auto &held, auto place) __attribute__((always_inline)) {
+        constexpr int kMany = sizeof(held) / sizeof(held[0]);
+#pragma unroll
+        for (int j = 0; j < kMany; ++j) {
+          const ulonglong2 *at =
+              reinterpret_cast<const ulonglong2 *>(keys + (min(place(j), n - 1) & ~3));
+          const ulonglong2 a = at[0], b = at[1];
+          held[j][0] = a.x;
+          held[j][1] = a.y;
+          held[j][2] = b.x;
+          held[j][3] = b.y;
+        }
+      },
       [&](int r, int i) __attribute__((always_inline)) {
         table[r] = row[i];
         if (chosen) chosen[r] = i;
       });
   if (chosen)
-    for (int i = count + threadIdx.x; i < p.budget; i += kSelectThreads) chosen[i] = -1;
+    for (int i = count + threadIdx.x; i < p.budget; i += kThreads) chosen[i] = -1;
   // The last block is always chosen, and the only one that may not be full.
   if (p.lens && kvh == 0 && threadIdx.x == 0)
     p.lens[seq] = count > 0 ? ctx - static_cast<int64_t>(n - count) * p.block_size : 0;
@@ -208,18 +311,22 @@ __global__ __launch_bounds__(kSelectThreads) void choose_blocks(SparseParams p) 
 
 template <typename T>
 int launch_scores(const SparseParams &p, hipStream_t stream) {
+  // Tiles of a wave: q is converted once for all of them, but a wave for every SIMD comes
+  // first.
+  const int64_t all = ceil_div(p.bt_width, 64) * p.hkv * p.seqs;  // of four waves
+  const int64_t cus = current_device_cus() > 0 ? current_device_cus() : 256;
+  const int tiles = static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(8, all / cus)));
   const unsigned grid =
-      static_cast<unsigned>(ceil_div(p.bt_width, kScoreBlocks) * p.hkv * p.seqs);
-  const int64_t lanes = ceil_div(p.d * static_cast<int64_t>(sizeof(T)), 16);
-  auto lds = [&](int l) {
-    return static_cast<size_t>(std::min<int64_t>(p.group, kHeldHeads)) * l * 64 / sizeof(T);
-  };
-  if (lanes <= 4) score_blocks<T, 4><<<grid, 256, lds(4), stream>>>(p);
-  else if (lanes <= 8) score_blocks<T, 8><<<grid, 256, lds(8), stream>>>(p);
-  else if (lanes <= 16) score_blocks<T, 16><<<grid, 256, lds(16), stream>>>(p);
-  else score_blocks<T, 32><<<grid, 256, lds(32), stream>>>(p);
+      static_cast<unsigned>(ceil_div(p.bt_width, 64 * tiles) * p.hkv * p.seqs);
+  const int64_t pieces = ceil_div(p.d * static_cast<int64_t>(sizeof(T)), 16);
+  if (pieces <= 4) score_blocks<T, 1><<<grid, 256, 0, stream>>>(p, tiles);
+  else if (pieces <= 8) score_blocks<T, 2><<<grid, 256, 0, stream>>>(p, tiles);
+  else if (pieces <= 16) score_blocks<T, 4><<<grid, 256, 0, stream>>>(p, tiles);
+  else score_blocks<T, 8><<<grid, 256, 0, stream>>>(p, tiles);
   return check_launch("score_blocks");
 }
+
+int64_t whole_fours(int64_t n) { return (n + 3) & ~int64_t(3); }
 
 struct Layout {
   size_t keys, table, lens, decode;
@@ -228,7 +335,7 @@ struct Layout {
 Layout layout_of(int64_t batch, int64_t hq, int64_t hkv, int64_t d, int64_t width,
                  int64_t block_size, int64_t budget) {
   const int64_t list = std::min(budget, width);
-  return Layout{align256(batch * hkv * width * sizeof(uint64_t)),
+  return Layout{align256(batch * hkv * whole_fours(width) * sizeof(uint64_t)),
                 align256(batch * hkv * list * sizeof(int64_t)), align256(batch * sizeof(int64_t)),
                 decode_workspace(batch, hq, hkv, d, list * block_size)};
 }
@@ -312,7 +419,7 @@ extern "C" int mlr_paged_decode_sparse(
                   seq_lens && out, "%s: null pointer", o.what);
   MLR_REQUIRE(reinterpret_cast<uintptr_t>(key_bounds) % 16 == 0,
               "%s: bounds must be 16-byte aligned", o.what);
-  MLR_REQUIRE(ceil_div(max_blocks, kScoreBlocks) * num_kv_heads * batch < (int64_t(1) << 31),
+  MLR_REQUIRE(ceil_div(max_blocks, 64) * num_kv_heads * batch < (int64_t(1) << 31),
               "%s: too many blocks", o.what);
   const size_t need = mlr_paged_decode_sparse_workspace_size(
       batch, num_q_heads, num_kv_heads, head_dim, max_blocks, block_size, budget);
@@ -324,7 +431,7 @@ extern "C" int mlr_paged_decode_sparse(
   SparseParams x{q, key_bounds, q_stride_b, q_stride_h, num_blocks, block_size, num_kv_heads,
                  group, head_dim, block_tables, bt_stride, max_blocks, seq_lens, batch, scale < 0,
                  static_cast<int>(sinks), static_cast<int>(recent), static_cast<int>(budget),
-                 static_cast<int>(list), nullptr, nullptr, nullptr, chosen};
+                 static_cast<int>(list), nullptr, whole_fours(max_blocks), nullptr, nullptr, chosen};
   int64_t max_keys = 0;
   if (need) {
     const Layout l = layout_of(batch, num_q_heads, num_kv_heads, head_dim, max_blocks, block_size,
@@ -347,7 +454,9 @@ extern "C" int mlr_paged_decode_sparse(
     o.ctx = x.lens;
   }
   if (need || chosen) {
-    choose_blocks<<<static_cast<unsigned>(batch * num_kv_heads), kSelectThreads, 0, s>>>(x);
+    const unsigned lists = static_cast<unsigned>(batch * num_kv_heads);
+    if (max_blocks <= 1024) choose_blocks<256, 1><<<lists, 256, 0, s>>>(x);
+    else choose_blocks<1024, 2><<<lists, 1024, 0, s>>>(x);
     if (const int rc = check_launch("choose_blocks")) return rc;
   }
   ScoredParams p = params_of(o, kModeDecode);
