@@ -821,7 +821,7 @@ int mlr_update_key_bounds(const void *k_cache, void *key_bounds, int64_t num_blo
 size_t mlr_paged_decode_sparse_workspace_size(int64_t batch, int64_t num_q_heads,
                                               int64_t num_kv_heads, int64_t head_dim,
                                               int64_t max_blocks, int64_t block_size,
-                                              int64_t budget);
+                                              int64_t budget, int dtype);
 int mlr_paged_decode_sparse(const void *q, int64_t q_stride_b, int64_t q_stride_h,
                             const void *k_cache, const void *v_cache, const void *key_bounds,
                             int64_t num_blocks, int64_t block_size, int64_t num_kv_heads,

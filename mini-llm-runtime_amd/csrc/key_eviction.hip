@@ -14,71 +14,182 @@ namespace mlr {
 namespace {
 
 constexpr float kLog2e = 1.4426950408889634f;
-constexpr int kChunk = 1024;  // keys of a workgroup of weigh_keys
-constexpr int kHeads = 64;    // heads whose statistics it holds at a time
+constexpr int kChunk = 256;  // keys of a wave of weigh_keys
+constexpr int kHeads = 64;   // heads whose statistics it holds at a time
 
-// The second pass of a weighing decode: scores, and (m, l) of each row's items, are in
-// the workspace. A workgroup joins the statistics of its KV head's rows, then adds
-// up the weights of its keys, four to a thread. Requests that share a block add to the
-// same entry, hence the atomic; where blocks are a request's own each entry has one
-// addend and the result does not depend on any order.
-__global__ __launch_bounds__(256) void weigh_keys(ScoredParams p, float *weights) {
-  __shared__ float s_m[kHeads], s_inv[kHeads];
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-  const int64_t b = blockIdx.x;
-  const int64_t seq = b % p.seqs;
-  const int kvh = static_cast<int>(b / p.seqs % p.hkv);
-  const int64_t chunk = b / p.seqs / p.hkv;
-  const int64_t ctx = clamp64(p.ctx[seq], 0, p.bt_width * p.block_size);
-  if (chunk * kChunk >= ctx) return;  // uniform
-  const int64_t key0 = chunk * kChunk + 4 * tid;
+// out = sum_i e^{m_i - M} O_i / sum_i e^{m_i - M} l_i over the items of row (sequence,
+// head) of a decode: 16 lanes side by side over its elements, four groups of lanes dealing
+// the items among them, joined in a fixed order.
+template <typename T, int D>
+__device__ __forceinline__ void join_row(const ScoredParams &p, int64_t row) {
+  constexpr int kVe = D / 16;
+  const int lane = threadIdx.x & 63, d0 = (lane & 15) * kVe, quarter = lane >> 4;
+  const int64_t seq = row / p.hq;
+  const int head = static_cast<int>(row - seq * p.hq), kvh = head / p.group;
+  const int in_group = head - kvh * p.group, tile = in_group / kRows;
+  const int64_t unit = seq * p.tiles + tile;
+  const int first = p.first[unit], count = p.first[unit + 1] - first;
+  const int64_t at = (static_cast<int64_t>(first) * p.hkv + kvh) * kRows + in_group - tile * kRows;
+  const int64_t step = static_cast<int64_t>(p.hkv) * kRows;
+  float m = -INFINITY;
+  for (int i = lane; i < count; i += 64) m = fmaxf(m, p.ml[2 * (at + i * step)]);
+  m = wave_max(m);
+  const float ref = m == -INFINITY ? 0.f : m;
+  float sum = 0.f, acc[kVe];
+#pragma unroll
+  for (int n = 0; n < kVe; ++n) acc[n] = 0.f;
+#pragma unroll 4
+  for (int i = quarter; i < count; i += 4) {
+    const float2 ml = *reinterpret_cast<const float2 *>(p.ml + 2 * (at + i * step));
+    const float f = __builtin_amdgcn_exp2f((ml.x - ref) * kLog2e);
+    sum += ml.y * f;
+#pragma unroll
+    for (int n = 0; n < kVe; n += 4) {
+      const float4 v = *reinterpret_cast<const float4 *>(p.acc + (at + i * step) * D + d0 + n);
+      acc[n] += v.x * f;
+      acc[n + 1] += v.y * f;
+      acc[n + 2] += v.z * f;
+      acc[n + 3] += v.w * f;
+    }
+  }
+  auto join = [](float v) {
+    v += __shfl_xor(v, 16);
+    return v + __shfl_xor(v, 32);
+  };
+  sum = join(sum);
+#pragma unroll
+  for (int n = 0; n < kVe; ++n) acc[n] = join(acc[n]);
+  if (quarter != 0) return;
+  const float inv = sum > 0.f ? 1.f / sum : sum == 0.f ? 0.f : sum;
+  T *dst = static_cast<T *>(p.out) + seq * p.o_st + head * p.o_sh;
+#pragma unroll
+  for (int n = 0; n < kVe; ++n)
+    if (d0 + n < p.d) dst[d0 + n] = Elem<T>::from_f32(acc[n] * inv);
+}
+
+// The second pass of a weighing decode: the scores, and (m, l) of each row's items, are
+// in the workspace. A wave joins the statistics of its KV head's rows and adds up the
+// weights of 256 keys, four to a lane. Requests that share a block add to the same
+// entry, hence the atomic; where blocks are a request's own each entry has one addend
+// and the result does not depend on any order.
+// Bound by latency, as the scores of 64 requests are 8 MB: what does not depend on the
+// statistics (table, scores of up to kAhead heads) is read before them.
+constexpr int kAhead = 8;
+__device__ __forceinline__ void weigh_keys(const ScoredParams &p, float *weights, int64_t task,
+                                           float (*s_ml)[2]) {
+  const int lane = threadIdx.x & 63;
+  const int64_t seq = task % p.seqs;
+  const int kvh = static_cast<int>(task / p.seqs % p.hkv);
+  const int64_t covered = p.bt_width * p.block_size;
+  const int64_t key0 = task / p.seqs / p.hkv * kChunk + 4 * lane;
+  const int64_t ctx = clamp64(p.ctx[seq], 0, covered);
+  const float *row = p.scores + (seq * p.hq + kvh * p.group) * p.scores_st +
+                     min(key0, p.scores_st - 4);
+  float4 x[kAhead];
+#pragma unroll
+  for (int h = 0; h < kAhead; ++h)
+    x[h] = *reinterpret_cast<const float4 *>(row + min(h, p.group - 1) * p.scores_st);
+  const uint32_t bs = static_cast<uint32_t>(p.block_size);
+  auto block_of = [&](uint32_t key) __attribute__((always_inline)) {
+    return p.bs_log2 >= 0 ? key >> p.bs_log2 : key / bs;
+  };
+  int64_t block[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+    block[i] = p.bt[seq * p.bt_st + block_of(static_cast<uint32_t>(min(key0 + i, covered - 1)))];
   float w[4] = {0.f, 0.f, 0.f, 0.f};
   for (int h0 = 0; h0 < p.group; h0 += kHeads) {
     const int heads = min(kHeads, p.group - h0);
-    for (int h = wave; h < heads; h += 4) {
+    // Eight lanes a head, its items dealt among them.
+    for (int h8 = 0; h8 < heads; h8 += 8) {
+      const int h = min(h8 + (lane >> 3), heads - 1);
       const int tile = (h0 + h) / kRows, rr = (h0 + h) - tile * kRows;
       const int64_t unit = seq * p.tiles + tile;
-      const int first = p.first[unit], count = p.first[unit + 1] - first;
+      const int first = p.whole ? static_cast<int>(unit) : p.first[unit];
+      const int count = p.whole ? 1 : p.first[unit + 1] - first;
       const int64_t at = (static_cast<int64_t>(first) * p.hkv + kvh) * kRows + rr;
       const int64_t step = static_cast<int64_t>(p.hkv) * kRows;
       float m = -INFINITY, l = 0.f;
-      for (int i = lane; i < count; i += 64) m = fmaxf(m, p.ml[2 * (at + i * step)]);
-      m = wave_max(m);
-      const float ref = m == -INFINITY ? 0.f : m;
-      for (int i = lane; i < count; i += 64)
-        l += p.ml[2 * (at + i * step) + 1] *
-             __builtin_amdgcn_exp2f((p.ml[2 * (at + i * step)] - ref) * kLog2e);
-      l = wave_sum(l);
-      if (lane == 0) {
-        s_m[h] = ref;
-        s_inv[h] = l > 0.f ? 1.f / l : l == 0.f ? 0.f : l;
+#pragma unroll 4
+      for (int i = lane & 7; i < count; i += 8) {
+        const float2 ml = *reinterpret_cast<const float2 *>(p.ml + 2 * (at + i * step));
+        const float top = fmaxf(m, ml.x), ref = top == -INFINITY ? 0.f : top;
+        l = l * __builtin_amdgcn_exp2f((m - ref) * kLog2e) +
+            ml.y * __builtin_amdgcn_exp2f((ml.x - ref) * kLog2e);
+        m = top;
+      }
+      float top = m;
+#pragma unroll
+      for (int o = 4; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor(top, o));
+      const float ref = top == -INFINITY ? 0.f : top;
+      l *= __builtin_amdgcn_exp2f((m - ref) * kLog2e);
+#pragma unroll
+      for (int o = 4; o > 0; o >>= 1) l += __shfl_xor(l, o);
+      if ((lane & 7) == 0) {
+        s_ml[h][0] = ref;
+        s_ml[h][1] = l > 0.f ? 1.f / l : l == 0.f ? 0.f : l;
       }
     }
-    __syncthreads();
-    if (key0 < ctx) {
-      const float *row = p.scores + (seq * p.hq + kvh * p.group + h0) * p.scores_st + key0;
-      for (int h = 0; h < heads; ++h) {
-        const float4 x = *reinterpret_cast<const float4 *>(row + h * p.scores_st);
-        w[0] += __builtin_amdgcn_exp2f((x.x - s_m[h]) * kLog2e) * s_inv[h];
-        w[1] += __builtin_amdgcn_exp2f((x.y - s_m[h]) * kLog2e) * s_inv[h];
-        w[2] += __builtin_amdgcn_exp2f((x.z - s_m[h]) * kLog2e) * s_inv[h];
-        w[3] += __builtin_amdgcn_exp2f((x.w - s_m[h]) * kLog2e) * s_inv[h];
-      }
+    // One wave's own rows of LDS: in order without a barrier.
+    auto add = [&](const float4 &v, int h) __attribute__((always_inline)) {
+      const float m = s_ml[h][0], inv = s_ml[h][1];
+      w[0] += __builtin_amdgcn_exp2f((v.x - m) * kLog2e) * inv;
+      w[1] += __builtin_amdgcn_exp2f((v.y - m) * kLog2e) * inv;
+      w[2] += __builtin_amdgcn_exp2f((v.z - m) * kLog2e) * inv;
+      w[3] += __builtin_amdgcn_exp2f((v.w - m) * kLog2e) * inv;
+    };
+    int h = 0;
+    if (h0 == 0) {
+#pragma unroll
+      for (int i = 0; i < kAhead; ++i)
+        if (i < heads) add(x[i], i);
+      h = min(kAhead, heads);
     }
-    __syncthreads();
+    for (; h < heads; ++h)
+      add(*reinterpret_cast<const float4 *>(row + (h0 + h) * p.scores_st), h);
   }
-  const int64_t *table = p.bt + seq * p.bt_st;
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
-    const int64_t key = key0 + i;
-    if (key >= ctx) break;
-    const int64_t at = key / p.block_size;
-    const int64_t block = table[at];
-    if (block < 0 || block >= p.num_blocks) continue;
-    float *entry = weights + (block * p.hkv + kvh) * p.block_size + (key - at * p.block_size);
-    if (key == ctx - 1) *entry = w[i];
+    if (key0 + i >= ctx || block[i] < 0 || block[i] >= p.num_blocks) continue;
+    const uint32_t key = static_cast<uint32_t>(key0 + i);
+    float *entry = weights + (block[i] * p.hkv + kvh) * p.block_size + (key - block_of(key) * bs);
+    if (key0 + i == ctx - 1) *entry = w[i];
     else unsafeAtomicAdd(entry, w[i]);
   }
+}
+
+// Both ends of a weighing decode that was cut into items: its results joined, a wave a
+// row, and its keys weighed, a wave for 256 of them.
+template <typename T, int D>
+__global__ __launch_bounds__(256) void weigh_and_join(ScoredParams p, float *weights,
+                                                      int64_t rows, int64_t tasks) {
+  __shared__ float s_ml[4][kHeads][2];
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  for (int64_t task = blockIdx.x * int64_t(4) + wave; task < rows + tasks;
+       task += gridDim.x * int64_t(4)) {
+    if (task < rows) join_row<T, D>(p, task);
+    else weigh_keys(p, weights, task - rows, s_ml[wave]);
+  }
+}
+
+int launch_weigh(const ScoredParams &p, float *weights, int64_t max_keys, int dtype,
+                 hipStream_t stream) {
+  const int64_t rows = p.whole ? 0 : static_cast<int64_t>(p.seqs) * p.hq;
+  const int64_t tasks = static_cast<int64_t>(p.seqs) * p.hkv * ceil_div(max_keys, kChunk);
+  const unsigned grid =
+      static_cast<unsigned>(std::min<int64_t>(ceil_div(rows + tasks, 4), 1 << 20));
+#define MLR_WEIGH(T)                                                                          \
+  if (p.d > 64) weigh_and_join<T, 128><<<grid, 256, 0, stream>>>(p, weights, rows, tasks);    \
+  else weigh_and_join<T, 64><<<grid, 256, 0, stream>>>(p, weights, rows, tasks)
+  if (dtype == MLR_DTYPE_F32) {
+    MLR_WEIGH(float);
+  } else if (dtype == MLR_DTYPE_F16) {
+    MLR_WEIGH(f16_t);
+  } else {
+    MLR_WEIGH(bf16_t);
+  }
+#undef MLR_WEIGH
+  return check_launch("weigh_and_join");
 }
 
 struct CacheParams {
@@ -404,8 +515,6 @@ extern "C" int mlr_paged_decode_weighted(
   const int64_t max_keys = max_blocks * block_size;
   const size_t need = mlr_paged_decode_weighted_workspace_size(batch, num_q_heads, num_kv_heads,
                                                                head_dim, max_keys);
-  const int64_t groups = batch * num_kv_heads * ceil_div(std::max<int64_t>(max_keys, 1), kChunk);
-  MLR_REQUIRE(groups < (int64_t(1) << 31), "%s: too many keys", o.what);
   MLR_REQUIRE(need == 0 || (workspace && workspace_bytes >= need),
               "%s: workspace of %zu bytes, %zu needed", o.what, workspace_bytes, need);
   ScoredParams p = params_of(o, kModeDecode);
@@ -416,12 +525,11 @@ extern "C" int mlr_paged_decode_weighted(
   char *ws = static_cast<char *>(workspace);
   p.scores = reinterpret_cast<float *>(ws);
   p.scores_st = (max_keys + 15) & ~int64_t(15);
-  p.force_partial = true;
+  p.whole = short_keys(max_keys, head_dim, dtype);
+  p.force_partial = !p.whole;
   const int64_t items = plan_decode(p, max_keys, ws + scores_bytes(batch, num_q_heads, max_keys));
   if (const int rc = launch_scored_rows(p, dtype, grid_of(items), s)) return rc;
-  weigh_keys<<<static_cast<unsigned>(groups), 256, 0, s>>>(p, key_weights);
-  if (const int rc = check_launch("weigh_keys")) return rc;
-  return merge_decode(p, dtype, s);
+  return launch_weigh(p, key_weights, max_keys, dtype, s);
 }
 
 extern "C" int mlr_evict_keys(void *k_cache, void *v_cache, float *key_weights,

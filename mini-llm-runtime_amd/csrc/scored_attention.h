@@ -194,12 +194,20 @@ ScoredParams params_of(const Operands &o, int mode);
 size_t decode_workspace(int64_t batch, int64_t hq, int64_t hkv, int64_t d, int64_t max_keys);
 // Plans a decode and places its partial results; the number of its items.
 int64_t plan_decode(ScoredParams &p, int64_t max_keys, char *workspace);
+// Whether units of up to max_keys keys are better left whole on that kernel: cutting them
+// costs each workgroup its planning and the call a launch to join the parts, some 8 us, and
+// a workgroup takes 2.5 us for 32 KB of keys (FP32, head size 64, whole and cut: 320 keys
+// 14.4 and 15.6 us, 640 keys 19.5 and 13.5 us).
+inline bool short_keys(int64_t max_keys, int64_t d, int dtype) {
+  return max_keys * (d > 64 ? 128 : 64) * dtype_size(dtype) <= 80 << 10;
+}
 unsigned grid_of(int64_t items);
 int merge_decode(const ScoredParams &p, int dtype, hipStream_t stream);
 size_t align256(size_t n);
 
-// Units of 128 rows; bf16 and fp16, block_size a power of two from 16 on.
-constexpr int kTileRows = 128;
+// Units of 128 rows; bf16 and fp16, block_size a power of two from 16 on. Drafted trees
+// that are not left whole: at most kTreeSeqs sequences.
+constexpr int kTileRows = 128, kTreeSeqs = 512;
 int launch_scored_tiles(const ScoredParams &p, int dtype, unsigned grid, hipStream_t stream);
 
 }  // namespace mlr

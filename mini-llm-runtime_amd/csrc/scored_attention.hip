@@ -89,6 +89,70 @@ __global__ __launch_bounds__(256) void scored_merge(ScoredParams p, int u0, int 
   }
 }
 
+// scored_merge for drafted trees, whose units have many rows of few items each: 16 lanes a
+// row, four rows a wave (41 units of 128 rows, 4 KV heads of 128: 16 us with a wave a
+// row, MEASURED us so).
+template <typename T, int D>
+__global__ __launch_bounds__(256) void tree_merge(ScoredParams p) {
+  constexpr int kVe = D / 16;
+  const int lane = threadIdx.x & 15, d0 = lane * kVe;
+  const int64_t slots = static_cast<int64_t>(p.units) * p.hkv * kTileRows;
+  for (int64_t slot = blockIdx.x * int64_t(16) + (threadIdx.x >> 4); slot < slots;
+       slot += gridDim.x * int64_t(16)) {
+    const int uk = static_cast<int>(slot / kTileRows), rr = static_cast<int>(slot % kTileRows);
+    const int u = uk / p.hkv, kvh = uk - u * p.hkv;
+    const int first = p.first[u], count = p.first[u + 1] - first;
+    if (count < 2) continue;  // no rows, or written already
+    const Unit t = unit_of(p, u, kTileRows);
+    const int r = t.r0 + rr;
+    if (r >= t.rows) continue;
+    const int64_t at = (static_cast<int64_t>(first) * p.hkv + kvh) * kTileRows + rr;
+    const int64_t step = static_cast<int64_t>(p.hkv) * kTileRows;
+    float m = -INFINITY;
+    for (int i = lane; i < count; i += 16) m = fmaxf(m, p.ml[2 * (at + i * step)]);
+#pragma unroll
+    for (int o = 8; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor(m, o));
+    const float ref = m == -INFINITY ? 0.f : m;
+    float sum = 0.f, acc[kVe];
+#pragma unroll
+    for (int n = 0; n < kVe; ++n) acc[n] = 0.f;
+#pragma unroll 8
+    for (int i = 0; i < count; ++i) {
+      const float2 ml = *reinterpret_cast<const float2 *>(p.ml + 2 * (at + i * step));
+      const float f = __builtin_amdgcn_exp2f((ml.x - ref) * kLog2e);
+      sum += ml.y * f;
+#pragma unroll
+      for (int n = 0; n < kVe; n += 4) {
+        const float4 v =
+            *reinterpret_cast<const float4 *>(p.acc + (at + i * step) * D + d0 + n);
+        acc[n] += v.x * f;
+        acc[n + 1] += v.y * f;
+        acc[n + 2] += v.z * f;
+        acc[n + 3] += v.w * f;
+      }
+    }
+    const float inv = sum > 0.f ? 1.f / sum : sum == 0.f ? 0.f : sum;
+    const int tok = r / p.group, g = r - tok * p.group;
+    T *dst = static_cast<T *>(p.out) + (t.q0 + tok) * p.o_st + (kvh * p.group + g) * p.o_sh;
+#pragma unroll
+    for (int n = 0; n < kVe; ++n)
+      if (d0 + n < p.d) dst[d0 + n] = Elem<T>::from_f32(acc[n] * inv);
+  }
+}
+
+int launch_tree_merge(const ScoredParams &p, int dtype, hipStream_t stream) {
+  const unsigned grid = static_cast<unsigned>(std::min<int64_t>(
+      ceil_div(static_cast<int64_t>(p.units) * p.hkv * kTileRows, 16), 1 << 20));
+  if (dtype == MLR_DTYPE_F16) {
+    if (p.d > 64) tree_merge<f16_t, 128><<<grid, 256, 0, stream>>>(p);
+    else tree_merge<f16_t, 64><<<grid, 256, 0, stream>>>(p);
+  } else {
+    if (p.d > 64) tree_merge<bf16_t, 128><<<grid, 256, 0, stream>>>(p);
+    else tree_merge<bf16_t, 64><<<grid, 256, 0, stream>>>(p);
+  }
+  return check_launch("tree_merge");
+}
+
 int launch_merge(const ScoredParams &p, int u0, int p_rows, const ScoredParams &x, int x_rows,
                  bool prefixed, int dtype, hipStream_t stream) {
   const int used = p.mode == kModePrefill ? p_rows : std::min(p_rows, p.group);
@@ -224,7 +288,7 @@ struct PrefillPlan {
   bool whole, parts;
 };
 PrefillPlan plan_prefill(int64_t seqs, int64_t max_q, int64_t max_keys, int64_t block_size,
-                         int64_t hq, int64_t hkv, int64_t d, int dtype) {
+                         int64_t hq, int64_t hkv, int64_t d, int dtype, bool tree) {
   const int64_t group = hq / hkv;
   PrefillPlan n;
   const bool tiles = takes_tiles(max_q * group, block_size, hkv, d, dtype);
@@ -234,6 +298,15 @@ PrefillPlan plan_prefill(int64_t seqs, int64_t max_q, int64_t max_keys, int64_t 
   n.items = max_items(n.units, hkv, max_keys, n.target);
   n.whole = tiles ? !splits_pay(n.units * hkv, max_keys, cus())
                   : part_bytes(n.units, n.items, kRows, d) > kMostParts;
+  if (tree && !tiles) {
+    n.whole = n.whole || short_keys(max_keys, d, dtype);
+  } else if (tree) {
+    // Items for all CUs once, cut by the kernel; batches that fill them four times over
+    // even out by themselves, and keys that no split is shorter than stay whole.
+    n.target = (d > 64 ? 1 : 2) * static_cast<int64_t>(cus());
+    n.items = max_items(n.units, hkv, max_keys, n.target);
+    n.whole = n.units * hkv > 4 * n.target || max_keys <= kMinSplit || seqs > kTreeSeqs;
+  }
   if (n.whole) {
     n.target = 1;  // a split as long as all keys
     n.items = n.units * hkv;
@@ -380,7 +453,7 @@ extern "C" size_t mlr_paged_prefill_scored_workspace_size(int64_t num_seqs, int6
       head_dim <= 0 || block_size <= 0)
     return 0;
   const PrefillPlan n = plan_prefill(num_seqs, max_query_len, max_blocks * block_size, block_size,
-                                     num_q_heads, num_kv_heads, head_dim, dtype);
+                                     num_q_heads, num_kv_heads, head_dim, dtype, false);
   return n.parts ? part_bytes(n.units, n.items, n.rows, head_dim) : 0;
 }
 
@@ -399,7 +472,7 @@ static int run_packed(const Operands &o, const int64_t *query_start_loc, const i
                   prefill_units(o.seqs, max_query_len, group, kRows) * o.hkv < (int64_t(1) << 25),
               "%s: too many query rows", o.what);
   const PrefillPlan n = plan_prefill(o.seqs, max_query_len, o.bt_width * o.block_size,
-                                     o.block_size, o.hq, o.hkv, o.d, o.dtype);
+                                     o.block_size, o.hq, o.hkv, o.d, o.dtype, bits != nullptr);
   const size_t need = n.parts ? part_bytes(n.units, n.items, n.rows, o.d) : 0;
   MLR_REQUIRE(need == 0 || (workspace && workspace_bytes >= need),
               "%s: workspace of %zu bytes, %zu needed", o.what, workspace_bytes, need);
@@ -414,13 +487,16 @@ static int run_packed(const Operands &o, const int64_t *query_start_loc, const i
   p.whole = n.whole;
   p.target = n.target;
   const int rows = static_cast<int>(n.rows);
+  MLR_REQUIRE(n.whole || n.parts || rows == kRows, "%s: splits without a workspace", o.what);
   if (n.parts) place_parts(p, static_cast<char *>(workspace), n.items, rows);
   hipStream_t s = static_cast<hipStream_t>(stream);
   const int rc = rows == kTileRows
                      ? launch_scored_tiles(p, o.dtype, static_cast<unsigned>(n.items), s)
                      : launch_scored_rows(p, o.dtype, grid_of(n.items), s);
   if (rc) return rc;
-  return n.parts ? launch_merge(p, 0, rows, p, rows, false, o.dtype, s) : MLR_OK;
+  if (!n.parts) return MLR_OK;
+  return bits && rows == kTileRows ? launch_tree_merge(p, o.dtype, s)
+                                   : launch_merge(p, 0, rows, p, rows, false, o.dtype, s);
 }
 
 extern "C" int mlr_paged_prefill_scored(
@@ -445,8 +521,12 @@ extern "C" size_t mlr_paged_attention_tree_workspace_size(int64_t num_seqs, int6
                                                           int64_t num_q_heads,
                                                           int64_t num_kv_heads, int64_t head_dim,
                                                           int dtype) {
-  return mlr_paged_prefill_scored_workspace_size(num_seqs, max_query_len, max_blocks, block_size,
-                                                 num_q_heads, num_kv_heads, head_dim, dtype);
+  if (num_seqs <= 0 || max_query_len <= 0 || num_kv_heads <= 0 || num_q_heads <= 0 ||
+      head_dim <= 0 || block_size <= 0)
+    return 0;
+  const PrefillPlan n = plan_prefill(num_seqs, max_query_len, max_blocks * block_size, block_size,
+                                     num_q_heads, num_kv_heads, head_dim, dtype, true);
+  return n.parts ? part_bytes(n.units, n.items, n.rows, head_dim) : 0;
 }
 
 extern "C" int mlr_paged_attention_tree(

@@ -234,72 +234,79 @@ __global__ __launch_bounds__(256) void scored_rows_kernel(ScoredParams p) {
   const int m16 = lane & 15, g = lane >> 4;
 
   // The cut: all keys, hence the split length; this thread's units and the
-  // items before them. -1: a unit without rows.
+  // items before them. -1: a unit without rows. Without splits an item is a unit.
   const int per = (p.units + 255) / 256;
   const int u_lo = min(tid * per, p.units), u_hi = min(u_lo + per, p.units);
   auto len_of = [&](int u) -> int64_t {
     const Unit t = unit_of(p, u, kRows);
     return t.r0 < t.rows ? unit_len(t) : -1;
   };
-  const int64_t len0 = u_lo < u_hi ? len_of(u_lo) : -1;  // mostly there is no other
+  int64_t len0 = -1;  // of the first; mostly there is no other
   auto items_at = [&](int u, int split) {
     const int64_t len = u == u_lo ? len0 : len_of(u);
     return len < 0 ? 0 : items_of(len, split);
   };
-  int64_t keys = max(len0, int64_t(0));
-  for (int u = u_lo + 1; u < u_hi; ++u) keys += max(len_of(u), int64_t(0));
+  int split = 0, own = 0, before = 0, items = p.units;
+  if (!p.whole) {
+    if (u_lo < u_hi) len0 = len_of(u_lo);
+    int64_t keys = max(len0, int64_t(0));
+    for (int u = u_lo + 1; u < u_hi; ++u) keys += max(len_of(u), int64_t(0));
 #pragma unroll
-  for (int o = 32; o > 0; o >>= 1) keys += __shfl_xor(keys, o);
-  if (lane == 0) s_keys[wv] = keys;
-  __syncthreads();
-  const int split = split_of(s_keys[0] + s_keys[1] + s_keys[2] + s_keys[3], p);
-  int own = 0;
-  for (int u = u_lo; u < u_hi; ++u) own += items_at(u, split);
-  int before = own;
+    for (int o = 32; o > 0; o >>= 1) keys += __shfl_xor(keys, o);
+    if (lane == 0) s_keys[wv] = keys;
+    __syncthreads();
+    split = split_of(s_keys[0] + s_keys[1] + s_keys[2] + s_keys[3], p);
+    for (int u = u_lo; u < u_hi; ++u) own += items_at(u, split);
+    before = own;
 #pragma unroll
-  for (int o = 1; o < 64; o <<= 1) {
-    const int x = __shfl_up(before, o);
-    if (lane >= o) before += x;
-  }
-  if (lane == 63) s_count[wv] = before;
-  before -= own;
-  __syncthreads();
-  int items = 0;
-  for (int i = 0; i < kWavesWg; ++i) {
-    if (i < wv) before += s_count[i];
-    items += s_count[i];
-  }
-  if (blockIdx.x == 0 && p.first) {
-    int at = before;
-    for (int u = u_lo; u < u_hi; ++u) {
-      p.first[u] = at;
-      at += items_at(u, split);
+    for (int o = 1; o < 64; o <<= 1) {
+      const int x = __shfl_up(before, o);
+      if (lane >= o) before += x;
     }
-    if (tid == 255) p.first[p.units] = items;
+    if (lane == 63) s_count[wv] = before;
+    before -= own;
+    __syncthreads();
+    items = 0;
+    for (int i = 0; i < kWavesWg; ++i) {
+      if (i < wv) before += s_count[i];
+      items += s_count[i];
+    }
+    if (blockIdx.x == 0 && p.first) {
+      int at = before;
+      for (int u = u_lo; u < u_hi; ++u) {
+        p.first[u] = at;
+        at += items_at(u, split);
+      }
+      if (tid == 255) p.first[p.units] = items;
+    }
   }
 
   const float inv_cap = kCap ? 1.f / p.cap : 0.f;
   for (int w = blockIdx.x; w < items * p.hkv; w += gridDim.x) {
     const int item = w / p.hkv, kvh = w - item * p.hkv;
-    if (item >= before && item < before + own) {
-      int at = before;
-      for (int u = u_lo; u < u_hi; ++u) {
-        const int n = items_at(u, split);
-        if (item < at + n) {
-          s_unit = u;
-          s_split = item - at;
-          s_of = n;
-          break;
+    int unit = item, part = 0, parts = 1;
+    if (!p.whole) {
+      if (item >= before && item < before + own) {
+        int at = before;
+        for (int u = u_lo; u < u_hi; ++u) {
+          const int n = items_at(u, split);
+          if (item < at + n) {
+            s_unit = u;
+            s_split = item - at;
+            s_of = n;
+            break;
+          }
+          at += n;
         }
-        at += n;
       }
+      __syncthreads();
+      unit = __builtin_amdgcn_readfirstlane(s_unit);
+      part = __builtin_amdgcn_readfirstlane(s_split);
+      parts = __builtin_amdgcn_readfirstlane(s_of);
     }
-    __syncthreads();
-    const int unit = __builtin_amdgcn_readfirstlane(s_unit);
-    const int part = __builtin_amdgcn_readfirstlane(s_split);
-    const int parts = __builtin_amdgcn_readfirstlane(s_of);
     const bool alone = parts == 1 && !p.force_partial;
     const Unit t = unit_of(p, unit, kRows);
+    if (t.r0 >= t.rows) continue;  // uniform: without splits, a unit without rows
     const int len = item_len(t, parts, 16);
     // Keys are below 2^31.
     const int64_t from = unit_base(t) + static_cast<int64_t>(part) * len;
@@ -511,12 +518,12 @@ __global__ __launch_bounds__(256) void scored_rows_kernel(ScoredParams p) {
       for (int n = 0; n < kVe; ++n) o[n] += s_acc[i][rr][d0 + n] * f;
     }
     const int orow = t.r0 + rr;
+    const int64_t at = static_cast<int64_t>(w) * kRows + rr;
+    if ((!alone || kKeep) && (tid & 15) == 0) {
+      p.ml[2 * at] = m_all;
+      p.ml[2 * at + 1] = sum;
+    }
     if (!alone) {
-      const int64_t at = static_cast<int64_t>(w) * kRows + rr;
-      if ((tid & 15) == 0) {
-        p.ml[2 * at] = m_all;
-        p.ml[2 * at + 1] = sum;
-      }
 #pragma unroll
       for (int n = 0; n < kVe; ++n) p.acc[at * D + d0 + n] = o[n];
     } else if (orow < t.rows) {

@@ -138,6 +138,7 @@ void scored_tiles_kernel(ScoredParams p) {
   __shared__ __align__(1024) unsigned char vs0[kHalves][kTileB], vs1[kHalves][kTileB];
   __shared__ int64_t s_keys[kThreads / 64];
   __shared__ int s_count[kThreads / 64], s_most[kThreads / 64], s_unit, s_part, s_of, s_all, s_odd;
+  __shared__ float s_time[kTree ? 16 : 1];
   const int tid = threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int w = wave & 3, half = wave >> 2;
@@ -192,6 +193,91 @@ void scored_tiles_kernel(ScoredParams p) {
       s_of = 1;
     }
     item = rank;
+  } else if (kTree) {
+    // The cut. A thread has one sequence, whose units see the same keys. Of some splits,
+    // from the one that would deal all keys evenly on and the longest unit cut in up to
+    // eight, that whose items, in rounds over the CUs, take the shortest time; an item
+    // costs as much as kStart keys more than its own (its planning, q and first tile).
+    constexpr int kStart = 400;
+    int *lens = reinterpret_cast<int *>(&ks0[0][0]), *units = lens + kThreads;
+    static_assert(kTreeSeqs <= kThreads && sizeof(ks0) >= 2 * kThreads * sizeof(int),
+                  "a thread has one sequence");
+    int own_units = 0, own_len = 0;
+    if (tid < p.seqs) {
+      const Unit t = unit_of(p, tid * p.tiles, kTileRows);
+      own_units = min((t.rows + kTileRows - 1) / kTileRows, p.tiles);
+      own_len = own_units > 0 ? static_cast<int>(unit_len(t)) : 0;
+    }
+    lens[tid] = own_len;
+    units[tid] = own_units;
+    int64_t keys = static_cast<int64_t>(own_len) * own_units;
+    int most = own_len;
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) {
+      keys += __shfl_xor(keys, o);
+      most = max(most, __shfl_xor(most, o));
+    }
+    if (lane == 0) {
+      s_keys[wave] = keys;
+      s_most[wave] = most;
+    }
+    if (tid == 0) s_unit = -1;
+    __syncthreads();
+    keys = 0;
+#pragma unroll
+    for (int i = 0; i < kThreads / 64; ++i) {
+      keys += s_keys[i];
+      most = max(most, s_most[i]);
+    }
+    const int slots = D == 64 ? 2 * p.ncu : p.ncu;
+    const float even = static_cast<float>(keys) * p.hkv / slots;
+    auto cut_of = [&](int i) __attribute__((always_inline)) {
+      const float x = i < 8 ? even * (1.f + 0.14f * i) : most / static_cast<float>(i - 7);
+      const float y = fminf(fmaxf(fmaxf(x, even), static_cast<float>(kMinSplit)), 2.0e9f);
+      return (static_cast<int>(y) + 64) & ~63;
+    };
+    for (int i = wave; i < 16; i += kThreads / 64) {
+      const int cut = cut_of(i);
+      int n = 0;
+      for (int q = lane; q < p.seqs; q += 64) n += units[q] * items_of(lens[q], cut);
+#pragma unroll
+      for (int o = 32; o > 0; o >>= 1) n += __shfl_xor(n, o);
+      const float rounds = static_cast<float>((n * p.hkv + slots - 1) / slots);
+      if (lane == 0) s_time[i] = rounds * (min(cut, most) + kStart);
+    }
+    __syncthreads();
+    int best = 0;
+#pragma unroll
+    for (int i = 1; i < 16; ++i) best = s_time[i] < s_time[best] ? i : best;
+    const int own_parts = items_of(own_len, cut_of(best)), own = own_units * own_parts;
+    int before = own;
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) {
+      const int x = __shfl_up(before, o);
+      if (lane >= o) before += x;
+    }
+    if (lane == 63) s_count[wave] = before;
+    before -= own;
+    __syncthreads();
+    int items = 0;
+#pragma unroll
+    for (int i = 0; i < kThreads / 64; ++i) {
+      if (i < wave) before += s_count[i];
+      items += s_count[i];
+    }
+    item = blockIdx.x / p.hkv;
+    kvh = blockIdx.x - static_cast<int>(item) * p.hkv;
+    if (item >= before && item < before + own) {
+      const int at = static_cast<int>(item) - before;
+      s_unit = tid * p.tiles + at / own_parts;
+      s_part = at % own_parts;
+      s_of = own_parts;
+    }
+    if (blockIdx.x == 0 && tid < p.seqs) {
+      for (int k = 0; k < p.tiles; ++k)
+        p.first[tid * p.tiles + k] = before + min(k, own_units) * own_parts;
+      if (tid == 0) p.first[p.units] = items;
+    }
   } else {
     const int per = (p.units + kThreads - 1) / kThreads;
     const int u_lo = min(tid * per, p.units), u_hi = min(u_lo + per, p.units);

@@ -333,11 +333,13 @@ struct Layout {
   size_t total() const { return keys + table + lens + decode; }
 };
 Layout layout_of(int64_t batch, int64_t hq, int64_t hkv, int64_t d, int64_t width,
-                 int64_t block_size, int64_t budget) {
+                 int64_t block_size, int64_t budget, int dtype) {
   const int64_t list = std::min(budget, width);
   return Layout{align256(batch * hkv * whole_fours(width) * sizeof(uint64_t)),
                 align256(batch * hkv * list * sizeof(int64_t)), align256(batch * sizeof(int64_t)),
-                decode_workspace(batch, hq, hkv, d, list * block_size)};
+                short_keys(list * block_size, d, dtype)
+                    ? 0
+                    : decode_workspace(batch, hq, hkv, d, list * block_size)};
 }
 
 }  // namespace
@@ -387,11 +389,11 @@ extern "C" int mlr_update_key_bounds(const void *k_cache, void *key_bounds, int6
 extern "C" size_t mlr_paged_decode_sparse_workspace_size(int64_t batch, int64_t num_q_heads,
                                                          int64_t num_kv_heads, int64_t head_dim,
                                                          int64_t max_blocks, int64_t block_size,
-                                                         int64_t budget) {
+                                                         int64_t budget, int dtype) {
   if (batch <= 0 || num_kv_heads <= 0 || num_q_heads <= 0 || max_blocks <= 0 || block_size <= 0 ||
       budget <= 0)
     return 0;
-  return layout_of(batch, num_q_heads, num_kv_heads, head_dim, max_blocks, block_size, budget)
+  return layout_of(batch, num_q_heads, num_kv_heads, head_dim, max_blocks, block_size, budget, dtype)
       .total();
 }
 
@@ -422,7 +424,7 @@ extern "C" int mlr_paged_decode_sparse(
   MLR_REQUIRE(ceil_div(max_blocks, 64) * num_kv_heads * batch < (int64_t(1) << 31),
               "%s: too many blocks", o.what);
   const size_t need = mlr_paged_decode_sparse_workspace_size(
-      batch, num_q_heads, num_kv_heads, head_dim, max_blocks, block_size, budget);
+      batch, num_q_heads, num_kv_heads, head_dim, max_blocks, block_size, budget, dtype);
   MLR_REQUIRE(need == 0 || (workspace && workspace_bytes >= need),
               "%s: workspace of %zu bytes, %zu needed", o.what, workspace_bytes, need);
   hipStream_t s = static_cast<hipStream_t>(stream);
@@ -435,7 +437,7 @@ extern "C" int mlr_paged_decode_sparse(
   int64_t max_keys = 0;
   if (need) {
     const Layout l = layout_of(batch, num_q_heads, num_kv_heads, head_dim, max_blocks, block_size,
-                               budget);
+                               budget, dtype);
     x.keys = reinterpret_cast<uint64_t *>(ws);
     x.table = reinterpret_cast<int64_t *>(ws += l.keys);
     x.lens = reinterpret_cast<int64_t *>(ws += l.table);
@@ -461,7 +463,8 @@ extern "C" int mlr_paged_decode_sparse(
   }
   ScoredParams p = params_of(o, kModeDecode);
   p.bt_sh = need ? list : 0;
-  const bool parts = max_keys > kMinSplit;
+  p.whole = short_keys(max_keys, head_dim, dtype);
+  const bool parts = !p.whole;
   const int64_t items = plan_decode(p, max_keys, parts ? ws : nullptr);
   if (const int rc = launch_scored_rows(p, dtype, grid_of(items), s)) return rc;
   return parts ? merge_decode(p, dtype, s) : MLR_OK;

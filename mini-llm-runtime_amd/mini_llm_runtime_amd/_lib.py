@@ -180,7 +180,7 @@ _PROTOTYPES = {
         [_c_ptr, _c_ptr, _c_i64, _c_i64, _c_i64, _c_i64, _c_ptr, _c_i64, _c_i64, _c_ptr, _c_ptr,
          _c_i64, _c_i64, _c_int, _c_ptr],
     ),
-    "mlr_paged_decode_sparse_workspace_size": (_c_size, [_c_i64] * 7),
+    "mlr_paged_decode_sparse_workspace_size": (_c_size, [_c_i64] * 7 + [_c_int]),
     "mlr_paged_decode_sparse": (
         _c_int,
         [_c_ptr, _c_i64, _c_i64, _c_ptr, _c_ptr, _c_ptr, _c_i64, _c_i64, _c_i64, _c_i64, _c_ptr,

@@ -150,10 +150,11 @@ def paged_attention_decode_sparse(
             _validate_tables(block_tables, seq_lens, block_size, num_blocks)
         q = _aligned_q(q)
         width = block_tables.shape[1]
+        dcode = _lib.DTYPE_CODES[q.dtype]
         lib = _lib.load()
         with _lib.on(device):
             nbytes = lib.mlr_paged_decode_sparse_workspace_size(
-                batch, num_q_heads, num_kv_heads, head_dim, width, block_size, budget)
+                batch, num_q_heads, num_kv_heads, head_dim, width, block_size, budget, dcode)
             ws = _workspace(nbytes, device)
             status = lib.mlr_paged_decode_sparse(
                 q.data_ptr(), q.stride(0), q.stride(1), k_cache.data_ptr(), v_cache.data_ptr(),
@@ -161,7 +162,7 @@ def paged_attention_decode_sparse(
                 block_tables.data_ptr(), block_tables.stride(0), width, seq_lens.data_ptr(),
                 batch, num_q_heads, budget, sinks, recent,
                 head_dim ** -0.5 if scale is None else scale, softcap,
-                _lib.DTYPE_CODES[q.dtype], None if blocks is None else blocks.data_ptr(),
+                dcode, None if blocks is None else blocks.data_ptr(),
                 None if ws is None else ws.data_ptr(), nbytes, out.data_ptr(), out.stride(0),
                 out.stride(1), _lib.stream_handle(device))
         _lib.check(status, "mlr_paged_decode_sparse")
