@@ -266,7 +266,7 @@ __global__ __launch_bounds__(kThreads) void choose_keys(CacheParams c, const int
           }
         }
       },
-      [&](int r, int i) __attribute__((always_inline)) { list[r] = i; });
+      [&](int r, int i, int) __attribute__((always_inline)) { list[r] = i; });
   for (int i = chosen + threadIdx.x; i < budget; i += kThreads) list[i] = -1;
   if (kvh == 0 && threadIdx.x == 0) lens[seq] = chosen;
 }

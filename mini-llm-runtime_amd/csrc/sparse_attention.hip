@@ -110,7 +110,9 @@ struct SparseParams {
   int64_t seqs;
   bool flip;  // a negative scale: the largest score is that of -q
   int sinks, recent, budget, list;  // list: columns of `table`, min(budget, bt_width)
-  uint64_t *keys;                   // [seqs, hkv, keys_st] scores as ordered keys
+  uint64_t *keys;                   // [seqs, hkv, keys_st] scores as ordered keys, or in
+                                    // 32 bits with their errors
+  uint64_t *exact;                  // as many, for choose_rough
   int64_t keys_st;                  // bt_width, in whole fours
   int64_t *table;                   // [seqs, hkv, list] physical blocks of the chosen
   int64_t *lens;                    // [seqs] keys of the chosen blocks
@@ -118,6 +120,9 @@ struct SparseParams {
 };
 
 typedef double f64x4_t __attribute__((ext_vector_type(4)));
+typedef float f32x4_t __attribute__((ext_vector_type(4)));
+typedef __bf16 bf16x8_t __attribute__((ext_vector_type(8)));
+typedef _Float16 f16x8_t __attribute__((ext_vector_type(8)));
 
 // Whether a 32-bit word of a row holds an infinity or NaN.
 template <typename T>
@@ -132,96 +137,85 @@ __device__ __forceinline__ bool odd(uint4 w) {
   return odd<T>(w.x) || odd<T>(w.y) || odd<T>(w.z) || odd<T>(w.w);
 }
 
-// Scores on v_mfma_f64_16x16x4: sum_d max(q low, q high) = [q-, q+].[low, high] with q- =
-// min(q, 0) and q+ = max(q, 0), 16 heads times 16 blocks. Operand A is q (lane l: head
-// l % 16), B the bounds (lane l: block l % 16); of a row lane group l / 16 has every
-// fourth piece of 16 bytes, so that its k-th elements are those of A and B alike. A
-// group of fewer heads repeats its last one, and the maximum over heads needs no mask.
-// Where a bound or q is not finite, 0 times it would be NaN where the larger of both
-// products is not: such tiles are added up product by product.
-//
-// Bound by the matrix unit where the heads of a group are many, by the reads of the bounds
-// where they are few: 8 requests of 2,048 blocks, 28/4 heads of 128, bf16, 33 MB in 26 us.
+// One request and KV head. Of a row, lane group l / 16 has every fourth piece of 16 bytes,
+// so that its k-th elements are those of a head (lane l: head l % 16) and of a block
+// (block l % 16) alike.
 template <typename T, int kT>
-__global__ __launch_bounds__(256) void score_blocks(SparseParams p, int tiles) {
-  constexpr int kE = 16 / sizeof(T);
-  const int tid = threadIdx.x, lane = tid & 63;
-  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const int col = lane & 15, g = lane >> 4;
-  const int64_t b = blockIdx.x;
-  const int64_t seq = b % p.seqs, kvh = b / p.seqs % p.hkv;
-  // A wave's tiles of 16 blocks: the workgroup's in turn.
-  const int64_t first = (b / p.seqs / p.hkv * 4 * tiles + wave) * 16;
-  const int64_t ctx = clamp64(p.ctx[seq], 0, p.bt_width * p.block_size);
-  const int64_t n = (ctx + p.block_size - 1) / p.block_size;
-  if (first >= n || n <= p.budget) return;  // nothing there, or nothing to choose
-  const int64_t *table = p.bt + seq * p.bt_st;
-  const T *bounds = static_cast<const T *>(p.bounds) + kvh * p.d;
-  const int64_t row = p.hkv * p.d;
-  const T *q = static_cast<const T *>(p.q) + seq * p.q_st + kvh * p.group * p.q_sh;
-  auto id_of = [&](int i) __attribute__((always_inline)) {
-    return table[min(first + 64 * i + col, n - 1)];
-  };
-  struct Tile {
-    uint4 low[kT], high[kT];
-    bool there;
-  };
-  auto read = [&](Tile &x, int i, int64_t id) __attribute__((always_inline)) {
-    x.there = first + 64 * i + col < n && id >= 0 && id < p.num_blocks;
-    const T *at = bounds + (x.there ? id : 0) * 2 * row;
+struct Pair {
+  static constexpr int kE = 16 / sizeof(T);
+  int64_t seq, kvh, n;  // n: blocks of the request
+  const int64_t *table;
+  const T *q, *bounds;
+  int64_t q_sh, row, d, num_blocks;
+  int heads, col, g;
+  bool flip;
+
+  __device__ __forceinline__ Pair(const SparseParams &p, int64_t pair_seq, int64_t pair_kvh)
+      : seq(pair_seq), kvh(pair_kvh), q_sh(p.q_sh), row(p.hkv * p.d), d(p.d),
+        num_blocks(p.num_blocks), heads(static_cast<int>(p.group)), col(threadIdx.x & 15),
+        g((threadIdx.x & 63) >> 4), flip(p.flip) {
+    const int64_t ctx = clamp64(p.ctx[seq], 0, p.bt_width * p.block_size);
+    n = (ctx + p.block_size - 1) / p.block_size;
+    table = p.bt + seq * p.bt_st;
+    q = static_cast<const T *>(p.q) + seq * p.q_st + kvh * p.group * p.q_sh;
+    bounds = static_cast<const T *>(p.bounds) + kvh * d;
+  }
+  // The lane's pieces of a block's bounds, zeros where there is none.
+  __device__ __forceinline__ bool read(uint4 (&low)[kT], uint4 (&high)[kT], int64_t id) const {
+    const bool there = id >= 0 && id < num_blocks;
+    const T *at = bounds + (there ? id : 0) * 2 * row;
 #pragma unroll
     for (int t = 0; t < kT; ++t) {
       const int e = (g + 4 * t) * kE;
-      x.low[t] = x.high[t] = make_uint4(0, 0, 0, 0);
-      if (e < p.d && x.there) {
-        x.low[t] = *reinterpret_cast<const uint4 *>(at + e);
-        x.high[t] = *reinterpret_cast<const uint4 *>(at + row + e);
+      low[t] = high[t] = make_uint4(0, 0, 0, 0);
+      if (e < d && there) {
+        low[t] = *reinterpret_cast<const uint4 *>(at + e);
+        high[t] = *reinterpret_cast<const uint4 *>(at + row + e);
       }
     }
-  };
-  const int heads = static_cast<int>(p.group);
-  const bool many = heads > 16;
-  // q of heads h0 ..: its negative and its positive part, in 64 bits.
-  double below[kT][kE], above[kT][kE];
-  bool q_odd = false;
-  auto read_q = [&](int h0) __attribute__((always_inline)) {
-    const T *mine = q + min(h0 + col, heads - 1) * p.q_sh;
-    q_odd = false;
+    return there;
+  }
+  // And of head h0 + l % 16; a group of fewer heads repeats its last one, so that a
+  // maximum over heads needs no mask.
+  __device__ __forceinline__ void read_q(uint4 (&x)[kT], int h0) const {
+    const T *mine = q + min(h0 + col, heads - 1) * q_sh;
 #pragma unroll
     for (int t = 0; t < kT; ++t) {
-      const int e0 = (g + 4 * t) * kE;
-      uint4 x = make_uint4(0, 0, 0, 0);
-      if (e0 < p.d) x = *reinterpret_cast<const uint4 *>(mine + e0);
-      q_odd = q_odd || odd<T>(x);
-      float f[kE];
-      unpack<T>(x, f);
-#pragma unroll
-      for (int e = 0; e < kE; ++e) {
-        const float v = p.flip ? -f[e] : f[e];
-        below[t][e] = fminf(v, 0.f);
-        above[t][e] = fmaxf(v, 0.f);
-      }
+      const int e = (g + 4 * t) * kE;
+      x[t] = make_uint4(0, 0, 0, 0);
+      if (e < d) x[t] = *reinterpret_cast<const uint4 *>(mine + e);
     }
-  };
-  auto score = [&](const Tile &x, int i) __attribute__((always_inline)) {
-    bool bound_odd = false;
-#pragma unroll
-    for (int t = 0; t < kT; ++t)
-      bound_odd = bound_odd || odd<T>(x.low[t]) || odd<T>(x.high[t]);
+  }
+
+  // The scores of a wave's 16 blocks, block l % 16's in lane l, in 64 bits on
+  // v_mfma_f64_16x16x4: sum_d max(q low, q high) = [q-, q+].[low, high] with q- = min(q, 0)
+  // and q+ = max(q, 0), heads as operand A, blocks as operand B. Where a bound or q is not
+  // finite, 0 times it would be NaN where the larger of both products is not: such tiles
+  // are added up product by product, and a sum that is NaN does not count.
+  __device__ __forceinline__ double score(int64_t id) const {
+    uint4 low[kT], high[kT];
+    const bool there = read(low, high, id);
     double best = -INFINITY;
     for (int h0 = 0; h0 < heads; h0 += 16) {
-      if (many) read_q(h0);
-      if (__builtin_expect(!__any(bound_odd || q_odd), 1)) {
+      uint4 x[kT];
+      read_q(x, h0);
+      bool strange = false;
+#pragma unroll
+      for (int t = 0; t < kT; ++t)
+        strange = strange || odd<T>(x[t]) || odd<T>(low[t]) || odd<T>(high[t]);
+      if (__builtin_expect(!__any(strange), 1)) {
         f64x4_t sum0 = {0., 0., 0., 0.}, sum1 = {0., 0., 0., 0.};
 #pragma unroll
         for (int t = 0; t < kT; ++t) {
-          float l[kE], u[kE];
-          unpack<T>(x.low[t], l);
-          unpack<T>(x.high[t], u);
+          float f[kE], l[kE], u[kE];
+          unpack<T>(x[t], f);
+          unpack<T>(low[t], l);
+          unpack<T>(high[t], u);
 #pragma unroll
           for (int e = 0; e < kE; ++e) {
-            sum0 = __builtin_amdgcn_mfma_f64_16x16x4f64(below[t][e], l[e], sum0, 0, 0, 0);
-            sum1 = __builtin_amdgcn_mfma_f64_16x16x4f64(above[t][e], u[e], sum1, 0, 0, 0);
+            const float v = flip ? -f[e] : f[e];
+            sum0 = __builtin_amdgcn_mfma_f64_16x16x4f64(fminf(v, 0.f), l[e], sum0, 0, 0, 0);
+            sum1 = __builtin_amdgcn_mfma_f64_16x16x4f64(fmaxf(v, 0.f), u[e], sum1, 0, 0, 0);
           }
         }
 #pragma unroll
@@ -232,110 +226,452 @@ __global__ __launch_bounds__(256) void score_blocks(SparseParams p, int tiles) {
 #pragma unroll
           for (int t = 0; t < kT; ++t) {
             float l[kE], u[kE];
-            unpack<T>(x.low[t], l);
-            unpack<T>(x.high[t], u);
+            unpack<T>(low[t], l);
+            unpack<T>(high[t], u);
 #pragma unroll
             for (int e = 0; e < kE; ++e) {
               const int at = (g + 4 * t) * kE + e;
-              if (at >= p.d) continue;
-              const float f = Elem<T>::to_f32(q[h * p.q_sh + at]);
-              const double v = p.flip ? -f : f;
+              if (at >= d) continue;
+              const float f = Elem<T>::to_f32(q[h * q_sh + at]);
+              const double v = flip ? -f : f;
               sum = fma(v, v >= 0. ? u[e] : l[e], sum);
             }
           }
           sum += __shfl_xor(sum, 16);
           sum += __shfl_xor(sum, 32);
-          best = sum > best ? sum : best;  // a sum that is NaN does not count
+          best = sum > best ? sum : best;
         }
       }
     }
     best = fmax(best, __shfl_xor(best, 16));
     best = fmax(best, __shfl_xor(best, 32));
-    const int64_t j = first + 64 * i + col;
-    if (g == 0 && j < n)
-      p.keys[(seq * p.hkv + kvh) * p.keys_st + j] = order_key(x.there ? best : -INFINITY);
+    return there ? best : -INFINITY;
+  }
+};
+
+// Scores in 64 bits of all blocks (FP32, and past kRoughBlocks), a wave for 16.
+template <typename T, int kT>
+__global__ __launch_bounds__(256) void score_blocks(SparseParams p) {
+  const int64_t b = blockIdx.x;
+  const Pair<T, kT> x(p, b % p.seqs, b / p.seqs % p.hkv);
+  const int64_t first = (b / p.seqs / p.hkv * 4 + (threadIdx.x >> 6)) * 16;
+  if (first >= x.n || x.n <= p.budget) return;  // nothing there, or nothing to choose
+  const int64_t j = first + x.col;
+  const double best = x.score(j < x.n ? x.table[j] : -1);
+  if (x.g == 0 && j < x.n)
+    p.keys[(x.seq * p.hkv + x.kvh) * p.keys_st + j] = order_key(best);
+}
+
+// For the 16-bit types, scores in 32 bits on the matrix instructions of the type, with how
+// far at most they are from those in 64: what that leaves undecided, a few blocks around the
+// last chosen one, is scored in 64 bits by choose_rough.
+//   |error| <= (2 d + 8) 2^-22 (sum_d |q_d|) (max_d |bound_d|)
+// for 2 d products, exact in 32 bits, added in any order with a relative error of 2^-22 each
+// (four times that of rounding to nearest), and 1e-30 of each factor for operands that
+// the matrix unit may take for 0. Not finite: no bound.
+// Bound by reading the bounds: 8 requests of 2,048 blocks, 4 KV heads of 128: 33 MB in
+// MEASURED us, where 64 bits throughout took 26 us.
+template <typename T> struct Rough;
+template <> struct Rough<bf16_t> {
+  __device__ static f32x4_t mfma(uint4 a, uint4 b, f32x4_t c) {
+    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8_t, a),
+                                                   __builtin_bit_cast(bf16x8_t, b), c, 0, 0, 0);
+  }
+};
+template <> struct Rough<f16_t> {
+  __device__ static f32x4_t mfma(uint4 a, uint4 b, f32x4_t c) {
+    return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8_t, a),
+                                                  __builtin_bit_cast(f16x8_t, b), c, 0, 0, 0);
+  }
+};
+
+template <typename T, int kT>
+__global__ __launch_bounds__(256) void score_rough(SparseParams p, int tiles) {
+  constexpr int kE = 8;
+  const int64_t b = blockIdx.x;
+  const Pair<T, kT> x(p, b % p.seqs, b / p.seqs % p.hkv);
+  // A wave's tiles of 16 blocks: the workgroup's in turn.
+  const int64_t first = (b / p.seqs / p.hkv * 4 * tiles + (threadIdx.x >> 6)) * 16;
+  if (first >= x.n || x.n <= p.budget) return;
+  auto id_of = [&](int i) __attribute__((always_inline)) {
+    const int64_t j = first + 64 * i + x.col;
+    const int64_t id = x.table[min(j, x.n - 1)];
+    return j < x.n ? id : int64_t(-1);
   };
-  Tile even, other;
-  const int count = static_cast<int>(min(int64_t(tiles), (n - first + 63) / 64));
-  read(even, 0, id_of(0));
+  auto sizes = [&](const uint4 (&w)[kT], bool add, float &v) __attribute__((always_inline)) {
+#pragma unroll
+    for (int t = 0; t < kT; ++t) {
+      float f[kE];
+      unpack<T>(w[t], f);
+#pragma unroll
+      for (int e = 0; e < kE; ++e) v = add ? v + fabsf(f[e]) : fmaxf(v, fabsf(f[e]));
+    }
+  };
+  // Halves of w whose sign is set, or is not; -0 makes no difference.
+  auto part = [&](uint4 w, bool negative) __attribute__((always_inline)) {
+    auto one = [&](uint32_t v) __attribute__((always_inline)) {
+      const uint32_t minus = (v >> 15 & 0x00010001u) * 0xffffu;
+      return negative ? v & minus : v & ~minus;
+    };
+    return make_uint4(one(w.x), one(w.y), one(w.z), one(w.w));
+  };
+  uint4 qw[kT];
+  float q_size = 0.f;  // the largest sum of |q| of a head
+  bool q_odd = false;
+  auto read_q = [&](int h0) __attribute__((always_inline)) {
+    x.read_q(qw, h0);
+    const uint32_t turn = x.flip ? 0x80008000u : 0u;
+#pragma unroll
+    for (int t = 0; t < kT; ++t) {
+      q_odd = q_odd || odd<T>(qw[t]);
+      qw[t] = make_uint4(qw[t].x ^ turn, qw[t].y ^ turn, qw[t].z ^ turn, qw[t].w ^ turn);
+    }
+    float sum = 0.f;
+    sizes(qw, true, sum);
+    sum += __shfl_xor(sum, 16);
+    q_size = fmaxf(q_size, sum + __shfl_xor(sum, 32));
+  };
+  uint4 low[2][kT], high[2][kT];
+  bool there[2];
+  auto score = [&](const uint4 (&l)[kT], const uint4 (&u)[kT], bool exists, int i)
+      __attribute__((always_inline)) {
+    float best = -INFINITY;
+    for (int h0 = 0; h0 < x.heads; h0 += 16) {
+      if (x.heads > 16) read_q(h0);
+      f32x4_t sum = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int t = 0; t < kT; ++t) {
+        sum = Rough<T>::mfma(part(qw[t], true), l[t], sum);
+        sum = Rough<T>::mfma(part(qw[t], false), u[t], sum);
+      }
+#pragma unroll
+      for (int r = 0; r < 4; ++r) best = __builtin_elementwise_maximum(best, sum[r]);  // NaN stays
+    }
+    best = __builtin_elementwise_maximum(best, __shfl_xor(best, 16));
+    best = __builtin_elementwise_maximum(best, __shfl_xor(best, 32));
+    float size = 0.f, most = q_size;
+    bool strange = q_odd;
+    sizes(l, false, size);
+    sizes(u, false, size);
+#pragma unroll
+    for (int t = 0; t < kT; ++t) strange = strange || odd<T>(l[t]) || odd<T>(u[t]);
+    size = fmaxf(size, __shfl_xor(size, 16));
+    size = fmaxf(size, __shfl_xor(size, 32));
+#pragma unroll
+    for (int o = 1; o < 16; o <<= 1) most = fmaxf(most, __shfl_xor(most, o));
+    strange = __any(strange);  // of the whole tile, for q is everyone's
+    const float d = static_cast<float>(x.d);
+    float off = (2.f * d + 8.f) * 0x1p-22f * most * size + 1e-30f * (most + d * size + d);
+    if (strange || !(fabsf(best) < 1e37f) || !(off < 1e37f)) {
+      best = 0.f;
+      off = INFINITY;
+    }
+    const int64_t j = first + 64 * i + x.col;
+    if (x.g == 0 && j < x.n)
+      reinterpret_cast<float2 *>(p.keys)[(x.seq * p.hkv + x.kvh) * p.keys_st + j] =
+          exists ? make_float2(best, off) : make_float2(-INFINITY, 0.f);
+  };
+  const int count = static_cast<int>(min(int64_t(tiles), (x.n - first + 63) / 64));
+  there[0] = x.read(low[0], high[0], id_of(0));
   int64_t id = id_of(1);
-  if (!many) read_q(0);
+  if (x.heads <= 16) read_q(0);
   for (int i = 0; i < count; i += 2) {
-    if (i + 1 < count) read(other, i + 1, id);
+    if (i + 1 < count) there[1] = x.read(low[1], high[1], id);
     id = id_of(i + 2);
-    score(even, i);
+    score(low[0], high[0], there[0], i);
     if (i + 1 >= count) break;
-    if (i + 2 < count) read(even, i + 2, id);
+    if (i + 2 < count) there[0] = x.read(low[0], high[0], id);
     id = id_of(i + 3);
-    score(other, i + 1);
+    score(low[1], high[1], there[1], i + 1);
   }
 }
 
-// A workgroup chooses the blocks of one request and KV head.
+// Where the chosen of a request and KV head go: a block table of their own, and their places.
+struct Chosen {
+  const int64_t *row;
+  int64_t *table, *chosen;
+  __device__ __forceinline__ Chosen(const SparseParams &p, int64_t seq, int64_t kvh)
+      : row(p.bt + seq * p.bt_st), table(p.table + (seq * p.hkv + kvh) * p.list),
+        chosen(p.chosen ? p.chosen + (seq * p.hkv + kvh) * p.budget : nullptr) {}
+  __device__ __forceinline__ void put(int r, int i, int64_t id) const {
+    table[r] = id;
+    if (chosen) chosen[r] = i;
+  }
+  __device__ __forceinline__ void operator()(int r, int i, int) const { put(r, i, row[i]); }
+  // The last block is always chosen, and the only one that may not be full.
+  __device__ __forceinline__ void finish(const SparseParams &p, int64_t seq, int64_t kvh,
+                                         int count, int threads) const {
+    if (chosen)
+      for (int i = count + threadIdx.x; i < p.budget; i += threads) chosen[i] = -1;
+    if (p.lens && kvh == 0 && threadIdx.x == 0) {
+      const int64_t ctx = clamp64(p.ctx[seq], 0, p.bt_width * p.block_size);
+      const int64_t n = (ctx + p.block_size - 1) / p.block_size;
+      p.lens[seq] = count > 0 ? ctx - (n - count) * p.block_size : 0;
+    }
+  }
+};
+
+__device__ __forceinline__ int blocks_of(const SparseParams &p, int64_t seq) {
+  const int64_t ctx = clamp64(p.ctx[seq], 0, p.bt_width * p.block_size);
+  return static_cast<int>((ctx + p.block_size - 1) / p.block_size);
+}
+
+// Loads four neighbouring keys of 64 bits at a time.
+__device__ __forceinline__ auto keys_from(const uint64_t *keys, int n) {
+  return [keys, n](auto &held, auto place) __attribute__((always_inline)) {
+    constexpr int kMany = sizeof(held) / sizeof(held[0]);
+#pragma unroll
+    for (int j = 0; j < kMany; ++j) {
+      const ulonglong2 *at = reinterpret_cast<const ulonglong2 *>(keys + (min(place(j), n - 1) & ~3));
+      const ulonglong2 a = at[0], b = at[1];
+      held[j][0] = a.x;
+      held[j][1] = a.y;
+      held[j][2] = b.x;
+      held[j][3] = b.y;
+    }
+  };
+}
+
+// A workgroup chooses the blocks of one request and KV head, from keys in the workspace.
 template <int kThreads, int kHeld>
 __global__ __launch_bounds__(kThreads) void choose_blocks(SparseParams p) {
   __shared__ SelectShared s;
   const int64_t seq = blockIdx.x % p.seqs, kvh = blockIdx.x / p.seqs;
-  const int64_t pair = seq * p.hkv + kvh;
-  const int64_t ctx = clamp64(p.ctx[seq], 0, p.bt_width * p.block_size);
-  const int n = static_cast<int>((ctx + p.block_size - 1) / p.block_size);
-  const uint64_t *keys = p.keys + pair * p.keys_st;
-  const int64_t *row = p.bt + seq * p.bt_st;
-  int64_t *table = p.table + pair * p.list;
-  int64_t *chosen = p.chosen ? p.chosen + pair * p.budget : nullptr;
+  const int n = blocks_of(p, seq);
+  const Chosen out(p, seq, kvh);
   const int count = select_places<uint64_t, kThreads, kHeld>(
       s, n, p.sinks, p.recent, p.budget,
-      [&](auto &held, auto place) __attribute__((always_inline)) {
-        constexpr int kMany = sizeof(held) / sizeof(held[0]);
+      keys_from(p.keys + (seq * p.hkv + kvh) * p.keys_st, n), out);
+  out.finish(p, seq, kvh, count, kThreads);
+}
+
+// The same for tables of few blocks, with their scores: one launch. Eight waves with up to
+// two tiles each; past that the scores of one request keep one CU too long.
+constexpr int kSmall = 256, kSmallThreads = 512;
+template <typename T, int kT>
+__global__ __launch_bounds__(kSmallThreads) void choose_small(SparseParams p) {
+  __shared__ SelectShared s;
+  __shared__ __align__(16) uint64_t s_keys[kSmall];
+  const Pair<T, kT> x(p, blockIdx.x % p.seqs, blockIdx.x / p.seqs);
+  const int n = static_cast<int>(x.n);
+  const Chosen out(p, x.seq, x.kvh);
+  if (n > p.budget) {  // uniform
+    for (int at = 16 * static_cast<int>(threadIdx.x >> 6); at < n; at += kSmallThreads / 4) {
+      const int j = at + x.col;
+      const double best = x.score(j < n ? x.table[j] : -1);
+      if (x.g == 0) s_keys[j] = order_key(best);
+    }
+    __syncthreads();
+  }
+  const int count = select_places<uint64_t, kSmallThreads, 1>(
+      s, n, p.sinks, p.recent, p.budget, keys_from(s_keys, n), out);
+  out.finish(p, x.seq, x.kvh, count, kSmallThreads);
+}
+
+// The choice from scores in 32 bits and how far off they may be. With T the last chosen of
+// them and R the largest error, a block below T - 2 R is worse than all down to T, and one
+// above T + 2 R is better than all from T on; those in between are scored in 64 bits. Where
+// they are more than kFew, all blocks are. Bound by latency, a dozen steps of 1 us: what a
+// later step needs of memory (block ids, q) is read with the scores.
+constexpr int kRoughThreads = 512, kRoughHeld = 2;
+constexpr int kRoughBlocks = 4 * kRoughThreads * kRoughHeld;  // at most
+template <typename T, int kT>
+__global__ __launch_bounds__(kRoughThreads) void choose_rough(SparseParams p) {
+  constexpr int kWaves = kRoughThreads / 64;
+  __shared__ SelectShared s;
+  __shared__ float s_off[kWaves];
+  __shared__ int64_t s_id[kFew];
+  __shared__ int s_sure[kWaves], s_open[kWaves], s_taken[kFew];
+  const Pair<T, kT> x(p, blockIdx.x % p.seqs, blockIdx.x / p.seqs);
+  const int n = static_cast<int>(x.n), lane = threadIdx.x & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const Chosen out(p, x.seq, x.kvh);
+  const int left = p.budget - p.sinks - p.recent;
+  if (n <= p.budget || left == 0) {  // uniform
+    const int count = min(n, p.budget);
+    for (int i = threadIdx.x; i < count; i += kRoughThreads)
+      out(i, n <= p.budget || i < p.sinks ? i : n - p.budget + i, -1);
+    out.finish(p, x.seq, x.kvh, count, kRoughThreads);
+    return;
+  }
+  const int lo = p.sinks, hi = n - p.recent;
+  const int64_t pair = x.seq * p.hkv + x.kvh;
+  const float2 *rough = reinterpret_cast<const float2 *>(p.keys) + pair * p.keys_st;
+  float off = 0.f;
+  int64_t ids[4 * kRoughHeld];
+  auto load = [&](auto &held, auto place) __attribute__((always_inline)) {
+    constexpr int kMany = sizeof(held) / sizeof(held[0]);
+    float4 a[kMany], b[kMany];
 #pragma unroll
-        for (int j = 0; j < kMany; ++j) {
-          const ulonglong2 *at =
-              reinterpret_cast<const ulonglong2 *>(keys + (min(place(j), n - 1) & ~3));
-          const ulonglong2 a = at[0], b = at[1];
-          held[j][0] = a.x;
-          held[j][1] = a.y;
-          held[j][2] = b.x;
-          held[j][3] = b.y;
+    for (int j = 0; j < kMany; ++j) {
+      const int at = min(place(j), n - 1) & ~3;
+      a[j] = *reinterpret_cast<const float4 *>(rough + at);
+      b[j] = *reinterpret_cast<const float4 *>(rough + at + 2);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) ids[4 * j + e] = x.table[min(at + e, n - 1)];
+    }
+#pragma unroll
+    for (int j = 0; j < kMany; ++j) {
+      const int at = min(place(j), n - 1) & ~3;
+      const float v[4] = {a[j].x, a[j].z, b[j].x, b[j].z};
+      const float r[4] = {a[j].y, a[j].w, b[j].y, b[j].w};
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        held[j][e] = order_key(v[e]);
+        if (at + e >= lo && at + e < hi) off = fmaxf(off, r[e]);
+      }
+    }
+  };
+  Places<uint32_t, kRoughThreads, kRoughHeld, decltype(load)> places(n, lo, hi, load);
+  off = wave_max(off);
+  if (lane == 0) s_off[wave] = off;
+  uint32_t last_key = 0;
+  int last_place = 0;
+  find_last<uint32_t, kRoughThreads>(s, places, left, last_key, last_place);
+#pragma unroll
+  for (int w = 0; w < kWaves; ++w) off = fmaxf(off, s_off[w]);
+  // That key may be below the last chosen one's, with none between: the window is as well
+  // around any score from there on.
+  const float last = __uint_as_float(last_key >> 31 ? last_key & 0x7fffffffu : ~last_key);
+  const float reach = 2.02f * off + 4e-7f * fabsf(last);
+  const bool bound = off < INFINITY;
+  const uint32_t from = bound ? order_key(last - reach) : 1u;
+  // Room for kFew numbers in between.
+  const uint32_t to = bound ? max(order_key(last + reach), from + kFew) : ~0u;
+  int sure = 0, open = 0;
+  places.each([&](int, const uint32_t(&k)[4]) __attribute__((always_inline)) {
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      sure += __popcll(__ballot(k[e] > to));
+      open += __popcll(__ballot(k[e] >= from && k[e] <= to));
+    }
+  });
+  if (lane == 0) {
+    s_sure[wave] = sure;
+    s_open[wave] = open;
+  }
+  if (threadIdx.x == 0) s.count = 0;
+  __syncthreads();
+  sure = open = 0;
+#pragma unroll
+  for (int w = 0; w < kWaves; ++w) {
+    sure += s_sure[w];
+    open += s_open[w];
+  }
+  const int need = left - sure;
+  if (open > kFew) {  // uniform
+    uint64_t *keys = p.exact + pair * p.keys_st;
+    for (int at = 16 * wave; at < n; at += 16 * kWaves) {
+      const int j = at + x.col;
+      const double best = x.score(j < n ? x.table[j] : -1);
+      if (x.g == 0 && j < n) keys[j] = order_key(best);
+    }
+    __threadfence_block();
+    __syncthreads();
+    const int count = select_places<uint64_t, kRoughThreads, 1>(s, n, p.sinks, p.recent, p.budget,
+                                                                keys_from(keys, n), out);
+    out.finish(p, x.seq, x.kvh, count, kRoughThreads);
+    return;
+  }
+  const bool few = open > need;
+  if (few) {
+    // The open ones in a list; a key of theirs becomes from + its place in it.
+#pragma unroll
+    for (int j = 0; j < kRoughHeld; ++j)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const int i = places.first + 256 * j + e;
+        uint32_t &k = places.keys[j][e];
+        if (j < places.steps && k >= from && k <= to) {
+          const int at = atomicAdd(&s.count, 1);
+          s.few_place[at] = i;
+          s_id[at] = ids[4 * j + e];
+          k = from + at;
         }
+      }
+    __syncthreads();
+    if (16 * wave < open) {
+      const int at = 16 * wave + x.col;
+      const double best = x.score(at < open ? s_id[min(at, open - 1)] : -1);
+      if (x.g == 0 && at < open) s.few_key[at] = order_key(best);
+    }
+    __syncthreads();
+    if (wave == 0) {
+      const int at = min(lane, open - 1);
+      const int better = rank_few(s.few_key[at], s.few_place[at], open);
+      if (lane < open) s_taken[lane] = better < need;
+    }
+    __syncthreads();
+  }
+  emit_places<uint32_t, kRoughThreads, kRoughHeld>(
+      s, places,
+      [&](int i, uint32_t k) __attribute__((always_inline)) {
+        if (k > to || places.forced(i)) return true;
+        return k >= from && (!few || s_taken[k - from] != 0);
       },
-      [&](int r, int i) __attribute__((always_inline)) {
-        table[r] = row[i];
-        if (chosen) chosen[r] = i;
-      });
-  if (chosen)
-    for (int i = count + threadIdx.x; i < p.budget; i += kThreads) chosen[i] = -1;
-  // The last block is always chosen, and the only one that may not be full.
-  if (p.lens && kvh == 0 && threadIdx.x == 0)
-    p.lens[seq] = count > 0 ? ctx - static_cast<int64_t>(n - count) * p.block_size : 0;
+      [&](int r, int i, int at) __attribute__((always_inline)) { out.put(r, i, ids[at]); });
+  out.finish(p, x.seq, x.kvh, p.budget, kRoughThreads);
 }
 
 template <typename T>
-int launch_scores(const SparseParams &p, hipStream_t stream) {
-  // Tiles of a wave: q is converted once for all of them, but a wave for every SIMD comes
-  // first.
-  const int64_t all = ceil_div(p.bt_width, 64) * p.hkv * p.seqs;  // of four waves
-  const int64_t cus = current_device_cus() > 0 ? current_device_cus() : 256;
-  const int tiles = static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(8, all / cus)));
-  const unsigned grid =
-      static_cast<unsigned>(ceil_div(p.bt_width, 64 * tiles) * p.hkv * p.seqs);
+int launch_choice(const SparseParams &p, hipStream_t stream) {
+  const int64_t pairs = p.hkv * p.seqs;
+  const unsigned lists = static_cast<unsigned>(pairs);
   const int64_t pieces = ceil_div(p.d * static_cast<int64_t>(sizeof(T)), 16);
-  if (pieces <= 4) score_blocks<T, 1><<<grid, 256, 0, stream>>>(p, tiles);
-  else if (pieces <= 8) score_blocks<T, 2><<<grid, 256, 0, stream>>>(p, tiles);
-  else if (pieces <= 16) score_blocks<T, 4><<<grid, 256, 0, stream>>>(p, tiles);
-  else score_blocks<T, 8><<<grid, 256, 0, stream>>>(p, tiles);
-  return check_launch("score_blocks");
+#define MLR_BY_PIECES(LAUNCH)                   \
+  if (pieces <= 4) LAUNCH(1);                   \
+  else if (pieces <= 8) LAUNCH(2);              \
+  else if (sizeof(T) == 2 || pieces <= 16) LAUNCH(4); \
+  else LAUNCH((sizeof(T) == 4 ? 8 : 4))
+  if (p.bt_width <= kSmall) {
+#define MLR_SMALL(N) choose_small<T, N><<<lists, kSmallThreads, 0, stream>>>(p)
+    MLR_BY_PIECES(MLR_SMALL);
+#undef MLR_SMALL
+    return check_launch("choose_small");
+  }
+  const bool all = p.bt_width <= p.budget;  // nothing to choose
+  if (sizeof(T) == 2 && !all && p.bt_width <= kRoughBlocks) {
+    if constexpr (sizeof(T) == 2) {
+      // Tiles of a wave: q is read once for all of them, but some waves for every SIMD
+      // come first.
+      const int64_t cus = current_device_cus() > 0 ? current_device_cus() : 256;
+      const int tiles = static_cast<int>(
+          std::max<int64_t>(1, std::min<int64_t>(8, ceil_div(p.bt_width, 64) * pairs / (2 * cus))));
+      const unsigned grid = static_cast<unsigned>(ceil_div(p.bt_width, 64 * tiles) * pairs);
+#define MLR_ROUGH(N)                                             \
+  {                                                              \
+    score_rough<T, N><<<grid, 256, 0, stream>>>(p, tiles);       \
+    choose_rough<T, N><<<lists, kRoughThreads, 0, stream>>>(p);  \
+  }
+      if (pieces <= 4) MLR_ROUGH(1) else if (pieces <= 8) MLR_ROUGH(2) else MLR_ROUGH(4)
+#undef MLR_ROUGH
+    }
+    return check_launch("choose_rough");
+  }
+  if (!all) {
+    const unsigned grid = static_cast<unsigned>(ceil_div(p.bt_width, 64) * pairs);
+#define MLR_SCORE(N) score_blocks<T, N><<<grid, 256, 0, stream>>>(p)
+    MLR_BY_PIECES(MLR_SCORE);
+#undef MLR_SCORE
+  }
+#undef MLR_BY_PIECES
+  if (p.bt_width <= 1024) choose_blocks<256, 1><<<lists, 256, 0, stream>>>(p);
+  else choose_blocks<1024, 2><<<lists, 1024, 0, stream>>>(p);
+  return check_launch("choose_blocks");
 }
 
 int64_t whole_fours(int64_t n) { return (n + 3) & ~int64_t(3); }
 
 struct Layout {
-  size_t keys, table, lens, decode;
-  size_t total() const { return keys + table + lens + decode; }
+  size_t keys, exact, table, lens, decode;
+  size_t total() const { return keys + exact + table + lens + decode; }
 };
 Layout layout_of(int64_t batch, int64_t hq, int64_t hkv, int64_t d, int64_t width,
                  int64_t block_size, int64_t budget, int dtype) {
   const int64_t list = std::min(budget, width);
-  return Layout{align256(batch * hkv * whole_fours(width) * sizeof(uint64_t)),
+  const size_t keys =
+      width > kSmall ? align256(batch * hkv * whole_fours(width) * sizeof(uint64_t)) : 0;
+  return Layout{keys, dtype_size(dtype) == 2 ? keys : 0,
                 align256(batch * hkv * list * sizeof(int64_t)), align256(batch * sizeof(int64_t)),
                 short_keys(list * block_size, d, dtype)
                     ? 0
@@ -433,39 +769,34 @@ extern "C" int mlr_paged_decode_sparse(
   SparseParams x{q, key_bounds, q_stride_b, q_stride_h, num_blocks, block_size, num_kv_heads,
                  group, head_dim, block_tables, bt_stride, max_blocks, seq_lens, batch, scale < 0,
                  static_cast<int>(sinks), static_cast<int>(recent), static_cast<int>(budget),
-                 static_cast<int>(list), nullptr, whole_fours(max_blocks), nullptr, nullptr, chosen};
+                 static_cast<int>(list), nullptr, nullptr, whole_fours(max_blocks), nullptr, nullptr,
+                 chosen};
   int64_t max_keys = 0;
   if (need) {
     const Layout l = layout_of(batch, num_q_heads, num_kv_heads, head_dim, max_blocks, block_size,
                                budget, dtype);
     x.keys = reinterpret_cast<uint64_t *>(ws);
-    x.table = reinterpret_cast<int64_t *>(ws += l.keys);
+    x.exact = reinterpret_cast<uint64_t *>(ws += l.keys);
+    x.table = reinterpret_cast<int64_t *>(ws += l.exact);
     x.lens = reinterpret_cast<int64_t *>(ws += l.table);
     ws += l.lens;
-    int rc = MLR_OK;
-    if (max_blocks > budget) {
-      if (dtype == MLR_DTYPE_F32) rc = launch_scores<float>(x, s);
-      else if (dtype == MLR_DTYPE_F16) rc = launch_scores<f16_t>(x, s);
-      else rc = launch_scores<bf16_t>(x, s);
-      if (rc) return rc;
-    }
     max_keys = list * block_size;
     o.bt = x.table;
     o.bt_st = num_kv_heads * list;
     o.bt_width = list;
     o.ctx = x.lens;
   }
-  if (need || chosen) {
-    const unsigned lists = static_cast<unsigned>(batch * num_kv_heads);
-    if (max_blocks <= 1024) choose_blocks<256, 1><<<lists, 256, 0, s>>>(x);
-    else choose_blocks<1024, 2><<<lists, 1024, 0, s>>>(x);
-    if (const int rc = check_launch("choose_blocks")) return rc;
-  }
+  int rc = MLR_OK;
+  if (dtype == MLR_DTYPE_F32) rc = launch_choice<float>(x, s);
+  else if (dtype == MLR_DTYPE_F16) rc = launch_choice<f16_t>(x, s);
+  else rc = launch_choice<bf16_t>(x, s);
+  if (rc) return rc;
   ScoredParams p = params_of(o, kModeDecode);
   p.bt_sh = need ? list : 0;
   p.whole = short_keys(max_keys, head_dim, dtype);
   const bool parts = !p.whole;
   const int64_t items = plan_decode(p, max_keys, parts ? ws : nullptr);
-  if (const int rc = launch_scored_rows(p, dtype, grid_of(items), s)) return rc;
+  rc = launch_scored_rows(p, dtype, grid_of(items), s);
+  if (rc) return rc;
   return parts ? merge_decode(p, dtype, s) : MLR_OK;
 }
