@@ -275,6 +275,22 @@ def test_compaction_of_long_rows_by_small_steps(device, drop):
     assert torch.equal(k.cpu(), want[0]) and torch.equal(v.cpu(), want[1])
 
 
+@pytest.mark.parametrize("block_size,n", [(1, 6000), (2, 9001), (48, 6000)])
+@pytest.mark.parametrize("hkv,d", [(1, 8), (5, 64)])
+def test_compaction_of_wide_tables(device, block_size, n, hkv, d):
+    """More blocks than a workgroup holds ids of, one list and several at a time."""
+    rng = random.Random(n)
+    k, v, tables = so.pool([n, 40], block_size, hkv, d, BF, 3)
+    kept = torch.full((2, n), -1)
+    for i, count in enumerate((n, 40)):
+        stay = sorted(rng.sample(range(count), count * 2 // 3))
+        kept[i, :len(stay)] = torch.tensor(stay)
+    want = moved(k, v, None, tables, kept, [0, 0], block_size)
+    k, v = k.to(device), v.to(device)
+    compact_keys(k, v, tables.to(device), kept.to(device), block_size)
+    assert torch.equal(k.cpu(), want[0]) and torch.equal(v.cpu(), want[1])
+
+
 def test_compaction_of_an_accepted_path_behind_a_shared_prefix(device):
     """Requests may share blocks before the start."""
     k, v, tables = so.pool([70, 70], 16, 2, 64, BF, 3)

@@ -136,17 +136,25 @@ def test_capped_and_negative_scale(device, dtype):
     run_case(device, dtype, (14, 2, 64), [300, 200], 5, scale=-0.1)
 
 
-def test_ties_go_to_the_lower_block(device):
+# Up to 256 blocks a table's scores and choice are one launch, past that two.
+WIDTHS = pytest.mark.parametrize("width", [None, 300])
+
+
+@WIDTHS
+@pytest.mark.parametrize("dtype", [BF, F32])
+def test_ties_go_to_the_lower_block(device, dtype, width):
     def change(q, k, v, bounds, tables):
         bounds[:, 0] = -1.0
         bounds[:, 1] = 1.0
         bounds[tables[0, 20], 1] = 2.0
 
-    _, blocks = run_case(device, BF, (14, 2, 64), [600], 6, change=change)
+    _, blocks = run_case(device, dtype, (14, 2, 64), [600], 6, change=change, width=width)
     assert blocks[0, 0].tolist() == [0, 1, 2, 3, 20, 37]
 
 
-def test_scores_apart_by_less_than_32_bits_hold(device):
+@WIDTHS
+@pytest.mark.parametrize("dtype", [BF, FP, F32])
+def test_scores_apart_by_less_than_32_bits_hold(device, dtype, width):
     """Sums of terms of unlike size, whose 32-bit sums would be equal."""
     def change(q, k, v, bounds, tables):
         q[:] = 1.0
@@ -156,12 +164,13 @@ def test_scores_apart_by_less_than_32_bits_hold(device):
         for j in (9, 5, 30):
             bounds[tables[0, j], 1, :, 1] = 1.0 + 2.0 ** -7
 
-    _, blocks = run_case(device, F32, (2, 1, 64), [600], 5, change=change)
+    _, blocks = run_case(device, dtype, (2, 1, 64), [600], 5, change=change, width=width)
     assert blocks[0, 0].tolist() == [0, 5, 9, 30, 37]
 
 
-@pytest.mark.parametrize("dtype", [BF, F32])
-def test_bounds_that_are_not_finite(device, dtype):
+@WIDTHS
+@pytest.mark.parametrize("dtype", [BF, FP, F32])
+def test_bounds_that_are_not_finite(device, dtype, width):
     """A head's NaN does not count, and a block of NaN scores lowest; infinities score."""
     def change(q, k, v, bounds, tables):
         bounds[tables[0, 3]] = float("nan")
@@ -169,11 +178,12 @@ def test_bounds_that_are_not_finite(device, dtype):
         bounds[tables[0, 6], 0, 0, 2] = -float("inf")
         q[0, 0, 2] = 0.0
 
-    run_case(device, dtype, (4, 2, 64), [400], 6, change=change)
+    run_case(device, dtype, (4, 2, 64), [400], 6, change=change, width=width)
 
 
+@WIDTHS
 @pytest.mark.parametrize("dtype", [BF, F32])
-def test_hidden_rows_are_not_read(device, dtype):
+def test_hidden_rows_are_not_read(device, dtype, width):
     """Blocks that are not chosen, and rows behind the last key, may hold anything."""
     def change(q, k, v, bounds, tables):
         for j in range(2, 24):
@@ -189,7 +199,7 @@ def test_hidden_rows_are_not_read(device, dtype):
         k[tables[0, 24], 9:] = float("nan")
         v[tables[0, 24], 9:] = float("nan")
 
-    got, _ = run_case(device, dtype, (14, 2, 64), [393], 4, change=change)
+    got, _ = run_case(device, dtype, (14, 2, 64), [393], 4, change=change, width=width)
     assert got.isfinite().all()
 
 
@@ -198,8 +208,9 @@ def test_padded_rows_and_wide_tables(device):
     assert (got[0] == 0).all() and (got[2] == 0).all() and (blocks[0] == -1).all()
 
 
-def test_bad_blocks_score_lowest_and_are_masked(device):
-    k, v, tables = so.pool([160], 16, 2, 64, BF, 0)
+@WIDTHS
+def test_bad_blocks_score_lowest_and_are_masked(device, width):
+    k, v, tables = so.pool([160], 16, 2, 64, BF, 0, width=width)
     bounds = bounds_of(k, tables, [160], None, 16, torch.zeros(k.shape[0], 2, 2, 64, dtype=BF))
     q = torch.randn(1, 14, 64, generator=torch.Generator().manual_seed(1)).to(BF)
     tables[0, 4] = 1 << 40
@@ -214,6 +225,49 @@ def test_bad_blocks_score_lowest_and_are_masked(device):
     want, bound, _, _ = so.attend(q, k.view(-1, 2, 64)[slot], v.view(-1, 2, 64)[slot], seen,
                                   0.125, 0.0, BF)
     so.assert_within(got, want, bound)
+
+
+@pytest.mark.parametrize("dtype", [BF, FP, F32])
+@pytest.mark.parametrize("heads", [(14, 2, 64), (8, 2, 128), (6, 2, 40), (40, 2, 24)])
+@pytest.mark.parametrize("left", [1, 40])
+def test_scores_that_32_bits_leave_open(device, dtype, heads, left):
+    """Groups of blocks that differ in the last place of one bound: some, more than are
+    compared one by one, and all of them open in 32 bits."""
+    for alike in (3, 50, 90, 400):
+        def change(q, k, v, bounds, tables):
+            at = tables[0, 10:10 + alike]
+            base = bounds[at[0]].clone()
+            bounds[at] = base
+            gen = torch.Generator().manual_seed(alike)
+            place = torch.randint(0, heads[2], (alike,), generator=gen)
+            step = 1.0 + torch.finfo(dtype).eps * torch.randint(-1, 2, (alike,), generator=gen)
+            for j, b in enumerate(at):
+                bounds[b, 1, :, place[j]] *= step[j].to(dtype)
+
+        run_case(device, dtype, heads, [16 * 420], left + 3, sinks=1, recent=2, change=change)
+
+
+@pytest.mark.parametrize("dtype", [BF, FP])
+def test_scores_past_what_32_bits_hold(device, dtype):
+    """Products and sums that overflow 32 bits, subnormal operands, and rows of zeros. The
+    blocks hold in all of them; with a query of 3e38 and keys past 1.2 the attention's own
+    products pass 3.41e38, the largest 32-bit number, and only the blocks are compared."""
+    big = 3e38 if dtype == BF else 65504.0
+    tiny = torch.finfo(dtype).tiny / 4
+
+    for kind in ("big", "tiny", "zeros", "mixed"):
+        def change(q, k, v, bounds, tables):
+            if kind == "zeros":
+                bounds.zero_()
+            elif kind == "tiny":
+                bounds.mul_(tiny)
+                q.mul_(tiny)
+            else:
+                bounds[tables[0, 5:200:3], 1, :, 3] = big
+                q[:, :, 3] = big if kind == "big" else 1.0
+
+        q_free = dict(scale=1e-9) if kind == "big" else {}
+        run_case(device, dtype, (14, 2, 64), [16 * 300], 20, recent=2, change=change, **q_free)
 
 
 @pytest.mark.parametrize("dtype", [BF, FP, F32])
