@@ -73,7 +73,8 @@ __device__ __forceinline__ void join_row(const ScoredParams &p, int64_t row) {
 // entry, hence the atomic; where blocks are a request's own each entry has one addend
 // and the result does not depend on any order.
 // Bound by latency, as the scores of 64 requests are 8 MB: what does not depend on the
-// statistics (table, scores of up to kAhead heads) is read before them.
+// statistics (table, scores of up to kAhead heads) is read before them. 64 requests of 128 to
+// 4,096 keys, 14 heads over 2 of 64: 9 us, with the join of the results.
 constexpr int kAhead = 8;
 __device__ __forceinline__ void weigh_keys(const ScoredParams &p, float *weights, int64_t task,
                                            float (*s_ml)[2]) {
@@ -217,7 +218,8 @@ struct CacheParams {
 
 // A workgroup chooses the places of one request and KV head. Bound by latency: the keys'
 // two loads (a table, then four neighbouring weights where a block holds a multiple of
-// four), two digits of the selection, the list.
+// four), the selection's histogram, the list. 32 lists of 16,384 keys 17 us to 20, of which the
+// histogram's atomics are 6; 128 lists of 1,040 keys 8 us.
 template <int kThreads, int kHeld>
 __global__ __launch_bounds__(kThreads) void choose_keys(CacheParams c, const int64_t *ctx,
                                                         int sinks, int recent, int budget,
@@ -281,7 +283,8 @@ __global__ __launch_bounds__(kThreads) void choose_keys(CacheParams c, const int
 //
 // Bound by what is in flight: each wave has two batches of 16 loads, one landing while the
 // other is written. The rows' places are made a batch ahead, from the list, which is read
-// two ahead, and the request's block table, which lies in LDS.
+// two ahead, and the request's block table, which lies in LDS. 4 lists of 6,144 rows for each of
+// 8 heads of 128, 201 MB read and written: 55 us, 3.7 TB/s.
 constexpr int kLanes = 4;    // of 16 bytes, of a row of a column
 constexpr int kLoads = 16;   // of a wave and batch
 constexpr int kWaveRows = 64 / kLanes * kLoads;
@@ -558,7 +561,9 @@ extern "C" int mlr_evict_keys(void *k_cache, void *v_cache, float *key_weights,
   choose_keys<T, H><<<lists, T, 0, s>>>(c, seq_lens, static_cast<int>(sinks),              \
                                         static_cast<int>(recent), static_cast<int>(budget), \
                                         kept, new_lens)
-  // As many waves as hold the longest row's keys in registers: fewer meet sooner.
+  // As many waves as hold the longest row's keys in registers: fewer meet sooner. us of the
+  // three: 128 lists of 1,040 keys 7.8, 11.1, 14.0 and of 2,047 10.7, 13.2, 16.2; 32 lists of
+  // 16,384 81, 20.0, 22.6 and of 32,760 145, 51, 26.7.
   const int64_t most = max_blocks * block_size;
   if (most <= 2048) MLR_CHOOSE(256, 2);
   else if (most <= 16384) MLR_CHOOSE(1024, 4);

@@ -59,7 +59,9 @@ __device__ __forceinline__ uint4 pack(const float *x) {
   }
 }
 
-// Thread: 16 bytes of a row of one changed block and KV head.
+// Thread: 16 bytes of a row of one changed block and KV head; a block's keys are read once.
+// Bound by the read: 4 requests of 7,000 to 8,192 keys, 8 KV heads of 128: 71 MB in 12.7 us,
+// some from the caches; one new key of 64 requests, 2 KV heads of 64, 8 us of launch and latency.
 template <typename T>
 __global__ __launch_bounds__(256) void bound_keys(BoundParams p) {
   constexpr int kE = 16 / sizeof(T);
@@ -249,7 +251,9 @@ struct Pair {
   }
 };
 
-// Scores in 64 bits of all blocks (FP32, and past kRoughBlocks), a wave for 16.
+// Scores in 64 bits of all blocks (FP32, and where score_rough is not taken), a wave for 16.
+// Bound by the 64-bit matrix instructions, half of whose work is with zeros: 8 requests of
+// 2,048 blocks, 4 KV heads of 128: 8.6 GFLOP of 16 heads in 26 us.
 template <typename T, int kT>
 __global__ __launch_bounds__(256) void score_blocks(SparseParams p) {
   const int64_t b = blockIdx.x;
@@ -270,7 +274,7 @@ __global__ __launch_bounds__(256) void score_blocks(SparseParams p) {
 // (four times that of rounding to nearest), and 1e-30 of each factor for operands that
 // the matrix unit may take for 0. Not finite: no bound.
 // Bound by reading the bounds: 8 requests of 2,048 blocks, 4 KV heads of 128: 33 MB in
-// MEASURED us, where 64 bits throughout took 26 us.
+// 13.6 us, where score_blocks takes 26 us.
 template <typename T> struct Rough;
 template <> struct Rough<bf16_t> {
   __device__ static f32x4_t mfma(uint4 a, uint4 b, f32x4_t c) {
@@ -445,9 +449,11 @@ __global__ __launch_bounds__(kThreads) void choose_blocks(SparseParams p) {
   out.finish(p, seq, kvh, count, kThreads);
 }
 
-// The same for tables of few blocks, with their scores: one launch. Eight waves with up to
-// two tiles each; past that the scores of one request keep one CU too long.
-constexpr int kSmall = 256, kSmallThreads = 512;
+// The same for tables of few blocks, with their scores: one launch. Eight waves with a tile
+// each; past that the scores of one request keep one CU too long. us of one launch and of
+// two, 16 requests, 4 KV heads of 128, by blocks: 64 13.7 and 15.8, 128 16.7 and 14.6, 256
+// 24.2 and 16.8; the second launch itself costs about 2 us more.
+constexpr int kSmall = 128, kSmallThreads = 512;
 template <typename T, int kT>
 __global__ __launch_bounds__(kSmallThreads) void choose_small(SparseParams p) {
   __shared__ SelectShared s;
@@ -471,10 +477,21 @@ __global__ __launch_bounds__(kSmallThreads) void choose_small(SparseParams p) {
 // The choice from scores in 32 bits and how far off they may be. With T the last chosen of
 // them and R the largest error, a block below T - 2 R is worse than all down to T, and one
 // above T + 2 R is better than all from T on; those in between are scored in 64 bits. Where
-// they are more than kFew, all blocks are. Bound by latency, a dozen steps of 1 us: what a
-// later step needs of memory (block ids, q) is read with the scores.
+// they are more than kFew, all blocks are. Bound by latency, a dozen steps of 1 us, 17 us for
+// 32 lists of 2,048 blocks: what a later step needs of memory (block ids, q) is read with the
+// scores.
 constexpr int kRoughThreads = 512, kRoughHeld = 2;
-constexpr int kRoughBlocks = 4 * kRoughThreads * kRoughHeld;  // at most
+constexpr int kRoughBlocks = 4 * kRoughThreads * kRoughHeld;  // at most, as they stay in registers
+
+// The second look costs some 6 us more than choose_blocks, so that 32 bits pay where the
+// scores in 64 take longer than that. us of scores and choice in 64 bits and in 32, by
+// lists x blocks x elements x tiles of 16 heads: 8 x 512 x 128 14 and 20, 4 x 4,096 x 128 20 and
+// 27, 128 x 512 x 64 20 and 20, 32 x 2,048 x 128 38 and 31, 64 x 4,096 x 128 98 and 66.
+bool takes_rough(int64_t pairs, int64_t group, int64_t d, int64_t width, int64_t budget,
+                 int dtype) {
+  return dtype != MLR_DTYPE_F32 && width > std::max<int64_t>(budget, kSmall) &&
+         width <= kRoughBlocks && pairs * width * d * ceil_div(group, 16) >= int64_t(6) << 20;
+}
 template <typename T, int kT>
 __global__ __launch_bounds__(kRoughThreads) void choose_rough(SparseParams p) {
   constexpr int kWaves = kRoughThreads / 64;
@@ -614,7 +631,7 @@ __global__ __launch_bounds__(kRoughThreads) void choose_rough(SparseParams p) {
 }
 
 template <typename T>
-int launch_choice(const SparseParams &p, hipStream_t stream) {
+int launch_choice(const SparseParams &p, bool rough, hipStream_t stream) {
   const int64_t pairs = p.hkv * p.seqs;
   const unsigned lists = static_cast<unsigned>(pairs);
   const int64_t pieces = ceil_div(p.d * static_cast<int64_t>(sizeof(T)), 16);
@@ -629,11 +646,11 @@ int launch_choice(const SparseParams &p, hipStream_t stream) {
 #undef MLR_SMALL
     return check_launch("choose_small");
   }
-  const bool all = p.bt_width <= p.budget;  // nothing to choose
-  if (sizeof(T) == 2 && !all && p.bt_width <= kRoughBlocks) {
+  if (rough) {
     if constexpr (sizeof(T) == 2) {
-      // Tiles of a wave: q is read once for all of them, but some waves for every SIMD
-      // come first.
+      // Tiles of a wave: q is read once for all of them, but two waves for every SIMD come
+      // first (us by 1, 2, 4 and as many as that: 128 lists of 512 blocks of 64 elements 9.0,
+      // -, 10.8 and 8.6; 64 of 4,096 of 128 58, -, 45 and 43).
       const int64_t cus = current_device_cus() > 0 ? current_device_cus() : 256;
       const int tiles = static_cast<int>(
           std::max<int64_t>(1, std::min<int64_t>(8, ceil_div(p.bt_width, 64) * pairs / (2 * cus))));
@@ -648,13 +665,15 @@ int launch_choice(const SparseParams &p, hipStream_t stream) {
     }
     return check_launch("choose_rough");
   }
-  if (!all) {
+  if (p.bt_width > p.budget) {  // something to choose
     const unsigned grid = static_cast<unsigned>(ceil_div(p.bt_width, 64) * pairs);
 #define MLR_SCORE(N) score_blocks<T, N><<<grid, 256, 0, stream>>>(p)
     MLR_BY_PIECES(MLR_SCORE);
 #undef MLR_SCORE
   }
 #undef MLR_BY_PIECES
+  // As many waves as hold the keys in registers: fewer meet sooner (us of 256 and 1,024
+  // threads: 16 lists of 512 blocks 6.6 and 11.3).
   if (p.bt_width <= 1024) choose_blocks<256, 1><<<lists, 256, 0, stream>>>(p);
   else choose_blocks<1024, 2><<<lists, 1024, 0, stream>>>(p);
   return check_launch("choose_blocks");
@@ -669,9 +688,10 @@ struct Layout {
 Layout layout_of(int64_t batch, int64_t hq, int64_t hkv, int64_t d, int64_t width,
                  int64_t block_size, int64_t budget, int dtype) {
   const int64_t list = std::min(budget, width);
+  const bool rough = takes_rough(batch * hkv, hq / hkv, d, width, budget, dtype);
   const size_t keys =
       width > kSmall ? align256(batch * hkv * whole_fours(width) * sizeof(uint64_t)) : 0;
-  return Layout{keys, dtype_size(dtype) == 2 ? keys : 0,
+  return Layout{keys, rough ? keys : 0,
                 align256(batch * hkv * list * sizeof(int64_t)), align256(batch * sizeof(int64_t)),
                 short_keys(list * block_size, d, dtype)
                     ? 0
@@ -701,7 +721,7 @@ extern "C" int mlr_update_key_bounds(const void *k_cache, void *key_bounds, int6
                   max_blocks >= 0 && max_blocks < (int64_t(1) << 31) / block_size,
               "%s: a block table must cover fewer than 2^31 positions", w);
   MLR_REQUIRE(max_new >= 0, "%s: max_new must be >= 0", w);
-  if (batch == 0 || max_blocks == 0 || max_new == 0) return MLR_OK;
+  if (batch == 0 || max_blocks == 0 || (starts && max_new == 0)) return MLR_OK;
   MLR_REQUIRE(k_cache && key_bounds && block_tables && seq_lens, "%s: null pointer", w);
   MLR_REQUIRE((reinterpret_cast<uintptr_t>(k_cache) | reinterpret_cast<uintptr_t>(key_bounds)) %
                       16 == 0, "%s: operands must be 16-byte aligned", w);
@@ -786,10 +806,12 @@ extern "C" int mlr_paged_decode_sparse(
     o.bt_width = list;
     o.ctx = x.lens;
   }
+  const bool rough = need && takes_rough(batch * num_kv_heads, group, head_dim, max_blocks, budget,
+                                         dtype);
   int rc = MLR_OK;
-  if (dtype == MLR_DTYPE_F32) rc = launch_choice<float>(x, s);
-  else if (dtype == MLR_DTYPE_F16) rc = launch_choice<f16_t>(x, s);
-  else rc = launch_choice<bf16_t>(x, s);
+  if (dtype == MLR_DTYPE_F32) rc = launch_choice<float>(x, rough, s);
+  else if (dtype == MLR_DTYPE_F16) rc = launch_choice<f16_t>(x, rough, s);
+  else rc = launch_choice<bf16_t>(x, rough, s);
   if (rc) return rc;
   ScoredParams p = params_of(o, kModeDecode);
   p.bt_sh = need ? list : 0;

@@ -72,9 +72,14 @@ def test_bounds_padded_rows_and_bad_blocks(device):
     assert torch.equal(got.cpu(), want)
 
 
+MANY = 4096  # blocks of a table
+
+
 def run_case(device, dtype, heads, lens, budget, sinks=1, recent=1, block_size=16, cap=0.0,
              scale=None, seed=0, validate=True, change=None, width=None):
     hq, hkv, d = heads
+    if width == MANY:  # scores in 32 bits first, which a few lists are not worth
+        lens = lens + [1] * (-(-(6 << 20) // (MANY * hkv * d)) - len(lens))
     k, v, tables = so.pool(lens, block_size, hkv, d, dtype, seed, width=width)
     gen = torch.Generator().manual_seed(seed + 1)
     q = torch.randn(len(lens), hq, d, generator=gen).to(dtype)
@@ -124,6 +129,16 @@ def test_budgets(device, budget, sinks, recent):
     run_case(device, BF, (14, 2, 64), [1, 80, 81, 400, 1000], budget, sinks, recent)
 
 
+@pytest.mark.parametrize("dtype", [BF, FP])
+@pytest.mark.parametrize("heads", [(14, 2, 64), (8, 2, 128), (4, 4, 96), (6, 2, 40), (40, 1, 16),
+                                   (80, 1, 32), (3, 1, 8)])
+def test_many_lists_of_long_tables(device, dtype, heads):
+    for budget, sinks, recent in ((8, 1, 2), (3, 0, 3), (40, 4, 1), (400, 0, 1)):
+        run_case(device, dtype, heads, [1, 16, 17, 1000, 5000, 5001, 65536], budget, sinks, recent,
+                 width=MANY)
+    run_case(device, dtype, heads, [3000, 200], 5, cap=10.0, scale=-0.1, width=MANY)
+
+
 @pytest.mark.parametrize("dtype", [BF, F32])
 def test_long_contexts(device, dtype):
     run_case(device, dtype, (4, 2, 64), [20000, 7], 100, recent=3)
@@ -136,8 +151,9 @@ def test_capped_and_negative_scale(device, dtype):
     run_case(device, dtype, (14, 2, 64), [300, 200], 5, scale=-0.1)
 
 
-# Up to 256 blocks a table's scores and choice are one launch, past that two.
-WIDTHS = pytest.mark.parametrize("width", [None, 300])
+# Up to 128 blocks a table's scores and choice are one launch, past that two, and with many
+# lists of long tables 16-bit scores are made in 32 bits first.
+WIDTHS = pytest.mark.parametrize("width", [None, 300, MANY])
 
 
 @WIDTHS
@@ -210,21 +226,22 @@ def test_padded_rows_and_wide_tables(device):
 
 @WIDTHS
 def test_bad_blocks_score_lowest_and_are_masked(device, width):
-    k, v, tables = so.pool([160], 16, 2, 64, BF, 0, width=width)
-    bounds = bounds_of(k, tables, [160], None, 16, torch.zeros(k.shape[0], 2, 2, 64, dtype=BF))
-    q = torch.randn(1, 14, 64, generator=torch.Generator().manual_seed(1)).to(BF)
+    lens = [160] + ([1] * 15 if width == MANY else [])
+    k, v, tables = so.pool(lens, 16, 2, 64, BF, 0, width=width)
+    bounds = bounds_of(k, tables, lens, None, 16, torch.zeros(k.shape[0], 2, 2, 64, dtype=BF))
+    q = torch.randn(len(lens), 14, 64, generator=torch.Generator().manual_seed(1)).to(BF)
     tables[0, 4] = 1 << 40
     got, blocks = paged_attention_decode_sparse(
         q.to(device), k.to(device), v.to(device), bounds.to(device), tables.to(device),
-        torch.tensor([160]).to(device), 16, 9, return_blocks=True, validate=False)
+        torch.tensor(lens).to(device), 16, 9, return_blocks=True, validate=False)
     assert blocks[0].tolist() == [[0, 1, 2, 3, 5, 6, 7, 8, 9]] * 2
     tables[0, 4] = 0
     seen = torch.ones(1, 160, dtype=torch.bool)
     seen[:, 64:80] = False
     slot = so.slots(tables[0], 160, 16)
-    want, bound, _, _ = so.attend(q, k.view(-1, 2, 64)[slot], v.view(-1, 2, 64)[slot], seen,
+    want, bound, _, _ = so.attend(q[:1], k.view(-1, 2, 64)[slot], v.view(-1, 2, 64)[slot], seen,
                                   0.125, 0.0, BF)
-    so.assert_within(got, want, bound)
+    so.assert_within(got[:1], want, bound)
 
 
 @pytest.mark.parametrize("dtype", [BF, FP, F32])
@@ -244,7 +261,8 @@ def test_scores_that_32_bits_leave_open(device, dtype, heads, left):
             for j, b in enumerate(at):
                 bounds[b, 1, :, place[j]] *= step[j].to(dtype)
 
-        run_case(device, dtype, heads, [16 * 420], left + 3, sinks=1, recent=2, change=change)
+        run_case(device, dtype, heads, [16 * 420], left + 3, sinks=1, recent=2, change=change,
+                 width=MANY)
 
 
 @pytest.mark.parametrize("dtype", [BF, FP])
@@ -267,7 +285,8 @@ def test_scores_past_what_32_bits_hold(device, dtype):
                 q[:, :, 3] = big if kind == "big" else 1.0
 
         q_free = dict(scale=1e-9) if kind == "big" else {}
-        run_case(device, dtype, (14, 2, 64), [16 * 300], 20, recent=2, change=change, **q_free)
+        run_case(device, dtype, (14, 2, 64), [16 * 300], 20, recent=2, change=change, width=MANY,
+                 **q_free)
 
 
 @pytest.mark.parametrize("dtype", [BF, FP, F32])
