@@ -73,8 +73,9 @@ def paged_attention_decode_weighted(
     weight, summed over the query heads of its KV head, to key_weights in place. The entry
     of a request's newest key, at position seq_lens[b] - 1, is set, whatever it held.
 
-    Requests may share blocks: each adds to the entries of the shared keys, in no
-    particular order, so that the last bits of such a sum may differ from run to run.
+    Requests may share blocks, but no request's newest key may be another's key too: each
+    adds to the entries of the shared keys, in no particular order, so that the last bits of
+    such a sum may differ from run to run.
     The workspace holds the scores of the batch: 4 bytes for every query head and every
     position that the tables cover.
     """

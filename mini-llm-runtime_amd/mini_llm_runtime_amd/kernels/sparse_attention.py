@@ -42,9 +42,10 @@ def update_key_bounds(
     them gives NaN.
 
     After a step that appended one token a request: starts = seq_lens - 1, max_new = 1.
-    max_new, at least the longest such range, sizes the launch; without it the tables'
-    width does. Blocks of full requests that others share may be written by each, with
-    the same values.
+    max_new, at least the longest such range, sizes the launch of a call with starts; without
+    it the tables' width does. Full blocks that requests share are written by each, with the
+    same values; the bounds of a shared block that one of them fills further than another
+    may be either's.
     """
     what = "update_key_bounds"
     if k_cache.ndim != 4:
