@@ -1303,8 +1303,9 @@ def bench_serving(device, steps=None, graphs=False):
 
 
 # Sources that hold none of the profiled kernels (decode, prefill, pre-attention).
-UNPROFILED_SOURCES = ("qk_norm_rope.hip", "sampling.hip", "scored_attention.h",
-                      "scored_attention.hip", "scored_rows.hip", "scored_tiles.hip")
+UNPROFILED_SOURCES = ("key_eviction.hip", "key_select.h", "qk_norm_rope.hip", "sampling.hip",
+                      "scored_attention.h", "scored_attention.hip", "scored_rows.hip",
+                      "scored_tiles.hip", "sparse_attention.hip", "tree_attention.hip")
 
 
 def kernel_sources_hash():

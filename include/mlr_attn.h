@@ -761,7 +761,8 @@ int mlr_paged_attention_tree(const void *q, int64_t q_stride_t, int64_t q_stride
  * mlr_paged_decode_weighted: mlr_paged_decode_scored (without a bias) that also adds to
  * key_weights, FP32 [num_blocks, num_kv_heads, block_size], each key's attention weight,
  * summed over the query heads of the KV head; the entry of a sequence's newest key is
- * set to it. Requests that share a block add to the same entries, in any order.
+ * set to it. Requests that share a block add to the same entries, in any order; no
+ * sequence's newest key may be another's key too.
  *
  * mlr_evict_keys: of each sequence and KV head the first `sinks` keys, the last `recent` and
  * of the others the heaviest by key_weights stay, `budget` in all (ties: the lower
@@ -802,7 +803,8 @@ int mlr_compact_keys(void *k_cache, void *v_cache, float *key_weights, int64_t n
  * mlr_update_key_bounds: key_bounds [num_blocks, 2, num_kv_heads, head_dim], in the cache's
  * type: the elementwise minimum and maximum of a block's keys that exist, NaN where one
  * is. Every block that holds a position of [starts[b], seq_lens[b]) (starts null: of all
- * blocks) is written anew; max_new is at least the longest such range.
+ * blocks) is written anew; max_new is at least the longest such range (not read where
+ * starts is null).
  *
  * mlr_paged_decode_sparse: mlr_paged_decode_scored (without a bias) over some blocks of each
  * sequence, chosen for each KV head: the first `sinks`, the last `recent` (at least 1, so
@@ -810,7 +812,8 @@ int mlr_compact_keys(void *k_cache, void *v_cache, float *key_weights, int64_t n
  * those of the largest score, `budget` in all (ties: the lower one), where
  *   score = max over the heads h of the group of sum_d max(q_hd min_d, q_hd max_d)
  * in 64 bits, of -q where scale is negative; a head's sum that is NaN does not count, and a
- * block id out of range scores -infinity. chosen [batch, num_kv_heads, budget] (may be
+ * block id out of range scores -infinity. The chosen blocks are made a table in the
+ * workspace and attended to from there. chosen [batch, num_kv_heads, budget] (may be
  * null): their places in order, -1 past the end.
  */
 int mlr_update_key_bounds(const void *k_cache, void *key_bounds, int64_t num_blocks,
