@@ -217,10 +217,13 @@ __device__ __forceinline__ void cap_scores(float (&x)[4], float cap, float inv_c
 // kPrefill: the rows are tokens of chunks, not requests. kUnlike: rows of a unit may
 // see different keys (chunks, and requests shorter than the prefix that they share).
 // kTree: of its sequence's last tokens a row sees those that its bits name. kKeep: the
-// scores stay for a pass that weighs the keys.
+// scores stay for a pass that weighs the keys. Both must not cost a D of 64 one of the three
+// workgroups of a CU that rows_target counts on: with a few registers too many, 16 FP32
+// trees of 3 to 5 tokens after 500 to 4,000 keys took 42 us, not 32.
 template <typename T, int D, bool kCap, bool kPaged16, bool kPrefill, bool kUnlike, bool kTree,
           bool kKeep>
-__global__ __launch_bounds__(256) void scored_rows_kernel(ScoredParams p) {
+__global__ __launch_bounds__(256, (kTree || kKeep) && D <= 64 ? 3 : 1) void scored_rows_kernel(
+    ScoredParams p) {
   constexpr int kVe = D / 16;  // elements of a row that a lane of P V holds
   constexpr int kE = 16 / sizeof(T);
   constexpr int kBatch = D * sizeof(T) <= 128 ? 4 : D * sizeof(T) <= 256 ? 2 : 1;
