@@ -626,7 +626,9 @@ __global__ __launch_bounds__(kRoughThreads) void choose_rough(SparseParams p) {
         if (k > to || places.forced(i)) return true;
         return k >= from && (!few || s_taken[k - from] != 0);
       },
-      [&](int r, int i, int at) __attribute__((always_inline)) { out.put(r, i, ids[at]); });
+      [&](int r, int i, int at) __attribute__((always_inline)) {
+        out.put(r, i, at < 0 ? out.row[i] : ids[at]);
+      });
   out.finish(p, x.seq, x.kvh, p.budget, kRoughThreads);
 }
 
