@@ -733,7 +733,7 @@ int mlr_sample_tokens(const void *logits, int64_t row_stride, int64_t num_logit_
  * [query_start_loc[s], query_start_loc[s+1]), the place of its parent among them (out of
  * range: none). ancestors [total_q, words]: bit j % 64 of word j / 64 of a row says
  * whether token j of the sequence is that token or one of its ancestors (tokens past
- * 64 * words have no bit).
+ * 64 * words have no bit; words is at most 64, and tokens past 4096 have no row).
  *
  * mlr_paged_attention_tree: packed sequences as for mlr_paged_prefill_scored, whose last
  * n keys of context_lens[s] are those of its n rows. A row sees every key before

@@ -1,4 +1,5 @@
-// What the scored attention kernels share: a call's operands, the cut of its
+// What the scored attention kernels, and those of drafted trees, weighed keys and selected
+// blocks, share: a call's operands, the cut of its
 // work into items, the scores, and the layout of partial results.
 //
 // A unit is a group of query rows that share their keys: kRows consecutive rows

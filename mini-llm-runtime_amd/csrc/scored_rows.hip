@@ -1,6 +1,6 @@
 // Paged attention with capped or biased scores, for few query rows per key: single
-// tokens and short chunks, and everything in FP32 or with a block_size that is no
-// power of two from 16 on.
+// tokens, short chunks and small trees of drafted tokens, and everything in FP32 or with a
+// block_size that is no power of two from 16 on.
 //
 //   x_ij = scale q_i.k_j;  cap: x = cap tanh(x / cap);  x -= slope_h |i - j|
 //   j visible iff lo <= j < limit_i;  out_i = softmax_j(x_ij) v_j
@@ -20,6 +20,8 @@
 // makes the error against 64 bits 1.4 times that of the one rounding of the result
 // (bf16 0.0023 and 0.0017 of the outputs' size). Scores, statistics and sums are FP32,
 // and the result is rounded once.
+// Drafted tokens see the keys before them and those that their bits name; a decode
+// that weighs its keys leaves the scores in the workspace (64 requests as below: 21 us).
 // The waves' results are joined through LDS. Splits of one unit leave (m, l, O)
 // in the workspace, added up by scored_merge in the next launch.
 //

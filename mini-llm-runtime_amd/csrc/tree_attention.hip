@@ -1,12 +1,14 @@
 // Ancestors of drafted tokens as bits, from their parents.
 //
 // Bit j of a token's row: whether token j of its sequence is the token itself or one of
-// its ancestors. A thread walks one token's path to its root; parents are read through
-// LDS where a sequence's fit there. A path ends at a parent that is no token of the
+// its ancestors. A thread walks one token's path to its root for four words of its row;
+// parents are read through LDS. A path ends at a parent that is no token of the
 // sequence, and after as many steps as there are tokens, so that it ends where
 // parents form a circle too.
 //
-// Bound by latency: a path of depth 16 is 16 dependent reads of LDS.
+// Bound by latency: a path of depth 16 is 16 dependent reads of LDS. A sequence of more than
+// 64 tokens has several workgroups, so that a chain of kMostNodes is walked once by each
+// thread, not by each in turn for all tokens.
 #include "mlr_common.h"
 
 #include <algorithm>
@@ -14,36 +16,34 @@
 namespace mlr {
 namespace {
 
-constexpr int kHeldParents = 4096;
+constexpr int kMostNodes = 4096;  // tokens of a sequence that are nodes
 
 __global__ __launch_bounds__(256) void tree_ancestors(const int64_t *parents, const int64_t *qsl,
                                                       int64_t total, int64_t words,
                                                       int64_t *ancestors) {
-  __shared__ int s_parent[kHeldParents];
+  __shared__ int s_parent[kMostNodes];
   const int64_t seq = blockIdx.x;
   const int64_t q0 = min(max(qsl[seq], int64_t(0)), total);
-  const int64_t n = min(max(qsl[seq + 1], q0), total) - q0;
-  const bool held = n <= kHeldParents;
-  auto parent_of = [&](int64_t i) {
+  const int n = static_cast<int>(
+      min(min(max(qsl[seq + 1], q0), total) - q0, static_cast<int64_t>(kMostNodes)));
+  for (int i = threadIdx.x; i < n; i += 256) {
     const int64_t up = parents[q0 + i];
-    return up >= 0 && up < n ? up : int64_t(-1);
-  };
-  if (held) {
-    for (int64_t i = threadIdx.x; i < n; i += 256) s_parent[i] = static_cast<int>(parent_of(i));
-    __syncthreads();
+    s_parent[i] = up >= 0 && up < n ? static_cast<int>(up) : -1;
   }
+  __syncthreads();
   // Four words of a token's row at a time; its path is walked once for these.
   const int64_t fours = (words + 3) / 4;
-  for (int64_t at = threadIdx.x; at < n * fours; at += 256) {
+  for (int64_t at = blockIdx.y * int64_t(256) + threadIdx.x; at < n * fours;
+       at += gridDim.y * int64_t(256)) {
     const int64_t token = at / fours, word = 4 * (at - token * fours);
     uint64_t bits[4] = {0, 0, 0, 0};
-    int64_t up = token;
-    for (int64_t steps = 0; steps < n && up >= 0; ++steps) {
+    int up = static_cast<int>(token);
+    for (int steps = 0; steps < n && up >= 0; ++steps) {
       const int64_t w = (up >> 6) - word;
 #pragma unroll
       for (int i = 0; i < 4; ++i)
         if (w == i) bits[i] |= uint64_t(1) << (up & 63);
-      up = held ? s_parent[up] : parent_of(up);
+      up = s_parent[up];
     }
 #pragma unroll
     for (int i = 0; i < 4; ++i)
@@ -61,11 +61,15 @@ extern "C" int mlr_tree_ancestors(const int64_t *parents, const int64_t *query_s
                                   int64_t *ancestors, void *stream) {
   clear_error();
   MLR_REQUIRE(num_seqs >= 0 && num_seqs < (1 << 24) && total_q >= 0 &&
-                  total_q < (int64_t(1) << 31) && words > 0 && words < (1 << 24),
-              "mlr_tree_ancestors: bad sizes");
+                  total_q < (int64_t(1) << 31) && words > 0 && words <= kMostNodes / 64,
+              "mlr_tree_ancestors: bad sizes (a row of ancestors has 1 to %d words)",
+              kMostNodes / 64);
   if (num_seqs == 0 || total_q == 0) return MLR_OK;
   MLR_REQUIRE(parents && query_start_loc && ancestors, "mlr_tree_ancestors: null pointer");
-  tree_ancestors<<<static_cast<unsigned>(num_seqs), 256, 0, static_cast<hipStream_t>(stream)>>>(
-      parents, query_start_loc, total_q, words, ancestors);
+  const int64_t nodes = std::min(total_q, 64 * words);
+  const dim3 grid(static_cast<unsigned>(num_seqs),
+                  static_cast<unsigned>(ceil_div(nodes * ceil_div(words, 4), 256)));
+  tree_ancestors<<<grid, 256, 0, static_cast<hipStream_t>(stream)>>>(parents, query_start_loc,
+                                                                     total_q, words, ancestors);
   return check_launch("tree_ancestors");
 }

@@ -71,7 +71,8 @@ def paged_attention_decode_weighted(
 ) -> torch.Tensor:
     """paged_attention_decode_scored (without a bias) that also adds each key's attention
     weight, summed over the query heads of its KV head, to key_weights in place. The entry
-    of a request's newest key, at position seq_lens[b] - 1, is set, whatever it held.
+    of a request's newest key, at position seq_lens[b] - 1, is set, whatever it held. With
+    validate=False a seq_lens of 0 (a padded row) gives zeros and adds nothing.
 
     Requests may share blocks, but no request's newest key may be another's key too: each
     adds to the entries of the shared keys, in no particular order, so that the last bits of
@@ -130,7 +131,7 @@ def evict_keys(
     `recent` (half the budget if None) and the heaviest of the others by key_weights (ties: the
     lower position; NaN counts as -infinity). What stays keeps its order and moves,
     with its key_weights, to the positions 0, 1, ... of the request, in place; what lies
-    behind is left as it is.
+    behind is left as it is. With validate=False a seq_lens of 0 (a padded row) keeps none.
 
     Returns (kept, new_lens): int64 [B, Hkv, budget], the positions that stayed, -1 past
     the end, and int64 [B], min(seq_lens, budget). A request no longer than the budget

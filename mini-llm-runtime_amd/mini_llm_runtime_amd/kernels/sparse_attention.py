@@ -71,10 +71,9 @@ def update_key_bounds(
         if starts.shape != (batch,):
             raise ValueError("starts must hold one position per request")
     width = block_tables.shape[1]
-    if max_new is None:
-        max_new = width * block_size
-    elif max_new < 0:
+    if max_new is not None and max_new < 0:
         raise ValueError("max_new cannot be negative")
+    max_new = width * block_size if max_new is None else min(max_new, width * block_size)
     if batch == 0:
         return
     if validate:

@@ -35,14 +35,14 @@ def tree_ancestors(
 
     parents [total_q] holds each token's parent as a place in its own sequence, whose
     rows are [query_start_loc[s], query_start_loc[s+1]); a place out of range (-1) is
-    none. Parents may stand behind their children. max_nodes is at least the longest
-    sequence: tokens past it have no bit.
+    none. Parents may stand behind their children. max_nodes, up to 4096, is at least the
+    longest sequence: tokens past it have no bit, and those past 4096 no row.
     """
     what = "tree_ancestors"
     if parents.ndim != 1:
         raise ValueError("parents must have shape [total_q]")
-    if max_nodes <= 0:
-        raise ValueError("max_nodes must be greater than 0")
+    if not 0 < max_nodes <= 4096:
+        raise ValueError("max_nodes must be greater than 0 and at most 4096")
     device = _lib.require_hip(parents, what=what)
     parents = _as_index_tensor(parents, device).contiguous()
     query_start_loc = _as_index_tensor(query_start_loc, device).contiguous()

@@ -169,7 +169,7 @@ def test_eviction(device, dtype, heads):
 
 
 @pytest.mark.parametrize("budget,sinks,recent", [
-    (1, 0, 0), (1, 1, 0), (1, 0, 1), (10, 10, 0), (10, 0, 10), (10, 4, 6), (64, 0, 0), (65, 1, 1)])
+    (0, 0, 0), (1, 0, 0), (1, 1, 0), (1, 0, 1), (10, 10, 0), (10, 0, 10), (10, 4, 6), (64, 0, 0), (65, 1, 1)])
 def test_eviction_budgets(device, budget, sinks, recent):
     cut(device, BF, (2, 64), [1, 9, 10, 11, 66, 200], budget, sinks, recent)
 

@@ -45,6 +45,21 @@ def test_bounds(device, dtype, heads, block_size):
         assert torch.equal(got.cpu(), bounds_of(k, tables, lens, starts, block_size, before))
 
 
+@pytest.mark.parametrize("most", [5, 1 << 40, 1 << 70])
+def test_bounds_of_a_range_said_to_be_long(device, most):
+    """max_new past what the tables cover, or past 64 bits, is all that they cover; without
+    starts it says nothing."""
+    lens, starts = [70, 33], [68, 28]
+    k, v, tables = so.pool(lens, 16, 2, 64, BF, 0)
+    before = torch.zeros(k.shape[0], 2, 2, 64, dtype=BF)
+    for first in (starts, None):
+        got = before.to(device)
+        update_key_bounds(k.to(device), got, tables.to(device), torch.tensor(lens).to(device), 16,
+                          starts=None if first is None else torch.tensor(first).to(device),
+                          max_new=most if first else 0)
+        assert torch.equal(got.cpu(), bounds_of(k, tables, lens, first, 16, before.clone()))
+
+
 @pytest.mark.parametrize("dtype", [BF, FP, F32])
 def test_bounds_of_odd_values(device, dtype):
     """A NaN stays, infinities bound, and what lies behind the last key is not read."""

@@ -231,7 +231,8 @@ def test_bad_blocks_are_masked(device, dtype):
     so.assert_within(got, want, bound)
 
 
-@pytest.mark.parametrize("counts", [[1], [5, 0, 64, 1], [65, 130, 300], [5000]])
+@pytest.mark.parametrize("counts", [[1], [5, 0, 64, 1], [65, 130, 300], [4096],
+                                    [700, 4000]])
 def test_ancestors(device, counts):
     rng = random.Random(sum(counts))
     parents = [so.random_parents(n, rng) for n in counts]
@@ -240,6 +241,21 @@ def test_ancestors(device, counts):
                          packed(parents).to(device), max(counts))
     want = torch.cat([bits_of(so.paths(p), words) for p in parents if p])
     assert torch.equal(got.cpu(), want)
+
+
+def test_ancestors_of_long_chains(device):
+    """Chains and circles of the most tokens that a tree may have, and of more: those past
+    it are no nodes and have no row."""
+    chain, circle = list(range(-1, 4095)), list(range(1, 4096)) + [0]
+    more = list(range(-1, 4999))
+    qsl = torch.tensor([0, 4096, 8192, 13192, 13195])
+    out = torch.full((13195, 64), 5, device=device)
+    got = tree_ancestors(torch.tensor(chain + circle + more + [-1, 0, 0]).to(device),
+                         qsl.to(device), 4096, out=out).cpu()
+    want = bits_of([range(i + 1) for i in range(4096)], 64)
+    assert torch.equal(got[:4096], want) and (got[4096:8192] == -1).all()
+    assert torch.equal(got[8192:8192 + 4096], want) and (got[8192 + 4096:13192] == 5).all()
+    assert torch.equal(got[13192:], bits_of([[0], [0, 1], [0, 2]], 64))
 
 
 def test_ancestors_of_odd_parents(device):

@@ -64,6 +64,7 @@ def test_attention_calls(change, error, needle):
     (torch.zeros(2, 2, dtype=torch.long), 4, ValueError, "parents"),
     (torch.zeros(2, dtype=torch.long), 0, ValueError, "max_nodes"),
     (torch.zeros(2, dtype=torch.long), -64, ValueError, "max_nodes"),
+    (torch.zeros(2, dtype=torch.long), 4097, ValueError, "max_nodes"),
     (torch.zeros(2, dtype=torch.long), 4, RuntimeError, "HIP devices")])
 def test_tree_ancestors(parents, max_nodes, error, needle):
     with pytest.raises(error, match=needle):
@@ -296,7 +297,7 @@ def test_ancestors_abi():
         return lib.mlr_tree_ancestors(*a.values())
 
     for change in (dict(parents=None), dict(qsl=None), dict(out=None), dict(seqs=-1),
-                   dict(seqs=1 << 24), dict(total=-1), dict(words=0)):
+                   dict(seqs=1 << 24), dict(total=-1), dict(words=0), dict(words=65)):
         assert ancestors(**change) == 1 and b"mlr_tree_ancestors" in lib.mlr_last_error(), change
     assert ancestors(seqs=0) == 0 and ancestors(total=0) == 0
 
