@@ -9,7 +9,8 @@
 // or so few that each is compared with all. 2,048 bins of equal width: mostly one
 // histogram is enough for a few thousand keys, as scores and weights lie close together.
 // Integers alone, so the order of the atomics does not matter. A wave holds a run of
-// neighbouring places, so the chosen are counted wave by wave and written in order.
+// neighbouring places, so the chosen are counted wave by wave and written in order. (4,096 and
+// 8,192 bins, which leave fewer keys in the last, took as long: 16,384 keys 20 us each.)
 #pragma once
 
 #include "mlr_common.h"
@@ -107,6 +108,16 @@ struct Places {
   }
 };
 
+// A value that all lanes share, in scalar registers: what depends on it branches once a wave.
+__device__ __forceinline__ int uniform(int x) { return __builtin_amdgcn_readfirstlane(x); }
+__device__ __forceinline__ uint32_t uniform(uint32_t x) {
+  return __builtin_amdgcn_readfirstlane(x);
+}
+__device__ __forceinline__ uint64_t uniform(uint64_t x) {
+  const uint32_t low = uniform(static_cast<uint32_t>(x));
+  return static_cast<uint64_t>(uniform(static_cast<uint32_t>(x >> 32))) << 32 | low;
+}
+
 // The `left`-th best, left > 0, of the places in [lo, hi), which are at least so many: the
 // largest key first, ties by the lower place. All threads of the workgroup call it.
 template <typename Key, int kThreads, class P>
@@ -142,7 +153,8 @@ __device__ __forceinline__ void find_last(SelectShared &s, P &places, int left, 
     least = static_cast<Key>(s.low[w]) < least ? static_cast<Key>(s.low[w]) : least;
     most = static_cast<Key>(s.high[w]) > most ? static_cast<Key>(s.high[w]) : most;
   }
-  Key base = least + 1, span = most - base;
+  most = uniform(most);
+  Key base = uniform(static_cast<Key>(least + 1)), span = most - base;
   int bits = span > 0 ? 64 - __clzll(static_cast<uint64_t>(span)) : 0;
   uint32_t place_base = 0;
   int place_bits = 32 - __clz(n);
@@ -150,22 +162,27 @@ __device__ __forceinline__ void find_last(SelectShared &s, P &places, int left, 
     return static_cast<uint32_t>(n - 1 - i);
   };
   // A key of 0 is further from base than the largest.
-  auto asked = [&](int i, Key k) __attribute__((always_inline)) {
-    return k - base <= span &&
-           (bits > 0 || (from_end(i) >= place_base && (from_end(i) - place_base) >> place_bits == 0));
+  auto in_span = [&](Key k) __attribute__((always_inline)) { return k - base <= span; };
+  auto in_places = [&](int i, Key k) __attribute__((always_inline)) {
+    return k == base && from_end(i) >= place_base && (from_end(i) - place_base) >> place_bits == 0;
   };
   for (;;) {
     const bool by_key = bits > 0;
     const int shift = max((by_key ? bits : place_bits) - kBinBits, 0);
-    auto bin_of = [&](int i, Key k) __attribute__((always_inline)) {
-      return by_key ? static_cast<int>((k - base) >> shift)
-                    : static_cast<int>((from_end(i) - place_base) >> shift);
-    };
-    places.each([&](int i, const Key(&k)[4]) __attribute__((always_inline)) {
+    if (by_key) {
+      places.each([&](int, const Key(&k)[4]) __attribute__((always_inline)) {
 #pragma unroll
-      for (int e = 0; e < 4; ++e)
-        if (asked(i + e, k[e])) atomicAdd(&s.hist[bin_of(i + e, k[e])], 1);
-    });
+        for (int e = 0; e < 4; ++e)
+          if (in_span(k[e])) atomicAdd(&s.hist[static_cast<int>((k[e] - base) >> shift)], 1);
+      });
+    } else {
+      places.each([&](int i, const Key(&k)[4]) __attribute__((always_inline)) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          if (in_places(i + e, k[e]))
+            atomicAdd(&s.hist[static_cast<int>((from_end(i + e) - place_base) >> shift)], 1);
+      });
+    }
     __syncthreads();
     // Thread t has the bins kBins - 1 - kOwn t and those below.
     constexpr int kOwn = kBins / kThreads;
@@ -195,14 +212,14 @@ __device__ __forceinline__ void find_last(SelectShared &s, P &places, int left, 
       }
     }
     __syncthreads();
-    const int count = s.hist[s.bin];
-    left = s.left;
+    const int bin = uniform(s.bin), count = uniform(s.hist[bin]);
+    left = uniform(s.left);
     if (by_key) {
-      base += static_cast<Key>(s.bin) << shift;
+      base += static_cast<Key>(bin) << shift;
       bits = shift;
       span = min(static_cast<Key>((Key(1) << shift) - 1), static_cast<Key>(most - base));
     } else {
-      place_base += static_cast<uint32_t>(s.bin) << shift;
+      place_base += static_cast<uint32_t>(bin) << shift;
       place_bits = shift;
     }
     if (count == left) {  // all of them
@@ -211,10 +228,11 @@ __device__ __forceinline__ void find_last(SelectShared &s, P &places, int left, 
       break;
     }
     if (count <= kFew) {
+      const bool whole = bits > 0;  // places do not matter yet
       places.each([&](int i, const Key(&k)[4]) __attribute__((always_inline)) {
 #pragma unroll
         for (int e = 0; e < 4; ++e)
-          if (asked(i + e, k[e])) {
+          if (whole ? in_span(k[e]) : in_places(i + e, k[e])) {
             const int at = atomicAdd(&s.count, 1);
             s.few_key[at] = k[e];
             s.few_place[at] = i + e;
