@@ -450,28 +450,49 @@ __global__ __launch_bounds__(kThreads) void choose_blocks(SparseParams p) {
 }
 
 // The same for tables of few blocks, with their scores: one launch. Eight waves with a tile
-// each; past that the scores of one request keep one CU too long. us of one launch and of
-// two, 16 requests, 4 KV heads of 128, by blocks: 64 13.7 and 15.8, 128 16.7 and 14.6, 256
-// 24.2 and 16.8; the second launch itself costs about 2 us more.
+// each; past that the scores of one request keep one CU too long. So few blocks need no
+// histogram: each is compared with all. us of one launch and of two, 16 requests, 4 KV heads
+// of 128, by blocks: 64 10.4 and 15.8, 128 14.0 and 15.1, 256 (sixteen waves) 36.6 and 15.8.
 constexpr int kSmall = 128, kSmallThreads = 512;
 template <typename T, int kT>
 __global__ __launch_bounds__(kSmallThreads) void choose_small(SparseParams p) {
-  __shared__ SelectShared s;
-  __shared__ __align__(16) uint64_t s_keys[kSmall];
+  static_assert(kSmallThreads == 4 * kSmall, "a tile a wave, four threads a block");
+  __shared__ uint64_t s_keys[kSmall];
+  __shared__ int s_count[kSmallThreads / 64];
   const Pair<T, kT> x(p, blockIdx.x % p.seqs, blockIdx.x / p.seqs);
-  const int n = static_cast<int>(x.n);
+  const int n = static_cast<int>(x.n), lane = threadIdx.x & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const Chosen out(p, x.seq, x.kvh);
+  const int i = threadIdx.x / 4;
+  bool chosen = i < n && threadIdx.x % 4 == 0;
   if (n > p.budget) {  // uniform
-    for (int at = 16 * static_cast<int>(threadIdx.x >> 6); at < n; at += kSmallThreads / 4) {
-      const int j = at + x.col;
+    const int j = 16 * wave + x.col;
+    if (16 * wave < n) {
       const double best = x.score(j < n ? x.table[j] : -1);
       if (x.g == 0) s_keys[j] = order_key(best);
     }
     __syncthreads();
+    // A block is compared with all that are asked, by four threads.
+    const int lo = p.sinks, hi = n - p.recent;
+    const uint64_t key = s_keys[min(i, n - 1)];
+    int better = 0;
+#pragma unroll 8
+    for (int o = lo + threadIdx.x % 4; o < hi; o += 4) {
+      const uint64_t other = s_keys[o];
+      better += other > key || (other == key && o < i);
+    }
+    better += __shfl_xor(better, 1);
+    better += __shfl_xor(better, 2);
+    chosen = chosen && (i < lo || i >= hi || better < p.budget - p.sinks - p.recent);
   }
-  const int count = select_places<uint64_t, kSmallThreads, 1>(
-      s, n, p.sinks, p.recent, p.budget, keys_from(s_keys, n), out);
-  out.finish(p, x.seq, x.kvh, count, kSmallThreads);
+  const uint64_t all = __ballot(chosen);
+  if (lane == 0) s_count[wave] = __popcll(all);
+  __syncthreads();
+  int r = __popcll(all & ((uint64_t(1) << lane) - 1));
+#pragma unroll
+  for (int w = 0; w < kSmallThreads / 64; ++w) r += w < wave ? s_count[w] : 0;
+  if (chosen) out(r, i, -1);
+  out.finish(p, x.seq, x.kvh, min(n, p.budget), kSmallThreads);
 }
 
 // The choice from scores in 32 bits and how far off they may be. With T the last chosen of
