@@ -33,13 +33,14 @@ def _check_weights(key_weights: torch.Tensor, k_cache: torch.Tensor) -> None:
 
 def _check_cache(k_cache, v_cache, block_size, what, *more) -> torch.device:
     _check_cache_pair(k_cache, v_cache)
-    if block_size != k_cache.shape[1]:
+    _, cache_block, _, head_dim = k_cache.shape
+    if block_size != cache_block:
         raise ValueError("block_size does not match KV cache layout")
-    if k_cache.dtype not in _DTYPES:
-        raise TypeError(f"{what}: unsupported dtype {k_cache.dtype}")
-    if v_cache.dtype != k_cache.dtype:
+    dtype = k_cache.dtype
+    if dtype not in _DTYPES:
+        raise TypeError(f"{what}: unsupported dtype {dtype}")
+    if v_cache.dtype != dtype:
         raise TypeError(f"{what}: k_cache and v_cache must share one dtype")
-    head_dim = k_cache.shape[3]
     if head_dim * k_cache.element_size() % 16 or not 0 < head_dim <= 1024:
         raise ValueError(f"{what} takes head_dim in multiples of 16 bytes, up to 1024 elements")
     if not (k_cache.is_contiguous() and v_cache.is_contiguous()):

@@ -32,6 +32,9 @@ _DEFAULT_TILE = 64
 
 def _as_index_tensor(values, device: torch.device) -> torch.Tensor:
     if isinstance(values, torch.Tensor):
+        # to() would return the same tensor, but takes 0.2 us longer to find that out.
+        if values.dtype is torch.long and values.device == device:
+            return values
         tensor = values.to(device=device, dtype=torch.long)
     else:
         tensor = torch.as_tensor(list(values), dtype=torch.long, device=device)

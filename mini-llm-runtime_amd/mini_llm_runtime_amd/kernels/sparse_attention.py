@@ -50,11 +50,11 @@ def update_key_bounds(
     what = "update_key_bounds"
     if k_cache.ndim != 4:
         raise ValueError("k_cache must have shape [num_blocks, block_size, Hkv, D]")
-    if block_size != k_cache.shape[1]:
+    num_blocks, cache_block, num_kv_heads, head_dim = k_cache.shape
+    if block_size != cache_block:
         raise ValueError("block_size does not match KV cache layout")
     if k_cache.dtype not in (torch.bfloat16, torch.float16, torch.float32):
         raise TypeError(f"{what}: unsupported dtype {k_cache.dtype}")
-    num_blocks, _, num_kv_heads, head_dim = k_cache.shape
     if head_dim * k_cache.element_size() % 16 or not 0 < head_dim <= 1024:
         raise ValueError(f"{what} takes head_dim in multiples of 16 bytes, up to 1024 elements")
     if not k_cache.is_contiguous():
