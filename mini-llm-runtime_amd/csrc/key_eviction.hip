@@ -135,7 +135,8 @@ __device__ __forceinline__ void weigh_keys(const ScoredParams &p, float *weights
         s_ml[h][1] = l > 0.f ? 1.f / l : l == 0.f ? 0.f : l;
       }
     }
-    // One wave's own rows of LDS: in order without a barrier.
+    // One wave's own part of LDS, here and below: in order without a barrier.
+    asm volatile("" ::: "memory");
     auto add = [&](const float4 &v, int h) __attribute__((always_inline)) {
       const float m = s_ml[h][0], inv = s_ml[h][1];
       w[0] += __builtin_amdgcn_exp2f((v.x - m) * kLog2e) * inv;
@@ -154,6 +155,7 @@ __device__ __forceinline__ void weigh_keys(const ScoredParams &p, float *weights
       add(*reinterpret_cast<const float4 *>(row + (h0 + h) * p.scores_st), h);
   }
   *reinterpret_cast<float4 *>(s_w + 4 * lane) = make_float4(w[0], w[1], w[2], w[3]);
+  asm volatile("" ::: "memory");
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
     const int64_t at = base + 64 * i + lane;
