@@ -498,8 +498,8 @@ __global__ __launch_bounds__(kSmallThreads) void choose_small(SparseParams p) {
 // The choice from scores in 32 bits and how far off they may be. With T the last chosen of
 // them and R the largest error, a block below T - 2 R is worse than all down to T, and one
 // above T + 2 R is better than all from T on; those in between are scored in 64 bits. Where
-// they are more than kFew, all blocks are. Bound by latency, a dozen steps of 1 us, 17 us for
-// 32 lists of 2,048 blocks: what a later step needs of memory (block ids, q) is read with the
+// they are more than kFew, all blocks are. Bound by latency, a dozen steps of 1 us, 16.5 us
+// for 32 lists of 2,048 blocks: what a later step needs of memory (block ids, q) is read with the
 // scores.
 constexpr int kRoughThreads = 512, kRoughHeld = 2;
 constexpr int kRoughBlocks = 4 * kRoughThreads * kRoughHeld;  // at most, as they stay in registers
