@@ -726,8 +726,9 @@ int mlr_sample_tokens(const void *logits, int64_t row_stride, int64_t num_logit_
  * bf16, fp16 and FP32, any block_size, fewer than 2^31 positions per table and 16-byte
  * aligned operands and row starts; the attention calls are over the operands of
  * mlr_paged_decode_scored and mlr_paged_prefill_scored (head_dim, softcap, lengths of 0,
- * block ids out of range, workspaces and roundings as there). No counterpart in the
- * reference.
+ * block ids out of range and workspaces as there). Scores, statistics and sums are FP32; a
+ * probability meets V to 2^-15 of itself in bf16 and 2^-21 in fp16, and the result is
+ * rounded once. No counterpart in the reference.
  *
  * mlr_tree_ancestors: parents [total_q] holds for each token of sequence s, at the rows
  * [query_start_loc[s], query_start_loc[s+1]), the place of its parent among them (out of

@@ -49,6 +49,8 @@ struct ScoredParams {
   int words;               // `words` words a row (null: causal)
   float *scores;           // kModeDecode: where to leave the scores (null: nowhere),
   int64_t scores_st;       // [seqs * hq][scores_st]
+  bool fine;               // kModeDecode: probabilities in two parts (two_parts); trees and
+                           // decodes that leave their scores always have them so
   void *out;
   int64_t o_st, o_sh;
   int mode, units;
@@ -80,6 +82,35 @@ __device__ __forceinline__ const int64_t *table_of(const ScoredParams &p, const 
 __device__ __forceinline__ bool bit_of(const ScoredParams &p, int64_t row, int node) {
   const int word = node >> 6;
   return word < p.words && (static_cast<uint64_t>(p.bits[row * p.words + word]) >> (node & 63) & 1);
+}
+
+// Two probabilities a and b as operands of 16 bits, hi + lo each, which a product with V adds
+// up in FP32: hi is cut off, not rounded, and lo is more than 0 wherever hi is, so that an
+// infinite V stays one (hi times it and lo times it have one sign, and 0 times it is met only
+// where the probability is 0). lo, up to 2^-7 of it in bf16 and 2^-10 in fp16, is rounded by
+// 2^-8 and 2^-11 of itself: 2^-15 and 2^-21 of the probability. fp16 takes numbers scaled up to
+// 2^15, of which it drops 2^-24 at most, 2^-39 of the largest.
+template <typename T>
+__device__ __forceinline__ void two_parts(float a, float b, uint32_t &hi, uint32_t &lo) {
+  typedef float f32x2_v __attribute__((ext_vector_type(2)));
+  if constexpr (std::is_same_v<T, bf16_t>) {
+    typedef __bf16 h2 __attribute__((ext_vector_type(2)));
+    const uint32_t ua = __float_as_uint(a), ub = __float_as_uint(b);
+    constexpr float kMore = 1.f + 0x1p-23f;
+    hi = __builtin_amdgcn_perm(ub, ua, 0x07060302);
+    lo = __builtin_bit_cast(
+        uint32_t, __builtin_convertvector(
+                      f32x2_v{fmaf(a, kMore, -__uint_as_float(ua & 0xffff0000u)),
+                              fmaf(b, kMore, -__uint_as_float(ub & 0xffff0000u))}, h2));
+  } else {
+    typedef _Float16 h2 __attribute__((ext_vector_type(2)));
+    const h2 cut = __builtin_bit_cast(h2, __builtin_amdgcn_cvt_pkrtz(a, b));
+    hi = __builtin_bit_cast(uint32_t, cut);
+    const float la = a - static_cast<float>(cut[0]), lb = b - static_cast<float>(cut[1]);
+    lo = __builtin_bit_cast(
+        uint32_t, __builtin_convertvector(f32x2_v{fmaxf(la, fminf(a, 0x1p-24f)),
+                                                  fmaxf(lb, fminf(b, 0x1p-24f))}, h2));
+  }
 }
 
 __device__ __forceinline__ int64_t clamp64(int64_t x, int64_t lo, int64_t hi) {

@@ -15,13 +15,15 @@
 //   O^T[D x 16 rows] += V^T P^T with P^T straight from the S^T registers: the
 //     k index of operand B is the key 4 (l / 16) + i. V as operand A: a lane
 //     holds D / 16 neighbouring elements of rows 4 (l / 16) + i.
-// 16-bit types round P to their type as operand (by at most 2^-8 of it in bf16, 2^-11
-// in fp16), at every head size: the matrix instructions take it in no other type. It
-// makes the error against 64 bits 1.4 times that of the one rounding of the result
-// (bf16 0.0023 and 0.0017 of the outputs' size). Scores, statistics and sums are FP32,
-// and the result is rounded once.
+// In 16-bit types P is an operand of their type. Chunks, plain decodes and shared prefixes
+// round it (by at most 2^-8 of it in bf16, 2^-11 in fp16), at every head size, which makes
+// the error against 64 bits 1.4 times that of the one rounding of the result (bf16 0.0023
+// and 0.0017 of the outputs' size). Drafted trees, weighing and sparse decodes hold it in
+// two parts (two_parts below), to 2^-15 and 2^-21 of it: the instruction with twice as many
+// keys takes both in the time of one. Scores, statistics and sums are FP32, and the result
+// is rounded once.
 // Drafted tokens see the keys before them and those that their bits name; a decode
-// that weighs its keys leaves the scores in the workspace (64 requests as below: 21 us).
+// that weighs its keys leaves the scores in the workspace (64 requests as below: 22 us).
 // The waves' results are joined through LDS. Splits of one unit leave (m, l, O)
 // in the workspace, added up by scored_merge in the next launch.
 //
@@ -53,6 +55,9 @@ template <> struct Mma16<bf16_t> {
     return __builtin_amdgcn_mfma_f32_16x16x16bf16_1k(__builtin_bit_cast(s16x4_t, v),
                                                      __builtin_bit_cast(s16x4_t, p), c, 0, 0, 0);
   }
+  __device__ static f32x4_t pv2(uint2 v, uint4 p, f32x4_t c) {
+    return qk(make_uint4(v.x, v.y, v.x, v.y), p, c);
+  }
 };
 template <> struct Mma16<f16_t> {
   using v8 = f16x8_t;
@@ -63,6 +68,9 @@ template <> struct Mma16<f16_t> {
   __device__ static f32x4_t pv(uint2 v, uint2 p, f32x4_t c) {
     return __builtin_amdgcn_mfma_f32_16x16x16f16(__builtin_bit_cast(f16x4_t, v),
                                                  __builtin_bit_cast(f16x4_t, p), c, 0, 0, 0);
+  }
+  __device__ static f32x4_t pv2(uint2 v, uint4 p, f32x4_t c) {
+    return qk(make_uint4(v.x, v.y, v.x, v.y), p, c);
   }
 };
 
@@ -219,13 +227,17 @@ __device__ __forceinline__ void cap_scores(float (&x)[4], float cap, float inv_c
 // kPrefill: the rows are tokens of chunks, not requests. kUnlike: rows of a unit may
 // see different keys (chunks, and requests shorter than the prefix that they share).
 // kTree: of its sequence's last tokens a row sees those that its bits name. kKeep: the
-// scores stay for a pass that weighs the keys. Both must not cost a D of 64 one of the three
+// scores stay for a pass that weighs the keys. kFine: probabilities in two parts, which
+// these two always have. None of them must cost a D of 64 one of the three
 // workgroups of a CU that rows_target counts on: with a few registers too many, 16 FP32
 // trees of 3 to 5 tokens after 500 to 4,000 keys took 42 us, not 32.
 template <typename T, int D, bool kCap, bool kPaged16, bool kPrefill, bool kUnlike, bool kTree,
-          bool kKeep>
-__global__ __launch_bounds__(256, (kTree || kKeep) && D <= 64 ? 3 : 1) void scored_rows_kernel(
+          bool kKeep, bool kFine>
+__global__ __launch_bounds__(256, kFine && D <= 64 ? 3 : 1) void scored_rows_kernel(
     ScoredParams p) {
+  static_assert(kFine || !(kTree || kKeep), "these are in two parts");
+  // What an fp16 probability, at most 1, is scaled by in two parts.
+  constexpr float kUp = kFine && std::is_same_v<T, f16_t> ? 32768.f : 1.f;
   constexpr int kVe = D / 16;  // elements of a row that a lane of P V holds
   constexpr int kE = 16 / sizeof(T);
   constexpr int kBatch = D * sizeof(T) <= 128 ? 4 : D * sizeof(T) <= 256 ? 2 : 1;
@@ -425,6 +437,7 @@ __global__ __launch_bounds__(256, (kTree || kKeep) && D <= 64 ? 3 : 1) void scor
         for (int i = 0; i < 4; ++i) {
           pr[i] = __builtin_amdgcn_exp2f((x[b][i] - ref) * kLog2e);
           l += pr[i];
+          pr[i] *= kUp;
         }
         bool plain = true;
         if (kUnlike && __builtin_expect(__any(own_end < min(b0 + b * step + 16, k1)), 0)) {
@@ -444,6 +457,11 @@ __global__ __launch_bounds__(256, (kTree || kKeep) && D <= 64 ? 3 : 1) void scor
           plain = __builtin_amdgcn_ballot_w64(bad) == 0;
         }
         if (__builtin_expect(plain, 1)) {
+          uint4 parts = make_uint4(0, 0, 0, 0);  // (hi, hi, lo, lo) of the four keys
+          if constexpr (kFine && sizeof(T) == 2) {
+            two_parts<T>(pr[0], pr[1], parts.x, parts.z);
+            two_parts<T>(pr[2], pr[3], parts.y, parts.w);
+          }
 #pragma unroll
           for (int n = 0; n < kVe; ++n) {
             if constexpr (sizeof(T) == 2) {
@@ -456,9 +474,13 @@ __global__ __launch_bounds__(256, (kTree || kKeep) && D <= 64 ? 3 : 1) void scor
                 w01 = __builtin_amdgcn_perm(tile[b].v[1][n / 2], tile[b].v[0][n / 2], 0x05040100);
                 w23 = __builtin_amdgcn_perm(tile[b].v[3][n / 2], tile[b].v[2][n / 2], 0x05040100);
               }
-              acc[n] = Mma16<T>::pv(make_uint2(w01, w23),
-                                    make_uint2(pack2<T>(pr[0], pr[1]), pack2<T>(pr[2], pr[3])),
-                                    acc[n]);
+              if constexpr (kFine) {
+                acc[n] = Mma16<T>::pv2(make_uint2(w01, w23), parts, acc[n]);
+              } else {
+                acc[n] = Mma16<T>::pv(make_uint2(w01, w23),
+                                      make_uint2(pack2<T>(pr[0], pr[1]), pack2<T>(pr[2], pr[3])),
+                                      acc[n]);
+              }
             } else {
 #pragma unroll
               for (int i = 0; i < 4; ++i)
@@ -493,6 +515,10 @@ __global__ __launch_bounds__(256, (kTree || kKeep) && D <= 64 ? 3 : 1) void scor
       }
     }
     l = sum_groups(l);
+    if constexpr (kUp != 1.f) {
+#pragma unroll
+      for (int n = 0; n < kVe; ++n) acc[n] *= 1.f / kUp;
+    }
 
     // Join the waves. acc[n][e] is element kVe (4 g + e) + n of row m16.
     if (g == 0) {
@@ -547,14 +573,15 @@ __global__ __launch_bounds__(256, (kTree || kKeep) && D <= 64 ? 3 : 1) void scor
 template <typename T, int D>
 int launch_rows(const ScoredParams &p, unsigned grid, hipStream_t stream) {
   const bool paged16 = p.block_size % 16 == 0;
-#define MLR_ROWS(C, B, F, U, R, K) \
-  scored_rows_kernel<T, D, C, B, F, U, R, K><<<grid, 256, 0, stream>>>(p)
+#define MLR_ROWS(C, B, F, U, R, K, E) \
+  scored_rows_kernel<T, D, C, B, F, U, R, K, E><<<grid, 256, 0, stream>>>(p)
 #define MLR_ROWS_B(C, B)                                                             \
-  if (p.mode == kModePrefill && p.bits) MLR_ROWS(C, B, true, true, true, false);     \
-  else if (p.mode == kModePrefill) MLR_ROWS(C, B, true, true, false, false);         \
-  else if (p.mode == kModePrefix) MLR_ROWS(C, B, false, true, false, false);         \
-  else if (p.scores) MLR_ROWS(C, B, false, false, false, true);                      \
-  else MLR_ROWS(C, B, false, false, false, false);
+  if (p.mode == kModePrefill && p.bits) MLR_ROWS(C, B, true, true, true, false, true);     \
+  else if (p.mode == kModePrefill) MLR_ROWS(C, B, true, true, false, false, false);        \
+  else if (p.mode == kModePrefix) MLR_ROWS(C, B, false, true, false, false, false);        \
+  else if (p.scores) MLR_ROWS(C, B, false, false, false, true, true);                      \
+  else if (p.fine && sizeof(T) == 2) MLR_ROWS(C, B, false, false, false, false, sizeof(T) == 2); \
+  else MLR_ROWS(C, B, false, false, false, false, false);
   if (p.cap > 0) {
     if (paged16) { MLR_ROWS_B(true, true) } else { MLR_ROWS_B(true, false) }
   } else {

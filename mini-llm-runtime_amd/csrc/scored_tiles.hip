@@ -16,9 +16,12 @@
 //   scores in base 2, relative to the row's reference point m, which follows
 //     the running maximum only when a tile exceeds it by 2^kLazy: probabilities
 //     stay below 2^kLazy, numerator and sum share m, and most tiles rescale nothing.
+//     (Trees in fp16: m lies kBelow below that maximum, so that the parts of a
+//     probability use the type's range, up to 2^15.)
 //   O^T[D x 32 rows] += V^T P^T: B = P^T straight from the S^T registers, rounded
 //     to the 16-bit type (by at most 2^-8 of it in bf16, 2^-11 in fp16; see
-//     scored_rows.hip), A = V^T by transposing LDS reads.
+//     scored_rows.hip), for trees in two parts, a product each (two_parts); A = V^T
+//     by transposing LDS reads.
 //
 // Tiles are taken from the last to the first, as a bias by distance makes the last
 // keys the heaviest, and the two key halves run their vector and matrix phases in
@@ -38,8 +41,9 @@
 //
 // Trees of drafted tokens are chunks of which a row sees the keys before them and
 // those of its bits: tiles that reach past those keys are masked bit by bit. 16 trees
-// of 20 to 48 tokens after 512 to 4,096 keys, 28/4 heads of 128: 24 GF in 61 us, bound by
-// the LDS reads of a tile, 32 rows a wave for each.
+// of 20 to 48 tokens after 512 to 4,096 keys, 28/4 heads of 128: 24 GF, and 12 more for
+// the second parts of the probabilities, in 71 us (60 with one part, whose rounding is
+// 2^-8); at 14/2 heads of 64 33 us (28).
 //
 // LDS rows are unpadded; the 16-byte chunk c of row r lies at c ^ swizzle(r),
 // which keeps the row reads of K and the transposing reads of V free of bank
@@ -137,6 +141,7 @@ void scored_tiles_kernel(ScoredParams p) {
   constexpr int kRowB = 2 * D, kChunks = D / 8;
   constexpr int kCopies = 16 * kRowB / 1024;  // 1 KB copies of a wave's 16 rows
   constexpr int kTileB = kTile * kRowB;
+  constexpr float kBelow = kTree && std::is_same_v<T, f16_t> ? 7.f : 0.f;
   // Each stage is an object of its own, so that the compiler does not make reads
   // of one wait for copies into another.
   __shared__ __align__(1024) unsigned char ks0[kHalves][kTileB], ks1[kHalves][kTileB];
@@ -541,7 +546,7 @@ void scored_tiles_kernel(ScoredParams p) {
   //        then scores and probabilities of tile i, packed for M_{i+1}
   // A wave waits for its own copies of the phase before, the barrier for all.
   f32x16_t s[KB];
-  uint32_t pk[KB][8];
+  uint32_t pk[KB][8], pl[KB][kTree ? 8 : 1];  // pl: the second parts
   auto active = [&](int i) __attribute__((always_inline)) {
     const int key0 = key_of(i);
     return key0 >= first_key && key0 < any;
@@ -561,18 +566,23 @@ void scored_tiles_kernel(ScoredParams p) {
         const uint2 hi = __builtin_bit_cast(
             uint2, __builtin_amdgcn_ds_read_tr16_b64_v4i16(
                        (lds_s16x4_t *)(vt + 16 * kb * kRowB + ((vo ^ 16 ^ (n << 6)) + 8 * kRowB))));
-        acc[n] = W::mfma(__builtin_bit_cast(v8, make_uint4(lo.x, lo.y, hi.x, hi.y)), pb, acc[n]);
+        const v8 va = __builtin_bit_cast(v8, make_uint4(lo.x, lo.y, hi.x, hi.y));
+        acc[n] = W::mfma(va, pb, acc[n]);
+        if constexpr (kTree) {
+          const uint32_t *y = &pl[kb >> 1][4 * (kb & 1)];
+          acc[n] = W::mfma(va, __builtin_bit_cast(v8, make_uint4(y[0], y[1], y[2], y[3])), acc[n]);
+        }
       }
     }
-    // Two MFMAs' V reads ahead of the MFMAs.
-    constexpr int kMfma = 2 * KB * NB;
+    // Two fragments' V reads ahead of the MFMAs.
+    constexpr int kFragments = 2 * KB * NB, kEach = kTree ? 2 : 1;
     __builtin_amdgcn_sched_group_barrier(0x100, 4, 0);
 #pragma unroll
-    for (int x = 0; x < kMfma - 2; ++x) {
-      __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+    for (int x = 0; x < kFragments - 2; ++x) {
+      __builtin_amdgcn_sched_group_barrier(0x008, kEach, 0);
       __builtin_amdgcn_sched_group_barrier(0x100, 2, 0);
     }
-    __builtin_amdgcn_sched_group_barrier(0x008, 2, 0);
+    __builtin_amdgcn_sched_group_barrier(0x008, 2 * kEach, 0);
   };
   // Where some row does not see some key, a V that is not finite would reach
   // it as 0 * V. So in such tiles each wave looks through the 16 rows that it has
@@ -745,13 +755,13 @@ void scored_tiles_kernel(ScoredParams p) {
       // Rows below their threshold keep m: a factor of 1. A row without a key so
       // far has sums of 0, whatever the factor.
       const bool move = rel > thr;
-      const float shift = move ? rel : 0.f;
+      const float shift = move ? rel - kBelow : 0.f;
       const float fall = move && thr > 0.f ? __builtin_amdgcn_exp2f(-shift) : 1.f;
       l *= fall;
 #pragma unroll
       for (int n = 0; n < NB; ++n) acc[n] *= fall;
       m += shift;
-      if (move) thr = kLazy;
+      if (move) thr = kLazy + kBelow;
 #pragma unroll
       for (int j = 0; j < KB; ++j)
 #pragma unroll
@@ -770,7 +780,10 @@ void scored_tiles_kernel(ScoredParams p) {
 #pragma unroll
     for (int j = 0; j < KB; ++j)
 #pragma unroll
-      for (int x = 0; x < 8; ++x) pk[j][x] = pack2<T>(s[j][2 * x], s[j][2 * x + 1]);
+      for (int x = 0; x < 8; ++x) {
+        if constexpr (kTree) two_parts<T>(s[j][2 * x], s[j][2 * x + 1], pk[j][x], pl[j][x]);
+        else pk[j][x] = pack2<T>(s[j][2 * x], s[j][2 * x + 1]);
+      }
   };
   // s_waitcnt: all but the newest batch of copies, and LDS; LDS and scalars alone.
   constexpr int kBatch = 2 * kCopies;
@@ -811,7 +824,10 @@ void scored_tiles_kernel(ScoredParams p) {
 #pragma unroll
       for (int j = 0; j < KB; ++j)
 #pragma unroll
-        for (int x = 0; x < 8; ++x) asm volatile("" : "=v"(pk[j][x]));
+        for (int x = 0; x < 8; ++x) {
+          asm volatile("" : "=v"(pk[j][x]));
+          if constexpr (kTree) asm volatile("" : "=v"(pl[j][x]));
+        }
     }
     asm volatile("" ::: "memory");
     __builtin_amdgcn_s_waitcnt(kWaitBatch);

@@ -838,6 +838,7 @@ extern "C" int mlr_paged_decode_sparse(
   if (rc) return rc;
   ScoredParams p = params_of(o, kModeDecode);
   p.bt_sh = need ? list : 0;
+  p.fine = true;
   p.whole = short_keys(max_keys, head_dim, dtype);
   const bool parts = !p.whole;
   const int64_t items = plan_decode(p, max_keys, parts ? ws : nullptr);

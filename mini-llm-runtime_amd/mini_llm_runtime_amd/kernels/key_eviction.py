@@ -9,7 +9,8 @@ of drafted tokens, or a choice of the caller's own.
 
 The sums are FP32, laid out like the cache with positions last: key_weights
 [num_blocks, Hkv, block_size]. A step sets its newest key's entry; the entries of a
-prompt's keys, which no step has set, are the caller's to clear.
+prompt's keys, which no step has set, are the caller's to clear. The decode's numbers are
+those of ``tree_attention``: FP32 sums, one rounding of the result.
 """
 
 from __future__ import annotations

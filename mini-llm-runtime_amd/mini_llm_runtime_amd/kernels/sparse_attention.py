@@ -6,7 +6,8 @@ calls of ``paged_attention``, with the same caches and tables.
 of its keys: key_bounds [num_blocks, 2, Hkv, D], in the cache's type.
 ``paged_attention_decode_sparse`` scores each block by the largest q.k that keys within
 its bounds could have and attends to the keys of the best blocks: of a long context
-it reads the bounds and `budget` blocks instead of all keys and values.
+it reads the bounds and `budget` blocks instead of all keys and values. Its numbers are
+those of ``tree_attention``: FP32 sums, one rounding of the result.
 """
 
 from __future__ import annotations

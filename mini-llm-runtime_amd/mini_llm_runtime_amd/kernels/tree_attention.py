@@ -9,8 +9,9 @@ these are is a row of bits a token, made once a step from the tokens' parents
 (``tree_ancestors``) or by the caller. ``key_eviction.compact_keys`` then moves the
 accepted path's rows together.
 
-bf16, fp16 and FP32; head_dim a multiple of 8 (FP32: 4) up to 128; any block size;
-roundings as for ``scored_attention``.
+bf16, fp16 and FP32; head_dim a multiple of 8 (FP32: 4) up to 128; any block size.
+Scores, statistics and sums are FP32, whatever the type, a probability meets V to 2^-15 of
+itself in bf16 and 2^-21 in fp16, and the result is rounded once.
 """
 
 from __future__ import annotations
