@@ -272,7 +272,8 @@ __global__ __launch_bounds__(256) void score_blocks(SparseParams p) {
 //   |error| <= (2 d + 8) 2^-22 (sum_d |q_d|) (max_d |bound_d|)
 // for 2 d products, exact in 32 bits, added in any order with a relative error of 2^-22 each
 // (four times that of rounding to nearest), and 1e-30 of each factor for operands that
-// the matrix unit may take for 0. Not finite: no bound.
+// the matrix unit may take for 0. Not finite, or (sum_d |q_d|) (max_d |bound_d|) so large that a
+// sum may overflow on its way to a smaller one: no bound.
 // Bound by reading the bounds: 8 requests of 2,048 blocks, 4 KV heads of 128: 33 MB in
 // 13.6 us, where score_blocks takes 26 us.
 template <typename T> struct Rough;
@@ -366,7 +367,7 @@ __global__ __launch_bounds__(256) void score_rough(SparseParams p, int tiles) {
     strange = __any(strange);  // of the whole tile, for q is everyone's
     const float d = static_cast<float>(x.d);
     float off = (2.f * d + 8.f) * 0x1p-22f * most * size + 1e-30f * (most + d * size + d);
-    if (strange || !(fabsf(best) < 1e37f) || !(off < 1e37f)) {
+    if (strange || !(most * size < 1e37f) || !(off < 1e37f)) {
       best = 0.f;
       off = INFINITY;
     }

@@ -304,6 +304,30 @@ def test_scores_past_what_32_bits_hold(device, dtype):
                  **q_free)
 
 
+@pytest.mark.parametrize("scale", [1e-19, -1e-19])
+def test_sums_that_overflow_on_their_way(device, scale):
+    """A block whose best head has products of -3e38 four times, then as many of 3e38, the
+    last two steps larger: its score, 4e36, is past those of many others, 5e35 to 2e36 and all
+    unlike, though a sum in 32 bits passes -infinity on its way and the block's other
+    heads score far less."""
+    sign = 1.0 if scale > 0 else -1.0
+
+    def change(q, k, v, bounds, tables):
+        q[0, 0] = 0.0
+        q[0, 0, :4], q[0, 0, 4:9] = -1e19 * sign, 1e19 * sign
+        at = tables[0, 5:200]
+        first = torch.tensor(5e16).to(BF).view(torch.int16)
+        bounds[at, 1, 0, 8] = (first + torch.arange(len(at), dtype=torch.int16)).view(BF)
+        one = tables[0, 100]
+        bounds[one, :, 0, :8] = 3e19
+        bounds[one, 1, 0, 7] *= 1 + 2.0 ** -6
+        bounds[one, 1, 0, 8] = 1.0
+
+    _, blocks = run_case(device, BF, (14, 2, 64), [16 * 300], 20, recent=2, scale=scale,
+                         change=change, width=MANY)
+    assert 100 in blocks[0, 0].tolist()
+
+
 @pytest.mark.parametrize("dtype", [BF, FP, F32])
 def test_whole_requests_are_the_scored_decode(device, dtype):
     """A budget of all blocks: no bounds are read, and the result is the decode's; both are
