@@ -193,7 +193,9 @@ struct Pair {
   // v_mfma_f64_16x16x4: sum_d max(q low, q high) = [q-, q+].[low, high] with q- = min(q, 0)
   // and q+ = max(q, 0), heads as operand A, blocks as operand B. Where a bound or q is not
   // finite, 0 times it would be NaN where the larger of both products is not: such tiles
-  // are added up product by product, and a sum that is NaN does not count.
+  // take a head at a time, in every row of A, and only the bound that it asks for; a sum
+  // that is NaN does not count. Both add up the same products in the same order, so that
+  // blocks of the same score have it to the last bit wherever they stand.
   __device__ __forceinline__ double score(int64_t id) const {
     uint4 low[kT], high[kT];
     const bool there = read(low, high, id);
@@ -224,7 +226,7 @@ struct Pair {
         for (int r = 0; r < 4; ++r) best = fmax(best, sum0[r] + sum1[r]);
       } else {
         for (int h = h0; h < min(h0 + 16, heads); ++h) {
-          double sum = 0.;
+          f64x4_t sum0 = {0., 0., 0., 0.}, sum1 = {0., 0., 0., 0.};
 #pragma unroll
           for (int t = 0; t < kT; ++t) {
             float l[kE], u[kE];
@@ -233,14 +235,16 @@ struct Pair {
 #pragma unroll
             for (int e = 0; e < kE; ++e) {
               const int at = (g + 4 * t) * kE + e;
-              if (at >= d) continue;
-              const float f = Elem<T>::to_f32(q[h * q_sh + at]);
-              const double v = flip ? -f : f;
-              sum = fma(v, v >= 0. ? u[e] : l[e], sum);
+              const float f = at < d ? Elem<T>::to_f32(q[h * q_sh + at]) : 0.f;
+              const float v = flip ? -f : f;
+              const bool below = v < 0.f;
+              sum0 = __builtin_amdgcn_mfma_f64_16x16x4f64(below ? v : 0.f, below ? l[e] : 0.f, sum0,
+                                                          0, 0, 0);
+              sum1 = __builtin_amdgcn_mfma_f64_16x16x4f64(below ? 0.f : v, below ? 0.f : u[e], sum1,
+                                                          0, 0, 0);
             }
           }
-          sum += __shfl_xor(sum, 16);
-          sum += __shfl_xor(sum, 32);
+          const double sum = sum0[0] + sum1[0];
           best = sum > best ? sum : best;
         }
       }

@@ -328,6 +328,22 @@ def test_sums_that_overflow_on_their_way(device, scale):
     assert 100 in blocks[0, 0].tolist()
 
 
+@pytest.mark.parametrize("dtype", [BF, F32])
+@pytest.mark.parametrize("width", [None, 200, MANY])
+@pytest.mark.parametrize("left", [1, 5, 8])
+def test_ties_beside_a_block_that_is_not_finite(device, dtype, width, left):
+    """Every block of the first sixteen stands sixteen places on once more, and one of the
+    first has a bound that is not finite: its whole tile still has the scores of the copies, to
+    the last bit, so that the lower place goes first."""
+    def change(q, k, v, bounds, tables):
+        for i in range(4):
+            bounds[tables[i, 16:32]] = bounds[tables[i, :16]]
+            bounds[tables[i, 3 + i], 1, :, 5] = float("nan")
+
+    run_case(device, dtype, (14, 2, 64), [16 * 33] * 4, left + 1, sinks=0, recent=1, change=change,
+             width=width)
+
+
 @pytest.mark.parametrize("dtype", [BF, FP, F32])
 def test_whole_requests_are_the_scored_decode(device, dtype):
     """A budget of all blocks: no bounds are read, and the result is the decode's; both are
