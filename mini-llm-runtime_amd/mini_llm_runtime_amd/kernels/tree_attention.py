@@ -63,6 +63,12 @@ def tree_ancestors(
     return out
 
 
+def _validate_words(query_start_loc, words) -> None:
+    """For a max_query_len that the words may not cover: whether they cover the sequences."""
+    if ((query_start_loc[1:] - query_start_loc[:-1]) > 64 * words).any():
+        raise ValueError("ancestors must hold a bit for every drafted token of a sequence")
+
+
 def paged_attention_tree(
     q: torch.Tensor,
     k_cache: torch.Tensor,
@@ -120,7 +126,7 @@ def paged_attention_tree(
         raise ValueError("max_query_len cannot be negative")
     max_query_len = min(max_query_len, total_q)
     if validate and max_query_len > 64 * words:
-        raise ValueError("ancestors must hold a bit for every drafted token of a sequence")
+        _validate_words(query_start_loc, words)
     q = _aligned_q(q)
     width = block_tables.shape[1]
     dcode = _lib.DTYPE_CODES[q.dtype]

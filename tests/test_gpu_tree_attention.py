@@ -209,6 +209,30 @@ def test_strides_and_padding(device):
 
 
 @pytest.mark.parametrize("dtype", [BF, F32])
+@pytest.mark.parametrize("count", [5, 40])
+def test_a_bound_past_the_words(device, dtype, count):
+    """max_query_len bounds the sequences from above: one past the bits of the words is taken
+    as long as no sequence is so long."""
+    lens = [count + 30] * 3
+    k, v, tables = so.pool(lens, 16, 2, 64, dtype, 5)
+    q = torch.randn(3 * count, 14, 64, generator=torch.Generator().manual_seed(1)).to(dtype)
+    sets = [so.paths(so.random_parents(count, random.Random(i))) for i in range(3)]
+    bits = torch.cat([bits_of(s, 1) for s in sets]).to(device)
+    args = [x.to(device) for x in (q, k, v, tables, packed(sets), torch.tensor(lens))]
+    for most in (count, 65, 1 << 40):
+        got = paged_attention_tree(*args, bits, 16, max_query_len=most)
+        for i, s in enumerate(sets):
+            seen = torch.zeros(count, lens[i], dtype=torch.bool)
+            seen[:, :30] = True
+            for r, path in enumerate(s):
+                seen[r, [30 + j for j in path]] = True
+            slot, rows = so.slots(tables[i], lens[i], 16), slice(i * count, (i + 1) * count)
+            want, bound, _, _ = so.attend(q[rows], k.view(-1, 2, 64)[slot],
+                                          v.view(-1, 2, 64)[slot], seen, 0.125, 0.0, dtype)
+            so.assert_within(got[rows], want, bound, f"bound {most}, sequence {i}")
+
+
+@pytest.mark.parametrize("dtype", [BF, F32])
 def test_bad_blocks_are_masked(device, dtype):
     """With validate=False a block id out of range hides its keys."""
     k, v, tables = so.pool([100], 16, 2, 64, dtype, 5)

@@ -71,6 +71,19 @@ def test_tree_ancestors(parents, max_nodes, error, needle):
         tree_attention.tree_ancestors(parents, torch.tensor([0, 2]), max_nodes)
 
 
+@pytest.mark.parametrize("lens,words,fits", [
+    ([], 1, True), ([64, 0, 64], 1, True), ([64, 65], 1, False), ([65, 128], 2, True),
+    ([129], 2, False)])
+def test_tree_words(lens, words, fits):
+    """Sequences are held against the words, whatever a caller gave as the most of them."""
+    qsl = torch.tensor([0, *lens]).cumsum(0)
+    if fits:
+        tree_attention._validate_words(qsl, words)
+    else:
+        with pytest.raises(ValueError, match="a bit for every drafted token"):
+            tree_attention._validate_words(qsl, words)
+
+
 def cache_args(**change):
     a = dict(k_cache=cache(), v_cache=cache(), block_size=BS)
     a.update(change)
