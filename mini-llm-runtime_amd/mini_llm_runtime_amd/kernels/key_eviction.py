@@ -57,6 +57,21 @@ def _shared(block_tables: torch.Tensor, first: torch.Tensor, end: torch.Tensor) 
     return ((ids[1:] == ids[:-1]) & (ids[1:] >= 0)).any()
 
 
+def _newest_is_shared(block_tables: torch.Tensor, seq_lens: torch.Tensor,
+                      block_size: int) -> torch.Tensor:
+    """Whether a request's newest key, in a block that it fills to `fill` keys, is a key of
+    another place in the tables too: whether the same block is filled as far there."""
+    column = torch.arange(block_tables.shape[1], device=block_tables.device)[None, :]
+    last = torch.div(seq_lens - 1, block_size, rounding_mode="floor")[:, None]
+    fill = (seq_lens[:, None] - column * block_size).clamp(max=block_size)
+    # By block, then by fill, and of those that fill alike the newest keys' first: such a
+    # place must have no other of its block behind it.
+    order = 2 * (block_tables * (block_size + 1) + fill) + (column != last)
+    order = torch.where(column <= last, order, -1).flatten().sort().values
+    block = torch.div(order, 2 * (block_size + 1), rounding_mode="floor")
+    return ((order[:-1] >= 0) & (order[:-1] % 2 == 0) & (block[1:] == block[:-1])).any()
+
+
 def paged_attention_decode_weighted(
     q: torch.Tensor,
     k_cache: torch.Tensor,
@@ -76,9 +91,9 @@ def paged_attention_decode_weighted(
     of a request's newest key, at position seq_lens[b] - 1, is set, whatever it held. With
     validate=False a seq_lens of 0 (a padded row) gives zeros and adds nothing.
 
-    Requests may share blocks, but no request's newest key may be another's key too: each
-    adds to the entries of the shared keys, in no particular order, so that the last bits of
-    such a sum may differ from run to run.
+    Requests may share blocks, but no request's newest key may be another's key too, which
+    validate=True checks with the tables: each adds to the entries of the shared keys, in
+    no particular order, so that the last bits of such a sum may differ from run to run.
     The workspace holds the scores of the batch: 4 bytes for every query head and every
     position that the tables cover.
     """
@@ -98,6 +113,8 @@ def paged_attention_decode_weighted(
     num_blocks, _, num_kv_heads, _ = k_cache.shape
     if validate:
         _validate_tables(block_tables, seq_lens, block_size, num_blocks)
+        if _newest_is_shared(block_tables, seq_lens, block_size):
+            raise ValueError("a request's newest key must be no other key too")
     q = _aligned_q(q)
     width = block_tables.shape[1]
     lib = _lib.load()

@@ -317,3 +317,22 @@ def test_compaction_with_bad_blocks(device):
     k, v = k.to(device), v.to(device)
     compact_keys(k, v, tables.to(device), kept.to(device), 16, validate=False)
     assert torch.equal(k.cpu(), want[0]) and torch.equal(v.cpu(), want[1])
+
+
+def test_weighing_refuses_a_newest_key_of_two_requests(device):
+    """Its entry would be set by one and added to by the other. What is shared and is no
+    request's newest key is fine."""
+    k, v, tables = so.pool([40, 40], 16, 2, 64, BF, 1)
+    q = torch.zeros(2, 4, 64, dtype=BF, device=device)
+    weights = torch.zeros(k.shape[0], 2, 16, device=device)
+    lens = torch.tensor([40, 40]).to(device)
+    for shared, fits in ((2, True), (3, False)):
+        tables[1, :shared] = tables[0, :shared]
+        args = (q, k.to(device), v.to(device), weights, tables.to(device), lens, 16)
+        if fits:
+            paged_attention_decode_weighted(*args)
+            continue
+        before = weights.clone()
+        with pytest.raises(ValueError, match="newest key"):
+            paged_attention_decode_weighted(*args)
+        assert torch.equal(weights, before)

@@ -179,6 +179,38 @@ def test_lists_and_their_blocks():
             check(table, None, both)
 
 
+@pytest.mark.parametrize("tables,lens,shared", [
+    ([[0, 1], [0, 2]], [20, 32], False),          # a whole first block in common
+    ([[0, 1], [0, 2]], [20, 16], True),           # whose last key is the second's newest
+    ([[0, 1], [0, 1]], [20, 20], True),           # the same keys throughout
+    ([[0, 1], [0, 1]], [20, 24], True),           # the first's newest is a key of the second
+    ([[0, 1], [2, 0]], [17, 18], True),           # at another place there
+    ([[0, 1], [2, 0]], [16, 17], True),
+    ([[0, 0]], [18], True),                       # twice in one request
+    ([[0, 1], [1, 0]], [16, 16], False),          # columns past the end are not used
+    ([[0, -1], [1, -1], [2, 0]], [1, 16, 16], False),
+    ([[3, 1], [3, 2], [3, 0]], [17, 18, 19], False), ([[2]], [1], False)])
+def test_newest_keys(tables, lens, shared):
+    got = key_eviction._newest_is_shared(torch.tensor(tables), torch.tensor(lens), BS)
+    assert bool(got) == shared
+
+
+def test_newest_keys_against_all_pairs():
+    """Random tables over few blocks, against a count of the requests that hold each key."""
+    gen, seen = torch.Generator().manual_seed(1), set()
+    for case in range(300):
+        bs, batch, width = 1 + case % 3, 1 + case % 4, 3
+        tables = torch.randint(0, 9, (batch, width), generator=gen)
+        lens = torch.randint(1, width * bs + 1, (batch,), generator=gen)
+        held = [(tables[b, i // bs].item(), i % bs) for b in range(batch) for i in range(lens[b])]
+        newest = [(tables[b, (lens[b] - 1) // bs].item(), ((lens[b] - 1) % bs).item())
+                  for b in range(batch)]
+        want = any(held.count(key) > 1 for key in newest)
+        assert bool(key_eviction._newest_is_shared(tables, lens, bs)) == want
+        seen.add(want)
+    assert seen == {True, False}
+
+
 P = 1 << 20  # a pointer that is aligned and never read
 
 
