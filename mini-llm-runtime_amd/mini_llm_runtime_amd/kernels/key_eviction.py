@@ -147,8 +147,9 @@ def evict_keys(
     validate: bool = True,
 ) -> tuple[torch.Tensor, torch.Tensor]:
     """Cuts each request to `budget` keys for each KV head: its first `sinks`, its last
-    `recent` (half the budget if None) and the heaviest of the others by key_weights (ties: the
-    lower position; NaN counts as -infinity). What stays keeps its order and moves,
+    `recent` (None: half the budget, or what the sinks leave of it) and the heaviest of the
+    others by key_weights (ties: the lower position; NaN counts as -infinity). `budget` is
+    at least `sinks` and `recent` together. What stays keeps its order and moves,
     with its key_weights, to the positions 0, 1, ... of the request, in place; what lies
     behind is left as it is. With validate=False a seq_lens of 0 (a padded row) keeps none.
 
@@ -161,7 +162,7 @@ def evict_keys(
     device = _check_cache(k_cache, v_cache, block_size, what, key_weights)
     _check_weights(key_weights, k_cache)
     if recent is None:
-        recent = budget // 2
+        recent = max(min(budget // 2, budget - sinks), 0)
     if sinks < 0 or recent < 0 or budget < sinks + recent:
         raise ValueError("budget must be at least sinks + recent, and none of them negative")
     if not 0 <= budget < 1 << 31:

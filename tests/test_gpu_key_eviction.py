@@ -336,3 +336,19 @@ def test_weighing_refuses_a_newest_key_of_two_requests(device):
         with pytest.raises(ValueError, match="newest key"):
             paged_attention_decode_weighted(*args)
         assert torch.equal(weights, before)
+
+
+@pytest.mark.parametrize("budget,recent", [(4, 0), (5, 1), (6, 2), (7, 3), (8, 4), (9, 4), (33, 16)])
+def test_eviction_with_as_many_recent_keys_as_fit(device, budget, recent):
+    """Without `recent`: half the budget, or what the sinks leave of a small one."""
+    k, v, tables = so.pool([5, 70], 16, 2, 64, F32, 1)
+    w = torch.rand(k.shape[0], 2, 16, generator=torch.Generator().manual_seed(2))
+    lens = torch.tensor([5, 70]).to(device)
+    results = []
+    for more in (dict(recent=recent), dict()):
+        own = [x.to(device, copy=True) for x in (k, v, w)]
+        results.append([*evict_keys(*own, tables.to(device), lens, 16, budget, **more), *own])
+    for x, y in zip(*results):
+        assert torch.equal(x, y)
+    with pytest.raises(ValueError, match="budget"):
+        evict_keys(*own, tables.to(device), lens, 16, 3)
