@@ -75,8 +75,10 @@ __device__ __forceinline__ void join_row(const ScoredParams &p, int64_t row) {
 // Bound by latency, as the scores of 64 requests are 8 MB: what does not depend on the
 // statistics (table, scores of up to kAhead heads) is read before them, and the weights change
 // lanes, so that the lanes' atomics go to neighbouring entries. 64 requests of 128 to 4,096
-// keys, 14 heads over 2 of 64: 7.6 us, with the join of the results (four neighbours a lane:
-// 9.0); 500 to 2,000 keys, 12 over 12: 13.5 us (20).
+// keys, 14 heads over 2 of 64: 7.2 us, with the join of the results (four neighbours a lane:
+// 9.0); 500 to 2,000 keys, 12 over 12: 11.2 us (20). A wave past its request's end leaves
+// before it reads scores, which nobody wrote there: 64 requests of 500 to 1,024 keys in tables of
+// 32,768 9.2 us, 22.4 with the work of all waves, 6.3 in tables of 1,024.
 constexpr int kAhead = 8;
 __device__ __forceinline__ void weigh_keys(const ScoredParams &p, float *weights, int64_t task,
                                            float (*s_ml)[2], float *s_w) {
@@ -86,6 +88,7 @@ __device__ __forceinline__ void weigh_keys(const ScoredParams &p, float *weights
   const int64_t covered = p.bt_width * p.block_size;
   const int64_t base = task / p.seqs / p.hkv * kChunk, key0 = base + 4 * lane;
   const int64_t ctx = clamp64(p.ctx[seq], 0, covered);
+  if (base >= ctx) return;  // uniform
   const float *row = p.scores + (seq * p.hq + kvh * p.group) * p.scores_st +
                      min(key0, p.scores_st - 4);
   float4 x[kAhead];

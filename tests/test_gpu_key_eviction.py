@@ -352,3 +352,28 @@ def test_eviction_with_as_many_recent_keys_as_fit(device, budget, recent):
         assert torch.equal(x, y)
     with pytest.raises(ValueError, match="budget"):
         evict_keys(*own, tables.to(device), lens, 16, 3)
+
+
+@pytest.mark.parametrize("dtype", [BF, F32])
+def test_weighing_in_wide_tables(device, dtype):
+    """Tables padded to far more columns than the requests fill: keys behind a request's end
+    get nothing, and the columns' ids are not looked at."""
+    lens = [1, 256, 257, 40, 1000]
+    k, v, tables = so.pool(lens, 16, 2, 64, dtype, 5, width=2048)
+    tables[:, 100:] = 1 << 40
+    q = torch.randn(5, 14, 64, generator=torch.Generator().manual_seed(1)).to(dtype)
+    weights = torch.zeros(k.shape[0], 2, 16, device=device)
+    got = paged_attention_decode_weighted(q.to(device), k.to(device), v.to(device), weights,
+                                          tables.to(device), torch.tensor(lens).to(device), 16)
+    want = torch.zeros(weights.shape, dtype=torch.float64)
+    size = torch.zeros_like(want)
+    for i, n in enumerate(lens):
+        slot = so.slots(tables[i], n, 16)
+        out, bound, p, pb = so.attend(q[i:i + 1], k.view(-1, 2, 64)[slot],
+                                      v.view(-1, 2, 64)[slot],
+                                      torch.ones(1, n, dtype=torch.bool), 0.125, 0.0, dtype)
+        so.assert_within(got[i:i + 1], out, bound, f"request {i}")
+        add = p[0].view(2, 7, n).sum(1).T
+        want[slot // 16, :, slot % 16] = add
+        size[slot // 16, :, slot % 16] = pb[0].view(2, 7, n).sum(1).T + 8 * 2.0 ** -24 * add
+    so.assert_within(weights, want, size, "weights")
