@@ -85,11 +85,11 @@ __device__ __forceinline__ bool bit_of(const ScoredParams &p, int64_t row, int n
 }
 
 // Two probabilities a and b as operands of 16 bits, hi + lo each, which a product with V adds
-// up in FP32: hi is cut off, not rounded, and lo is more than 0 wherever hi is, so that an
-// infinite V stays one (hi times it and lo times it have one sign, and 0 times it is met only
-// where the probability is 0). lo, up to 2^-7 of it in bf16 and 2^-10 in fp16, is rounded by
-// 2^-8 and 2^-11 of itself: 2^-15 and 2^-21 of the probability. fp16 takes numbers scaled up to
-// 2^15, of which it drops 2^-24 at most, 2^-39 of the largest.
+// up in FP32: hi is cut off, not rounded, and lo is more than 0 wherever hi is (in bf16 down
+// to probabilities of 2^-103), so that an infinite V stays one: hi times it and lo times it
+// have one sign, and neither is 0 times it. lo, up to 2^-7 of the probability in bf16 and
+// 2^-10 in fp16, is rounded by 2^-8 and 2^-11 of itself: 2^-15 and 2^-21 of the probability.
+// fp16 takes numbers scaled up to 2^15, of which it drops 2^-24 at most, 2^-39 of that.
 template <typename T>
 __device__ __forceinline__ void two_parts(float a, float b, uint32_t &hi, uint32_t &lo) {
   typedef float f32x2_v __attribute__((ext_vector_type(2)));
